@@ -91,7 +91,7 @@ def draw(rng):
         return case
     if kind == "norm":
         H = _hidden(rng)
-        return {"kind": kind, "grad": grad, "tokens": _log(rng, 1, min(20000, 16384 * 4096 // (H * (2 if grad else 1)))),
+        return {"kind": kind, "grad": grad, "tokens": _log(rng, 1, min(20000, 14000 * 4096 // (H * (2 if grad else 1)))),
                 "hidden": H, "residual": rng.choice(["fp32", "bf16"]), "gate": rng.choice(["none", "token", "channel", "full"]),
                 "sigmoid": rng.random() < 0.5, "post": rng.random() < 0.75, "offset": rng.choice([0.0, 1.0])}
     V = rng.choice([VOCAB, rng.randint(500, 160000), rng.randint(20000, 160000)])
