@@ -81,7 +81,7 @@ def draw(rng):
     if kind in ("sort", "back"):
         H, E = _hidden(rng), rng.randint(8, 512)
         k = rng.randint(1, min(E, 12))
-        T = _log(rng, 1, min(16384, 4096 * 8 * 7168 // (k * H)))
+        T = _log(rng, 1, min(16384, 4096 * 6 * 7168 // (k * H)))
         case = {"kind": kind, "grad": grad, "tokens": T, "k": k, "experts": E, "hidden": H,
                 "type": rng.choice(["bf16", "bf16", "fp32"]), "absent": rng.choice([0.0, 0.0, 0.1, 0.5])}
         if case["type"] == "fp32":
