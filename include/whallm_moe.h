@@ -148,6 +148,39 @@ WM_EXPORT int wm_permute(const int32_t* indices, int64_t pairs, int32_t experts,
                          int32_t* order, int32_t* inverse, int32_t* offsets, int32_t* tiles,
                          int32_t* tile_count, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- token rows to their experts and back -----------------------------------
+ * For expert products outside this library (other weight formats, experts in training): the rows
+ * of a batch sorted by expert, the products' rows back to their tokens, and the gradients of both
+ * (the gather, inverse gather and weighted sum of qwen4_exp.py:865-904, :1048-1051; the reference
+ * has no gradients). rows [tokens * k, hidden], x, y, dx, dy, add [tokens, hidden] hold bf16, or
+ * fp32 where `fp32` is 1, aligned to their elements (16-byte aligned rows of a multiple of 16
+ * bytes are moved 16 bytes at a time). hidden 1..1048576, k 1..64, tokens * k below 2^31. inverse
+ * [tokens * k] is the row of each pair, -1 for a pair without one (wm_sort_tokens, wm_permute).
+ * Outputs must not overlap inputs, except that y may be add. */
+/* Sorts the pairs as wm_permute does (experts 1..1024) and copies x[t] to the rows of t's pairs;
+ * the lists as wm_permute's, and behind their ends: order -1, tiles (-1, -1), rows zero.
+ * tiles [ceil(tokens * k / tile_rows) + experts][2], 8-byte aligned.
+ * workspace: wm_sort_tokens_workspace_size bytes. */
+WM_EXPORT size_t wm_sort_tokens_workspace_size(int32_t tokens, int32_t k, int32_t experts);
+WM_EXPORT int wm_sort_tokens(const void* x, int32_t fp32, int32_t tokens, int32_t hidden, const int32_t* indices,
+                             int32_t k, int32_t experts, int32_t tile_rows, void* rows, int32_t* order,
+                             int32_t* inverse, int32_t* offsets, int32_t* tiles, int32_t* tile_count, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* dx[t] = sum_j drows[inverse[t, j]] over the pairs that have a row, fp32 in j order. */
+WM_EXPORT int wm_sort_tokens_backward(const void* drows, int32_t fp32, const int32_t* inverse, int32_t tokens,
+                                      int32_t k, int32_t hidden, void* dx, void* stream);
+/* y[t] = sum_j weights[t, j] * rows[inverse[t, j]] (+ add[t], nullable), fp32 in j order; weights
+ * fp32 [tokens, k]. wm_combine_pairs for rows in expert order. */
+WM_EXPORT int wm_combine_rows(const void* rows, int32_t fp32, const float* weights, const int32_t* inverse,
+                              int32_t tokens, int32_t k, int32_t hidden, const void* add, void* y, void* stream);
+/* The gradients of wm_combine_rows from dy: drows[inverse[t, j]] = weights[t, j] * dy[t], zero in
+ * the rows from *present on (device; the number of pairs with a row, offsets[experts] of the
+ * sort), dweights[t, j] = dy[t] . rows[inverse[t, j]] (fp32; 0 for a pair without a row). The
+ * gradient of add is dy itself. */
+WM_EXPORT int wm_combine_rows_backward(const void* dy, const void* rows, int32_t fp32, const float* weights,
+                                       const int32_t* inverse, const int32_t* present, int32_t tokens, int32_t k,
+                                       int32_t hidden, void* drows, float* dweights, void* stream);
+
 /* ---- MXFP4 expert FFN -----------------------------------------------------
  * One MoE layer, Qwen form (SparseMoE.__call__, qwen4_exp.py:1015-1051):
  *   y[t] = sum_k weights[t,k] * FFN_{indices[t,k]}(x[t]) + sigmoid(x[t] . shared_gate) * FFN_shared(x[t])

@@ -1,0 +1,103 @@
+"""Refusals of the calls around the expert products, without a GPU: the C entry points' argument checks
+and the Python layer's, both before any launch."""
+import pytest
+import torch
+
+from whallm_amd import _lib, ops
+
+A = 0x10000   # an aligned address that is never read
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The Python checks on CPU tensors; a call that gets past them fails the test."""
+    def reached(device, name, *args):
+        raise AssertionError(f"{name} was called")
+    monkeypatch.setattr(ops, "_require_device", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(ops, "_launch", reached)
+
+
+def sort_args(**kw):
+    a = dict(x=A, fp32=0, tokens=4, hidden=64, indices=A, k=2, experts=8, tile_rows=16, rows=A, order=A, inverse=A, offsets=A,
+             tiles=A, tile_count=A, workspace=A, workspace_bytes=1 << 30, stream=None)
+    a.update(kw)
+    return a.values()
+
+
+@pytest.mark.parametrize("kw,msg", [
+    ({"tokens": -1}, "negative"), ({"k": 0}, "k must be"), ({"k": 65}, "k must be"), ({"hidden": 0}, "hidden must be"),
+    ({"hidden": 1 << 21}, "hidden must be"), ({"fp32": 2}, "fp32 must be"), ({"experts": 0}, "experts must be"),
+    ({"experts": 1025}, "experts must be"), ({"tile_rows": 0}, "tile_rows"), ({"tokens": 1 << 30, "k": 2}, "below 2"),
+    ({"x": None}, "null pointer"), ({"indices": None}, "null pointer"), ({"rows": None}, "null pointer"),
+    ({"offsets": None}, "null pointer"), ({"workspace": None}, "null pointer"), ({"workspace_bytes": 8}, "workspace too small"),
+    ({"x": A + 1}, "aligned"), ({"rows": A + 2, "fp32": 1}, "aligned"), ({"tiles": A + 4}, "aligned"),
+])
+def test_sort_tokens_c_refusals(kw, msg):
+    with pytest.raises(_lib.WhallmError, match=msg):
+        _lib.call("wm_sort_tokens", *sort_args(**kw))
+
+
+def test_rows_c_refusals():
+    def backward(drows=A, fp32=0, inverse=A, tokens=4, k=2, hidden=64, dx=A):
+        _lib.call("wm_sort_tokens_backward", drows, fp32, inverse, tokens, k, hidden, dx, None)
+
+    def combine(rows=A, fp32=0, weights=A, inverse=A, tokens=4, k=2, hidden=64, add=None, y=A):
+        _lib.call("wm_combine_rows", rows, fp32, weights, inverse, tokens, k, hidden, add, y, None)
+
+    def grads(dy=A, rows=A, fp32=0, weights=A, inverse=A, present=A, tokens=4, k=2, hidden=64, drows=A, dweights=A):
+        _lib.call("wm_combine_rows_backward", dy, rows, fp32, weights, inverse, present, tokens, k, hidden, drows, dweights, None)
+
+    for call in (backward, combine, grads):
+        for kw, msg in (({"tokens": -2}, "negative"), ({"k": 0}, "k must be"), ({"k": 65}, "k must be"),
+                        ({"hidden": 0}, "hidden must be"), ({"fp32": -1}, "fp32 must be"), ({"inverse": None}, "null pointer")):
+            with pytest.raises(_lib.WhallmError, match=msg):
+                call(**kw)
+        call(tokens=0)   # nothing to do
+    for call, kw in ((backward, {"dx": A + 1}), (combine, {"add": A + 1}), (combine, {"fp32": 1, "y": A + 2}), (grads, {"dy": A + 1})):
+        with pytest.raises(_lib.WhallmError, match="aligned"):
+            call(**kw)
+    for kw in ({"present": None}, {"drows": None}, {"dweights": None}):
+        with pytest.raises(_lib.WhallmError, match="null pointer"):
+            grads(**kw)
+
+
+def test_rows_take_device_tensors_only():
+    x, idx = torch.zeros(2, 8), torch.zeros(2, 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="device"):
+        ops.sort_tokens(x, idx, 4)
+
+
+def test_rows_python_refusals(on_cpu):
+    x, idx, w = torch.zeros(6, 8), torch.zeros(6, 2, dtype=torch.int32), torch.zeros(6, 2)
+    rows = torch.zeros(12, 8)
+    p = ops.Permutation(*(torch.zeros(n, dtype=torch.int32) for n in (12, 12, 5, 8, 1)))
+    with pytest.raises(ValueError, match="bfloat16 or float32"):
+        ops.sort_tokens(x.half(), idx, 4)
+    with pytest.raises(ValueError, match="indices must be"):
+        ops.sort_tokens(x, idx.long(), 4)
+    with pytest.raises(ValueError, match="indices must be"):
+        ops.sort_tokens(x, idx[:5], 4)
+    with pytest.raises(ValueError, match="positive"):
+        ops.sort_tokens(x[:, :0], idx, 4)
+    with pytest.raises(ValueError, match="autograd"):
+        ops.sort_tokens(x.clone().requires_grad_(), idx, 4)
+    with pytest.raises(ValueError, match="not that of these rows"):
+        ops.sort_tokens_backward(rows[:10], p, 2)
+    with pytest.raises(ValueError, match="k rows of every token"):
+        ops.sort_tokens_backward(rows, p, 5)
+    with pytest.raises(ValueError, match="weights"):
+        ops.combine_rows(rows, w[:5], p)
+    with pytest.raises(ValueError, match="weights must be torch.float32"):
+        ops.combine_rows(rows, w.double(), p)
+    with pytest.raises(ValueError, match="add must be"):
+        ops.combine_rows(rows, w, p, x.bfloat16())
+    with pytest.raises(ValueError, match="add must be"):
+        ops.combine_rows(rows, w, p, x[:5])
+    with pytest.raises(ValueError, match="autograd"):
+        ops.combine_rows(rows, w.clone().requires_grad_(), p)
+    with pytest.raises(ValueError, match="dy must be"):
+        ops.combine_rows_backward(x.bfloat16(), rows, w, p)
+    with pytest.raises(ValueError, match="dy must be"):
+        ops.combine_rows_backward(x[:, :4], rows, w, p)
+    with torch.no_grad(), pytest.raises(AssertionError, match="wm_combine_rows was called"):
+        ops.combine_rows(rows.requires_grad_(), w, p)

@@ -59,6 +59,12 @@ _SIGNATURES = {
     "wm_linear_bf16": (c_int, [_P, _P, c_int32, c_int32, c_int32, _P, _P]),
     "wm_permute_workspace_size": (c_size_t, [c_int64, c_int32]),
     "wm_permute": (c_int, [_P, c_int64, c_int32, c_int32, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "wm_sort_tokens_workspace_size": (c_size_t, [c_int32, c_int32, c_int32]),
+    "wm_sort_tokens": (c_int, [_P, c_int32, c_int32, c_int32, _P, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P, _P, _P,
+                               c_size_t, _P]),
+    "wm_sort_tokens_backward": (c_int, [_P, c_int32, _P, c_int32, c_int32, c_int32, _P, _P]),
+    "wm_combine_rows": (c_int, [_P, c_int32, _P, _P, c_int32, c_int32, c_int32, _P, _P, _P]),
+    "wm_combine_rows_backward": (c_int, [_P, _P, c_int32, _P, _P, _P, c_int32, c_int32, c_int32, _P, _P, _P]),
     "wm_moe_mxfp4_workspace_size": (c_size_t, [c_int32, c_int32, POINTER(MXFP4ExpertsC)]),
     "wm_moe_mxfp4": (c_int, [_P, c_int32, _P, _P, c_int32, POINTER(MXFP4ExpertsC), POINTER(MXFP4ExpertsC), _P,
                              _P, _P, c_size_t, _P]),

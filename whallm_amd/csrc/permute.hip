@@ -201,6 +201,12 @@ __global__ void __launch_bounds__(64) permute_scatter_kernel(const int32_t* __re
   }
 }
 
+void permute_count(const int32_t* indices, int64_t pairs, int experts, const PermuteWorkspace& ws, hipStream_t s) {
+  hipLaunchKernelGGL(permute_count_kernel, dim3((unsigned)permute_count_blocks(pairs)), dim3(64 * PERMUTE_COUNT_WAVES), 0, s,
+                     indices, pairs, experts, ws.counts, ws.done);
+  check_launch("permute_count");
+}
+
 // See moe_internal.h.
 void permute_lists(const int32_t* indices, int64_t pairs, int experts, int tile_rows, int cold_rows, int32_t* order,
                    int32_t* inverse, int32_t* row_token, int k, int32_t* offsets, int32_t* tiles, int32_t* cold_tiles,
@@ -247,9 +253,7 @@ WM_EXPORT int wm_permute(const int32_t* indices, int64_t pairs, int32_t experts,
     if (!offsets || !tile_count || !workspace || (pairs > 0 && (!indices || !order || !inverse || !tiles)))
       fail("wm_permute: null pointer");
     const PermuteWorkspace ws = permute_workspace(workspace, pairs, experts);
-    hipLaunchKernelGGL(permute_count_kernel, dim3((unsigned)permute_count_blocks(pairs)), dim3(64 * PERMUTE_COUNT_WAVES), 0,
-                       as_stream(stream), indices, pairs, experts, ws.counts, ws.done);
-    check_launch("permute_count");
+    permute_count(indices, pairs, experts, ws, as_stream(stream));
     permute_lists(indices, pairs, experts, tile_rows, 0, order, inverse, nullptr, 1, offsets, tiles, nullptr, tile_count, ws,
                   as_stream(stream));
   });

@@ -304,6 +304,147 @@ def permute(indices: torch.Tensor, experts: int, tile_rows: int = 128) -> Permut
     return Permutation(order, inverse, offsets, tiles, count)
 
 
+# ----------------------------------------------------------------------------- token rows to experts and back
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """One call on ``device``'s current stream (its last argument), whatever the current device is."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream)
+
+
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _no_autograd(name: str, *tensors: torch.Tensor | None) -> None:
+    """Refuses inputs whose gradient would be lost: these calls are not recorded by autograd."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        how = "it has no gradient" if name.endswith("_backward") else f"its gradients are {name}_backward's"
+        raise ValueError(f"{name} is not recorded by autograd ({how}): call it under torch.no_grad()")
+
+
+def _rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{name} must be bfloat16 or float32, got {t.dtype}")
+    if like is not None and t.dtype != like.dtype:
+        raise ValueError(f"{name} must be {like.dtype} like the other rows, got {t.dtype}")
+    return t.contiguous()
+
+
+def _pair_rows(rows: torch.Tensor, permutation: Permutation, k: int) -> int:
+    """The tokens of rows [T * K, H] in the order of ``permutation``."""
+    if rows.dim() != 2:
+        raise ValueError("rows must be [tokens * k, hidden]")
+    pairs = rows.shape[0]
+    inverse = permutation.inverse
+    if k < 1 or pairs % k:
+        raise ValueError("rows must hold k rows of every token")
+    if inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.numel() != pairs:
+        raise ValueError("the permutation is not that of these rows")
+    return pairs // k
+
+
+def sort_tokens(x: torch.Tensor, indices: torch.Tensor, experts: int,
+                tile_rows: int = 128) -> tuple[torch.Tensor, Permutation]:
+    """x [.., H] (bf16 or fp32) with the experts of every token, indices int32 [.., K] -> (rows [T * K, H] in
+    expert order, the Permutation of ``permute``): expert e's tokens are rows[offsets[e]:offsets[e + 1]].
+    A pair whose id is no expert (padding, not resident) has no row; the rows behind the last pair are zero,
+    ``order`` and ``tiles`` -1 behind their ends (wm_sort_tokens)."""
+    device = _require_device(x, indices)
+    _no_autograd("sort_tokens", x)
+    x = _rows(x, "x")
+    if x.dim() < 1 or indices.dim() != x.dim() or indices.shape[:-1] != x.shape[:-1]:
+        raise ValueError("indices must be [.., K] for x [.., H]")
+    if indices.dtype != torch.int32:
+        raise ValueError(f"indices must be {torch.int32}, got {indices.dtype}")
+    indices = indices.contiguous()
+    H, k = x.shape[-1], indices.shape[-1]
+    if H < 1 or k < 1 or experts < 1 or tile_rows < 1:
+        raise ValueError("hidden, k, experts and tile_rows must be positive")
+    T = x.numel() // H
+    P = T * k
+    max_tiles = -(-P // tile_rows) + experts
+    ws_bytes = _lib.load().wm_sort_tokens_workspace_size(T, k, experts)
+    rows = torch.empty(P, H, dtype=x.dtype, device=device)
+    # the lists and the workspace in one allocation, tiles first (8-byte aligned)
+    tiles, order, inverse, offsets, count, ws = torch.empty(
+        2 * max_tiles + 2 * P + experts + 2 + -(-ws_bytes // 4), dtype=torch.int32, device=device).split(
+        [2 * max_tiles, P, P, experts + 1, 1, -(-ws_bytes // 4)])
+    _launch(device, "wm_sort_tokens", x.data_ptr(), int(x.dtype == torch.float32), T, H, indices.data_ptr(), k, experts,
+            tile_rows, rows.data_ptr(), order.data_ptr(), inverse.data_ptr(), offsets.data_ptr(), tiles.data_ptr(),
+            count.data_ptr(), ws.data_ptr(), ws_bytes)
+    return rows, Permutation(order, inverse, offsets, tiles.view(max_tiles, 2), count)
+
+
+def sort_tokens_backward(drows: torch.Tensor, permutation: Permutation, k: int) -> torch.Tensor:
+    """The gradient of sort_tokens: drows [T * K, H] -> dx [T, H] = the sum over each token's rows, fp32 in k
+    order, rounded once to drows' type (wm_sort_tokens_backward)."""
+    device = _require_device(drows, permutation.inverse)
+    _no_autograd("sort_tokens_backward", drows)
+    drows = _rows(drows, "drows")
+    T, H = _pair_rows(drows, permutation, k), drows.shape[1]
+    dx = torch.empty(T, H, dtype=drows.dtype, device=device)
+    _launch(device, "wm_sort_tokens_backward", drows.data_ptr(), int(drows.dtype == torch.float32),
+            permutation.inverse.data_ptr(), T, k, H, dx.data_ptr())
+    return dx
+
+
+def combine_rows(rows: torch.Tensor, weights: torch.Tensor, permutation: Permutation,
+                 add: torch.Tensor | None = None) -> torch.Tensor:
+    """The expert products' rows [T * K, H] (bf16 or fp32, in expert order) back to their tokens:
+    y[.., :] = sum_k weights[.., k] * rows[inverse] (+ add), fp32 in k order, rounded once; weights fp32
+    [.., K], y and add [.., H] in rows' type (wm_combine_rows; combine_pairs takes rows in router order)."""
+    device = _require_device(rows, weights, permutation.inverse, add)
+    _no_autograd("combine_rows", rows, weights, add)
+    rows = _rows(rows, "rows")
+    weights = _contig(weights, torch.float32, "weights")
+    if weights.dim() < 1:
+        raise ValueError("weights must be [.., K]")
+    k = weights.shape[-1]
+    T, H = _pair_rows(rows, permutation, k), rows.shape[1]
+    if weights.numel() != T * k:
+        raise ValueError("weights must be [.., K] matching rows")
+    shape = (*weights.shape[:-1], H)
+    if add is not None:
+        add = _rows(add, "add", rows)
+        if add.shape != shape:
+            raise ValueError("add must be [.., H] matching weights")
+    y = torch.empty(shape, dtype=rows.dtype, device=device)
+    _launch(device, "wm_combine_rows", rows.data_ptr(), int(rows.dtype == torch.float32), weights.data_ptr(),
+            permutation.inverse.data_ptr(), T, k, H, _at(add), y.data_ptr())
+    return y
+
+
+def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor,
+                          permutation: Permutation) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of combine_rows from dy [.., H]: (drows [T * K, H] in rows' type, zero behind the last
+    pair; dweights fp32 [.., K], 0 where a pair has no row). The gradient of ``add`` is dy itself
+    (wm_combine_rows_backward)."""
+    device = _require_device(dy, rows, weights, permutation.inverse, permutation.offsets)
+    _no_autograd("combine_rows_backward", dy, rows, weights)
+    rows = _rows(rows, "rows")
+    dy = _rows(dy, "dy", rows)
+    weights = _contig(weights, torch.float32, "weights")
+    if weights.dim() < 1:
+        raise ValueError("weights must be [.., K]")
+    k = weights.shape[-1]
+    T, H = _pair_rows(rows, permutation, k), rows.shape[1]
+    if weights.numel() != T * k or dy.shape != (*weights.shape[:-1], H):
+        raise ValueError("dy must be [.., H] and weights [.., K] matching rows")
+    offsets = permutation.offsets
+    if offsets.dtype != torch.int32 or not offsets.is_contiguous() or offsets.numel() < 1:
+        raise ValueError("the permutation's offsets must be contiguous int32")
+    drows, dweights = torch.empty_like(rows), torch.empty_like(weights)
+    _launch(device, "wm_combine_rows_backward", dy.data_ptr(), rows.data_ptr(), int(rows.dtype == torch.float32),
+            weights.data_ptr(), permutation.inverse.data_ptr(), offsets.data_ptr() + 4 * (offsets.numel() - 1), T, k, H,
+            drows.data_ptr(), dweights.data_ptr())
+    return drows, dweights
+
+
 # ----------------------------------------------------------------------------- expert FFN
 
 def _check_indices(indices: torch.Tensor, experts: int, validate: bool) -> None:
