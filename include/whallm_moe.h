@@ -333,6 +333,42 @@ WM_EXPORT int wm_norm_router(const float* residual, const void* y, const void* n
 WM_EXPORT size_t wm_router_packed_bytes(int32_t experts, int32_t hidden, int32_t has_gate);
 WM_EXPORT int wm_repack_router(const void* router, const void* shared_gate, int32_t experts, int32_t hidden,
                                void* packed, void* stream);
+/* The norms around a block (the step of wm_residual_rmsnorm for layers that also norm, gate or
+ * scale what a block adds; the reference has neither these nor their gradients):
+ *   z = y * rsqrt(mean(y^2) + eps) * (weight_offset + post_weight)   (post_norm 0: z = y)
+ *   residual_out = residual + scale * g * z
+ *   x = residual_out * rsqrt(mean(residual_out^2) + eps) * (weight_offset + pre_weight)
+ * over rows of hidden values, fp32 inside, x from residual_out as it is stored. y and x bf16,
+ * residual and residual_out bf16 or fp32 [tokens, hidden], weights bf16 [hidden] (null: the norm
+ * alone, no offset), the gate g bf16 or fp32, through a sigmoid with gate_sigmoid. hidden 1..16384;
+ * rows of a multiple of 8 values at 16-byte aligned addresses are read 16 bytes at a time, others
+ * value by value. */
+typedef struct wm_block_norm_form {
+  const void* post_weight;
+  const void* pre_weight;
+  const void* gate;
+  float weight_offset;           /* 1 for weights stored as their distance from 1 */
+  float scale;
+  float eps;
+  int32_t post_norm;
+  int32_t gate_kind;             /* 0 none (g = 1), 1 [tokens], 2 [hidden], 3 [tokens, hidden] */
+  int32_t gate_fp32;
+  int32_t gate_sigmoid;
+  int32_t residual_fp32;
+} wm_block_norm_form;
+/* residual_out may be residual; no other output overlaps an input. */
+WM_EXPORT int wm_block_norm(const wm_block_norm_form* form, const void* residual, const void* y, int32_t tokens,
+                            int32_t hidden, void* residual_out, void* x, void* stream);
+/* The gradients from dx (bf16) and dresidual_out (in the residual's type, nullable: zero), given the
+ * residual_out and y of the forward pass: dresidual (the residual's type; may be dresidual_out), dy
+ * (bf16; may be dx), dpost_weight and dpre_weight fp32 [hidden], dgate fp32 for a gate of kind 1 or 2
+ * and in the gate's type for kind 3. The gradient outputs of absent weights and gates are null.
+ * workspace: wm_block_norm_backward_workspace_size bytes, 16-byte aligned. */
+WM_EXPORT size_t wm_block_norm_backward_workspace_size(int32_t tokens, int32_t hidden);
+WM_EXPORT int wm_block_norm_backward(const wm_block_norm_form* form, const void* dx, const void* dresidual_out,
+                                     const void* residual_out, const void* y, int32_t tokens, int32_t hidden,
+                                     void* dresidual, void* dy, float* dpost_weight, float* dpre_weight, void* dgate,
+                                     void* workspace, size_t workspace_bytes, void* stream);
 /* `layers` MoE layers chained as x_l = rmsnorm(r_l), r_{l+1} = r_l + MoE_l(x_l), routing
  * from logits [layers, T, E] on the device (no host synchronisation; graph-capturable).
  * experts / shared / shared_gates are host arrays of `layers` entries (shared and

@@ -101,3 +101,69 @@ def test_rows_python_refusals(on_cpu):
         ops.combine_rows_backward(x[:, :4], rows, w, p)
     with torch.no_grad(), pytest.raises(AssertionError, match="wm_combine_rows was called"):
         ops.combine_rows(rows.requires_grad_(), w, p)
+
+
+# ----------------------------------------------------------------------------- block norm
+
+def norm_form(**kw):
+    f = dict(post_weight=A, pre_weight=A, gate=None, weight_offset=0.0, scale=1.0, eps=1e-6, post_norm=1, gate_kind=0, gate_fp32=0,
+             gate_sigmoid=0, residual_fp32=1)
+    f.update(kw)
+    return _lib.BlockNormFormC(*f.values())
+
+
+def norm_call(form=None, residual=A, y=A, tokens=2, hidden=64, residual_out=A, x=A, **kw):
+    _lib.call("wm_block_norm", form or norm_form(**kw), residual, y, tokens, hidden, residual_out, x, None)
+
+
+def norm_grad_call(dx=A, dres=A, residual_out=A, y=A, tokens=2, hidden=64, dr=A, dy=A, dpost=A, dpre=A, dgate=None, ws=A,
+                   ws_bytes=1 << 30, **kw):
+    _lib.call("wm_block_norm_backward", norm_form(**kw), dx, dres, residual_out, y, tokens, hidden, dr, dy, dpost, dpre, dgate, ws,
+              ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    ({"tokens": -1}, "negative"), ({"hidden": 0}, "hidden must be"), ({"hidden": 16385}, "hidden must be"),
+    ({"gate_kind": 4, "gate": A}, "gate_kind"), ({"gate_kind": 1}, "go together"), ({"gate": A}, "go together"),
+    ({"post_norm": 0}, "needs the post norm"), ({"eps": -1.0}, "eps"), ({"eps": float("nan")}, "eps"), ({"y": None}, "null pointer"),
+    ({"y": A + 1}, "aligned"), ({"gate_kind": 2, "gate_fp32": 1, "gate": A + 2, "dgate": A}, "aligned"),
+])
+def test_block_norm_c_refusals(kw, msg):
+    with pytest.raises(_lib.WhallmError, match=msg):
+        norm_call(**{k: v for k, v in kw.items() if k != "dgate"})
+    with pytest.raises(_lib.WhallmError, match="go with their gradients" if kw.get("gate") and "dgate" not in kw and kw.get("gate_kind") in (1, 2, 3) else msg):
+        norm_grad_call(**kw)
+
+
+def test_block_norm_c_refusals_of_one_side():
+    for kw, msg in (({"residual": None}, "null pointer"), ({"residual_out": None}, "null pointer"), ({"x": None}, "null pointer"),
+                    ({"residual": A + 2}, "aligned")):
+        with pytest.raises(_lib.WhallmError, match=msg):
+            norm_call(**kw)
+    with pytest.raises(_lib.WhallmError, match="null form"):
+        _lib.call("wm_block_norm", None, A, A, 1, 64, A, A, None)
+    for kw, msg in (({"dx": None}, "null pointer"), ({"dr": None}, "null pointer"), ({"dy": None}, "null pointer"),
+                    ({"ws": None}, "null pointer"), ({"ws_bytes": 64}, "workspace too small"), ({"ws": A + 4}, "misaligned"),
+                    ({"dpost": None}, "gradients"), ({"dpre": None}, "gradients"), ({"dgate": A}, "gradients"),
+                    ({"gate": A, "gate_kind": 1}, "gradients"), ({"dpre": A + 2}, "aligned"), ({"dres": A + 2}, "aligned")):
+        with pytest.raises(_lib.WhallmError, match=msg):
+            norm_grad_call(**kw)
+    norm_call(tokens=0)
+    lib = _lib.load()
+    assert lib.wm_block_norm_backward_workspace_size(-1, 64) == 0 and lib.wm_block_norm_backward_workspace_size(4, 0) == 0
+
+
+def test_block_norm_python_refusals(on_cpu):
+    r, y, w = torch.zeros(3, 8), torch.zeros(3, 8, dtype=torch.bfloat16), torch.zeros(8, dtype=torch.bfloat16)
+    for args, kw, msg in (
+            ((r.half(), y), {}, "residual must be"), ((r, y.float()), {}, "y must be"), ((r, y[:2]), {}, "match residual"),
+            ((r, y, w.float()), {}, "post_weight must be"), ((r, y, w[:4]), {}, "weights must be"),
+            ((r, y, w), {"post_norm": False}, "needs post_norm"), ((r, y), {"eps": -1.0}, "eps"),
+            ((r, y), {"gate": torch.zeros(3)}, "gate must be"), ((r, y), {"gate": torch.zeros(3, 1).double()}, "gate must be"),
+            ((r, y), {"residual_out": torch.zeros(8, 3).t()}, "residual_out"), ((r.clone().requires_grad_(), y), {}, "autograd")):
+        with pytest.raises(ValueError, match=msg):
+            ops.block_norm(*args, **kw)
+    for dx, dres, msg in ((y.float(), None, "dx must be"), (y[:2], None, "dx must match"), (y, y, "dresidual must be"),
+                          (y, r[:2], "dresidual must be")):
+        with pytest.raises(ValueError, match=msg):
+            ops.block_norm_backward(dx, dres, r, y)

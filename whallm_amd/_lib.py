@@ -46,6 +46,16 @@ class DecodeLayerC(ctypes.Structure):
     ]
 
 
+class BlockNormFormC(ctypes.Structure):
+    """wm_block_norm_form (include/whallm_moe.h)."""
+    _fields_ = [
+        ("post_weight", c_void_p), ("pre_weight", c_void_p), ("gate", c_void_p),
+        ("weight_offset", c_float), ("scale", c_float), ("eps", c_float),
+        ("post_norm", c_int32), ("gate_kind", c_int32), ("gate_fp32", c_int32), ("gate_sigmoid", c_int32),
+        ("residual_fp32", c_int32),
+    ]
+
+
 _P = c_void_p
 _SIGNATURES = {
     "wm_last_error": (c_char_p, []),
@@ -78,6 +88,10 @@ _SIGNATURES = {
     "wm_mlp_bf16": (c_int, [_P, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
     "wm_repack_prefill_fp8": (c_int, [POINTER(FP8ExpertsC), _P, _P, _P, _P, _P]),
     "wm_residual_rmsnorm": (c_int, [_P, _P, c_int32, c_int32, c_float, _P, _P]),
+    "wm_block_norm": (c_int, [POINTER(BlockNormFormC), _P, _P, c_int32, c_int32, _P, _P, _P]),
+    "wm_block_norm_backward_workspace_size": (c_size_t, [c_int32, c_int32]),
+    "wm_block_norm_backward": (c_int, [POINTER(BlockNormFormC), _P, _P, _P, _P, c_int32, c_int32, _P, _P, _P, _P, _P, _P,
+                                       c_size_t, _P]),
     "wm_norm_router": (c_int, [_P, _P, _P, c_int32, c_int32, c_float, _P, c_int32, _P, _P, c_size_t, _P, _P, _P, _P,
                                _P]),
     "wm_router_packed_bytes": (c_size_t, [c_int32, c_int32, c_int32]),

@@ -682,6 +682,114 @@ def residual_rmsnorm(residual: torch.Tensor, y: torch.Tensor | None, eps: float 
     return x
 
 
+def _norm_form(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, eps, weight_offset, post_norm):
+    """The checked wm_block_norm_form and the contiguous (y, weights, gate) it points to."""
+    if residual.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"residual must be float32 or bfloat16, got {residual.dtype}")
+    if residual.dim() < 1 or residual.shape[-1] < 1:
+        raise ValueError("residual must be [.., H]")
+    H = residual.shape[-1]
+    y = _contig(y, torch.bfloat16, "y")
+    if y.shape != residual.shape:
+        raise ValueError("y must match residual")
+    if post_weight is not None and not post_norm:
+        raise ValueError("post_weight needs post_norm")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    if post_weight is not None:
+        post_weight = _contig(post_weight, torch.bfloat16, "post_weight")
+    if pre_weight is not None:
+        pre_weight = _contig(pre_weight, torch.bfloat16, "pre_weight")
+    if any(w is not None and w.shape != (H,) for w in (post_weight, pre_weight)):
+        raise ValueError("weights must be [H]")
+    kind = 0
+    if gate is not None:
+        if gate.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"gate must be float32 or bfloat16, got {gate.dtype}")
+        if gate.shape == (H,):
+            kind = 2
+        elif gate.shape == (*residual.shape[:-1], 1):
+            kind = 1
+        elif gate.shape == residual.shape:
+            kind = 3
+        else:
+            raise ValueError("gate must be [H], [.., 1] or [.., H]")
+        gate = gate.contiguous()
+    form = _lib.BlockNormFormC(_at(post_weight), _at(pre_weight), _at(gate), weight_offset, scale, eps, int(post_norm), kind,
+                               int(gate is not None and gate.dtype == torch.float32), int(bool(gate_sigmoid)),
+                               int(residual.dtype == torch.float32))
+    return form, y, post_weight, pre_weight, gate, kind
+
+
+def block_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Tensor | None = None,
+               pre_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_sigmoid: bool = False,
+               scale: float = 1.0, eps: float = 1e-6, weight_offset: float = 0.0, post_norm: bool = True,
+               residual_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The norms after one block and before the next (wm_block_norm): z = rmsnorm(y) * (weight_offset +
+    post_weight) (y itself without ``post_norm``), residual' = residual + scale * g * z, x =
+    bf16(rmsnorm(residual') * (weight_offset + pre_weight)). Returns (x, residual').
+
+    residual [.., H] fp32 or bf16, y [.., H] bf16, weights bf16 [H] (None: the norm alone); ``gate`` fp32 or bf16:
+    [H], one value a token [.., 1], or [.., H], through a sigmoid with ``gate_sigmoid`` (norm_router's shared
+    logit as [.., 1]). ``residual_out`` receives residual' and may be the residual itself."""
+    device = _require_device(residual, y, post_weight, pre_weight, gate, residual_out)
+    _no_autograd("block_norm", residual, y, post_weight, pre_weight, gate)
+    form, y, post_weight, pre_weight, gate, _ = _norm_form(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, eps,
+                                                           weight_offset, post_norm)
+    if residual_out is None:
+        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=device)
+    elif residual_out.dtype != residual.dtype or residual_out.shape != residual.shape or not residual_out.is_contiguous():
+        raise ValueError("residual_out must be a contiguous tensor shaped and typed like residual")
+    residual = residual.contiguous()
+    H = residual.shape[-1]
+    x = torch.empty(residual.shape, dtype=torch.bfloat16, device=device)
+    _launch(device, "wm_block_norm", form, residual.data_ptr(), y.data_ptr(), residual.numel() // H, H,
+            residual_out.data_ptr(), x.data_ptr())
+    return x, residual_out
+
+
+@dataclass
+class BlockNormGrads:
+    """block_norm_backward's gradients; None for an input that was not there."""
+    residual: torch.Tensor
+    y: torch.Tensor
+    post_weight: torch.Tensor | None
+    pre_weight: torch.Tensor | None
+    gate: torch.Tensor | None
+
+
+def block_norm_backward(dx: torch.Tensor, dresidual: torch.Tensor | None, residual_out: torch.Tensor, y: torch.Tensor,
+                        post_weight: torch.Tensor | None = None, pre_weight: torch.Tensor | None = None,
+                        gate: torch.Tensor | None = None, gate_sigmoid: bool = False, scale: float = 1.0, eps: float = 1e-6,
+                        weight_offset: float = 0.0, post_norm: bool = True) -> BlockNormGrads:
+    """The gradients of block_norm from those of x (``dx``, bf16) and residual' (``dresidual``, in its type; None:
+    zero), given the residual' that the forward pass returned and its other inputs (wm_block_norm_backward).
+    The weights' gradients and a gate's of [H] or [.., 1] are fp32, a [.., H] gate's has the gate's type."""
+    device = _require_device(dx, dresidual, residual_out, y, post_weight, pre_weight, gate)
+    _no_autograd("block_norm_backward", dx, dresidual, residual_out, y, post_weight, pre_weight, gate)
+    form, y, post_weight, pre_weight, gate, kind = _norm_form(residual_out, y, post_weight, pre_weight, gate, gate_sigmoid,
+                                                              scale, eps, weight_offset, post_norm)
+    dx = _contig(dx, torch.bfloat16, "dx")
+    if dx.shape != residual_out.shape:
+        raise ValueError("dx must match residual_out")
+    if dresidual is not None:
+        if dresidual.dtype != residual_out.dtype or dresidual.shape != residual_out.shape:
+            raise ValueError("dresidual must be shaped and typed like residual_out")
+        dresidual = dresidual.contiguous()
+    residual_out = residual_out.contiguous()
+    H = residual_out.shape[-1]
+    T = residual_out.numel() // H
+    dr, dy = torch.empty_like(residual_out), torch.empty_like(y)
+    dpost = None if post_weight is None else torch.empty(H, dtype=torch.float32, device=device)
+    dpre = None if pre_weight is None else torch.empty(H, dtype=torch.float32, device=device)
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype if kind == 3 else torch.float32, device=device)
+    ws_bytes = _lib.load().wm_block_norm_backward_workspace_size(T, H)
+    ws = _workspace(ws_bytes, device)
+    _launch(device, "wm_block_norm_backward", form, dx.data_ptr(), _at(dresidual), residual_out.data_ptr(), y.data_ptr(), T, H,
+            dr.data_ptr(), dy.data_ptr(), _at(dpost), _at(dpre), _at(dgate), ws.data_ptr(), ws_bytes)
+    return BlockNormGrads(dr, dy, dpost, dpre, dgate)
+
+
 def repack_router(router: torch.Tensor, shared_gate: torch.Tensor | None = None) -> torch.Tensor:
     """The router rows (+ the shared gate row) in MFMA fragment order (wm_repack_router).
     norm_router(..., router_packed=) still accepts it and checks its size, but reads the rows as stored,
