@@ -625,6 +625,49 @@ WM_EXPORT int wm_slot_cache_route_rebalance(wm_slot_cache* cache);
 WM_EXPORT int wm_slot_cache_route_state(wm_slot_cache* cache, double* scores, int32_t* quotas, double* short_rates,
                                         double* long_rates, int64_t* tokens, double* read_cost, int64_t* counters);
 
+/* ---- logits to acceptance ------------------------------------------------------
+ * The steps between a head's logits and sampling or acceptance (wm_mtp_verify_greedy takes logits,
+ * wm_mtp_verify_rejection log-probabilities): penalties for tokens already said, biases, a
+ * grammar's mask, the temperature and the log-softmax. For logits [rows, vocab] (bf16, or fp32
+ * where `fp32` is 1) and out fp32 [rows, vocab], in fp32 and in this order:
+ *   l = l > 0 ? l / repetition : l * repetition    for every token of the row's history
+ *   l -= frequency * count + presence              for every token of the history's answer part
+ *   l += bias                                      for every listed token
+ *   l /= temperature                               (where it is > 0)
+ *   l = -inf                                       where the mask's bit is 0
+ *   l -= max + log(sum(exp(l - max)))              with log_probs; -inf stays -inf, also in a row
+ *                                                  that has nothing else; a NaN that no mask
+ *                                                  hides makes its row's other values NaN
+ * Every pointer of the rules is nullable (the step is left out) and every per-row value is on the
+ * device, so a captured call follows them. out may be logits where they are fp32; it overlaps no
+ * other input. vocab up to 4194304. workspace (log_probs only):
+ * wm_process_logits_workspace_size bytes, 8-byte aligned. */
+typedef struct wm_logit_rules {
+  const int32_t* history;        /* token ids, row r at history + r * history_stride (0: one
+                                    history for all rows, as the rows of a verify round have); an id
+                                    outside the vocabulary counts nowhere */
+  int64_t history_stride;
+  int32_t history_len;           /* ids a row has room for, up to 1048575 */
+  int32_t biases;                /* listed biases of a row, up to 2047 */
+  const int32_t* lengths;        /* [rows] ids that count, clamped to 0..history_len (null: all) */
+  const int32_t* prompt_lengths; /* [rows] of these the first that are prompt (null: none) */
+  const float* repetition;       /* [rows] */
+  const float* frequency;        /* [rows] */
+  const float* presence;         /* [rows] */
+  const int32_t* bias_ids;       /* row r at + r * bias_stride; outside the vocabulary: none; of a
+                                    token listed twice the last value */
+  const float* bias_values;      /* laid out like bias_ids */
+  int64_t bias_stride;
+  const void* mask;              /* 32-bit words, bit v % 32 of word v / 32 set: token v is allowed;
+                                    row r at + r * mask_stride words */
+  int64_t mask_stride;
+  const float* temperature;      /* [rows]; 0 or less leaves the row unscaled */
+} wm_logit_rules;
+WM_EXPORT size_t wm_process_logits_workspace_size(int32_t rows, int32_t vocab);
+WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab,
+                                const wm_logit_rules* rules, int32_t log_probs, float* out, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 /* ---- MTP acceptance ----------------------------------------------------------
  * Verify n draft tokens (n <= 15) against n + 1 target rows [n + 1, vocab] fp32.
  * out: device int32[2] = (accepted drafts, next token).

@@ -167,3 +167,46 @@ def test_block_norm_python_refusals(on_cpu):
                           (y, r[:2], "dresidual must be")):
         with pytest.raises(ValueError, match=msg):
             ops.block_norm_backward(dx, dres, r, y)
+
+
+# ----------------------------------------------------------------------------- logits
+
+def logits_call(logits=A, fp32=1, rows=2, vocab=100, log_probs=1, out=A, ws=A, ws_bytes=1 << 20, **kw):
+    r = dict(history=None, history_stride=0, history_len=0, biases=0, lengths=None, prompt_lengths=None, repetition=None,
+             frequency=None, presence=None, bias_ids=None, bias_values=None, bias_stride=0, mask=None, mask_stride=0, temperature=None)
+    r.update(kw)
+    _lib.call("wm_process_logits", logits, fp32, rows, vocab, _lib.LogitRulesC(*r.values()), log_probs, out, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    ({"rows": -1}, "rows must"), ({"vocab": 0}, "vocab must"), ({"vocab": (1 << 22) + 1}, "vocab must"), ({"fp32": 3}, "fp32 must"),
+    ({"rows": 1 << 30, "vocab": 1 << 22}, "too many rows"), ({"history": A, "history_len": 1 << 20}, "history_len"),
+    ({"history": A, "history_len": -1}, "history_len"), ({"biases": 2048}, "biases must"), ({"biases": -1}, "biases must"),
+    ({"history_stride": -1}, "strides"), ({"lengths": A}, "without a history"), ({"prompt_lengths": A}, "without a history"),
+    ({"bias_ids": A}, "go together"), ({"bias_values": A}, "go together"), ({"logits": None}, "null pointer"),
+    ({"out": None}, "null pointer"), ({"logits": A + 2}, "aligned"), ({"out": A + 2}, "aligned"), ({"mask": A + 1}, "aligned"),
+    ({"ws": None}, "workspace"), ({"ws_bytes": 0}, "workspace"), ({"ws": A + 4}, "workspace"),
+])
+def test_process_logits_c_refusals(kw, msg):
+    with pytest.raises(_lib.WhallmError, match=msg):
+        logits_call(**kw)
+
+
+def test_process_logits_python_refusals(on_cpu):
+    logits = torch.zeros(3, 40)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(_lib.WhallmError, match="null rules"):
+        _lib.call("wm_process_logits", A, 1, 1, 10, None, 0, A, None, 0, None)
+    logits_call(rows=0)
+    for args, kw, msg in (
+            ((logits.half(),), {}, "bfloat16 or float32"), ((logits[0],), {}, "logits must be"),
+            ((logits,), {"history": i32(2, 5)}, "history must be"), ((logits,), {"history": torch.zeros(3, 5)}, "history must be"),
+            ((logits,), {"lengths": i32(3)}, "need a history"), ((logits,), {"history": i32(3, 5), "lengths": i32(2)}, "lengths must be"),
+            ((logits,), {"history": i32(3, 5), "lengths": torch.zeros(3).long()}, "lengths must be"),
+            ((logits,), {"repetition": torch.zeros(2)}, "repetition must be"), ((logits,), {"temperature": torch.zeros(3).double()}, "temperature must be"),
+            ((logits,), {"bias_ids": i32(3, 2)}, "go together"), ((logits,), {"bias_ids": i32(3, 2), "bias_values": torch.zeros(3, 3)}, "one shape"),
+            ((logits,), {"mask": i32(3, 1)}, "a bit for every token"), ((logits,), {"mask": torch.zeros(3, 2).bool()}, "mask must be"),
+            ((logits,), {"out": torch.zeros(3, 40).bfloat16()}, "out must be"), ((logits,), {"out": torch.zeros(40, 3).t()}, "out must be"),
+            ((logits.clone().requires_grad_(),), {}, "autograd")):
+        with pytest.raises(ValueError, match=msg):
+            ops.process_logits(*args, **kw)

@@ -56,6 +56,16 @@ class BlockNormFormC(ctypes.Structure):
     ]
 
 
+class LogitRulesC(ctypes.Structure):
+    """wm_logit_rules (include/whallm_moe.h)."""
+    _fields_ = [
+        ("history", c_void_p), ("history_stride", c_int64), ("history_len", c_int32), ("biases", c_int32),
+        ("lengths", c_void_p), ("prompt_lengths", c_void_p), ("repetition", c_void_p), ("frequency", c_void_p),
+        ("presence", c_void_p), ("bias_ids", c_void_p), ("bias_values", c_void_p), ("bias_stride", c_int64),
+        ("mask", c_void_p), ("mask_stride", c_int64), ("temperature", c_void_p),
+    ]
+
+
 _P = c_void_p
 _SIGNATURES = {
     "wm_last_error": (c_char_p, []),
@@ -135,6 +145,8 @@ _SIGNATURES = {
     "wm_moe_fp8": (c_int, [_P, c_int32, _P, _P, c_int32, POINTER(FP8ExpertsC), POINTER(FP8ExpertsC), _P, _P, _P,
                            c_size_t, _P]),
     "wm_experts_fp8": (c_int, [_P, c_int32, _P, c_int32, POINTER(FP8ExpertsC), _P, _P, c_size_t, _P]),
+    "wm_process_logits_workspace_size": (c_size_t, [c_int32, c_int32]),
+    "wm_process_logits": (c_int, [_P, c_int32, c_int32, c_int32, POINTER(LogitRulesC), c_int32, _P, _P, c_size_t, _P]),
     "wm_mtp_workspace_size": (c_size_t, [c_int32, c_int32]),
     "wm_mtp_verify_greedy": (c_int, [_P, _P, c_int32, c_int32, _P, _P, c_size_t, _P]),
     "wm_verify_step_fp8_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, _P]),

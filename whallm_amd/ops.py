@@ -1090,6 +1090,89 @@ class PersistentDecodeStack:
         return bool(r)
 
 
+# ----------------------------------------------------------------------------- logits to acceptance
+
+def _row_lists(t: torch.Tensor, rows: int, name: str) -> tuple[torch.Tensor, int]:
+    """[rows, n], or [1, n] for a list that all rows share -> (contiguous, elements between rows)."""
+    if t.dim() != 2 or t.shape[0] not in (rows, 1):
+        raise ValueError(f"{name} must be [rows, n], or [1, n] for all rows")
+    t = t.contiguous()
+    return t, 0 if t.shape[0] == 1 else t.shape[1]
+
+
+def _row_values(t: torch.Tensor | None, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    t = _contig(t, dtype, name)
+    if t.shape != (rows,):
+        raise ValueError(f"{name} must be [rows]")
+    return t
+
+
+def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                   prompt_lengths: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                   frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                   bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
+                   mask: torch.Tensor | None = None, temperature: torch.Tensor | None = None, log_probs: bool = False,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties, biases, grammar mask and temperature on logits [rows, V] (fp32 or bf16), and with ``log_probs``
+    the log-softmax: what mtp_verify_greedy and mtp_verify_rejection take (wm_process_logits has the formula).
+
+    ``history`` int32 [rows, L] holds the token ids said so far, [1, L] one history for every row (the rows of a
+    verify round: the context and the drafts, ``lengths`` growing by one a row); ``lengths`` and
+    ``prompt_lengths`` int32 [rows] say how many count and how many of these are prompt, which only
+    ``repetition`` sees. repetition, frequency, presence and temperature are fp32 [rows]; bias_ids int32 and
+    bias_values fp32 [rows, n] or [1, n]; mask int32 [rows, ceil(V / 32)] or [1, ..], a set bit allows its token.
+    Returns fp32 [rows, V]; ``out`` may be fp32 logits themselves."""
+    device = _require_device(logits, history, lengths, prompt_lengths, repetition, frequency, presence, bias_ids, bias_values,
+                             mask, temperature, out)
+    _no_autograd("process_logits", logits, bias_values)
+    logits = _rows(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be [rows, vocab]")
+    R, V = logits.shape
+    lengths, prompt_lengths = (_row_values(t, R, torch.int32, n) for t, n in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths")))
+    repetition, frequency, presence, temperature = (
+        _row_values(t, R, torch.float32, n) for t, n in ((repetition, "repetition"), (frequency, "frequency"),
+                                                         (presence, "presence"), (temperature, "temperature")))
+    history_stride = history_len = biases = bias_stride = mask_stride = 0
+    if history is not None:
+        history, history_stride = _row_lists(_contig(history, torch.int32, "history"), R, "history")
+        history_len = history.shape[1]
+        if history_len == 0:
+            history = lengths = prompt_lengths = None
+    elif lengths is not None or prompt_lengths is not None:
+        raise ValueError("lengths need a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values go together")
+    if bias_ids is not None:
+        if bias_ids.shape != bias_values.shape:
+            raise ValueError("bias_ids and bias_values must have one shape")
+        bias_ids, bias_stride = _row_lists(_contig(bias_ids, torch.int32, "bias_ids"), R, "bias_ids")
+        bias_values = _contig(bias_values, torch.float32, "bias_values")
+        biases = bias_ids.shape[1]
+        if biases == 0:
+            bias_ids = bias_values = None
+    if mask is not None:
+        mask, mask_stride = _row_lists(_contig(mask, torch.int32, "mask"), R, "mask")
+        if mask.shape[1] != -(-V // 32):
+            raise ValueError("mask must hold a bit for every token, 32 in a word")
+    if out is None:
+        out = torch.empty(R, V, dtype=torch.float32, device=device)
+    elif out.dtype != torch.float32 or out.shape != (R, V) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous float32 tensor shaped like logits")
+    rules = _lib.LogitRulesC(_at(history), history_stride, history_len, biases, _at(lengths), _at(prompt_lengths), _at(repetition),
+                             _at(frequency), _at(presence), _at(bias_ids), _at(bias_values), bias_stride, _at(mask), mask_stride,
+                             _at(temperature))
+    ws, ws_bytes = None, 0
+    if log_probs:
+        ws_bytes = _lib.load().wm_process_logits_workspace_size(R, V)
+        ws = _workspace(ws_bytes, device)
+    _launch(device, "wm_process_logits", logits.data_ptr(), int(logits.dtype == torch.float32), R, V, rules, int(bool(log_probs)),
+            out.data_ptr(), _at(ws), ws_bytes)
+    return out
+
+
 # ----------------------------------------------------------------------------- MTP acceptance
 
 def _mtp_rows(t: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int]:
