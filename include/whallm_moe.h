@@ -160,7 +160,7 @@ WM_EXPORT int wm_permute(const int32_t* indices, int64_t pairs, int32_t experts,
 /* Sorts the pairs as wm_permute does (experts 1..1024) and copies x[t] to the rows of t's pairs;
  * the lists as wm_permute's, and behind their ends: order -1, tiles (-1, -1), rows zero.
  * tiles [ceil(tokens * k / tile_rows) + experts][2], 8-byte aligned.
- * workspace: wm_sort_tokens_workspace_size bytes. */
+ * workspace: wm_sort_tokens_workspace_size bytes, 4-byte aligned; 0 for the calls that need none. */
 WM_EXPORT size_t wm_sort_tokens_workspace_size(int32_t tokens, int32_t k, int32_t experts);
 WM_EXPORT int wm_sort_tokens(const void* x, int32_t fp32, int32_t tokens, int32_t hidden, const int32_t* indices,
                              int32_t k, int32_t experts, int32_t tile_rows, void* rows, int32_t* order,

@@ -29,7 +29,8 @@ def sort_args(**kw):
     ({"hidden": 1 << 21}, "hidden must be"), ({"fp32": 2}, "fp32 must be"), ({"experts": 0}, "experts must be"),
     ({"experts": 1025}, "experts must be"), ({"tile_rows": 0}, "tile_rows"), ({"tokens": 1 << 30, "k": 2}, "below 2"),
     ({"x": None}, "null pointer"), ({"indices": None}, "null pointer"), ({"rows": None}, "null pointer"),
-    ({"offsets": None}, "null pointer"), ({"workspace": None}, "null pointer"), ({"workspace_bytes": 8}, "workspace too small"),
+    ({"offsets": None}, "null pointer"), ({"workspace": None, "tokens": 1 << 20}, "null pointer"),
+    ({"workspace_bytes": 8, "tokens": 1 << 20}, "workspace too small"),
     ({"x": A + 1}, "aligned"), ({"rows": A + 2, "fp32": 1}, "aligned"), ({"tiles": A + 4}, "aligned"),
 ])
 def test_sort_tokens_c_refusals(kw, msg):

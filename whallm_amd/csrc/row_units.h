@@ -66,6 +66,27 @@ struct RowUnit<true, false> {
   static __device__ __forceinline__ Raw zero() { return 0.0f; }
 };
 
+// A unit with the non-temporal hint, for rows that pass once.
+__device__ __forceinline__ uint4 load_once(const uint4* p) { return gload16_nt(p); }
+__device__ __forceinline__ float4 load_once(const float4* p) {
+  const uint4 v = gload16_nt(p);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+template <typename T>
+__device__ __forceinline__ T load_once(const T* p) {
+  return __builtin_nontemporal_load(p);
+}
+__device__ __forceinline__ void store_once(uint4* p, uint4 v) {
+  const wm_u32x4 u = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(u, (__attribute__((address_space(1))) wm_u32x4*)(p));
+}
+__device__ __forceinline__ void store_once(float4* p, float4 v) {
+  store_once(reinterpret_cast<uint4*>(p), make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)));
+}
+__device__ __forceinline__ void store_once(uint32_t* p, uint32_t v) { __builtin_nontemporal_store(v, p); }
+__device__ __forceinline__ void store_once(uint16_t* p, uint16_t v) { __builtin_nontemporal_store(v, p); }
+__device__ __forceinline__ void store_once(float* p, float v) { __builtin_nontemporal_store(v, p); }
+
 // A launch of 256 threads over rows of `units` units: 2^log2 threads side by side in a row, 256 >> log2
 // rows a block; grid (row blocks, unit blocks).
 struct RowGrid {

@@ -21,45 +21,210 @@ namespace wm {
 
 constexpr int SORT_MAX_K = 64;
 
-// ---- sort: the lists are there, x's rows go to theirs. Block (t / rows a block, unit block).
-template <typename Unit>
-__global__ void __launch_bounds__(256) sort_move_kernel(const Unit* __restrict__ x, int64_t tokens, int64_t units, int log2,
-                                                       int k, int experts, const int32_t* __restrict__ inverse,
-                                                       const int32_t* __restrict__ offsets, Unit* __restrict__ rows,
-                                                       int32_t* __restrict__ order, int32_t* __restrict__ tiles,
-                                                       const int32_t* __restrict__ tile_count, int64_t max_tiles) {
-  const int64_t t = (int64_t)blockIdx.x * (256 >> log2) + (threadIdx.x >> log2);
-  const int64_t c = ((int64_t)blockIdx.y << log2) + (threadIdx.x & ((1 << log2) - 1));
-  const int64_t pairs = tokens * k;
-  // Behind the ends: -1 in the lists (first unit block), zero rows.
-  const int32_t present = offsets[experts];
-  if (blockIdx.y == 0) {
-    const int64_t step = (int64_t)gridDim.x * 256;
-    const int64_t me = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    for (int64_t r = present + me; r < pairs; r += step) order[r] = -1;
-    for (int64_t i = tile_count[0] + me; i < max_tiles; i += step) reinterpret_cast<int2*>(tiles)[i] = make_int2(-1, -1);
+// ---- sort. A workgroup owns a chunk of tokens (256 pairs at most) and a range of units. It finds its
+// pairs' rows in LDS: the first row of each expert for this chunk, plus a pair's place among the chunk's
+// earlier pairs of its expert. Where the first rows come from is what differs:
+//   ONE   every workgroup counts all pairs itself, those before its chunk apart. One launch and no
+//         workspace, and the counting is repeated by every workgroup, so it is for few pairs.
+//   else  permute_count and permute_scan have left them in memory.
+constexpr int SORT_THREADS = 512;
+constexpr int SORT_CHUNK = 256;
+
+struct SortArgs {
+  const void* x;
+  const int32_t* indices;
+  int64_t tokens, units;
+  int k, experts, tile_rows;
+  int chunk_tokens, split_units, log2;  // 2^log2 threads side by side in a row
+  void* rows;
+  int32_t *order, *inverse, *offsets, *tiles, *tile_count;
+  int64_t max_tiles;
+  const int32_t* chunk_base;
+};
+
+// Exclusive prefix sums over the workgroup's threads, and the total. Every thread calls it.
+__device__ __forceinline__ int32_t sort_scan(int32_t v, int32_t* total) {
+  __shared__ int32_t wave_sum[SORT_THREADS / 64];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  int32_t incl = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += o;
   }
-  if (t >= tokens || c >= units) return;
-  const Unit v = x[t * units + c];
-  for (int j = 0; j < k; ++j) {
-    const int64_t p = t * k + j;
-    const int32_t r = inverse[p];
-    if (r >= 0) rows[r * units + c] = v;
-    if (p >= present) rows[p * units + c] = Unit{};
+  if (lane == 63) wave_sum[wave] = incl;
+  __syncthreads();
+  int32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < SORT_THREADS / 64; ++w) {
+    before += w < wave ? wave_sum[w] : 0;
+    all += wave_sum[w];
   }
+  __syncthreads();  // wave_sum is free again
+  *total = all;
+  return before + incl - v;
+}
+
+template <typename Unit, bool ONE>
+__global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
+  // base: counts, then the chunk's first row of each expert; later the first row of each expert (offsets)
+  __shared__ int32_t base[PERMUTE_MAX_EXPERTS], later[PERMUTE_MAX_EXPERTS + 1];
+  __shared__ int32_t tile_start[ONE ? PERMUTE_MAX_EXPERTS : 1];
+  __shared__ __align__(16) int32_t key[SORT_CHUNK];
+  __shared__ int32_t row[SORT_CHUNK];
+  const int64_t pairs = a.tokens * a.k;
+  const int64_t t0 = (int64_t)blockIdx.x * a.chunk_tokens;
+  const int64_t p0 = t0 * a.k;
+  const int tokens = (int)max((int64_t)0, min((int64_t)a.chunk_tokens, a.tokens - t0));
+  const int n = tokens * a.k;
+  const int E = a.experts;
+  int32_t present;
+  if (threadIdx.x < n) {
+    const int32_t e = a.indices[p0 + threadIdx.x];
+    key[threadIdx.x] = (uint32_t)e < (uint32_t)E ? e : -1;
+  }
+  if constexpr (ONE) {
+    for (int e = threadIdx.x; e < E; e += SORT_THREADS) base[e] = later[e] = 0;
+    __syncthreads();
+    // 16 ids in flight a thread, as four 16-byte loads where the list allows them
+    const bool quads = (uintptr_t)a.indices % 16 == 0;
+    for (int64_t q0 = 4 * threadIdx.x; q0 < pairs; q0 += 16 * SORT_THREADS) {
+      int32_t e[4][4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int64_t q = q0 + b * 4 * SORT_THREADS;
+        if (quads && q + 4 <= pairs) {
+          const int4 v = *reinterpret_cast<const int4*>(a.indices + q);
+          e[b][0] = v.x, e[b][1] = v.y, e[b][2] = v.z, e[b][3] = v.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[b][i] = q + i < pairs ? a.indices[q + i] : -1;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((uint32_t)e[b][i] < (uint32_t)E)
+            atomicAdd(q0 + b * 4 * SORT_THREADS + i < p0 ? &base[e[b][i]] : &later[e[b][i]], 1);
+    }
+    __syncthreads();
+    const int e0 = 2 * threadIdx.x, e1 = e0 + 1;  // two experts a thread
+    const int32_t b0 = e0 < E ? base[e0] : 0, b1 = e1 < E ? base[e1] : 0;
+    const int32_t n0 = e0 < E ? b0 + later[e0] : 0, n1 = e1 < E ? b1 + later[e1] : 0;
+    const int32_t first = sort_scan(n0 + n1, &present);
+    if (e0 < E) base[e0] = first + b0, later[e0] = first;
+    if (e1 < E) base[e1] = first + n0 + b1, later[e1] = first + n0;
+    if (blockIdx.x == 0 && blockIdx.y == 0) {  // the lists that have no pair to them
+      if (e0 < E) a.offsets[e0] = first;
+      if (e1 < E) a.offsets[e1] = first + n0;
+      if (threadIdx.x == 0) a.offsets[E] = present;
+      const int32_t t0s = (n0 + a.tile_rows - 1) / a.tile_rows, t1s = (n1 + a.tile_rows - 1) / a.tile_rows;
+      int32_t count;
+      const int32_t tile = sort_scan(t0s + t1s, &count);
+      if (threadIdx.x == 0) a.tile_count[0] = count;
+      if (e0 < E) tile_start[e0] = tile;
+      if (e1 < E) tile_start[e1] = tile + t0s;
+      __syncthreads();
+      // Tile i belongs to the last expert whose first tile is <= i: experts without tiles share their start
+      // with the next one that has some, and come before it.
+      for (int32_t i = threadIdx.x; i < count; i += SORT_THREADS) {
+        int lo = 0, hi = E - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (tile_start[mid] <= i) lo = mid; else hi = mid - 1;
+        }
+        reinterpret_cast<int2*>(a.tiles)[i] = make_int2(lo, later[lo] + (i - tile_start[lo]) * a.tile_rows);
+      }
+      for (int64_t i = count + threadIdx.x; i < a.max_tiles; i += SORT_THREADS)
+        reinterpret_cast<int2*>(a.tiles)[i] = make_int2(-1, -1);
+    }
+  } else {
+    present = a.offsets[E];
+    if (blockIdx.y == 0)
+      for (int64_t i = a.tile_count[0] + (int64_t)blockIdx.x * SORT_THREADS + threadIdx.x; i < a.max_tiles;
+           i += (int64_t)gridDim.x * SORT_THREADS)
+        reinterpret_cast<int2*>(a.tiles)[i] = make_int2(-1, -1);
+  }
+  __syncthreads();
+  if (threadIdx.x < SORT_CHUNK) {  // whole waves: ballots
+    const bool in_range = threadIdx.x < n;
+    const int32_t e = in_range ? key[threadIdx.x] : -1;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int bits = 32 - __clz(E);
+    uint64_t peers = __ballot(e >= 0);  // the wave's pairs of the same expert
+    for (int bit = 0; bit < bits; ++bit) {
+      const uint64_t set = __ballot((e >> bit) & 1);
+      peers &= ((e >> bit) & 1) ? set : ~set;
+    }
+    int32_t r = __popcll(peers & (lane == 0 ? 0ull : ~0ull >> (64 - lane)));
+    const int4* earlier = reinterpret_cast<const int4*>(key);
+#pragma unroll 4
+    for (int j = 0; j < 16 * wave; ++j) {  // the pairs of the waves before, all of the chunk
+      const int4 v = earlier[j];
+      r += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
+    }
+    if (in_range) {
+      if (e >= 0) r += ONE ? base[e] : a.chunk_base[(int64_t)blockIdx.x * E + e] + a.offsets[e];
+      else r = -1;
+      row[threadIdx.x] = r;
+      const int64_t p = p0 + threadIdx.x;
+      if (blockIdx.y == 0) {
+        a.inverse[p] = r;
+        if (r >= 0) a.order[r] = (int32_t)p;
+        if (p >= present) a.order[p] = -1;
+      }
+    }
+  }
+  __syncthreads();
+  const Unit* x = (const Unit*)a.x;
+  Unit* rows = (Unit*)a.rows;
+  const int64_t c0 = (int64_t)blockIdx.y * a.split_units, c1 = min(a.units, c0 + a.split_units);
+  for (int t = threadIdx.x >> a.log2; t < tokens; t += SORT_THREADS >> a.log2) {
+    for (int64_t c = c0 + (threadIdx.x & ((1 << a.log2) - 1)); c < c1; c += 1 << a.log2) {
+      const Unit v = x[(t0 + t) * a.units + c];
+#pragma unroll 4
+      for (int j = 0; j < a.k; ++j) {
+        const int32_t r = row[t * a.k + j];
+        if (r >= 0) store_once(&rows[r * a.units + c], v);
+      }
+    }
+  }
+  // The rows behind the last pair, spread over the workgroups: the few that own the last pairs would take
+  // twice as long (4096 tokens x 8, hidden 7168, 2% of the pairs absent: 112 us, spread 103).
+  for (int64_t r = present + (int64_t)blockIdx.x; r < pairs; r += gridDim.x)
+    for (int64_t c = c0 + threadIdx.x; c < c1; c += SORT_THREADS) store_once(&rows[r * a.units + c], Unit{});
+}
+
+// Up to this many pairs a call is one launch.
+constexpr int64_t SORT_ONE_MAX = 32768;
+
+static int sort_chunk_tokens(int64_t tokens, int k, bool one) {
+  const int most = SORT_CHUNK / k > 0 ? SORT_CHUNK / k : 1;
+  if (!one) return most;
+  const int64_t want = (tokens + 255) / 256;  // few tokens: a workgroup each
+  return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 template <typename Unit>
-static void sort_move(const void* x, int64_t tokens, int64_t units, int k, int experts, int32_t* order, const int32_t* inverse,
-                      const int32_t* offsets, void* rows, int32_t* tiles, const int32_t* tile_count, int64_t max_tiles,
-                      hipStream_t s) {
-  const RowGrid g = row_grid(tokens > 0 ? tokens : 1, units);  // without tokens the list of tiles still ends
-  hipLaunchKernelGGL(sort_move_kernel<Unit>, g.grid, dim3(256), 0, s, (const Unit*)x, tokens, units, g.log2, k, experts,
-                     inverse, offsets, (Unit*)rows, order, tiles, tile_count, max_tiles);
-  check_launch("sort_move");
+static void sort_launch(SortArgs a, bool one, hipStream_t s) {
+  const int64_t chunks = a.tokens > 0 ? (a.tokens + a.chunk_tokens - 1) / a.chunk_tokens : 1;
+  // columns are split until the chip has work for every CU
+  const int64_t most = (a.units + 255) / 256;
+  int64_t splits = chunks >= 512 ? 1 : (511 + chunks) / chunks;
+  if (splits > most) splits = most;
+  a.split_units = (int)((a.units + splits - 1) / splits);
+  a.log2 = 0;
+  while (a.log2 < 9 && (1 << a.log2) < a.split_units) ++a.log2;
+  const dim3 grid((unsigned)chunks, (unsigned)splits);
+  if (one) hipLaunchKernelGGL((sort_kernel<Unit, true>), grid, dim3(SORT_THREADS), 0, s, a);
+  else hipLaunchKernelGGL((sort_kernel<Unit, false>), grid, dim3(SORT_THREADS), 0, s, a);
+  check_launch("sort");
 }
 
 // ---- back (WEIGHTED) and the sort's gradient: a thread owns one unit of a token, sums its k rows.
+constexpr int GATHER_BATCH = 8;  // rows in flight
+
 template <bool F32, bool WIDE, bool WEIGHTED>
 __global__ void __launch_bounds__(256) gather_sum_kernel(const void* __restrict__ rows_, const float* __restrict__ weights,
                                                         const int32_t* __restrict__ inverse, int64_t tokens, int64_t units,
@@ -72,15 +237,24 @@ __global__ void __launch_bounds__(256) gather_sum_kernel(const void* __restrict_
   const Raw* rows = (const Raw*)rows_;
   const uint32_t pairs = (uint32_t)(tokens * k);
   float acc[U::N] = {};
-  for (int j = 0; j < k; ++j) {
-    const int64_t p = t * k + j;
-    const uint32_t r = (uint32_t)inverse[p];
-    if (r >= pairs) continue;
-    float f[U::N];
-    U::unpack(rows[r * units + c], f);
-    const float w = WEIGHTED ? weights[p] : 1.0f;
+  for (int j0 = 0; j0 < k; j0 += GATHER_BATCH) {
+    uint32_t r[GATHER_BATCH];
+    Raw v[GATHER_BATCH];
 #pragma unroll
-    for (int i = 0; i < U::N; ++i) acc[i] = WEIGHTED ? fmaf(w, f[i], acc[i]) : acc[i] + f[i];
+    for (int q = 0; q < GATHER_BATCH; ++q) r[q] = j0 + q < k ? (uint32_t)inverse[t * k + j0 + q] : 0xffffffffu;
+#pragma unroll
+    for (int q = 0; q < GATHER_BATCH; ++q)
+      if (r[q] < pairs) v[q] = load_once(&rows[r[q] * units + c]);
+#pragma unroll
+    for (int q = 0; q < GATHER_BATCH; ++q) {
+      if (r[q] < pairs) {
+        const float w = WEIGHTED ? weights[t * k + j0 + q] : 1.0f;
+        float f[U::N];
+        U::unpack(v[q], f);
+#pragma unroll
+        for (int i = 0; i < U::N; ++i) acc[i] = WEIGHTED ? fmaf(w, f[i], acc[i]) : acc[i] + f[i];
+      }
+    }
   }
   if (add_) {
     float f[U::N];
@@ -127,7 +301,9 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
   const Raw* rows = (const Raw*)rows_;
   Raw* drows = (Raw*)drows_;
   const uint32_t pairs = (uint32_t)(tokens * k);
-  const int32_t present = *present_;
+  // the rows without a pair, spread over the tokens
+  for (int64_t r = *present_ + t; r < tokens * k; r += tokens)
+    for (int64_t c = threadIdx.x; c < units; c += 256) store_once(&drows[r * units + c], U::zero());
   for (int j0 = 0; j0 < k; j0 += BACK_BATCH) {
     uint32_t r[BACK_BATCH];
     float w[BACK_BATCH], dot[BACK_BATCH] = {};
@@ -144,15 +320,14 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
       for (int q = 0; q < BACK_BATCH; ++q) {
         if (r[q] < pairs) {
           float f[U::N], o[U::N];
-          U::unpack(rows[r[q] * units + c], f);
+          U::unpack(load_once(&rows[r[q] * units + c]), f);
 #pragma unroll
           for (int i = 0; i < U::N; ++i) {
             dot[q] = fmaf(d[i], f[i], dot[q]);
             o[i] = w[q] * d[i];
           }
-          drows[r[q] * units + c] = U::pack(o);
+          store_once(&drows[r[q] * units + c], U::pack(o));
         }
-        if (j0 + q < k && t * k + j0 + q >= present) drows[(t * k + j0 + q) * units + c] = U::zero();
       }
     }
 #pragma unroll
@@ -167,6 +342,13 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
     }
     __syncthreads();
   }
+}
+
+// Chunk counts, the experts' totals and the scan's counter.
+static PermuteWorkspace sort_workspace(void* workspace, int64_t pairs, int experts, int chunk_pairs) {
+  int32_t* counts = (int32_t*)workspace;
+  int32_t* totals = counts + (pairs + chunk_pairs - 1) / chunk_pairs * experts;
+  return {counts, totals, totals + experts};
 }
 
 static void check_rows(const char* name, int64_t tokens, int k, int64_t hidden, int f32) {
@@ -185,8 +367,10 @@ using namespace wm;
 extern "C" {
 
 WM_EXPORT size_t wm_sort_tokens_workspace_size(int32_t tokens, int32_t k, int32_t experts) {
-  if (tokens < 0 || k < 1 || experts < 1) return 0;
-  return wm_permute_workspace_size((int64_t)tokens * k, experts);
+  const int64_t pairs = (int64_t)tokens * k;
+  if (tokens < 0 || k < 1 || k > SORT_MAX_K || experts < 1 || pairs <= SORT_ONE_MAX) return 0;
+  const int64_t chunk_pairs = (int64_t)sort_chunk_tokens(tokens, k, false) * k;
+  return ((size_t)((pairs + chunk_pairs - 1) / chunk_pairs + 1) * experts + 1) * sizeof(int32_t);
 }
 
 WM_EXPORT int wm_sort_tokens(const void* x, int32_t fp32, int32_t tokens, int32_t hidden, const int32_t* indices, int32_t k,
@@ -198,24 +382,38 @@ WM_EXPORT int wm_sort_tokens(const void* x, int32_t fp32, int32_t tokens, int32_
     const int64_t pairs = (int64_t)tokens * k;
     if (experts < 1 || experts > PERMUTE_MAX_EXPERTS) fail("wm_sort_tokens: experts must be in 1..1024");
     if (tile_rows < 1) fail("wm_sort_tokens: tile_rows must be positive");
-    if (!offsets || !tiles || !tile_count || !workspace || (pairs > 0 && (!x || !indices || !rows || !order || !inverse)))
+    const size_t need = wm_sort_tokens_workspace_size(tokens, k, experts);
+    if (!offsets || !tiles || !tile_count || (need > 0 && !workspace) || (pairs > 0 && (!x || !indices || !rows || !order || !inverse)))
       fail("wm_sort_tokens: null pointer");
     if (((uintptr_t)x | (uintptr_t)rows) % (fp32 ? 4 : 2) || (uintptr_t)tiles % 8)
       fail("wm_sort_tokens: rows must be aligned to their elements and tiles to 8 bytes");
-    if (workspace_bytes < wm_sort_tokens_workspace_size(tokens, k, experts)) fail("wm_sort_tokens: workspace too small");
+    if (workspace_bytes < need || (uintptr_t)workspace % 4) fail("wm_sort_tokens: workspace too small or misaligned");
     hipStream_t s = as_stream(stream);
-    const PermuteWorkspace ws = permute_workspace(workspace, pairs, experts);
-    permute_count(indices, pairs, experts, ws, s);
-    permute_lists(indices, pairs, experts, tile_rows, 0, order, inverse, nullptr, 1, offsets, tiles, nullptr, tile_count, ws, s);
+    const bool one = pairs <= SORT_ONE_MAX;
+    SortArgs a = {};
+    a.x = x, a.indices = indices, a.tokens = tokens, a.k = k, a.experts = experts, a.tile_rows = tile_rows;
+    a.chunk_tokens = sort_chunk_tokens(tokens, k, one);
+    a.rows = rows, a.order = order, a.inverse = inverse, a.offsets = offsets, a.tiles = tiles, a.tile_count = tile_count;
+    a.max_tiles = (pairs + tile_rows - 1) / tile_rows + experts;
+    if (!one) {
+      const int chunk_pairs = a.chunk_tokens * k;
+      const PermuteWorkspace ws = sort_workspace(workspace, pairs, experts, chunk_pairs);
+      permute_count(indices, pairs, experts, chunk_pairs, ws, s);
+      permute_scan((pairs + chunk_pairs - 1) / chunk_pairs, experts, tile_rows, 0, offsets, tiles, nullptr, tile_count, ws, s);
+      a.chunk_base = ws.counts;
+    }
     const int64_t bytes = (int64_t)hidden * (fp32 ? 4 : 2);
-    const int64_t max_tiles = (pairs + tile_rows - 1) / tile_rows + experts;
     const uintptr_t at = (uintptr_t)x | (uintptr_t)rows | (uintptr_t)bytes;
-    if (at % 16 == 0)
-      sort_move<uint4>(x, tokens, bytes / 16, k, experts, order, inverse, offsets, rows, tiles, tile_count, max_tiles, s);
-    else if (at % 4 == 0)
-      sort_move<uint32_t>(x, tokens, bytes / 4, k, experts, order, inverse, offsets, rows, tiles, tile_count, max_tiles, s);
-    else
-      sort_move<uint16_t>(x, tokens, bytes / 2, k, experts, order, inverse, offsets, rows, tiles, tile_count, max_tiles, s);
+    if (at % 16 == 0) {
+      a.units = bytes / 16;
+      sort_launch<uint4>(a, one, s);
+    } else if (at % 4 == 0) {
+      a.units = bytes / 4;
+      sort_launch<uint32_t>(a, one, s);
+    } else {
+      a.units = bytes / 2;
+      sort_launch<uint16_t>(a, one, s);
+    }
   });
 }
 
