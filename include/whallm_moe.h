@@ -630,11 +630,12 @@ WM_EXPORT int wm_slot_cache_route_state(wm_slot_cache* cache, double* scores, in
  * wm_mtp_verify_rejection log-probabilities): penalties for tokens already said, biases, a
  * grammar's mask, the temperature and the log-softmax. For logits [rows, vocab] (bf16, or fp32
  * where `fp32` is 1) and out fp32 [rows, vocab], in fp32 and in this order:
- *   l = l > 0 ? l / repetition : l * repetition    for every token of the row's history
+ *   l = l > 0 ? l / repetition : l * repetition    for every token of the row's history (by the
+ *                                                  reciprocal)
  *   l -= frequency * count + presence              for every token of the history's answer part
  *   l += bias                                      for every listed token
- *   l /= temperature                               (where it is > 0)
  *   l = -inf                                       where the mask's bit is 0
+ *   l /= temperature                               (where it is in 2^-126..2^126), by its reciprocal
  *   l -= max + log(sum(exp(l - max)))              with log_probs; -inf stays -inf, also in a row
  *                                                  that has nothing else; a NaN that no mask
  *                                                  hides makes its row's other values NaN
@@ -661,7 +662,7 @@ typedef struct wm_logit_rules {
   const void* mask;              /* 32-bit words, bit v % 32 of word v / 32 set: token v is allowed;
                                     row r at + r * mask_stride words */
   int64_t mask_stride;
-  const float* temperature;      /* [rows]; 0 or less leaves the row unscaled */
+  const float* temperature;      /* [rows]; outside 2^-126..2^126 (0 among it) the row is left unscaled */
 } wm_logit_rules;
 WM_EXPORT size_t wm_process_logits_workspace_size(int32_t rows, int32_t vocab);
 WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab,

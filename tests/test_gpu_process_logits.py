@@ -1,9 +1,11 @@
 """GPU parity of the logit steps before acceptance (wm_process_logits) against the formula in 64 bits.
 
-Bar: the running error of the same steps in fp32 (running_error.py). The log-softmax: exp is good to 2
-units and takes the error of its argument, a row's sum passes at most 16 values of a thread, 6 steps of a
-wave, 4 waves and as many again over the chunks, the logarithm is good to 2 units and has the sum's
-relative error, and two subtractions follow.
+Bar: the running error of the same steps in fp32 (running_error.py). The log-softmax: a term exp(l - top)
+is exp2 of the difference times log2 e, three roundings of the argument, over the five levels at
+which maxima meet (thread, wave, workgroup, chunks, wave): their differences add up to l - top, and each
+level adds an exp2 (2 units) and a product (1). A row's sum passes at most 32 values of a thread, 6 steps
+of a wave, 6 of a workgroup, the chunks of a lane and 6 steps again. The logarithm is good to 2 units and
+has the sum's relative error, and two subtractions follow.
 """
 import numpy as np
 import pytest
@@ -14,7 +16,7 @@ from running_error import Fp32, U, check
 
 pytestmark = pytest.mark.gpu
 
-SUM = 16 + 6 + 4 + 16 + 6 + 4
+SUM = 32 + 6 + 6 + 14 + 6
 
 
 def f64(t):
@@ -40,7 +42,7 @@ def want_logits(logits, log_probs=False, history=None, lengths=None, prompt_leng
             seen = np.bincount(ok(h[:end]), minlength=V) > 0
             count = np.bincount(ok(h[p:end]), minlength=V).astype(np.float64)
             rep = per(repetition, r, 1.0)
-            div, mul = l / rep, l * rep
+            div, mul = l * (Fp32(1.0) / Fp32(rep)), l * rep    # by the reciprocal
             pos = l.v > 0
             l = Fp32(np.where(seen, np.where(pos, div.v, mul.v), l.v), np.where(seen, np.where(pos, div.e, mul.e), l.e))
             l = l - Fp32(per(frequency, r, 0.0)) * Fp32(count) - Fp32(per(presence, r, 0.0) * (count > 0))
@@ -52,7 +54,7 @@ def want_logits(logits, log_probs=False, history=None, lengths=None, prompt_leng
             l = l + Fp32(b)
         t = per(temperature, r, 1.0)
         if t > 0:
-            l = l / Fp32(t)
+            l = l * (Fp32(1.0) / Fp32(t))    # by the reciprocal
         if mask is not None:
             bits = np.unpackbits(row(mask, r).view(np.uint8), bitorder="little")[:V] != 0
             l = Fp32(np.where(bits, l.v, -np.inf), np.where(bits, l.e, 0.0))
@@ -68,10 +70,10 @@ def log_softmax(l):
         return l
     with np.errstate(invalid="ignore", over="ignore"):
         arg = l.v - top
-        e_arg = np.where(np.isneginf(l.v), 0.0, 2 * l.e.max() + U * np.abs(np.where(np.isneginf(l.v), 0.0, arg)))
+        e_arg = np.where(np.isneginf(l.v), 0.0, 2 * l.e.max() + 3.01 * U * np.abs(np.where(np.isneginf(l.v), 0.0, arg)))
         term = np.exp(arg)
         total = term.sum()
-        rel = (term * (e_arg * 1.01 + 4 * U)).sum() / total + SUM * U
+        rel = (term * (e_arg * 1.01 + 5 * 4 * U)).sum() / total + SUM * U
         log = np.log(total)
         v = np.where(np.isneginf(l.v), -np.inf, l.v - top - log)
         e = l.e + l.e.max() + rel * 1.01 + 4 * U * abs(log) + 2 * U * (np.abs(np.where(np.isneginf(l.v), 0, arg)) + abs(log))

@@ -7,165 +7,318 @@
 //   l = allowed[v] ? l / temperature : -inf
 //   log-probabilities: l - max l - log sum exp(l - max l), where -inf stays -inf
 //
-// Bound by HBM: the logits are read and the results written. A workgroup owns a chunk of a row's
-// vocabulary. It counts the row's whole history (a few thousand tokens, from L2 after the first
-// workgroup) into one LDS word per token of the chunk, so no count table exists in memory and nothing
-// is left to clear. A word holds the answer's count (20 bits), whether a prompt holds the token (1) and
-// the place of its bias in the list (11, the last one where a token is listed twice): integer
-// additions and maxima, so the result does not depend on their order.
+// Bound by HBM: the logits are read and the results written; log-probabilities read the logits twice, once
+// for the rows' maxima and sums (a chunk's go to the workspace) and once to write, which is less than
+// writing the processed logits and going over them again. A workgroup owns a chunk of a row's vocabulary, a
+// thread units of 4 tokens, so that a wave's stores are 1 KB without a gap (with 8 tokens a thread, 16 bytes
+// in every 32 a store, 192 rows of 129,280 take 34 us to write, so 23). It counts the row's whole history (a
+// few thousand tokens, from L2 after the first workgroup) into one LDS word per token of the chunk, so no
+// count table exists in memory and nothing is left to clear. A word holds the answer's count (20 bits), whether
+// a prompt holds the token (1) and the place of its bias in the list (11, the last one where a token is
+// listed twice): integer additions and maxima, so the result does not depend on their order.
+//
+// The lists cost latency, not work: the ids' way from memory, three barriers, then the logits'. So the chunk's
+// logits, the first ids of the history and the biases are all loaded before the first barrier. A history
+// names a few percent of the tokens, which is enough for most waves to hold one and take the penalties' way:
+// they are products with the penalty or its reciprocal, no divisions.
+#include <cmath>
+
 #include "row_units.h"
 
 namespace wm {
 
-constexpr int LOGIT_CHUNK = 4096;
 constexpr int LOGIT_THREADS = 256;
+constexpr int LOGIT_UNIT = 4;  // a wave's units are 1 KB of results without a gap
 constexpr int LOGIT_MAX_HISTORY = (1 << 20) - 1;
 constexpr int LOGIT_MAX_BIASES = (1 << 11) - 1;
 constexpr uint32_t LOGIT_COUNT = (1u << 20) - 1, LOGIT_PROMPT = 1u << 20;
 constexpr int LOGIT_BIAS_SHIFT = 21;
+constexpr float LOG2E = 1.4426950408889634f;
 
+// The maximum of some values and their sum of exp(l - top). Of nothing but -inf the sum is 0; a NaN, which no
+// maximum sees, makes the sum NaN.
 struct LogitPart {
-  float top, sum;  // the chunk's maximum and its sum of exp(l - top)
+  float top, sum;
 };
 
-__device__ __forceinline__ float block_max(float v, float* part) {
-  v = segment_max<64>(v);
-  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
-  __syncthreads();
-  v = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-  __syncthreads();
-  return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* part) {
-  v = segment_sum<64>(v);
-  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
-  __syncthreads();
-  v = (part[0] + part[1]) + (part[2] + part[3]);
-  __syncthreads();
-  return v;
+__device__ __forceinline__ float finite_top(float top) { return top == -INFINITY ? 0.0f : top; }
+
+// Over a wave, in every lane.
+__device__ __forceinline__ LogitPart wave_part(LogitPart p) {
+  const float top = segment_max<64>(p.top);
+  const float sum = p.sum * __builtin_amdgcn_exp2f((p.top - finite_top(top)) * LOG2E);
+  return {top, segment_sum<64>(sum)};
 }
 
-template <bool F32, bool WIDE>
-__global__ void __launch_bounds__(LOGIT_THREADS) logit_chunk_kernel(const void* logits, int vocab, int chunks,
-                                                                   wm_logit_rules r, float* out,
-                                                                   LogitPart* __restrict__ parts) {
-  __shared__ uint32_t word[LOGIT_CHUNK];
-  __shared__ float part[4];
-  const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int lo = chunk * LOGIT_CHUNK, n = min(LOGIT_CHUNK, vocab - lo);
-  for (int i = threadIdx.x; i < LOGIT_CHUNK; i += LOGIT_THREADS) word[i] = 0;
+// A row's values that do not depend on the token.
+struct LogitRow {
+  float rep, inv_rep, freq, pres, inv_temp;
+  const float* bias;
+  const uint8_t* mask;
+};
+__device__ __forceinline__ LogitRow logit_row(const wm_logit_rules& r, int row) {
+  const float temp = r.temperature ? r.temperature[row] : 1.0f;
+  // temperatures whose reciprocal is a normal number
+  const bool scaled = temp >= 0x1p-126f && temp <= 0x1p126f;
+  const float rep = r.repetition ? r.repetition[row] : 1.0f;
+  return {rep, 1.0f / rep, r.frequency ? r.frequency[row] : 0.0f,
+          r.presence ? r.presence[row] : 0.0f, scaled ? 1.0f / temp : 1.0f,
+          r.bias_values ? r.bias_values + row * r.bias_stride : nullptr,
+          r.mask ? (const uint8_t*)((const uint32_t*)r.mask + row * r.mask_stride) : nullptr};
+}
+
+// A unit's raw logits, `n` of them there.
+template <bool F32>
+struct LogitRaw;
+template <>
+struct LogitRaw<true> {
+  wm_u32x4 a;
+  __device__ __forceinline__ void load(const void* logits, int64_t at) { a = load16((const float*)logits + at); }
+  __device__ __forceinline__ void load_part(const void* logits, int64_t at, int n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = e < n ? ((const uint32_t*)logits)[at + e] : 0u;
+  }
+  __device__ __forceinline__ void unpack(float l[LOGIT_UNIT]) const { RowUnit<true, true>::unpack(a, l); }
+  static __device__ __forceinline__ float one(const void* logits, int64_t at) { return ((const float*)logits)[at]; }
+};
+template <>
+struct LogitRaw<false> {
+  wm_u32x2 a;
+  __device__ __forceinline__ void load(const void* logits, int64_t at) { a = load8((const uint16_t*)logits + at); }
+  __device__ __forceinline__ void load_part(const void* logits, int64_t at, int n) {
+    const uint16_t* p = (const uint16_t*)logits + at;
+    a[0] = p[0] | (n > 1 ? (uint32_t)p[1] << 16 : 0u);
+    a[1] = n > 2 ? p[2] : 0u;
+  }
+  __device__ __forceinline__ void unpack(float l[LOGIT_UNIT]) const {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      l[2 * m] = __uint_as_float(a[m] << 16);
+      l[2 * m + 1] = __uint_as_float(a[m] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ float one(const void* logits, int64_t at) {
+    return bf16_bits_to_f32(((const uint16_t*)logits)[at]);
+  }
+};
+
+// The words of a chunk of n tokens from lo on. Every thread of the workgroup calls it; ends with a barrier.
+template <int CHUNK>
+__device__ __forceinline__ void count_words(const wm_logit_rules& r, int row, int lo, int n, uint32_t (&word)[CHUNK]) {
+  const int32_t* bias_ids = r.bias_ids ? r.bias_ids + row * r.bias_stride : nullptr;
+  const int biases = bias_ids ? r.biases : 0;
+  const int32_t* ids = r.history ? r.history + row * r.history_stride : nullptr;
+  const int len = !ids ? 0 : r.lengths ? max(0, min(r.lengths[row], r.history_len)) : r.history_len;
+  const int prompt = r.prompt_lengths ? r.prompt_lengths[row] : 0;
+  // 16 ids in flight a thread, by 16 bytes at any alignment; -1 behind the end
+  wm_u32x4 v[4];
+  auto fetch = [&](int j0) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int j = j0 + b * 4 * LOGIT_THREADS;
+      if (j + 4 <= len) {
+        v[b] = load16(ids + j);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[b][i] = j + i < len ? (uint32_t)ids[j + i] : 0xffffffffu;
+      }
+    }
+  };
+  const int first_bias = (int)threadIdx.x < biases ? bias_ids[threadIdx.x] : -1;
+  fetch(4 * threadIdx.x);
+#pragma unroll
+  for (int i = 4 * threadIdx.x; i < CHUNK; i += 4 * LOGIT_THREADS) *reinterpret_cast<uint4*>(&word[i]) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  const float* bias = nullptr;
-  if (r.bias_ids) {
-    const int32_t* ids = r.bias_ids + row * r.bias_stride;
-    bias = r.bias_values + row * r.bias_stride;
-    for (int j = threadIdx.x; j < r.biases; j += LOGIT_THREADS) {
-      const int id = ids[j];
+  if (biases > 0) {
+    for (int j = threadIdx.x; j < biases; j += LOGIT_THREADS) {
+      const int id = j < LOGIT_THREADS ? first_bias : bias_ids[j];
       const uint32_t at = (uint32_t)id - (uint32_t)lo;
       if (id >= 0 && at < (uint32_t)n) atomicMax(&word[at], (uint32_t)(j + 1) << LOGIT_BIAS_SHIFT);
     }
-    __syncthreads();
+    __syncthreads();  // the words' lower bits are 0 until here
   }
-  if (r.history) {
-    const int32_t* ids = r.history + row * r.history_stride;
-    const int len = r.lengths ? max(0, min(r.lengths[row], r.history_len)) : r.history_len;
-    const int prompt = r.prompt_lengths ? r.prompt_lengths[row] : 0;
-    for (int j = threadIdx.x; j < len; j += LOGIT_THREADS) {
-      const int id = ids[j];
-      const uint32_t at = (uint32_t)id - (uint32_t)lo;
-      if (id >= 0 && at < (uint32_t)n) {
-        if (j < prompt) atomicOr(&word[at], LOGIT_PROMPT);
-        else atomicAdd(&word[at], 1u);
-      }
-    }
-    __syncthreads();
-  }
-  const float rep = r.repetition ? r.repetition[row] : 1.0f;
-  const float freq = r.frequency ? r.frequency[row] : 0.0f;
-  const float pres = r.presence ? r.presence[row] : 0.0f;
-  float temp = r.temperature ? r.temperature[row] : 1.0f;
-  if (!(temp > 0.0f)) temp = 1.0f;
-  const uint32_t* mask = r.mask ? (const uint32_t*)r.mask + row * r.mask_stride : nullptr;
-  typedef RowUnit<F32, WIDE> U;
-  typedef typename U::Raw Raw;
-  constexpr int N = U::N, PER = LOGIT_CHUNK / LOGIT_THREADS / N;
-  float v[PER][N];
-  const int64_t base = (int64_t)row * vocab + lo;
-  float top = -INFINITY;
+  for (int j0 = 4 * threadIdx.x; j0 < len; j0 += 16 * LOGIT_THREADS) {
+    if (j0 >= 16 * LOGIT_THREADS) fetch(j0);
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int i = (k * LOGIT_THREADS + threadIdx.x) * N;
-    if (i < n) {
-      U::unpack(((const Raw*)((const typename U::Elem*)logits + base))[i / N], v[k]);
-      const uint32_t bits = mask ? mask[(lo + i) / 32] >> ((lo + i) % 32) : 0xffffffffu;
+    for (int b = 0; b < 4; ++b) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint32_t w = word[i + e];
-        const uint32_t count = w & LOGIT_COUNT;
-        float l = v[k][e];
-        if (w & (LOGIT_COUNT | LOGIT_PROMPT)) {
-          l = l > 0.0f ? l / rep : l * rep;
-          if (count) l = l - freq * (float)count - pres;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t at = v[b][i] - (uint32_t)lo;
+        if ((int32_t)v[b][i] >= 0 && at < (uint32_t)n) {
+          if (j0 + b * 4 * LOGIT_THREADS + i < prompt) atomicOr(&word[at], LOGIT_PROMPT);
+          else atomicAdd(&word[at], 1u);
         }
-        if (w >> LOGIT_BIAS_SHIFT) l += bias[(w >> LOGIT_BIAS_SHIFT) - 1];
-        l = (bits >> e) & 1u ? l / temp : -INFINITY;
-        v[k][e] = l;
-        top = fmaxf(top, l);
-      }
-      if constexpr (N == 1) {
-        out[base + i] = v[k][0];
-      } else {
-#pragma unroll
-        for (int q = 0; q < N; q += 4)
-          *reinterpret_cast<float4*>(out + base + i + q) = make_float4(v[k][q], v[k][q + 1], v[k][q + 2], v[k][q + 3]);
       }
     }
   }
-  if (!parts) return;
-  top = block_max(top, part);
-  float sum = 0.0f;
-  if (top > -INFINITY) {
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      if ((k * LOGIT_THREADS + threadIdx.x) * N < n) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) sum += expf(v[k][e] - top);
-      }
-    }
-  } else {
-    // a chunk without an allowed token adds nothing, one of NaN (which no maximum sees) spoils its row
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      if ((k * LOGIT_THREADS + threadIdx.x) * N < n) {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (isnan(v[k][e])) sum = v[k][e];
-      }
-    }
-  }
-  sum = block_sum(sum, part);
-  if (threadIdx.x == 0) parts[blockIdx.x] = LogitPart{top, sum};
+  __syncthreads();
 }
 
-// The rows' logarithms of the sum, from their chunks, and out -= them.
-__global__ void __launch_bounds__(LOGIT_THREADS) logit_norm_kernel(float* __restrict__ out, int vocab, int chunks,
-                                                                  const LogitPart* __restrict__ parts) {
-  __shared__ float part[4];
-  const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const LogitPart* mine = parts + (int64_t)row * chunks;
-  float top = -INFINITY, sum = 0.0f;
-  for (int c = threadIdx.x; c < chunks; c += LOGIT_THREADS) top = fmaxf(top, mine[c].top);
-  top = block_max(top, part);
-  for (int c = threadIdx.x; c < chunks; c += LOGIT_THREADS)
-    sum += mine[c].top > -INFINITY ? mine[c].sum * expf(mine[c].top - top) : mine[c].sum;
-  sum = block_sum(sum, part);
-  const float log_sum = logf(sum);
-  const int lo = chunk * LOGIT_CHUNK, n = min(LOGIT_CHUNK, vocab - lo);
-  float* o = out + (int64_t)row * vocab + lo;
-  for (int i = threadIdx.x; i < n; i += LOGIT_THREADS) {
-    const float l = o[i];
-    if (l != -INFINITY) o[i] = l - top - log_sum;
+// Penalties and bias of a unit's logits, by their words.
+__device__ __forceinline__ void apply_words(const uint32_t* words, const LogitRow& r, float l[LOGIT_UNIT]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(words);
+  if ((a.x | a.y | a.z | a.w) == 0) return;
+  const uint32_t w[LOGIT_UNIT] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int e = 0; e < LOGIT_UNIT; ++e) {
+    const uint32_t count = w[e] & LOGIT_COUNT;
+    if (w[e] & (LOGIT_COUNT | LOGIT_PROMPT)) l[e] *= l[e] > 0.0f ? r.inv_rep : r.rep;
+    if (count) l[e] = l[e] - r.freq * (float)count - r.pres;
+    if (w[e] >> LOGIT_BIAS_SHIFT) l[e] += r.bias[(w[e] >> LOGIT_BIAS_SHIFT) - 1];
   }
+}
+
+// Mask and temperature of a unit's logits; `bits` says which are allowed.
+__device__ __forceinline__ void mask_and_scale(uint32_t bits, bool masked, float inv_temp, float l[LOGIT_UNIT]) {
+  if (masked) {
+#pragma unroll
+    for (int e = 0; e < LOGIT_UNIT; ++e) {
+      const uint32_t keep = (uint32_t)((int32_t)(bits << (31 - e)) >> 31);  // all ones where the token is allowed
+      l[e] = __uint_as_float((__float_as_uint(l[e]) & keep) | (0xff800000u & ~keep));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < LOGIT_UNIT; ++e) l[e] *= inv_temp;  // finite and above 0: -inf stays
+}
+
+// A unit's results to out, `n` of them there.
+__device__ __forceinline__ void store_unit(float* out, int64_t at, int n, const float l[LOGIT_UNIT]) {
+  if (n >= LOGIT_UNIT) {
+    store16_nt(out + at, RowUnit<true, true>::pack(l));
+  } else {
+#pragma unroll
+    for (int e = 0; e < LOGIT_UNIT; ++e)
+      if (e < n) out[at + e] = l[e];
+  }
+}
+
+// A workgroup's chunk: the raw logits, and which of their tokens are allowed, loaded before anything else.
+template <bool F32, int PER>
+struct LogitChunk {
+  LogitRaw<F32> raw[PER];
+  uint32_t bits[PER];
+  __device__ __forceinline__ void load(const void* logits, int64_t base, int lo, int n, const uint8_t* mask) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
+      if (i + LOGIT_UNIT <= n) raw[k].load(logits, base + i);
+      else if (i < n) raw[k].load_part(logits, base + i, n - i);
+      bits[k] = mask && i < n ? mask[(lo + i) / 8] >> (i & 4) : 0xfu;
+    }
+  }
+};
+
+// The chunks' maxima and sums.
+template <bool F32, int PER>
+__global__ void __launch_bounds__(LOGIT_THREADS) logit_stats_kernel(const void* __restrict__ logits, int vocab, int chunks,
+                                                                   wm_logit_rules r, LogitPart* __restrict__ parts) {
+  constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
+  __shared__ __align__(16) uint32_t word[CHUNK];
+  __shared__ LogitPart part[LOGIT_THREADS / 64];
+  const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
+  const bool lists = r.history || r.bias_ids;
+  const LogitRow lr = logit_row(r, row);
+  LogitChunk<F32, PER> c;
+  c.load(logits, (int64_t)row * vocab + lo, lo, n, lr.mask);
+  if (lists) count_words<CHUNK>(r, row, lo, n, word);
+  float l[PER][LOGIT_UNIT];
+  LogitPart p = {-INFINITY, 0.0f};
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
+    if (i < n) {
+      c.raw[k].unpack(l[k]);
+      if (lists) apply_words(&word[i], lr, l[k]);
+      mask_and_scale(c.bits[k], lr.mask != nullptr, lr.inv_temp, l[k]);
+#pragma unroll
+      for (int e = 0; e < LOGIT_UNIT; ++e) {
+        if (i + e >= n) l[k][e] = -INFINITY;
+        p.top = fmaxf(p.top, l[k][e]);
+      }
+    }
+  }
+  const float top = finite_top(p.top);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if ((k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT < n) {
+#pragma unroll
+      for (int e = 0; e < LOGIT_UNIT; ++e) p.sum += __builtin_amdgcn_exp2f((l[k][e] - top) * LOG2E);
+    }
+  }
+  p = wave_part(p);
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = p;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    p = threadIdx.x < LOGIT_THREADS / 64 ? part[threadIdx.x] : LogitPart{-INFINITY, 0.0f};
+    p = wave_part(p);
+    if (threadIdx.x == 0) parts[blockIdx.x] = p;
+  }
+}
+
+// The results. parts (nullable): the rows' chunks, for log-probabilities.
+template <bool F32, int PER>
+__global__ void __launch_bounds__(LOGIT_THREADS) logit_write_kernel(const void* logits, int vocab, int chunks, wm_logit_rules r,
+                                                                   const LogitPart* __restrict__ parts, float* out) {
+  constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
+  __shared__ __align__(16) uint32_t word[CHUNK];
+  __shared__ LogitPart whole;
+  const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
+  const int64_t base = (int64_t)row * vocab + lo;
+  const bool lists = r.history || r.bias_ids;
+  const LogitRow lr = logit_row(r, row);
+  LogitChunk<F32, PER> c;
+  c.load(logits, base, lo, n, lr.mask);
+  if (parts && threadIdx.x < 64) {
+    LogitPart p = {-INFINITY, 0.0f};
+    for (int q = threadIdx.x; q < chunks; q += 64) {
+      const LogitPart o = parts[(int64_t)row * chunks + q];
+      const float top = fmaxf(p.top, o.top);
+      p.sum = p.sum * __builtin_amdgcn_exp2f((p.top - finite_top(top)) * LOG2E) +
+              o.sum * __builtin_amdgcn_exp2f((o.top - finite_top(top)) * LOG2E);
+      p.top = top;
+    }
+    p = wave_part(p);
+    if (threadIdx.x == 0) whole = p;
+  }
+  if (lists) count_words<CHUNK>(r, row, lo, n, word);
+  else __syncthreads();
+  const float top = parts ? finite_top(whole.top) : 0.0f, log_sum = parts ? logf(whole.sum) : 0.0f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
+    if (i >= n) break;
+    float l[LOGIT_UNIT];
+    c.raw[k].unpack(l);
+    if (lists) apply_words(&word[i], lr, l);
+    mask_and_scale(c.bits[k], lr.mask != nullptr, lr.inv_temp, l);
+    if (parts) {
+#pragma unroll
+      for (int e = 0; e < LOGIT_UNIT; ++e) l[e] = l[e] == -INFINITY ? l[e] : (l[e] - top) - log_sum;
+    }
+    store_unit(out, base + i, n - i, l);
+  }
+}
+
+// Units of a thread, by how many workgroups the rows make.
+static int logit_per(int64_t rows, int64_t vocab) {
+  return rows * ((vocab + 4095) / 4096) >= 512 ? 4 : 2;
+}
+static int64_t logit_chunks(int64_t rows, int64_t vocab) {
+  const int64_t chunk = LOGIT_THREADS * LOGIT_UNIT * logit_per(rows, vocab);
+  return (vocab + chunk - 1) / chunk;
+}
+
+template <bool F32, int PER>
+static void process_logits(const void* logits, int rows, int vocab, const wm_logit_rules& r, float* out, LogitPart* parts,
+                           hipStream_t s) {
+  const int chunks = (int)logit_chunks(rows, vocab);
+  const dim3 grid((unsigned)(rows * chunks));
+  if (parts) {
+    hipLaunchKernelGGL((logit_stats_kernel<F32, PER>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts);
+    check_launch("logit_stats");
+  }
+  hipLaunchKernelGGL((logit_write_kernel<F32, PER>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts, out);
+  check_launch("logit_write");
 }
 
 }  // namespace wm
@@ -176,7 +329,7 @@ extern "C" {
 
 WM_EXPORT size_t wm_process_logits_workspace_size(int32_t rows, int32_t vocab) {
   if (rows < 0 || vocab < 1) return 0;
-  return (size_t)rows * ((vocab + LOGIT_CHUNK - 1) / LOGIT_CHUNK) * sizeof(LogitPart);
+  return (size_t)(rows * logit_chunks(rows, vocab)) * sizeof(LogitPart);
 }
 
 WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab, const wm_logit_rules* rules,
@@ -185,8 +338,7 @@ WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, 
     if (!rules) fail("wm_process_logits: null rules");
     if (rows < 0) fail("wm_process_logits: rows must not be negative");
     if (vocab < 1 || vocab > 1 << 22) fail("wm_process_logits: vocab must be in 1..4194304");
-    const int64_t chunks = (vocab + LOGIT_CHUNK - 1) / LOGIT_CHUNK;
-    if (rows * chunks > (int64_t)0x7fffffff) fail("wm_process_logits: too many rows");
+    if (rows * logit_chunks(rows, vocab) > (int64_t)0x7fffffff) fail("wm_process_logits: too many rows");
     if (fp32 != 0 && fp32 != 1) fail("wm_process_logits: fp32 must be 0 (bf16 logits) or 1");
     const wm_logit_rules& r = *rules;
     if (r.history_len < 0 || r.history_len > LOGIT_MAX_HISTORY) fail("wm_process_logits: history_len must be in 0..1048575");
@@ -200,24 +352,16 @@ WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, 
       fail("wm_process_logits: tensors must be aligned to their elements");
     if (log_probs && (!workspace || workspace_bytes < wm_process_logits_workspace_size(rows, vocab) || (uintptr_t)workspace % 8))
       fail("wm_process_logits: workspace too small or misaligned");
-    const bool wide = rows_wide(vocab, fp32 != 0, {logits, out});
     LogitPart* parts = log_probs ? (LogitPart*)workspace : nullptr;
     hipStream_t s = as_stream(stream);
-#define WM_LOGITS(F, W)                                                                                                      \
-  hipLaunchKernelGGL((logit_chunk_kernel<F, W>), dim3((unsigned)(rows * chunks)), dim3(LOGIT_THREADS), 0, s, logits, vocab, \
-                     (int)chunks, r, out, parts)
+    const int per = logit_per(rows, vocab);
+#define WM_LOGITS(F, P) process_logits<F, P>(logits, rows, vocab, r, out, parts, s)
     if (fp32) {
-      if (wide) WM_LOGITS(true, true); else WM_LOGITS(true, false);
+      if (per == 4) WM_LOGITS(true, 4); else WM_LOGITS(true, 2);
     } else {
-      if (wide) WM_LOGITS(false, true); else WM_LOGITS(false, false);
+      if (per == 4) WM_LOGITS(false, 4); else WM_LOGITS(false, 2);
     }
 #undef WM_LOGITS
-    check_launch("logit_chunk");
-    if (log_probs) {
-      hipLaunchKernelGGL(logit_norm_kernel, dim3((unsigned)(rows * chunks)), dim3(LOGIT_THREADS), 0, s, out, vocab, (int)chunks,
-                         parts);
-      check_launch("logit_norm");
-    }
   });
 }
 

@@ -11,8 +11,6 @@
 // All four are bound by HBM and walk the tokens, not the permuted rows: a token's row is read or written
 // once and its k permuted rows once each. Sums are fp32 in j order, so a result does not depend on the
 // grid, and are rounded once.
-#include <initializer_list>
-
 #include "moe_internal.h"
 #include "permute_device.h"
 #include "row_units.h"
@@ -33,7 +31,8 @@ constexpr int SORT_CHUNK = 256;
 struct SortArgs {
   const void* x;
   const int32_t* indices;
-  int64_t tokens, units;
+  int64_t tokens, length;  // a row's length in 2-byte elements: rows are moved, whatever they hold
+  RowUnits row;
   int k, experts, tile_rows;
   int chunk_tokens, split_units, log2;  // 2^log2 threads side by side in a row
   void* rows;
@@ -65,7 +64,7 @@ __device__ __forceinline__ int32_t sort_scan(int32_t v, int32_t* total) {
   return before + incl - v;
 }
 
-template <typename Unit, bool ONE>
+template <bool ONE>
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
   // base: counts, then the chunk's first row of each expert; later the first row of each expert (offsets)
   __shared__ int32_t base[PERMUTE_MAX_EXPERTS], later[PERMUTE_MAX_EXPERTS + 1];
@@ -177,23 +176,32 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
     }
   }
   __syncthreads();
-  const Unit* x = (const Unit*)a.x;
-  Unit* rows = (Unit*)a.rows;
-  const int64_t c0 = (int64_t)blockIdx.y * a.split_units, c1 = min(a.units, c0 + a.split_units);
+  const uint16_t* x = (const uint16_t*)a.x;
+  uint16_t* rows = (uint16_t*)a.rows;
+  const int c0 = blockIdx.y * a.split_units, c1 = min(a.row.units, c0 + a.split_units);
   for (int t = threadIdx.x >> a.log2; t < tokens; t += SORT_THREADS >> a.log2) {
-    for (int64_t c = c0 + (threadIdx.x & ((1 << a.log2) - 1)); c < c1; c += 1 << a.log2) {
-      const Unit v = x[(t0 + t) * a.units + c];
+    for (int c = c0 + (threadIdx.x & ((1 << a.log2) - 1)); c < c1; c += 1 << a.log2) {
+      auto move = [&](auto unit, int64_t at) {
+        typedef decltype(unit) U;
+        const auto v = U::load(x + (t0 + t) * a.length + at);
 #pragma unroll 4
-      for (int j = 0; j < a.k; ++j) {
-        const int32_t r = row[t * a.k + j];
-        if (r >= 0) store_once(&rows[r * a.units + c], v);
-      }
+        for (int j = 0; j < a.k; ++j) {
+          const int32_t r = row[t * a.k + j];
+          if (r >= 0) U::store_once(rows + r * a.length + at, v);
+        }
+      };
+      if (c < a.row.wide) move(RowUnit<false, true>(), 8 * (int64_t)c);
+      else move(RowUnit<false, false>(), 8 * (int64_t)a.row.wide + c - a.row.wide);
     }
   }
   // The rows behind the last pair, spread over the workgroups: the few that own the last pairs would take
   // twice as long (4096 tokens x 8, hidden 7168, 2% of the pairs absent: 112 us, spread 103).
-  for (int64_t r = present + (int64_t)blockIdx.x; r < pairs; r += gridDim.x)
-    for (int64_t c = c0 + threadIdx.x; c < c1; c += SORT_THREADS) store_once(&rows[r * a.units + c], Unit{});
+  for (int64_t r = present + (int64_t)blockIdx.x; r < pairs; r += gridDim.x) {
+    for (int c = c0 + threadIdx.x; c < c1; c += SORT_THREADS) {
+      if (c < a.row.wide) store16_nt(rows + r * a.length + 8 * (int64_t)c, wm_u32x4{0, 0, 0, 0});
+      else rows[r * a.length + 8 * (int64_t)a.row.wide + c - a.row.wide] = 0;
+    }
+  }
 }
 
 // Up to this many pairs a call is one launch.
@@ -206,45 +214,37 @@ static int sort_chunk_tokens(int64_t tokens, int k, bool one) {
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-template <typename Unit>
 static void sort_launch(SortArgs a, bool one, hipStream_t s) {
   const int64_t chunks = a.tokens > 0 ? (a.tokens + a.chunk_tokens - 1) / a.chunk_tokens : 1;
   // columns are split until the chip has work for every CU
-  const int64_t most = (a.units + 255) / 256;
+  const int64_t most = (a.row.units + 255) / 256;
   int64_t splits = chunks >= 512 ? 1 : (511 + chunks) / chunks;
   if (splits > most) splits = most;
-  a.split_units = (int)((a.units + splits - 1) / splits);
+  a.split_units = (int)((a.row.units + splits - 1) / splits);
   a.log2 = 0;
   while (a.log2 < 9 && (1 << a.log2) < a.split_units) ++a.log2;
   const dim3 grid((unsigned)chunks, (unsigned)splits);
-  if (one) hipLaunchKernelGGL((sort_kernel<Unit, true>), grid, dim3(SORT_THREADS), 0, s, a);
-  else hipLaunchKernelGGL((sort_kernel<Unit, false>), grid, dim3(SORT_THREADS), 0, s, a);
+  if (one) hipLaunchKernelGGL((sort_kernel<true>), grid, dim3(SORT_THREADS), 0, s, a);
+  else hipLaunchKernelGGL((sort_kernel<false>), grid, dim3(SORT_THREADS), 0, s, a);
   check_launch("sort");
 }
 
 // ---- back (WEIGHTED) and the sort's gradient: a thread owns one unit of a token, sums its k rows.
 constexpr int GATHER_BATCH = 8;  // rows in flight
 
-template <bool F32, bool WIDE, bool WEIGHTED>
-__global__ void __launch_bounds__(256) gather_sum_kernel(const void* __restrict__ rows_, const float* __restrict__ weights,
-                                                        const int32_t* __restrict__ inverse, int64_t tokens, int64_t units,
-                                                        int log2, int k, const void* add_, void* y_) {
-  typedef RowUnit<F32, WIDE> U;
-  typedef typename U::Raw Raw;
-  const int64_t t = (int64_t)blockIdx.x * (256 >> log2) + (threadIdx.x >> log2);
-  const int64_t c = ((int64_t)blockIdx.y << log2) + (threadIdx.x & ((1 << log2) - 1));
-  if (t >= tokens || c >= units) return;
-  const Raw* rows = (const Raw*)rows_;
-  const uint32_t pairs = (uint32_t)(tokens * k);
+template <typename U, bool WEIGHTED>
+__device__ __forceinline__ void gather_unit(const typename U::Elem* __restrict__ rows, const float* __restrict__ weights,
+                                            const int32_t* __restrict__ inverse, uint32_t pairs, int64_t hidden, int64_t t,
+                                            int64_t at, int k, const typename U::Elem* add, typename U::Elem* y) {
   float acc[U::N] = {};
   for (int j0 = 0; j0 < k; j0 += GATHER_BATCH) {
     uint32_t r[GATHER_BATCH];
-    Raw v[GATHER_BATCH];
+    typename U::Raw v[GATHER_BATCH];
 #pragma unroll
     for (int q = 0; q < GATHER_BATCH; ++q) r[q] = j0 + q < k ? (uint32_t)inverse[t * k + j0 + q] : 0xffffffffu;
 #pragma unroll
     for (int q = 0; q < GATHER_BATCH; ++q)
-      if (r[q] < pairs) v[q] = load_once(&rows[r[q] * units + c]);
+      if (r[q] < pairs) v[q] = U::load_once(rows + r[q] * hidden + at);
 #pragma unroll
     for (int q = 0; q < GATHER_BATCH; ++q) {
       if (r[q] < pairs) {
@@ -256,30 +256,44 @@ __global__ void __launch_bounds__(256) gather_sum_kernel(const void* __restrict_
       }
     }
   }
-  if (add_) {
+  if (add) {
     float f[U::N];
-    U::unpack(((const Raw*)add_)[t * units + c], f);
+    U::unpack(U::load(add + t * hidden + at), f);
 #pragma unroll
     for (int i = 0; i < U::N; ++i) acc[i] += f[i];
   }
-  ((Raw*)y_)[t * units + c] = U::pack(acc);
+  U::store(y + t * hidden + at, U::pack(acc));
+}
+
+template <bool F32, bool WEIGHTED>
+__global__ void __launch_bounds__(256) gather_sum_kernel(const void* __restrict__ rows_, const float* __restrict__ weights,
+                                                        const int32_t* __restrict__ inverse, int64_t tokens, int64_t hidden,
+                                                        RowUnits row, int log2, int k, const void* add_, void* y_) {
+  typedef typename RowUnit<F32, true>::Elem Elem;
+  const int64_t t = (int64_t)blockIdx.x * (256 >> log2) + (threadIdx.x >> log2);
+  const int c = ((int)blockIdx.y << log2) + (threadIdx.x & ((1 << log2) - 1));
+  if (t >= tokens || c >= row.units) return;
+  constexpr int N = RowUnit<F32, true>::N;
+  const uint32_t pairs = (uint32_t)(tokens * k);
+  const Elem *rows = (const Elem*)rows_, *add = (const Elem*)add_;
+  if (c < row.wide)
+    gather_unit<RowUnit<F32, true>, WEIGHTED>(rows, weights, inverse, pairs, hidden, t, (int64_t)c * N, k, add, (Elem*)y_);
+  else
+    gather_unit<RowUnit<F32, false>, WEIGHTED>(rows, weights, inverse, pairs, hidden, t, (int64_t)row.wide * N + c - row.wide, k,
+                                               add, (Elem*)y_);
 }
 
 template <bool WEIGHTED>
 static void gather_sum(const void* rows, bool f32, const float* weights, const int32_t* inverse, int64_t tokens, int k,
                        int64_t hidden, const void* add, void* y, hipStream_t s) {
-  const bool wide = rows_wide(hidden, f32, {rows, add, y});
-  const int64_t units = wide ? hidden / (f32 ? 4 : 8) : hidden;
-  const RowGrid g = row_grid(tokens, units);
-#define WM_GS(F, W)                                                                                                     \
-  hipLaunchKernelGGL((gather_sum_kernel<F, W, WEIGHTED>), g.grid, dim3(256), 0, s, rows, weights, inverse, tokens, units, \
-                     g.log2, k, add, y)
-  if (f32) {
-    if (wide) WM_GS(true, true); else WM_GS(true, false);
-  } else {
-    if (wide) WM_GS(false, true); else WM_GS(false, false);
-  }
-#undef WM_GS
+  const RowUnits row = row_units(hidden, f32);
+  const RowGrid g = row_grid(tokens, row.units);
+  if (f32)
+    hipLaunchKernelGGL((gather_sum_kernel<true, WEIGHTED>), g.grid, dim3(256), 0, s, rows, weights, inverse, tokens, hidden, row,
+                       g.log2, k, add, y);
+  else
+    hipLaunchKernelGGL((gather_sum_kernel<false, WEIGHTED>), g.grid, dim3(256), 0, s, rows, weights, inverse, tokens, hidden, row,
+                       g.log2, k, add, y);
   check_launch("gather_sum");
 }
 
@@ -287,23 +301,28 @@ static void gather_sum(const void* rows, bool f32, const float* weights, const i
 // pairs, so a pair's row is read once, its gradient written, and its dot product summed over the block.
 constexpr int BACK_BATCH = 8;
 
-template <bool F32, bool WIDE>
+template <bool F32>
 __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__ dy_, const void* __restrict__ rows_,
                                                        const float* __restrict__ weights, const int32_t* __restrict__ inverse,
-                                                       const int32_t* __restrict__ present_, int64_t tokens, int64_t units,
-                                                       int k, void* __restrict__ drows_, float* __restrict__ dweights) {
-  typedef RowUnit<F32, WIDE> U;
-  typedef typename U::Raw Raw;
+                                                       const int32_t* __restrict__ present_, int64_t tokens, int64_t hidden,
+                                                       RowUnits row, int k, void* __restrict__ drows_,
+                                                       float* __restrict__ dweights) {
+  typedef typename RowUnit<F32, true>::Elem Elem;
+  constexpr int N = RowUnit<F32, true>::N;
   __shared__ float part[BACK_BATCH][4];
   const int64_t t = blockIdx.x;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const Raw* dy = (const Raw*)dy_ + t * units;
-  const Raw* rows = (const Raw*)rows_;
-  Raw* drows = (Raw*)drows_;
+  const Elem* dy = (const Elem*)dy_ + t * hidden;
+  const Elem* rows = (const Elem*)rows_;
+  Elem* drows = (Elem*)drows_;
   const uint32_t pairs = (uint32_t)(tokens * k);
   // the rows without a pair, spread over the tokens
-  for (int64_t r = *present_ + t; r < tokens * k; r += tokens)
-    for (int64_t c = threadIdx.x; c < units; c += 256) store_once(&drows[r * units + c], U::zero());
+  for (int64_t r = *present_ + t; r < tokens * k; r += tokens) {
+    for (int c = threadIdx.x; c < row.units; c += 256) {
+      if (c < row.wide) store16_nt(drows + r * hidden + (int64_t)c * N, wm_u32x4{0, 0, 0, 0});
+      else drows[r * hidden + (int64_t)row.wide * N + c - row.wide] = 0;
+    }
+  }
   for (int j0 = 0; j0 < k; j0 += BACK_BATCH) {
     uint32_t r[BACK_BATCH];
     float w[BACK_BATCH], dot[BACK_BATCH] = {};
@@ -313,23 +332,30 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
       r[q] = j0 + q < k ? (uint32_t)inverse[p] : 0xffffffffu;
       w[q] = j0 + q < k ? weights[p] : 0.0f;
     }
-    for (int64_t c = threadIdx.x; c < units; c += 256) {
+    auto unit = [&](auto u, int64_t at) {
+      typedef decltype(u) U;
       float d[U::N];
-      U::unpack(dy[c], d);
+      typename U::Raw v[BACK_BATCH];
+      U::unpack(U::load(dy + at), d);
+#pragma unroll
+      for (int q = 0; q < BACK_BATCH; ++q)
+        if (r[q] < pairs) v[q] = U::load_once(rows + r[q] * hidden + at);
 #pragma unroll
       for (int q = 0; q < BACK_BATCH; ++q) {
         if (r[q] < pairs) {
           float f[U::N], o[U::N];
-          U::unpack(load_once(&rows[r[q] * units + c]), f);
+          U::unpack(v[q], f);
 #pragma unroll
           for (int i = 0; i < U::N; ++i) {
             dot[q] = fmaf(d[i], f[i], dot[q]);
             o[i] = w[q] * d[i];
           }
-          store_once(&drows[r[q] * units + c], U::pack(o));
+          U::store_once(drows + r[q] * hidden + at, U::pack(o));
         }
       }
-    }
+    };
+    for (int c = threadIdx.x; c < row.wide; c += 256) unit(RowUnit<F32, true>(), (int64_t)c * N);
+    if (threadIdx.x < row.units - row.wide) unit(RowUnit<F32, false>(), (int64_t)row.wide * N + threadIdx.x);
 #pragma unroll
     for (int q = 0; q < BACK_BATCH; ++q) {
       const float v = segment_sum<64>(dot[q]);
@@ -402,18 +428,9 @@ WM_EXPORT int wm_sort_tokens(const void* x, int32_t fp32, int32_t tokens, int32_
       permute_scan((pairs + chunk_pairs - 1) / chunk_pairs, experts, tile_rows, 0, offsets, tiles, nullptr, tile_count, ws, s);
       a.chunk_base = ws.counts;
     }
-    const int64_t bytes = (int64_t)hidden * (fp32 ? 4 : 2);
-    const uintptr_t at = (uintptr_t)x | (uintptr_t)rows | (uintptr_t)bytes;
-    if (at % 16 == 0) {
-      a.units = bytes / 16;
-      sort_launch<uint4>(a, one, s);
-    } else if (at % 4 == 0) {
-      a.units = bytes / 4;
-      sort_launch<uint32_t>(a, one, s);
-    } else {
-      a.units = bytes / 2;
-      sort_launch<uint16_t>(a, one, s);
-    }
+    a.length = (int64_t)hidden * (fp32 ? 2 : 1);
+    a.row = row_units(a.length, false);
+    sort_launch(a, one, s);
   });
 }
 
@@ -449,18 +466,14 @@ WM_EXPORT int wm_combine_rows_backward(const void* dy, const void* rows, int32_t
     if (!dy || !rows || !weights || !inverse || !present || !drows || !dweights) fail("wm_combine_rows_backward: null pointer");
     if (((uintptr_t)dy | (uintptr_t)rows | (uintptr_t)drows) % (fp32 ? 4 : 2))
       fail("wm_combine_rows_backward: rows must be aligned to their elements");
-    const bool f32 = fp32 != 0, wide = rows_wide(hidden, f32, {dy, rows, drows});
-    const int64_t units = wide ? hidden / (f32 ? 4 : 8) : hidden;
+    const RowUnits row = row_units(hidden, fp32 != 0);
     hipStream_t s = as_stream(stream);
-#define WM_BG(F, W)                                                                                                      \
-  hipLaunchKernelGGL((back_grad_kernel<F, W>), dim3((unsigned)tokens), dim3(256), 0, s, dy, rows, weights, inverse, present, \
-                     (int64_t)tokens, units, k, drows, dweights)
-    if (f32) {
-      if (wide) WM_BG(true, true); else WM_BG(true, false);
-    } else {
-      if (wide) WM_BG(false, true); else WM_BG(false, false);
-    }
-#undef WM_BG
+    if (fp32)
+      hipLaunchKernelGGL((back_grad_kernel<true>), dim3((unsigned)tokens), dim3(256), 0, s, dy, rows, weights, inverse, present,
+                         (int64_t)tokens, (int64_t)hidden, row, k, drows, dweights);
+    else
+      hipLaunchKernelGGL((back_grad_kernel<false>), dim3((unsigned)tokens), dim3(256), 0, s, dy, rows, weights, inverse, present,
+                         (int64_t)tokens, (int64_t)hidden, row, k, drows, dweights);
     check_launch("back_grad");
   });
 }
