@@ -102,60 +102,87 @@ struct LogitRaw<false> {
   }
 };
 
-// The words of a chunk of n tokens from lo on. Every thread of the workgroup calls it; ends with a barrier.
 template <int CHUNK>
-__device__ __forceinline__ void count_words(const wm_logit_rules& r, int row, int lo, int n, uint32_t (&word)[CHUNK]) {
-  const int32_t* bias_ids = r.bias_ids ? r.bias_ids + row * r.bias_stride : nullptr;
-  const int biases = bias_ids ? r.biases : 0;
-  const int32_t* ids = r.history ? r.history + row * r.history_stride : nullptr;
-  const int len = !ids ? 0 : r.lengths ? max(0, min(r.lengths[row], r.history_len)) : r.history_len;
-  const int prompt = r.prompt_lengths ? r.prompt_lengths[row] : 0;
-  // 16 ids in flight a thread, by 16 bytes at any alignment; -1 behind the end
+struct LogitWords {
+  uint32_t word[CHUNK];
+  float bias[LOGIT_THREADS];  // the first biases' values, for the threads that meet them
+};
+
+// A row's lists, and the first of them a thread has in flight: 16 ids by 16 bytes at any alignment, -1 where there
+// are none, one of the last ids that make no 16 bytes, and a bias. Loaded before the logits, since a wait
+// for a load is a wait for those before it, and without a use of what is loaded.
+struct LogitIds {
+  const int32_t *ids, *bias_ids;
+  int len, prompt, biases, bias_id;
+  float bias_value;
+  uint32_t last;
   wm_u32x4 v[4];
-  auto fetch = [&](int j0) {
+
+  __device__ __forceinline__ void fetch(int j0) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const int j = j0 + b * 4 * LOGIT_THREADS;
-      if (j + 4 <= len) {
-        v[b] = load16(ids + j);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[b][i] = j + i < len ? (uint32_t)ids[j + i] : 0xffffffffu;
-      }
+      v[b] = wm_u32x4{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      if (j + 4 <= len) v[b] = load16(ids + j);
     }
-  };
-  const int first_bias = (int)threadIdx.x < biases ? bias_ids[threadIdx.x] : -1;
-  fetch(4 * threadIdx.x);
+  }
+  __device__ __forceinline__ void load(const wm_logit_rules& r, int row) {
+    ids = r.history ? r.history + row * r.history_stride : nullptr;
+    len = !ids ? 0 : r.lengths ? max(0, min(r.lengths[row], r.history_len)) : r.history_len;
+    prompt = r.prompt_lengths ? r.prompt_lengths[row] : 0;
+    bias_ids = r.bias_ids ? r.bias_ids + row * r.bias_stride : nullptr;
+    biases = bias_ids ? r.biases : 0;
+    bias_id = -1;
+    bias_value = 0.0f;
+    if ((int)threadIdx.x < biases) {
+      bias_id = bias_ids[threadIdx.x];
+      bias_value = r.bias_values[row * r.bias_stride + threadIdx.x];
+    }
+    last = 0xffffffffu;
+    if ((int)threadIdx.x < len % 4) last = (uint32_t)ids[len - len % 4 + threadIdx.x];
+    fetch(4 * threadIdx.x);
+  }
+};
+
+// The words of a chunk of n tokens from lo on. Every thread of the workgroup calls it; ends with a barrier.
+template <int CHUNK>
+__device__ __forceinline__ void count_words(LogitIds& f, int lo, int n, LogitWords<CHUNK>& s) {
+  uint32_t(&word)[CHUNK] = s.word;
 #pragma unroll
   for (int i = 4 * threadIdx.x; i < CHUNK; i += 4 * LOGIT_THREADS) *reinterpret_cast<uint4*>(&word[i]) = make_uint4(0, 0, 0, 0);
+  s.bias[threadIdx.x] = f.bias_value;
   __syncthreads();
-  if (biases > 0) {
-    for (int j = threadIdx.x; j < biases; j += LOGIT_THREADS) {
-      const int id = j < LOGIT_THREADS ? first_bias : bias_ids[j];
-      const uint32_t at = (uint32_t)id - (uint32_t)lo;
-      if (id >= 0 && at < (uint32_t)n) atomicMax(&word[at], (uint32_t)(j + 1) << LOGIT_BIAS_SHIFT);
+  if (f.biases > 0) {
+    for (int j = threadIdx.x; j < f.biases; j += LOGIT_THREADS) {
+      const int id = j < LOGIT_THREADS ? f.bias_id : f.bias_ids[j];
+      const uint32_t at = (uint32_t)id - (uint32_t)lo;  // a negative id is beyond every chunk's end
+      if (at < (uint32_t)n) atomicMax(&word[at], (uint32_t)(j + 1) << LOGIT_BIAS_SHIFT);
     }
     __syncthreads();  // the words' lower bits are 0 until here
   }
-  for (int j0 = 4 * threadIdx.x; j0 < len; j0 += 16 * LOGIT_THREADS) {
-    if (j0 >= 16 * LOGIT_THREADS) fetch(j0);
+  auto count = [&](uint32_t id, int j) {
+    const uint32_t at = id - (uint32_t)lo;
+    if (at < (uint32_t)n) {
+      if (j < f.prompt) atomicOr(&word[at], LOGIT_PROMPT);
+      else atomicAdd(&word[at], 1u);
+    }
+  };
+  for (int j0 = 4 * threadIdx.x; j0 + 4 <= f.len; j0 += 16 * LOGIT_THREADS) {
+    if (j0 >= 16 * LOGIT_THREADS) f.fetch(j0);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
+      const int j = j0 + b * 4 * LOGIT_THREADS;
+      if (j + 4 > f.len) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t at = v[b][i] - (uint32_t)lo;
-        if ((int32_t)v[b][i] >= 0 && at < (uint32_t)n) {
-          if (j0 + b * 4 * LOGIT_THREADS + i < prompt) atomicOr(&word[at], LOGIT_PROMPT);
-          else atomicAdd(&word[at], 1u);
-        }
-      }
+      for (int i = 0; i < 4; ++i) count(f.v[b][i], j + i);
     }
   }
+  count(f.last, f.len - f.len % 4 + threadIdx.x);
   __syncthreads();
 }
 
 // Penalties and bias of a unit's logits, by their words.
-__device__ __forceinline__ void apply_words(const uint32_t* words, const LogitRow& r, float l[LOGIT_UNIT]) {
+__device__ __forceinline__ void apply_words(const uint32_t* words, const float* biases, const LogitRow& r, float l[LOGIT_UNIT]) {
   const uint4 a = *reinterpret_cast<const uint4*>(words);
   if ((a.x | a.y | a.z | a.w) == 0) return;
   const uint32_t w[LOGIT_UNIT] = {a.x, a.y, a.z, a.w};
@@ -164,7 +191,8 @@ __device__ __forceinline__ void apply_words(const uint32_t* words, const LogitRo
     const uint32_t count = w[e] & LOGIT_COUNT;
     if (w[e] & (LOGIT_COUNT | LOGIT_PROMPT)) l[e] *= l[e] > 0.0f ? r.inv_rep : r.rep;
     if (count) l[e] = l[e] - r.freq * (float)count - r.pres;
-    if (w[e] >> LOGIT_BIAS_SHIFT) l[e] += r.bias[(w[e] >> LOGIT_BIAS_SHIFT) - 1];
+    const uint32_t j = w[e] >> LOGIT_BIAS_SHIFT;
+    if (j) l[e] += j <= LOGIT_THREADS ? biases[j - 1] : r.bias[j - 1];
   }
 }
 
@@ -192,47 +220,57 @@ __device__ __forceinline__ void store_unit(float* out, int64_t at, int n, const 
   }
 }
 
-// A workgroup's chunk: the raw logits, and which of their tokens are allowed, loaded before anything else.
-template <bool F32, int PER>
+// A workgroup's chunk: the raw logits, and the mask's bytes that hold their tokens' bits. WHOLE: a chunk that the
+// vocabulary does not end in, without a branch between the loads.
+template <bool F32, int PER, bool WHOLE>
 struct LogitChunk {
   LogitRaw<F32> raw[PER];
-  uint32_t bits[PER];
-  __device__ __forceinline__ void load(const void* logits, int64_t base, int lo, int n, const uint8_t* mask) {
+  uint8_t mask[PER];
+  static constexpr int STEP = LOGIT_THREADS * LOGIT_UNIT;
+  __device__ __forceinline__ void load(const void* logits, int64_t base, int lo, int n, const uint8_t* bytes) {
+    const int at = threadIdx.x * LOGIT_UNIT;
+    if (bytes) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (WHOLE || k * STEP + at < n) mask[k] = bytes[(lo + k * STEP + at) / 8];
+    }
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
-      if (i + LOGIT_UNIT <= n) raw[k].load(logits, base + i);
+      const int i = k * STEP + at;
+      if (WHOLE || i + LOGIT_UNIT <= n) raw[k].load(logits, base + i);
       else if (i < n) raw[k].load_part(logits, base + i, n - i);
-      bits[k] = mask && i < n ? mask[(lo + i) / 8] >> (i & 4) : 0xfu;
     }
+  }
+  // Logits of unit k after the rules; words null: without lists.
+  __device__ __forceinline__ void apply(int k, const uint32_t* words, const float* biases, const LogitRow& r,
+                                        float l[LOGIT_UNIT]) const {
+    raw[k].unpack(l);
+    if (words) apply_words(words + k * STEP + threadIdx.x * LOGIT_UNIT, biases, r, l);
+    mask_and_scale((uint32_t)mask[k] >> (threadIdx.x % 2 * LOGIT_UNIT), r.mask != nullptr, r.inv_temp, l);
   }
 };
 
-// The chunks' maxima and sums.
-template <bool F32, int PER>
-__global__ void __launch_bounds__(LOGIT_THREADS) logit_stats_kernel(const void* __restrict__ logits, int vocab, int chunks,
-                                                                   wm_logit_rules r, LogitPart* __restrict__ parts) {
-  constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
-  __shared__ __align__(16) uint32_t word[CHUNK];
-  __shared__ LogitPart part[LOGIT_THREADS / 64];
-  const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
+// The maximum and the sum of a chunk: in part[0] .. of the waves.
+template <bool F32, int PER, bool WHOLE>
+__device__ __forceinline__ void chunk_stats(const void* logits, int vocab, const wm_logit_rules& r, int row, int lo, int n,
+                                            LogitWords<LOGIT_THREADS * LOGIT_UNIT * PER>& s, LogitPart* part) {
   const bool lists = r.history || r.bias_ids;
   const LogitRow lr = logit_row(r, row);
-  LogitChunk<F32, PER> c;
+  LogitIds f;
+  if (lists) f.load(r, row);
+  LogitChunk<F32, PER, WHOLE> c;
   c.load(logits, (int64_t)row * vocab + lo, lo, n, lr.mask);
-  if (lists) count_words<CHUNK>(r, row, lo, n, word);
+  if (lists) count_words(f, lo, n, s);
   float l[PER][LOGIT_UNIT];
   LogitPart p = {-INFINITY, 0.0f};
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
-    if (i < n) {
-      c.raw[k].unpack(l[k]);
-      if (lists) apply_words(&word[i], lr, l[k]);
-      mask_and_scale(c.bits[k], lr.mask != nullptr, lr.inv_temp, l[k]);
+    if (WHOLE || i < n) {
+      c.apply(k, lists ? s.word : nullptr, s.bias, lr, l[k]);
 #pragma unroll
       for (int e = 0; e < LOGIT_UNIT; ++e) {
-        if (i + e >= n) l[k][e] = -INFINITY;
+        if (!WHOLE && i + e >= n) l[k][e] = -INFINITY;
         p.top = fmaxf(p.top, l[k][e]);
       }
     }
@@ -240,63 +278,86 @@ __global__ void __launch_bounds__(LOGIT_THREADS) logit_stats_kernel(const void* 
   const float top = finite_top(p.top);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    if ((k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT < n) {
+    if (WHOLE || (k * LOGIT_THREADS + (int)threadIdx.x) * LOGIT_UNIT < n) {
 #pragma unroll
       for (int e = 0; e < LOGIT_UNIT; ++e) p.sum += __builtin_amdgcn_exp2f((l[k][e] - top) * LOG2E);
     }
   }
   p = wave_part(p);
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = p;
+}
+
+// The chunks' maxima and sums.
+template <bool F32, int PER>
+__global__ void __launch_bounds__(LOGIT_THREADS) logit_stats_kernel(const void* __restrict__ logits, int vocab, int chunks,
+                                                                   wm_logit_rules r, LogitPart* __restrict__ parts) {
+  constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
+  __shared__ __align__(16) LogitWords<CHUNK> s;
+  __shared__ LogitPart part[LOGIT_THREADS / 64];
+  const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
+  if (n == CHUNK) chunk_stats<F32, PER, true>(logits, vocab, r, row, lo, n, s, part);
+  else chunk_stats<F32, PER, false>(logits, vocab, r, row, lo, n, s, part);
   __syncthreads();
   if (threadIdx.x < 64) {
-    p = threadIdx.x < LOGIT_THREADS / 64 ? part[threadIdx.x] : LogitPart{-INFINITY, 0.0f};
+    LogitPart p = threadIdx.x < LOGIT_THREADS / 64 ? part[threadIdx.x] : LogitPart{-INFINITY, 0.0f};
     p = wave_part(p);
     if (threadIdx.x == 0) parts[blockIdx.x] = p;
   }
 }
 
-// The results. parts (nullable): the rows' chunks, for log-probabilities.
-template <bool F32, int PER>
-__global__ void __launch_bounds__(LOGIT_THREADS) logit_write_kernel(const void* logits, int vocab, int chunks, wm_logit_rules r,
-                                                                   const LogitPart* __restrict__ parts, float* out) {
-  constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
-  __shared__ __align__(16) uint32_t word[CHUNK];
-  __shared__ LogitPart whole;
-  const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
+// A chunk's results. parts (nullable): the row's chunks, for log-probabilities.
+template <bool F32, int PER, bool WHOLE>
+__device__ __forceinline__ void chunk_write(const void* logits, int vocab, int chunks, const wm_logit_rules& r, int row, int lo,
+                                            int n, const LogitPart* __restrict__ parts, float* out,
+                                            LogitWords<LOGIT_THREADS * LOGIT_UNIT * PER>& s, LogitPart* whole) {
   const int64_t base = (int64_t)row * vocab + lo;
   const bool lists = r.history || r.bias_ids;
   const LogitRow lr = logit_row(r, row);
-  LogitChunk<F32, PER> c;
+  LogitIds f;
+  if (lists) f.load(r, row);
+  LogitPart o = {-INFINITY, 0.0f};
+  if (parts && threadIdx.x < 64 && (int)threadIdx.x < chunks) o = parts[threadIdx.x];
+  LogitChunk<F32, PER, WHOLE> c;
   c.load(logits, base, lo, n, lr.mask);
   if (parts && threadIdx.x < 64) {
-    LogitPart p = {-INFINITY, 0.0f};
-    for (int q = threadIdx.x; q < chunks; q += 64) {
-      const LogitPart o = parts[(int64_t)row * chunks + q];
+    LogitPart p = o;
+    for (int q = 64 + threadIdx.x; q < chunks; q += 64) {
+      o = parts[q];
       const float top = fmaxf(p.top, o.top);
       p.sum = p.sum * __builtin_amdgcn_exp2f((p.top - finite_top(top)) * LOG2E) +
               o.sum * __builtin_amdgcn_exp2f((o.top - finite_top(top)) * LOG2E);
       p.top = top;
     }
     p = wave_part(p);
-    if (threadIdx.x == 0) whole = p;
+    if (threadIdx.x == 0) *whole = p;
   }
-  if (lists) count_words<CHUNK>(r, row, lo, n, word);
+  if (lists) count_words(f, lo, n, s);
   else __syncthreads();
-  const float top = parts ? finite_top(whole.top) : 0.0f, log_sum = parts ? logf(whole.sum) : 0.0f;
+  const float top = parts ? finite_top(whole->top) : 0.0f, log_sum = parts ? logf(whole->sum) : 0.0f;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
-    if (i >= n) break;
+    if (!WHOLE && i >= n) break;
     float l[LOGIT_UNIT];
-    c.raw[k].unpack(l);
-    if (lists) apply_words(&word[i], lr, l);
-    mask_and_scale(c.bits[k], lr.mask != nullptr, lr.inv_temp, l);
+    c.apply(k, lists ? s.word : nullptr, s.bias, lr, l);
     if (parts) {
 #pragma unroll
       for (int e = 0; e < LOGIT_UNIT; ++e) l[e] = l[e] == -INFINITY ? l[e] : (l[e] - top) - log_sum;
     }
-    store_unit(out, base + i, n - i, l);
+    store_unit(out, base + i, WHOLE ? LOGIT_UNIT : n - i, l);
   }
+}
+
+template <bool F32, int PER>
+__global__ void __launch_bounds__(LOGIT_THREADS) logit_write_kernel(const void* logits, int vocab, int chunks, wm_logit_rules r,
+                                                                   const LogitPart* __restrict__ parts, float* out) {
+  constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
+  __shared__ __align__(16) LogitWords<CHUNK> s;
+  __shared__ LogitPart whole;
+  const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
+  const LogitPart* mine = parts ? parts + (int64_t)row * chunks : nullptr;
+  if (n == CHUNK) chunk_write<F32, PER, true>(logits, vocab, chunks, r, row, lo, n, mine, out, s, &whole);
+  else chunk_write<F32, PER, false>(logits, vocab, chunks, r, row, lo, n, mine, out, s, &whole);
 }
 
 // Units of a thread, by how many workgroups the rows make.
