@@ -10,78 +10,93 @@
 //   b = s g dr',  c = b (o + w_post)               dy = p c - y p^3 mean(c y)     dw_post = sum_t b y p
 //   dg = s dr' z (by sigmoid'), summed over what g is broadcast over
 //
-// Bound by HBM: every tensor passes once. A workgroup holds a token's row in registers (a thread has VEC
-// consecutive columns, V times), sums over the row twice at most, and goes on to the next token with the
-// weights still in registers. Sums over tokens (weight gradients) stay in the threads' registers, go to
-// the workspace once per workgroup and are added up by a second launch in the workgroups' order. All
-// arithmetic is fp32; bf16 outputs are rounded once, from values that no earlier rounding touched but
-// r''s own (x is the norm of the residual that the next block reads).
-#include "wm_common.h"
+// Bound by HBM: every tensor passes once. A workgroup holds a token's row in registers, 8 or 16 columns a
+// thread, sums over the row twice at most, and goes on to the next token with the weights still in
+// registers. Sums over tokens (weight gradients) stay in the threads' registers, go to the workspace once
+// per workgroup and are added up by a second launch in the workgroups' order. All arithmetic is fp32; bf16
+// outputs are rounded once, from values that no earlier rounding touched but r''s own (x is the norm of
+// the residual that the next block reads).
+#include <initializer_list>
+
+#include "row_units.h"
 
 namespace wm {
 
 constexpr int NORM_MAX_HIDDEN = 16384;
-enum { GATE_NONE = 0, GATE_TOKEN = 1, GATE_CHANNEL = 2, GATE_FULL = 3 };
+enum { GATE_NONE = 0, GATE_TOKEN = 1, GATE_CHANNEL = 2, GATE_FULL = 3, GATE_FULL_F32 = 4 };  // 4: kernels only
 
-// VEC consecutive elements from index i: bf16, or fp32.
-template <int VEC>
-__device__ __forceinline__ void load_bf16(const void* p, int64_t i, float f[VEC]) {
-  if constexpr (VEC == 8) {
-    const uint4 v = *reinterpret_cast<const uint4*>((const uint16_t*)p + i);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+// Eight consecutive elements of a row as they are stored, from an address aligned to the elements; `n` of
+// them are there, the others 0. WHOLE: all are, which the launch knows from hidden % 8 == 0.
+template <bool F32>
+struct Row8;
+template <>
+struct Row8<false> {
+  wm_u32x4 a;
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const void* p, int64_t i, int n) {
+    const uint16_t* q = (const uint16_t*)p + i;
+    if (WHOLE || n >= 8) {
+      a = load16(q);
+    } else {
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      f[2 * m] = __uint_as_float(u[m] << 16);
-      f[2 * m + 1] = __uint_as_float(u[m] & 0xffff0000u);
+      for (int e = 0; e < 4; ++e) a[e] = (2 * e < n ? q[2 * e] : 0u) | (2 * e + 1 < n ? (uint32_t)q[2 * e + 1] << 16 : 0u);
+    }
+  }
+  __device__ __forceinline__ void clear() { a = wm_u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float(i % 2 ? a[i / 2] & 0xffff0000u : a[i / 2] << 16); }
+};
+template <>
+struct Row8<true> {
+  wm_u32x4 a, b;
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const void* p, int64_t i, int n) {
+    const float* q = (const float*)p + i;
+    if (WHOLE || n >= 8) {
+      a = load16(q);
+      b = load16(q + 4);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = e < n ? __float_as_uint(q[e]) : 0u;
+        b[e] = 4 + e < n ? __float_as_uint(q[4 + e]) : 0u;
+      }
+    }
+  }
+  __device__ __forceinline__ void clear() { a = b = wm_u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float(i < 4 ? a[i] : b[i - 4]); }
+};
+template <bool WHOLE>
+__device__ __forceinline__ void store8(void* p, bool f32, int64_t i, int n, const float f[8]) {
+  if (f32) {
+    float* q = (float*)p + i;
+    if (WHOLE || n >= 8) {
+      store16(q, RowUnit<true, true>::pack(f));
+      store16(q + 4, RowUnit<true, true>::pack(f + 4));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) q[e] = f[e];
     }
   } else {
-    f[0] = bf16_bits_to_f32(((const uint16_t*)p)[i]);
-  }
-}
-template <int VEC>
-__device__ __forceinline__ void load_f32(const void* p, int64_t i, float f[VEC]) {
-  if constexpr (VEC == 8) {
-    const float4 a = *reinterpret_cast<const float4*>((const float*)p + i);
-    const float4 b = *reinterpret_cast<const float4*>((const float*)p + i + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    f[0] = ((const float*)p)[i];
-  }
-}
-template <int VEC>
-__device__ __forceinline__ void load_any(const void* p, bool f32, int64_t i, float f[VEC]) {
-  if (f32) load_f32<VEC>(p, i, f); else load_bf16<VEC>(p, i, f);
-}
-template <int VEC>
-__device__ __forceinline__ void store_bf16(void* p, int64_t i, const float f[VEC]) {
-  if constexpr (VEC == 8) {
-    uint32_t u[4];
+    uint16_t* q = (uint16_t*)p + i;
+    if (WHOLE || n >= 8) {
+      store16(q, RowUnit<false, true>::pack(f));
+    } else {
 #pragma unroll
-    for (int m = 0; m < 4; ++m) u[m] = f32_to_bf16_bits(f[2 * m]) | ((uint32_t)f32_to_bf16_bits(f[2 * m + 1]) << 16);
-    *reinterpret_cast<uint4*>((uint16_t*)p + i) = make_uint4(u[0], u[1], u[2], u[3]);
-  } else {
-    ((uint16_t*)p)[i] = f32_to_bf16_bits(f[0]);
-  }
-}
-template <int VEC>
-__device__ __forceinline__ void store_any(void* p, bool f32, int64_t i, const float f[VEC]) {
-  if (!f32) {
-    store_bf16<VEC>(p, i, f);
-  } else if constexpr (VEC == 8) {
-    *reinterpret_cast<float4*>((float*)p + i) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>((float*)p + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    ((float*)p)[i] = f[0];
+      for (int e = 0; e < 8; ++e)
+        if (e < n) q[e] = (uint16_t)pack_bf16(f[e], 0.0f);
+    }
   }
 }
 
 __device__ __forceinline__ float sigmoid_f32(float v) { return 1.0f / (1.0f + expf(-v)); }
 
-// Sums N values over the workgroup (whole waves, 16 at most) in a fixed order; every thread gets them.
-// `part` is not used again before every thread is past this sum: the caller alternates two.
+// Sums N values over the workgroup (whole waves, 16 at most) in a fixed order; every thread gets them. `part`
+// holds zeros behind the waves, and is written again only behind another sum's barrier: the callers
+// alternate between two or three.
 template <int N>
 __device__ __forceinline__ void block_sums(float v[N], float (*part)[16]) {
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     v[n] = segment_sum<64>(v[n]);
@@ -89,11 +104,11 @@ __device__ __forceinline__ void block_sums(float v[N], float (*part)[16]) {
   }
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    float s = part[n][0];
-    for (int w = 1; w < waves; ++w) s += part[n][w];
-    v[n] = s;
-  }
+  for (int n = 0; n < N; ++n) v[n] = segment_sum<16>(part[n][lane % 16]);
+}
+__device__ __forceinline__ void clear_parts(float* part, int n) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) part[i] = 0.0f;
+  __syncthreads();
 }
 
 struct NormArgs {
@@ -108,101 +123,108 @@ struct NormArgs {
   int hidden;
 };
 
-// The gate of a thread's columns: its value (through the sigmoid) for element (t, c).
-template <int VEC>
-__device__ __forceinline__ void gate_values(const NormArgs& a, int64_t t, int c, float g[VEC]) {
-  if (a.gate_kind == GATE_NONE) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) g[i] = 1.0f;
-    return;
+// The weights of a thread's columns as they are stored: ones without weights, which then have no offset.
+struct Weight8 {
+  Row8<false> w;
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const uint16_t* p, int c, int n) {
+    w.a = wm_u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    if (p) w.template load<WHOLE>(p, c, n);
   }
-  if (a.gate_kind == GATE_TOKEN) {
-    float v[1];
-    load_any<1>(a.gate, a.gate_f32, t, v);
-    if (a.gate_sigmoid) v[0] = sigmoid_f32(v[0]);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) g[i] = v[0];
-    return;
-  }
-  load_any<VEC>(a.gate, a.gate_f32, (a.gate_kind == GATE_FULL ? t * a.hidden : 0) + c, g);
-  if (a.gate_sigmoid) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) g[i] = sigmoid_f32(g[i]);
-  }
+  __device__ __forceinline__ float get(float offset, int i) const { return w.get(i) + offset; }
+};
+
+// One value of a gate (through the sigmoid).
+__device__ __forceinline__ float gate_value(const NormArgs& a, int64_t i) {
+  const float g = a.gate_f32 ? ((const float*)a.gate)[i] : bf16_bits_to_f32(((const uint16_t*)a.gate)[i]);
+  return a.gate_sigmoid ? sigmoid_f32(g) : g;
 }
 
-// o + w for a thread's columns, 1 without weights.
-template <int VEC>
-__device__ __forceinline__ void norm_weights(const uint16_t* w, float offset, int c, float f[VEC]) {
-  if (!w) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = 1.0f;
-    return;
-  }
-  load_bf16<VEC>(w, c, f);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) f[i] += offset;
-}
-
-template <bool F32, int VEC, int V>
-__global__ void __launch_bounds__(1024) block_norm_kernel(NormArgs a, void* residual_out, uint16_t* __restrict__ x) {
-  __shared__ float part[2][1][16];
+// A thread has columns 8 (v blockDim + thread) .. + 7 of every row, v < V.
+template <bool F32, int V, bool WHOLE, int GATE, int THREADS>
+__global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* residual_out, uint16_t* __restrict__ x) {
+  __shared__ float part[3][1][16];
+  clear_parts(&part[0][0][0], 48);
   const int H = a.hidden;
-  float wpost[V][VEC], wpre[V][VEC];
+  const float opost = a.post ? a.offset : 0.0f, opre = a.pre ? a.offset : 0.0f;
+  Weight8 wpost[V], wpre[V];
+  float channel[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * VEC;
+    const int c = (v * blockDim.x + threadIdx.x) * 8;
     if (c < H) {
-      norm_weights<VEC>(a.post, a.offset, c, wpost[v]);
-      norm_weights<VEC>(a.pre, a.offset, c, wpre[v]);
+      wpost[v].template load<WHOLE>(a.post, c, H - c);
+      wpre[v].template load<WHOLE>(a.pre, c, H - c);
+      if (GATE == GATE_CHANNEL) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) channel[v][i] = WHOLE || i < H - c ? a.scale * gate_value(a, c + i) : 0.0f;
+      }
     }
   }
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    float r[V][VEC], y[V][VEC];
+  int odd = 0;
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x, odd ^= 1) {
+    Row8<F32> raw[V];
+    Row8<false> y[V];
+    Row8<GATE == GATE_FULL_F32> gate[V];
+    float r[V][8];
     float sum[1] = {0.0f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * VEC;
+      const int c = (v * blockDim.x + threadIdx.x) * 8;
       if (c < H) {
-        load_any<VEC>(a.residual, F32, t * H + c, r[v]);
-        load_bf16<VEC>(a.y, t * H + c, y[v]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[0] = fmaf(y[v][i], y[v][i], sum[0]);
+        y[v].template load<WHOLE>(a.y, t * H + c, H - c);
+        raw[v].template load<WHOLE>(a.residual, t * H + c, H - c);
+        if (GATE >= GATE_FULL) gate[v].template load<WHOLE>(a.gate, t * H + c, H - c);
       }
     }
+    const float g1 = GATE == GATE_TOKEN ? a.scale * gate_value(a, t) : a.scale;
     float p = 1.0f;
     if (a.post_norm) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if ((int)((v * blockDim.x + threadIdx.x) * 8) < H) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[0] = fmaf(y[v].get(i), y[v].get(i), sum[0]);
+        }
+      }
       block_sums<1>(sum, part[0]);
       p = rsqrtf(sum[0] / (float)H + a.eps);
     }
     sum[0] = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * VEC;
+      const int c = (v * blockDim.x + threadIdx.x) * 8;
       if (c < H) {
-        float g[VEC];
-        gate_values<VEC>(a, t, c, g);
+        float g[8];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          r[v][i] = fmaf(a.scale * g[i], y[v][i] * p * wpost[v][i], r[v][i]);
-          if (!F32) r[v][i] = bf16_bits_to_f32(f32_to_bf16_bits(r[v][i]));
-          sum[0] = fmaf(r[v][i], r[v][i], sum[0]);
+        for (int i = 0; i < 8; ++i) g[i] = GATE == GATE_CHANNEL ? channel[v][i] : g1;
+        if (GATE >= GATE_FULL) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] = a.gate_sigmoid ? sigmoid_f32(gate[v].get(i)) : gate[v].get(i);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] *= a.scale;
         }
-        store_any<VEC>(residual_out, F32, t * H + c, r[v]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          r[v][i] = fmaf(g[i], y[v].get(i) * p * wpost[v].get(opost, i), raw[v].get(i));
+        if (!F32) RowUnit<false, true>::unpack(RowUnit<false, true>::pack(r[v]), r[v]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (WHOLE || i < H - c) sum[0] = fmaf(r[v][i], r[v][i], sum[0]);
+        store8<WHOLE>(residual_out, F32, t * H + c, H - c, r[v]);
       }
     }
-    block_sums<1>(sum, part[1]);
+    block_sums<1>(sum, part[1 + odd]);  // without the post norm no other barrier stands between two of these
     const float q = rsqrtf(sum[0] / (float)H + a.eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * VEC;
+      const int c = (v * blockDim.x + threadIdx.x) * 8;
       if (c < H) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) r[v][i] *= q * wpre[v][i];
-        store_bf16<VEC>(x, t * H + c, r[v]);
+        for (int i = 0; i < 8; ++i) r[v][i] *= q * wpre[v].get(opre, i);
+        store8<WHOLE>(x, false, t * H + c, H - c, r[v]);
       }
     }
-    __syncthreads();  // part is free again
   }
 }
 
@@ -211,47 +233,73 @@ struct NormGrads {
   const void* dres;  // null: zero
   void* dr;
   uint16_t* dy;
-  void* dgate;    // token: fp32 [T]; full: in the gate's type
-  float* partial;  // [workgroups][3][H]: post, pre, channel gate
+  void* dgate;     // token: fp32 [T]; full: in the gate's type
+  float* partial;  // [3][workgroups][H]: post, pre, channel gate
 };
 
-template <bool F32, int VEC, int V>
-__global__ void __launch_bounds__(1024) block_norm_grad_kernel(NormArgs a, NormGrads d) {
+// What a thread loads of a token's row. (Loading the next token's meanwhile takes the registers of a second
+// workgroup a CU and is no faster: 74.0 us for 4001 tokens of 5120 with a full gate, 72.7 without.)
+template <bool F32, int V, bool WHOLE, int GATE>
+struct NormRow {
+  Row8<F32> r[V], dr[V];
+  Row8<false> y[V], dx[V];
+  Row8<GATE == GATE_FULL_F32> gate[V];
+  __device__ __forceinline__ void load(const NormArgs& a, const NormGrads& d, int64_t t) {
+    const int H = a.hidden;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * blockDim.x + threadIdx.x) * 8;
+      if (c < H) {
+        r[v].template load<WHOLE>(a.residual, t * H + c, H - c);
+        dx[v].template load<WHOLE>(d.dx, t * H + c, H - c);
+        y[v].template load<WHOLE>(a.y, t * H + c, H - c);
+        if (d.dres) dr[v].template load<WHOLE>(d.dres, t * H + c, H - c);
+        if (GATE >= GATE_FULL) gate[v].template load<WHOLE>(a.gate, t * H + c, H - c);
+      }
+    }
+  }
+};
+
+template <bool F32, int V, bool WHOLE, int GATE, int THREADS>
+__global__ void __launch_bounds__(THREADS) block_norm_grad_kernel(NormArgs a, NormGrads d) {
   __shared__ float part[2][3][16];
+  clear_parts(&part[0][0][0], 96);
   const int H = a.hidden;
-  float wpost[V][VEC], wpre[V][VEC], dpost[V][VEC], dpre[V][VEC], dch[V][VEC];
+  const float opost = a.post ? a.offset : 0.0f, opre = a.pre ? a.offset : 0.0f;
+  Weight8 wpost[V], wpre[V];
+  float channel[V][8];
+  float dpost[V][8], dpre[V][8], dch[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * VEC;
+    const int c = (v * blockDim.x + threadIdx.x) * 8;
     if (c < H) {
-      norm_weights<VEC>(a.post, a.offset, c, wpost[v]);
-      norm_weights<VEC>(a.pre, a.offset, c, wpre[v]);
+      wpost[v].template load<WHOLE>(a.post, c, H - c);
+      wpre[v].template load<WHOLE>(a.pre, c, H - c);
+      if (GATE == GATE_CHANNEL) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) channel[v][i] = WHOLE || i < H - c ? gate_value(a, c + i) : 0.0f;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) dpost[v][i] = dpre[v][i] = dch[v][i] = 0.0f;
+    for (int i = 0; i < 8; ++i) dpost[v][i] = dpre[v][i] = dch[v][i] = 0.0f;
   }
   const float inv = 1.0f / (float)H;
+  NormRow<F32, V, WHOLE, GATE> row;
+#pragma unroll
+  for (int v = 0; v < V; ++v) row.dr[v].clear();
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    float r[V][VEC], y[V][VEC], dx[V][VEC], dr[V][VEC];
+    row.load(a, d, t);
+    const float g1 = GATE == GATE_TOKEN ? gate_value(a, t) : 1.0f;
     float sum[3] = {0.0f, 0.0f, 0.0f};  // r'^2, a r', y^2
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * VEC;
-      if (c < H) {
-        load_any<VEC>(a.residual, F32, t * H + c, r[v]);
-        load_bf16<VEC>(d.dx, t * H + c, dx[v]);
-        load_bf16<VEC>(a.y, t * H + c, y[v]);
-        if (d.dres) {
-          load_any<VEC>(d.dres, F32, t * H + c, dr[v]);
-        } else {
+      if ((int)((v * blockDim.x + threadIdx.x) * 8) < H) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) dr[v][i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          sum[0] = fmaf(r[v][i], r[v][i], sum[0]);
-          sum[1] = fmaf(dx[v][i] * wpre[v][i], r[v][i], sum[1]);
-          sum[2] = fmaf(y[v][i], y[v][i], sum[2]);
+        for (int i = 0; i < 8; ++i) {  // behind a row's end r', dx and y are 0
+          const float r = row.r[v].get(i), y = row.y[v].get(i);
+          sum[0] = fmaf(r, r, sum[0]);
+          sum[1] = fmaf(row.dx[v].get(i) * wpre[v].get(opre, i), r, sum[1]);
+          sum[2] = fmaf(y, y, sum[2]);
         }
       }
     }
@@ -260,81 +308,115 @@ __global__ void __launch_bounds__(1024) block_norm_grad_kernel(NormArgs a, NormG
     const float p = a.post_norm ? rsqrtf(sum[2] * inv + a.eps) : 1.0f;
     const float k1 = q * q * q * (sum[1] * inv);
     float sum2[2] = {0.0f, 0.0f};  // c y, the token's gate gradient
+    float cc[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * VEC;
+      const int c = (v * blockDim.x + threadIdx.x) * 8;
       if (c < H) {
-        float g[VEC], dg[VEC];
-        gate_values<VEC>(a, t, c, g);
+        float dr[8], dg[8], g[8];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          dr[v][i] += fmaf(q, dx[v][i] * wpre[v][i], -r[v][i] * k1);
-          dpre[v][i] = fmaf(dx[v][i] * q, r[v][i], dpre[v][i]);
-          const float n = y[v][i] * p;
-          const float sdr = a.scale * dr[v][i];
-          dg[i] = sdr * n * wpost[v][i] * (a.gate_sigmoid ? g[i] * (1.0f - g[i]) : 1.0f);
+        for (int i = 0; i < 8; ++i) g[i] = GATE == GATE_CHANNEL ? channel[v][i] : GATE >= GATE_FULL ? row.gate[v].get(i) : g1;
+        if (GATE >= GATE_FULL && a.gate_sigmoid) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] = sigmoid_f32(g[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float r = row.r[v].get(i), dx = row.dx[v].get(i), n = row.y[v].get(i) * p;
+          dr[i] = row.dr[v].get(i) + fmaf(q * dx, wpre[v].get(opre, i), -r * k1);
+          dpre[v][i] = fmaf(q * dx, r, dpre[v][i]);
+          const float sdr = a.scale * dr[i], w = wpost[v].get(opost, i);
           const float b = sdr * g[i];
           dpost[v][i] = fmaf(b, n, dpost[v][i]);
-          dch[v][i] += dg[i];
-          sum2[1] += dg[i];
-          dx[v][i] = b * wpost[v][i];  // c from here on
-          sum2[0] = fmaf(dx[v][i], y[v][i], sum2[0]);
+          if (GATE != GATE_NONE) dg[i] = sdr * (n * w);
+          cc[v][i] = b * w;
+          sum2[0] = fmaf(cc[v][i], row.y[v].get(i), sum2[0]);
         }
-        store_any<VEC>(d.dr, F32, t * H + c, dr[v]);
-        if (a.gate_kind == GATE_FULL) store_any<VEC>(d.dgate, a.gate_f32, t * H + c, dg);
+        store8<WHOLE>(d.dr, F32, t * H + c, H - c, dr);
+        if (GATE != GATE_NONE) {
+          if (a.gate_sigmoid) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dg[i] *= g[i] * (1.0f - g[i]);
+          }
+          if (GATE >= GATE_FULL) store8<WHOLE>(d.dgate, GATE == GATE_FULL_F32, t * H + c, H - c, dg);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (GATE == GATE_CHANNEL) dch[v][i] += dg[i];
+            if (GATE == GATE_TOKEN) sum2[1] += dg[i];
+          }
+        }
       }
     }
-    block_sums<2>(sum2, part[1]);
+    if (a.post_norm || GATE == GATE_TOKEN) block_sums<GATE == GATE_TOKEN ? 2 : 1>(sum2, part[1]);
+    else __syncthreads();
     const float k2 = a.post_norm ? p * p * p * (sum2[0] * inv) : 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * VEC;
+      const int c = (v * blockDim.x + threadIdx.x) * 8;
       if (c < H) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) dx[v][i] = fmaf(p, dx[v][i], -y[v][i] * k2);
-        store_bf16<VEC>(d.dy, t * H + c, dx[v]);
+        for (int i = 0; i < 8; ++i) cc[v][i] = fmaf(p, cc[v][i], -row.y[v].get(i) * k2);
+        store8<WHOLE>(d.dy, false, t * H + c, H - c, cc[v]);
       }
     }
-    if (a.gate_kind == GATE_TOKEN && threadIdx.x == 0) ((float*)d.dgate)[t] = sum2[1];
-    __syncthreads();  // part is free again
+    if (GATE == GATE_TOKEN && threadIdx.x == 0) ((float*)d.dgate)[t] = sum2[1];
   }
-  float* out = d.partial + (int64_t)blockIdx.x * 3 * H;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * VEC;
+    const int c = (v * blockDim.x + threadIdx.x) * 8;
     if (c < H) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (a.post) out[c + i] = dpost[v][i];
-        if (a.pre) out[H + c + i] = dpre[v][i];
-        if (a.gate_kind == GATE_CHANNEL) out[2 * H + c + i] = dch[v][i];
-      }
+      const int64_t at = (int64_t)blockIdx.x * H + c, all = (int64_t)gridDim.x * H;
+      if (a.post) store8<WHOLE>(d.partial, true, at, H - c, dpost[v]);
+      if (a.pre) store8<WHOLE>(d.partial, true, all + at, H - c, dpre[v]);
+      if (GATE == GATE_CHANNEL) store8<WHOLE>(d.partial, true, 2 * all + at, H - c, dch[v]);
     }
   }
 }
 
-// out[which][c] = the sum of partial[b][which][c] over the workgroups: 16 columns x 16 slices of workgroups
-// a block, then the slices in order.
-__global__ void __launch_bounds__(256) norm_columns_kernel(const float* __restrict__ partial, int blocks, int hidden,
-                                                          float* dpost, float* dpre, float* dgate) {
-  __shared__ float slice[16][17];
+// out[which][c] = the sum of partial[which][b][c] over the workgroups b: a workgroup has 64 columns, each of its
+// 16 waves every 16th b, and the waves' sums are added in their order.
+__global__ void __launch_bounds__(1024) norm_columns_kernel(const float* __restrict__ partial, int blocks, int hidden,
+                                                           float* dpost, float* dpre, float* dgate) {
+  __shared__ float wave_sum[16][64];
   float* out = blockIdx.y == 0 ? dpost : blockIdx.y == 1 ? dpre : dgate;
   if (!out) return;
-  const int col = threadIdx.x % 16, part = threadIdx.x / 16;
-  const int c = blockIdx.x * 16 + col;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int c = blockIdx.x * 64 + lane;
+  const float* mine = partial + (int64_t)blockIdx.y * blocks * hidden + c;
   float sum = 0.0f;
-  if (c < hidden)
-    for (int b = part; b < blocks; b += 16) sum += partial[((int64_t)b * 3 + blockIdx.y) * hidden + c];
-  slice[part][col] = sum;
+  if (c < hidden) {
+#pragma unroll 8
+    for (int b = wave; b < blocks; b += 16) sum += mine[(int64_t)b * hidden];
+  }
+  wave_sum[wave][lane] = sum;
   __syncthreads();
-  if (part == 0 && c < hidden) {
-    for (int s = 1; s < 16; ++s) sum += slice[s][col];
+  if (wave == 0 && c < hidden) {
+    for (int w = 1; w < 16; ++w) sum += wave_sum[w][lane];
     out[c] = sum;
   }
 }
 
-// Workgroups of the gradient pass: each adds a row to the second launch's work.
-static int norm_grad_blocks(int64_t tokens) { return (int)(tokens < 512 ? tokens : 512); }
+// A workgroup's threads: 8 columns each where 1024 threads suffice, else 16.
+struct NormShape {
+  int v, threads;
+};
+static NormShape norm_shape(int hidden) {
+  const int units = (hidden + 7) / 8, v = units <= 1024 ? 1 : 2;
+  return {v, ((units + v - 1) / v + 63) / 64 * 64};
+}
+
+// Workgroups of a pass by the waves a CU gets, two workgroups at least. (The forward pass with 64, twice what a
+// CU holds, 152 us for 16384 tokens of 4096, with 32 157 us, with a workgroup a token 218.)
+static int norm_blocks(int64_t tokens, int hidden, int waves) {
+  const int64_t per_cu = waves * 64 / norm_shape(hidden).threads, want = 256 * (per_cu > 2 ? per_cu : 2);
+  return (int)(tokens < want ? tokens : want);
+}
+// The gradient pass adds a row a workgroup to the second launch's work: 8 tokens each or more, unless that
+// leaves CUs without one.
+static int norm_grad_blocks(int64_t tokens, int hidden) {
+  const int64_t most = tokens / 8 > 512 ? tokens / 8 : 512, blocks = norm_blocks(tokens, hidden, 16);
+  return (int)(blocks < most ? blocks : most);
+}
 
 static NormArgs norm_args(const char* name, const wm_block_norm_form* f, const void* residual, const void* y, int tokens,
                           int hidden) {
@@ -353,42 +435,53 @@ static NormArgs norm_args(const char* name, const wm_block_norm_form* f, const v
           tokens, hidden};
 }
 
-// Elements of `f32` tensors aligned to themselves; returns whether all rows can be read 16 bytes at a time.
-static bool norm_aligned(const char* name, const wm_block_norm_form* f, int hidden, std::initializer_list<const void*> bf16,
-                         std::initializer_list<const void*> residuals, const void* f32_or_null, const void* gate2) {
-  uintptr_t all = (uintptr_t)f->post_weight | (uintptr_t)f->pre_weight, wide = all;
-  for (const void* p : bf16) all |= (uintptr_t)p;
-  wide |= all;
-  uintptr_t res = 0, gate = (uintptr_t)f->gate | (uintptr_t)gate2;
+// Every tensor is aligned to its elements.
+static void norm_aligned(const char* name, const wm_block_norm_form* f, std::initializer_list<const void*> bf16,
+                         std::initializer_list<const void*> residuals, std::initializer_list<const void*> f32,
+                         const void* full_gate) {
+  uintptr_t two = (uintptr_t)f->post_weight | (uintptr_t)f->pre_weight, res = 0, four = 0;
+  for (const void* p : bf16) two |= (uintptr_t)p;
   for (const void* p : residuals) res |= (uintptr_t)p;
-  if (all % 2 || res % (f->residual_fp32 ? 4 : 2) || gate % (f->gate_fp32 ? 4 : 2) || (uintptr_t)f32_or_null % 4)
+  for (const void* p : f32) four |= (uintptr_t)p;
+  const uintptr_t gate = (uintptr_t)f->gate | (uintptr_t)full_gate;
+  if (two % 2 || res % (f->residual_fp32 ? 4 : 2) || gate % (f->gate_fp32 ? 4 : 2) || four % 4)
     fail(std::string(name) + ": tensors must be aligned to their elements");
-  wide |= res;
-  if (f->gate_kind >= GATE_CHANNEL) wide |= gate;
-  return hidden % 8 == 0 && wide % 16 == 0;
 }
 
-// Threads of a workgroup: a thread has V runs of VEC columns of the row.
-struct NormShape {
-  int vec, v, threads;
-};
-static NormShape norm_shape(int hidden, bool wide) {
-  const int units = wide ? hidden / 8 : hidden;
-  const int v = wide ? (units <= 1024 ? 1 : 2) : (units <= 1024 ? 1 : units <= 4096 ? 4 : 16);
-  const int threads = (units + v - 1) / v;
-  return {wide ? 8 : 1, v, (threads + 63) / 64 * 64};
-}
-
-#define WM_NORM_SHAPES(F32, LAUNCH)                 \
-  if (s.vec == 8) {                                 \
-    if (s.v == 1) LAUNCH(F32, 8, 1); else LAUNCH(F32, 8, 2); \
-  } else if (s.v == 1) {                            \
-    LAUNCH(F32, 1, 1);                              \
-  } else if (s.v == 4) {                            \
-    LAUNCH(F32, 1, 4);                              \
-  } else {                                          \
-    LAUNCH(F32, 1, 16);                             \
+// The kernels' instances: the residual's type, 8 columns a thread in up to 512 or 1024 threads or 16 in up to
+// 1024 (fewer threads leave each more registers), whole rows of eights or not, the gate.
+#define WM_NORM_GATES(KERNEL, F, V, W, N, ...)                                                          \
+  switch (gate) {                                                                                      \
+    case GATE_NONE: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_NONE, N>), __VA_ARGS__); break;           \
+    case GATE_TOKEN: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_TOKEN, N>), __VA_ARGS__); break;         \
+    case GATE_CHANNEL: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_CHANNEL, N>), __VA_ARGS__); break;     \
+    case GATE_FULL: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_FULL, N>), __VA_ARGS__); break;           \
+    default: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_FULL_F32, N>), __VA_ARGS__);                     \
   }
+#define WM_NORM_WHOLE(KERNEL, F, V, N, ...)                              \
+  if (a.hidden % 8 == 0) { WM_NORM_GATES(KERNEL, F, V, true, N, __VA_ARGS__) } \
+  else { WM_NORM_GATES(KERNEL, F, V, false, N, __VA_ARGS__) }
+#define WM_NORM_SHAPES(KERNEL, F, ...)                                                   \
+  if (shape.v == 2) { WM_NORM_WHOLE(KERNEL, F, 2, 1024, __VA_ARGS__) }                   \
+  else if (shape.threads > 512) { WM_NORM_WHOLE(KERNEL, F, 1, 1024, __VA_ARGS__) }       \
+  else { WM_NORM_WHOLE(KERNEL, F, 1, 512, __VA_ARGS__) }
+#define WM_NORM_LAUNCH(KERNEL, ...)                                                       \
+  const NormShape shape = norm_shape(a.hidden);                                           \
+  const int gate = a.gate_kind == GATE_FULL && a.gate_f32 ? GATE_FULL_F32 : a.gate_kind;  \
+  const dim3 threads(shape.threads);                                                      \
+  if (f32) { WM_NORM_SHAPES(KERNEL, true, __VA_ARGS__) } else { WM_NORM_SHAPES(KERNEL, false, __VA_ARGS__) }
+
+static void norm_forward(const NormArgs& a, bool f32, void* residual_out, uint16_t* x, hipStream_t s) {
+  const dim3 blocks((unsigned)norm_blocks(a.tokens, a.hidden, 64));
+  WM_NORM_LAUNCH(block_norm_kernel, blocks, threads, 0, s, a, residual_out, x)
+  check_launch("block_norm");
+}
+
+static void norm_grad(const NormArgs& a, bool f32, const NormGrads& d, int grid, hipStream_t s) {
+  const dim3 blocks((unsigned)grid);
+  WM_NORM_LAUNCH(block_norm_grad_kernel, blocks, threads, 0, s, a, d)
+  check_launch("block_norm_grad");
+}
 
 }  // namespace wm
 
@@ -402,25 +495,14 @@ WM_EXPORT int wm_block_norm(const wm_block_norm_form* form, const void* residual
     const NormArgs a = norm_args("wm_block_norm", form, residual, y, tokens, hidden);
     if (tokens == 0) return;
     if (!residual_out || !x) fail("wm_block_norm: null pointer");
-    const NormShape s = norm_shape(hidden, norm_aligned("wm_block_norm", form, hidden, {y, x}, {residual, residual_out}, nullptr,
-                                                        nullptr));
-    const unsigned blocks = (unsigned)(tokens < 2048 ? tokens : 2048);
-#define WM_NORM(F, VEC, V)                                                                                          \
-  hipLaunchKernelGGL((block_norm_kernel<F, VEC, V>), dim3(blocks), dim3(s.threads), 0, as_stream(stream), a, residual_out, \
-                     (uint16_t*)x)
-    if (form->residual_fp32) {
-      WM_NORM_SHAPES(true, WM_NORM)
-    } else {
-      WM_NORM_SHAPES(false, WM_NORM)
-    }
-#undef WM_NORM
-    check_launch("block_norm");
+    norm_aligned("wm_block_norm", form, {y, x}, {residual, residual_out}, {}, nullptr);
+    norm_forward(a, form->residual_fp32 != 0, residual_out, (uint16_t*)x, as_stream(stream));
   });
 }
 
 WM_EXPORT size_t wm_block_norm_backward_workspace_size(int32_t tokens, int32_t hidden) {
-  if (tokens < 0 || hidden < 1) return 0;
-  return (size_t)norm_grad_blocks(tokens) * 3 * hidden * sizeof(float);
+  if (tokens < 0 || hidden < 1 || hidden > NORM_MAX_HIDDEN) return 0;
+  return (size_t)norm_grad_blocks(tokens, hidden) * 3 * hidden * sizeof(float);
 }
 
 WM_EXPORT int wm_block_norm_backward(const wm_block_norm_form* form, const void* dx, const void* dresidual_out,
@@ -435,28 +517,17 @@ WM_EXPORT int wm_block_norm_backward(const wm_block_norm_form* form, const void*
     if (tokens > 0 && (!dx || !dresidual || !dy || !workspace)) fail("wm_block_norm_backward: null pointer");
     if (workspace_bytes < wm_block_norm_backward_workspace_size(tokens, hidden) || (uintptr_t)workspace % 16)
       fail("wm_block_norm_backward: workspace too small or misaligned");
-    const bool wide = norm_aligned("wm_block_norm_backward", form, hidden, {y, dx, dy}, {residual_out, dresidual_out, dresidual},
-                                   (const void*)((uintptr_t)dpost_weight | (uintptr_t)dpre_weight |
-                                                 (form->gate_kind == GATE_FULL ? 0 : (uintptr_t)dgate)),
-                                   form->gate_kind == GATE_FULL ? dgate : nullptr);
-    const NormShape s = norm_shape(hidden, wide);
-    const int blocks = norm_grad_blocks(tokens);
+    norm_aligned("wm_block_norm_backward", form, {y, dx, dy}, {residual_out, dresidual_out, dresidual},
+                 {dpost_weight, dpre_weight, form->gate_kind == GATE_FULL ? nullptr : dgate},
+                 form->gate_kind == GATE_FULL ? dgate : nullptr);
+    const int blocks = norm_grad_blocks(tokens, hidden);
     const NormGrads d = {(const uint16_t*)dx, dresidual_out, dresidual, (uint16_t*)dy, dgate, (float*)workspace};
-    if (blocks > 0) {
-#define WM_NORM(F, VEC, V) \
-  hipLaunchKernelGGL((block_norm_grad_kernel<F, VEC, V>), dim3(blocks), dim3(s.threads), 0, as_stream(stream), a, d)
-      if (form->residual_fp32) {
-        WM_NORM_SHAPES(true, WM_NORM)
-      } else {
-        WM_NORM_SHAPES(false, WM_NORM)
-      }
-#undef WM_NORM
-      check_launch("block_norm_grad");
-    }
+    hipStream_t s = as_stream(stream);
+    if (blocks > 0) norm_grad(a, form->residual_fp32 != 0, d, blocks, s);
     float* dchannel = form->gate_kind == GATE_CHANNEL ? (float*)dgate : nullptr;
     if (dpost_weight || dpre_weight || dchannel) {
-      hipLaunchKernelGGL(norm_columns_kernel, dim3((hidden + 15) / 16, 3), dim3(256), 0, as_stream(stream), d.partial, blocks,
-                         hidden, dpost_weight, dpre_weight, dchannel);
+      hipLaunchKernelGGL(norm_columns_kernel, dim3((hidden + 63) / 64, 3), dim3(1024), 0, s, d.partial, blocks, hidden,
+                         dpost_weight, dpre_weight, dchannel);
       check_launch("norm_columns");
     }
   });

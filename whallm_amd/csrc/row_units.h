@@ -28,8 +28,10 @@ __device__ __forceinline__ wm_u32x2 load8(const void* p) {
   return *(const __attribute__((address_space(1))) wm_u32x2_any*)(p);
 }
 
+// Two fp32 to bf16, to nearest even, by the one instruction that does it (V_CVT_PK_BF16_F32).
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  return f32_to_bf16_bits(lo) | ((uint32_t)f32_to_bf16_bits(hi) << 16);
+  const wm_bf16x2 v = {(__bf16)lo, (__bf16)hi};
+  return bf16x2_to_bits(v);
 }
 
 // Sixteen bytes of a row (WIDE) or one element.
@@ -68,7 +70,7 @@ struct RowUnit<false, false> {
   static __device__ __forceinline__ void store(Elem* p, Raw v) { *p = v; }
   static __device__ __forceinline__ void store_once(Elem* p, Raw v) { *p = v; }
   static __device__ __forceinline__ void unpack(Raw v, float f[N]) { f[0] = bf16_bits_to_f32(v); }
-  static __device__ __forceinline__ Raw pack(const float f[N]) { return f32_to_bf16_bits(f[0]); }
+  static __device__ __forceinline__ Raw pack(const float f[N]) { return (Raw)pack_bf16(f[0], 0.0f); }
 };
 
 template <>
