@@ -306,7 +306,9 @@ def permute(indices: torch.Tensor, experts: int, tile_rows: int = 128) -> Permut
 
 # ----------------------------------------------------------------------------- token rows to experts and back
 
-# The handle of a device's current stream without the Stream object around it (1.7 us of a call).
+# A few microseconds on the GPU are this module's small calls, so they are written for the host's time: the
+# handle of a device's current stream without the Stream object around it (1.7 us), empty_like or sizes as
+# arguments rather than torch.empty of a shape (1.6 us).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -327,9 +329,12 @@ def _at(t: torch.Tensor | None) -> int | None:
 
 def _no_autograd(name: str, *tensors: torch.Tensor | None) -> None:
     """Refuses inputs whose gradient would be lost: these calls are not recorded by autograd."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        how = "it has no gradient" if name.endswith("_backward") else f"its gradients are {name}_backward's"
-        raise ValueError(f"{name} is not recorded by autograd ({how}): call it under torch.no_grad()")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            how = "it has no gradient" if name.endswith("_backward") else f"its gradients are {name}_backward's"
+            raise ValueError(f"{name} is not recorded by autograd ({how}): call it under torch.no_grad()")
 
 
 def _rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
@@ -375,14 +380,15 @@ def sort_tokens(x: torch.Tensor, indices: torch.Tensor, experts: int,
     max_tiles = -(-P // tile_rows) + experts
     ws_bytes = _lib.load().wm_sort_tokens_workspace_size(T, k, experts)
     rows = torch.empty(P, H, dtype=x.dtype, device=device)
-    # the lists and the workspace in one allocation, tiles first (8-byte aligned)
-    tiles, order, inverse, offsets, count, ws = torch.empty(
-        2 * max_tiles + 2 * P + experts + 2 + -(-ws_bytes // 4), dtype=torch.int32, device=device).split(
-        [2 * max_tiles, P, P, experts + 1, 1, -(-ws_bytes // 4)])
+    tiles = torch.empty(max_tiles, 2, dtype=torch.int32, device=device)
+    words = -(-ws_bytes // 4)
+    # the other lists and the workspace in one allocation
+    lists = torch.empty(2 * P + experts + 2 + words, dtype=torch.int32, device=device)
+    order, inverse, offsets, count, ws = lists.split_with_sizes([P, P, experts + 1, 1, words])
     _launch(device, "wm_sort_tokens", x.data_ptr(), int(x.dtype == torch.float32), T, H, indices.data_ptr(), k, experts,
             tile_rows, rows.data_ptr(), order.data_ptr(), inverse.data_ptr(), offsets.data_ptr(), tiles.data_ptr(),
-            count.data_ptr(), ws.data_ptr(), ws_bytes)
-    return rows, Permutation(order, inverse, offsets, tiles.view(max_tiles, 2), count)
+            count.data_ptr(), ws.data_ptr() if words else None, ws_bytes)
+    return rows, Permutation(order, inverse, offsets, tiles, count)
 
 
 def sort_tokens_backward(drows: torch.Tensor, permutation: Permutation, k: int) -> torch.Tensor:
@@ -418,7 +424,7 @@ def combine_rows(rows: torch.Tensor, weights: torch.Tensor, permutation: Permuta
         add = _rows(add, "add", rows)
         if add.shape != shape:
             raise ValueError("add must be [.., H] matching weights")
-    y = torch.empty(shape, dtype=rows.dtype, device=device)
+    y = torch.empty(*shape, dtype=rows.dtype, device=device) if add is None else torch.empty_like(add)
     _launch(device, "wm_combine_rows", rows.data_ptr(), int(rows.dtype == torch.float32), weights.data_ptr(),
             permutation.inverse.data_ptr(), T, k, H, _at(add), y.data_ptr())
     return y
@@ -703,26 +709,28 @@ def _norm_form(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, 
         raise ValueError("eps must not be negative")
     if post_weight is not None:
         post_weight = _contig(post_weight, torch.bfloat16, "post_weight")
+        if post_weight.dim() != 1 or post_weight.numel() != H:
+            raise ValueError("weights must be [H]")
     if pre_weight is not None:
         pre_weight = _contig(pre_weight, torch.bfloat16, "pre_weight")
-    if any(w is not None and w.shape != (H,) for w in (post_weight, pre_weight)):
-        raise ValueError("weights must be [H]")
+        if pre_weight.dim() != 1 or pre_weight.numel() != H:
+            raise ValueError("weights must be [H]")
     kind = 0
     if gate is not None:
         if gate.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"gate must be float32 or bfloat16, got {gate.dtype}")
-        if gate.shape == (H,):
+        if gate.dim() == 1 and gate.shape[0] == H:
             kind = 2
+        elif gate.shape == residual.shape:
+            kind = 3 if H > 1 else 1
         elif gate.shape == (*residual.shape[:-1], 1):
             kind = 1
-        elif gate.shape == residual.shape:
-            kind = 3
         else:
             raise ValueError("gate must be [H], [.., 1] or [.., H]")
         gate = gate.contiguous()
-    form = _lib.BlockNormFormC(_at(post_weight), _at(pre_weight), _at(gate), weight_offset, scale, eps, int(post_norm), kind,
-                               int(gate is not None and gate.dtype == torch.float32), int(bool(gate_sigmoid)),
-                               int(residual.dtype == torch.float32))
+    form = _lib.BlockNormFormC(_at(post_weight), _at(pre_weight), _at(gate), weight_offset, scale, eps, bool(post_norm), kind,
+                               gate is not None and gate.dtype == torch.float32, bool(gate_sigmoid),
+                               residual.dtype == torch.float32)
     return form, y, post_weight, pre_weight, gate, kind
 
 
@@ -741,13 +749,14 @@ def block_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Tenso
     _no_autograd("block_norm", residual, y, post_weight, pre_weight, gate)
     form, y, post_weight, pre_weight, gate, _ = _norm_form(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, eps,
                                                            weight_offset, post_norm)
-    if residual_out is None:
-        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=device)
-    elif residual_out.dtype != residual.dtype or residual_out.shape != residual.shape or not residual_out.is_contiguous():
+    if residual_out is not None and (residual_out.dtype != residual.dtype or residual_out.shape != residual.shape
+                                     or not residual_out.is_contiguous()):
         raise ValueError("residual_out must be a contiguous tensor shaped and typed like residual")
     residual = residual.contiguous()
+    if residual_out is None:
+        residual_out = torch.empty_like(residual)
     H = residual.shape[-1]
-    x = torch.empty(residual.shape, dtype=torch.bfloat16, device=device)
+    x = torch.empty_like(y)
     _launch(device, "wm_block_norm", form, residual.data_ptr(), y.data_ptr(), residual.numel() // H, H,
             residual_out.data_ptr(), x.data_ptr())
     return x, residual_out
@@ -1108,10 +1117,11 @@ def _row_lists(t: torch.Tensor, rows: int, name: str) -> tuple[torch.Tensor, int
 def _row_values(t: torch.Tensor | None, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor | None:
     if t is None:
         return None
-    t = _contig(t, dtype, name)
-    if t.shape != (rows,):
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 1 or t.numel() != rows:
         raise ValueError(f"{name} must be [rows]")
-    return t
+    return t.contiguous()
 
 
 def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
@@ -1136,10 +1146,12 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, vocab]")
     R, V = logits.shape
-    lengths, prompt_lengths = (_row_values(t, R, torch.int32, n) for t, n in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths")))
-    repetition, frequency, presence, temperature = (
-        _row_values(t, R, torch.float32, n) for t, n in ((repetition, "repetition"), (frequency, "frequency"),
-                                                         (presence, "presence"), (temperature, "temperature")))
+    lengths = _row_values(lengths, R, torch.int32, "lengths")
+    prompt_lengths = _row_values(prompt_lengths, R, torch.int32, "prompt_lengths")
+    repetition = _row_values(repetition, R, torch.float32, "repetition")
+    frequency = _row_values(frequency, R, torch.float32, "frequency")
+    presence = _row_values(presence, R, torch.float32, "presence")
+    temperature = _row_values(temperature, R, torch.float32, "temperature")
     history_stride = history_len = biases = bias_stride = mask_stride = 0
     if history is not None:
         history, history_stride = _row_lists(_contig(history, torch.int32, "history"), R, "history")
