@@ -204,5 +204,27 @@ def call(name: str, *args) -> None:
         raise kind(f"{name}: {lib.wm_last_error().decode(errors='replace')}")
 
 
+_host_calls = None
+
+
+def host_calls():
+    """The compiled host side of the small calls (csrc/host_calls.cpp), linked to the same library;
+    raises when it is not built or cannot load."""
+    global _host_calls
+    if _host_calls is None:
+        import importlib.util
+
+        from .build import host_calls_path
+        load()
+        path = host_calls_path()
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m whallm_amd.build`")
+        spec = importlib.util.spec_from_file_location("_host_calls", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _host_calls = module
+    return _host_calls
+
+
 def exported_symbols() -> list[str]:
     return sorted(_SIGNATURES)

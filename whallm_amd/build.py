@@ -76,40 +76,61 @@ def build(force: bool = False, jobs: int | None = None) -> Path:
 
 
 HOST_META_SRC = CSRC / "host_meta.cpp"
+HOST_CALLS_SRC = CSRC / "host_calls.cpp"
 
 
-def host_meta_path() -> Path:
-    """Where the operator mirrors' host helper (csrc/host_meta.cpp) is built."""
+def _extension_path(module: str) -> Path:
     import sysconfig
-    return LIB.parent / ("_host_meta" + sysconfig.get_config_var("EXT_SUFFIX"))
+    return LIB.parent / (module + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def build_host_meta(force: bool = False) -> Path:
-    """Compile csrc/host_meta.cpp into a CPython extension against the installed torch (host
-    code only, g++); returns its path."""
+def _build_extension(source: Path, module: str, force: bool, link: list[str] = ()) -> Path:
+    """A CPython extension against the installed torch (host code only, g++); returns its path."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
-    out = host_meta_path()
-    if not force and out.exists() and out.stat().st_mtime >= HOST_META_SRC.stat().st_mtime:
+    out = _extension_path(module)
+    newest = max(source.stat().st_mtime, *(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
+    if not force and out.exists() and out.stat().st_mtime >= newest:
         return out
     LIB.parent.mkdir(exist_ok=True)
     tmp = out.with_name(out.name + ".tmp")
-    cmd = ["g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-DTORCH_EXTENSION_NAME=_host_meta",
+    cmd = ["g++", "-O2", "-shared", "-fPIC", "-std=c++17", f"-DTORCH_EXTENSION_NAME={module}",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in cpp_extension.include_paths()], f"-I{sysconfig.get_paths()['include']}",
-           str(HOST_META_SRC), "-o", str(tmp),
-           *[f"-L{p}" for p in cpp_extension.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+           str(source), "-o", str(tmp),
+           *[f"-L{p}" for p in cpp_extension.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", *link]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"g++ failed on {HOST_META_SRC.name}:\n{result.stderr}")
+        raise RuntimeError(f"g++ failed on {source.name}:\n{result.stderr}")
     os.replace(tmp, out)
     return out
+
+
+def host_meta_path() -> Path:
+    """Where the operator mirrors' host helper (csrc/host_meta.cpp) is built."""
+    return _extension_path("_host_meta")
+
+
+def build_host_meta(force: bool = False) -> Path:
+    return _build_extension(HOST_META_SRC, "_host_meta", force)
+
+
+def host_calls_path() -> Path:
+    """Where the host side of the small calls (csrc/host_calls.cpp) is built."""
+    return _extension_path("_host_calls")
+
+
+def build_host_calls(force: bool = False) -> Path:
+    """Linked against the library beside it, which is built first."""
+    return _build_extension(HOST_CALLS_SRC, "_host_calls", force,
+                            [f"-L{LIB.parent}", "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN"])
 
 
 if __name__ == "__main__":
     path = build(force="--force" in sys.argv)
     print(path)
     print(build_host_meta(force="--force" in sys.argv))
+    print(build_host_calls(force="--force" in sys.argv))

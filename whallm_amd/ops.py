@@ -305,58 +305,11 @@ def permute(indices: torch.Tensor, experts: int, tile_rows: int = 128) -> Permut
 
 
 # ----------------------------------------------------------------------------- token rows to experts and back
-
-# A few microseconds on the GPU are this module's small calls, so they are written for the host's time: the
-# handle of a device's current stream without the Stream object around it (1.7 us), empty_like or sizes as
-# arguments rather than torch.empty of a shape (1.6 us).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _launch(device: torch.device, name: str, *args) -> None:
-    """One call on ``device``'s current stream (its last argument), whatever the current device is."""
-    stream = _raw_stream(device.index)
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, stream)
-    else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, stream)
-
-
-def _at(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
-
-
-def _no_autograd(name: str, *tensors: torch.Tensor | None) -> None:
-    """Refuses inputs whose gradient would be lost: these calls are not recorded by autograd."""
-    if not torch.is_grad_enabled():
-        return
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            how = "it has no gradient" if name.endswith("_backward") else f"its gradients are {name}_backward's"
-            raise ValueError(f"{name} is not recorded by autograd ({how}): call it under torch.no_grad()")
-
-
-def _rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
-    if t.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{name} must be bfloat16 or float32, got {t.dtype}")
-    if like is not None and t.dtype != like.dtype:
-        raise ValueError(f"{name} must be {like.dtype} like the other rows, got {t.dtype}")
-    return t.contiguous()
-
-
-def _pair_rows(rows: torch.Tensor, permutation: Permutation, k: int) -> int:
-    """The tokens of rows [T * K, H] in the order of ``permutation``."""
-    if rows.dim() != 2:
-        raise ValueError("rows must be [tokens * k, hidden]")
-    pairs = rows.shape[0]
-    inverse = permutation.inverse
-    if k < 1 or pairs % k:
-        raise ValueError("rows must hold k rows of every token")
-    if inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.numel() != pairs:
-        raise ValueError("the permutation is not that of these rows")
-    return pairs // k
-
+#
+# These calls, the block norms and process_logits take a few microseconds on the GPU: their checks, outputs and
+# launches are compiled (csrc/host_calls.cpp). They run on the tensors' device, whatever the current one is, and
+# on its current stream. None is recorded by autograd: inputs that require gradients are refused outside
+# torch.no_grad(), and each backward function gives the gradients.
 
 def sort_tokens(x: torch.Tensor, indices: torch.Tensor, experts: int,
                 tile_rows: int = 128) -> tuple[torch.Tensor, Permutation]:
@@ -364,44 +317,14 @@ def sort_tokens(x: torch.Tensor, indices: torch.Tensor, experts: int,
     expert order, the Permutation of ``permute``): expert e's tokens are rows[offsets[e]:offsets[e + 1]].
     A pair whose id is no expert (padding, not resident) has no row; the rows behind the last pair are zero,
     ``order`` and ``tiles`` -1 behind their ends (wm_sort_tokens)."""
-    device = _require_device(x, indices)
-    _no_autograd("sort_tokens", x)
-    x = _rows(x, "x")
-    if x.dim() < 1 or indices.dim() != x.dim() or indices.shape[:-1] != x.shape[:-1]:
-        raise ValueError("indices must be [.., K] for x [.., H]")
-    if indices.dtype != torch.int32:
-        raise ValueError(f"indices must be {torch.int32}, got {indices.dtype}")
-    indices = indices.contiguous()
-    H, k = x.shape[-1], indices.shape[-1]
-    if H < 1 or k < 1 or experts < 1 or tile_rows < 1:
-        raise ValueError("hidden, k, experts and tile_rows must be positive")
-    T = x.numel() // H
-    P = T * k
-    max_tiles = -(-P // tile_rows) + experts
-    ws_bytes = _lib.load().wm_sort_tokens_workspace_size(T, k, experts)
-    rows = torch.empty(P, H, dtype=x.dtype, device=device)
-    tiles = torch.empty(max_tiles, 2, dtype=torch.int32, device=device)
-    words = -(-ws_bytes // 4)
-    # the other lists and the workspace in one allocation
-    lists = torch.empty(2 * P + experts + 2 + words, dtype=torch.int32, device=device)
-    order, inverse, offsets, count, ws = lists.split_with_sizes([P, P, experts + 1, 1, words])
-    _launch(device, "wm_sort_tokens", x.data_ptr(), int(x.dtype == torch.float32), T, H, indices.data_ptr(), k, experts,
-            tile_rows, rows.data_ptr(), order.data_ptr(), inverse.data_ptr(), offsets.data_ptr(), tiles.data_ptr(),
-            count.data_ptr(), ws.data_ptr() if words else None, ws_bytes)
-    return rows, Permutation(order, inverse, offsets, tiles, count)
+    rows, *lists = _lib.host_calls().sort_tokens(x, indices, experts, tile_rows)
+    return rows, Permutation(*lists)
 
 
 def sort_tokens_backward(drows: torch.Tensor, permutation: Permutation, k: int) -> torch.Tensor:
     """The gradient of sort_tokens: drows [T * K, H] -> dx [T, H] = the sum over each token's rows, fp32 in k
     order, rounded once to drows' type (wm_sort_tokens_backward)."""
-    device = _require_device(drows, permutation.inverse)
-    _no_autograd("sort_tokens_backward", drows)
-    drows = _rows(drows, "drows")
-    T, H = _pair_rows(drows, permutation, k), drows.shape[1]
-    dx = torch.empty(T, H, dtype=drows.dtype, device=device)
-    _launch(device, "wm_sort_tokens_backward", drows.data_ptr(), int(drows.dtype == torch.float32),
-            permutation.inverse.data_ptr(), T, k, H, dx.data_ptr())
-    return dx
+    return _lib.host_calls().sort_tokens_backward(drows, permutation.inverse, k)
 
 
 def combine_rows(rows: torch.Tensor, weights: torch.Tensor, permutation: Permutation,
@@ -409,25 +332,7 @@ def combine_rows(rows: torch.Tensor, weights: torch.Tensor, permutation: Permuta
     """The expert products' rows [T * K, H] (bf16 or fp32, in expert order) back to their tokens:
     y[.., :] = sum_k weights[.., k] * rows[inverse] (+ add), fp32 in k order, rounded once; weights fp32
     [.., K], y and add [.., H] in rows' type (wm_combine_rows; combine_pairs takes rows in router order)."""
-    device = _require_device(rows, weights, permutation.inverse, add)
-    _no_autograd("combine_rows", rows, weights, add)
-    rows = _rows(rows, "rows")
-    weights = _contig(weights, torch.float32, "weights")
-    if weights.dim() < 1:
-        raise ValueError("weights must be [.., K]")
-    k = weights.shape[-1]
-    T, H = _pair_rows(rows, permutation, k), rows.shape[1]
-    if weights.numel() != T * k:
-        raise ValueError("weights must be [.., K] matching rows")
-    shape = (*weights.shape[:-1], H)
-    if add is not None:
-        add = _rows(add, "add", rows)
-        if add.shape != shape:
-            raise ValueError("add must be [.., H] matching weights")
-    y = torch.empty(*shape, dtype=rows.dtype, device=device) if add is None else torch.empty_like(add)
-    _launch(device, "wm_combine_rows", rows.data_ptr(), int(rows.dtype == torch.float32), weights.data_ptr(),
-            permutation.inverse.data_ptr(), T, k, H, _at(add), y.data_ptr())
-    return y
+    return _lib.host_calls().combine_rows(rows, weights, permutation.inverse, add)
 
 
 def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor,
@@ -435,25 +340,7 @@ def combine_rows_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.T
     """The gradients of combine_rows from dy [.., H]: (drows [T * K, H] in rows' type, zero behind the last
     pair; dweights fp32 [.., K], 0 where a pair has no row). The gradient of ``add`` is dy itself
     (wm_combine_rows_backward)."""
-    device = _require_device(dy, rows, weights, permutation.inverse, permutation.offsets)
-    _no_autograd("combine_rows_backward", dy, rows, weights)
-    rows = _rows(rows, "rows")
-    dy = _rows(dy, "dy", rows)
-    weights = _contig(weights, torch.float32, "weights")
-    if weights.dim() < 1:
-        raise ValueError("weights must be [.., K]")
-    k = weights.shape[-1]
-    T, H = _pair_rows(rows, permutation, k), rows.shape[1]
-    if weights.numel() != T * k or dy.shape != (*weights.shape[:-1], H):
-        raise ValueError("dy must be [.., H] and weights [.., K] matching rows")
-    offsets = permutation.offsets
-    if offsets.dtype != torch.int32 or not offsets.is_contiguous() or offsets.numel() < 1:
-        raise ValueError("the permutation's offsets must be contiguous int32")
-    drows, dweights = torch.empty_like(rows), torch.empty_like(weights)
-    _launch(device, "wm_combine_rows_backward", dy.data_ptr(), rows.data_ptr(), int(rows.dtype == torch.float32),
-            weights.data_ptr(), permutation.inverse.data_ptr(), offsets.data_ptr() + 4 * (offsets.numel() - 1), T, k, H,
-            drows.data_ptr(), dweights.data_ptr())
-    return drows, dweights
+    return _lib.host_calls().combine_rows_backward(dy, rows, weights, permutation.inverse, permutation.offsets)
 
 
 # ----------------------------------------------------------------------------- expert FFN
@@ -693,47 +580,6 @@ def residual_rmsnorm(residual: torch.Tensor, y: torch.Tensor | None, eps: float 
     return x
 
 
-def _norm_form(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, eps, weight_offset, post_norm):
-    """The checked wm_block_norm_form and the contiguous (y, weights, gate) it points to."""
-    if residual.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"residual must be float32 or bfloat16, got {residual.dtype}")
-    if residual.dim() < 1 or residual.shape[-1] < 1:
-        raise ValueError("residual must be [.., H]")
-    H = residual.shape[-1]
-    y = _contig(y, torch.bfloat16, "y")
-    if y.shape != residual.shape:
-        raise ValueError("y must match residual")
-    if post_weight is not None and not post_norm:
-        raise ValueError("post_weight needs post_norm")
-    if not eps >= 0:
-        raise ValueError("eps must not be negative")
-    if post_weight is not None:
-        post_weight = _contig(post_weight, torch.bfloat16, "post_weight")
-        if post_weight.dim() != 1 or post_weight.numel() != H:
-            raise ValueError("weights must be [H]")
-    if pre_weight is not None:
-        pre_weight = _contig(pre_weight, torch.bfloat16, "pre_weight")
-        if pre_weight.dim() != 1 or pre_weight.numel() != H:
-            raise ValueError("weights must be [H]")
-    kind = 0
-    if gate is not None:
-        if gate.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"gate must be float32 or bfloat16, got {gate.dtype}")
-        if gate.dim() == 1 and gate.shape[0] == H:
-            kind = 2
-        elif gate.shape == residual.shape:
-            kind = 3 if H > 1 else 1
-        elif gate.shape == (*residual.shape[:-1], 1):
-            kind = 1
-        else:
-            raise ValueError("gate must be [H], [.., 1] or [.., H]")
-        gate = gate.contiguous()
-    form = _lib.BlockNormFormC(_at(post_weight), _at(pre_weight), _at(gate), weight_offset, scale, eps, bool(post_norm), kind,
-                               gate is not None and gate.dtype == torch.float32, bool(gate_sigmoid),
-                               residual.dtype == torch.float32)
-    return form, y, post_weight, pre_weight, gate, kind
-
-
 def block_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Tensor | None = None,
                pre_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_sigmoid: bool = False,
                scale: float = 1.0, eps: float = 1e-6, weight_offset: float = 0.0, post_norm: bool = True,
@@ -745,21 +591,8 @@ def block_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Tenso
     residual [.., H] fp32 or bf16, y [.., H] bf16, weights bf16 [H] (None: the norm alone); ``gate`` fp32 or bf16:
     [H], one value a token [.., 1], or [.., H], through a sigmoid with ``gate_sigmoid`` (norm_router's shared
     logit as [.., 1]). ``residual_out`` receives residual' and may be the residual itself."""
-    device = _require_device(residual, y, post_weight, pre_weight, gate, residual_out)
-    _no_autograd("block_norm", residual, y, post_weight, pre_weight, gate)
-    form, y, post_weight, pre_weight, gate, _ = _norm_form(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, eps,
-                                                           weight_offset, post_norm)
-    if residual_out is not None and (residual_out.dtype != residual.dtype or residual_out.shape != residual.shape
-                                     or not residual_out.is_contiguous()):
-        raise ValueError("residual_out must be a contiguous tensor shaped and typed like residual")
-    residual = residual.contiguous()
-    if residual_out is None:
-        residual_out = torch.empty_like(residual)
-    H = residual.shape[-1]
-    x = torch.empty_like(y)
-    _launch(device, "wm_block_norm", form, residual.data_ptr(), y.data_ptr(), residual.numel() // H, H,
-            residual_out.data_ptr(), x.data_ptr())
-    return x, residual_out
+    return _lib.host_calls().block_norm(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, eps, weight_offset,
+                                        post_norm, residual_out)
 
 
 @dataclass
@@ -779,29 +612,8 @@ def block_norm_backward(dx: torch.Tensor, dresidual: torch.Tensor | None, residu
     """The gradients of block_norm from those of x (``dx``, bf16) and residual' (``dresidual``, in its type; None:
     zero), given the residual' that the forward pass returned and its other inputs (wm_block_norm_backward).
     The weights' gradients and a gate's of [H] or [.., 1] are fp32, a [.., H] gate's has the gate's type."""
-    device = _require_device(dx, dresidual, residual_out, y, post_weight, pre_weight, gate)
-    _no_autograd("block_norm_backward", dx, dresidual, residual_out, y, post_weight, pre_weight, gate)
-    form, y, post_weight, pre_weight, gate, kind = _norm_form(residual_out, y, post_weight, pre_weight, gate, gate_sigmoid,
-                                                              scale, eps, weight_offset, post_norm)
-    dx = _contig(dx, torch.bfloat16, "dx")
-    if dx.shape != residual_out.shape:
-        raise ValueError("dx must match residual_out")
-    if dresidual is not None:
-        if dresidual.dtype != residual_out.dtype or dresidual.shape != residual_out.shape:
-            raise ValueError("dresidual must be shaped and typed like residual_out")
-        dresidual = dresidual.contiguous()
-    residual_out = residual_out.contiguous()
-    H = residual_out.shape[-1]
-    T = residual_out.numel() // H
-    dr, dy = torch.empty_like(residual_out), torch.empty_like(y)
-    dpost = None if post_weight is None else torch.empty(H, dtype=torch.float32, device=device)
-    dpre = None if pre_weight is None else torch.empty(H, dtype=torch.float32, device=device)
-    dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype if kind == 3 else torch.float32, device=device)
-    ws_bytes = _lib.load().wm_block_norm_backward_workspace_size(T, H)
-    ws = _workspace(ws_bytes, device)
-    _launch(device, "wm_block_norm_backward", form, dx.data_ptr(), _at(dresidual), residual_out.data_ptr(), y.data_ptr(), T, H,
-            dr.data_ptr(), dy.data_ptr(), _at(dpost), _at(dpre), _at(dgate), ws.data_ptr(), ws_bytes)
-    return BlockNormGrads(dr, dy, dpost, dpre, dgate)
+    return BlockNormGrads(*_lib.host_calls().block_norm_backward(dx, dresidual, residual_out, y, post_weight, pre_weight, gate,
+                                                                 gate_sigmoid, scale, eps, weight_offset, post_norm))
 
 
 def repack_router(router: torch.Tensor, shared_gate: torch.Tensor | None = None) -> torch.Tensor:
@@ -1106,24 +918,6 @@ class PersistentDecodeStack:
 
 # ----------------------------------------------------------------------------- logits to acceptance
 
-def _row_lists(t: torch.Tensor, rows: int, name: str) -> tuple[torch.Tensor, int]:
-    """[rows, n], or [1, n] for a list that all rows share -> (contiguous, elements between rows)."""
-    if t.dim() != 2 or t.shape[0] not in (rows, 1):
-        raise ValueError(f"{name} must be [rows, n], or [1, n] for all rows")
-    t = t.contiguous()
-    return t, 0 if t.shape[0] == 1 else t.shape[1]
-
-
-def _row_values(t: torch.Tensor | None, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor | None:
-    if t is None:
-        return None
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 1 or t.numel() != rows:
-        raise ValueError(f"{name} must be [rows]")
-    return t.contiguous()
-
-
 def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
                    prompt_lengths: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
                    frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
@@ -1139,55 +933,8 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
     ``repetition`` sees. repetition, frequency, presence and temperature are fp32 [rows]; bias_ids int32 and
     bias_values fp32 [rows, n] or [1, n]; mask int32 [rows, ceil(V / 32)] or [1, ..], a set bit allows its token.
     Returns fp32 [rows, V]; ``out`` may be fp32 logits themselves."""
-    device = _require_device(logits, history, lengths, prompt_lengths, repetition, frequency, presence, bias_ids, bias_values,
-                             mask, temperature, out)
-    _no_autograd("process_logits", logits, bias_values)
-    logits = _rows(logits, "logits")
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError("logits must be [rows, vocab]")
-    R, V = logits.shape
-    lengths = _row_values(lengths, R, torch.int32, "lengths")
-    prompt_lengths = _row_values(prompt_lengths, R, torch.int32, "prompt_lengths")
-    repetition = _row_values(repetition, R, torch.float32, "repetition")
-    frequency = _row_values(frequency, R, torch.float32, "frequency")
-    presence = _row_values(presence, R, torch.float32, "presence")
-    temperature = _row_values(temperature, R, torch.float32, "temperature")
-    history_stride = history_len = biases = bias_stride = mask_stride = 0
-    if history is not None:
-        history, history_stride = _row_lists(_contig(history, torch.int32, "history"), R, "history")
-        history_len = history.shape[1]
-        if history_len == 0:
-            history = lengths = prompt_lengths = None
-    elif lengths is not None or prompt_lengths is not None:
-        raise ValueError("lengths need a history")
-    if (bias_ids is None) != (bias_values is None):
-        raise ValueError("bias_ids and bias_values go together")
-    if bias_ids is not None:
-        if bias_ids.shape != bias_values.shape:
-            raise ValueError("bias_ids and bias_values must have one shape")
-        bias_ids, bias_stride = _row_lists(_contig(bias_ids, torch.int32, "bias_ids"), R, "bias_ids")
-        bias_values = _contig(bias_values, torch.float32, "bias_values")
-        biases = bias_ids.shape[1]
-        if biases == 0:
-            bias_ids = bias_values = None
-    if mask is not None:
-        mask, mask_stride = _row_lists(_contig(mask, torch.int32, "mask"), R, "mask")
-        if mask.shape[1] != -(-V // 32):
-            raise ValueError("mask must hold a bit for every token, 32 in a word")
-    if out is None:
-        out = torch.empty(R, V, dtype=torch.float32, device=device)
-    elif out.dtype != torch.float32 or out.shape != (R, V) or not out.is_contiguous():
-        raise ValueError("out must be a contiguous float32 tensor shaped like logits")
-    rules = _lib.LogitRulesC(_at(history), history_stride, history_len, biases, _at(lengths), _at(prompt_lengths), _at(repetition),
-                             _at(frequency), _at(presence), _at(bias_ids), _at(bias_values), bias_stride, _at(mask), mask_stride,
-                             _at(temperature))
-    ws, ws_bytes = None, 0
-    if log_probs:
-        ws_bytes = _lib.load().wm_process_logits_workspace_size(R, V)
-        ws = _workspace(ws_bytes, device)
-    _launch(device, "wm_process_logits", logits.data_ptr(), int(logits.dtype == torch.float32), R, V, rules, int(bool(log_probs)),
-            out.data_ptr(), _at(ws), ws_bytes)
-    return out
+    return _lib.host_calls().process_logits(logits, history, lengths, prompt_lengths, repetition, frequency, presence, bias_ids,
+                                            bias_values, mask, temperature, log_probs, out)
 
 
 # ----------------------------------------------------------------------------- MTP acceptance
