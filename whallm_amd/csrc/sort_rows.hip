@@ -20,11 +20,16 @@ namespace wm {
 constexpr int SORT_MAX_K = 64;
 
 // ---- sort. A workgroup owns a chunk of tokens (256 pairs at most) and a range of units. It finds its
-// pairs' rows in LDS: the first row of each expert for this chunk, plus a pair's place among the chunk's
-// earlier pairs of its expert. Where the first rows come from is what differs:
-//   ONE   every workgroup counts all pairs itself, those before its chunk apart. One launch and no
-//         workspace, and the counting is repeated by every workgroup, so it is for few pairs.
-//   else  permute_count and permute_scan have left them in memory.
+// pairs' rows in LDS, and moves the tokens' units to them. Three ways to the rows, by the number of pairs:
+//   up to 256     (sort_few_kernel) a workgroup a token; each has all ids in LDS and counts, for each of its
+//                 pairs, the pairs before it in expert order. The token's units are on their way meanwhile.
+//   up to 32768   (sort_kernel<true>) every workgroup counts all pairs by expert, those before its chunk apart,
+//                 so it knows the first row of each expert for this chunk; a pair's row is that plus its
+//                 place among the chunk's earlier pairs of its expert. One launch and no workspace, the
+//                 counting repeated by every workgroup: with 32768 pairs of 512 values 17 us a call, three
+//                 launches 20; with 65536 pairs 33 against 28.
+//   more          (sort_kernel<false>) permute_count and permute_scan leave the first rows in memory.
+// One launch has one workgroup more, for the lists that belong to no pair.
 constexpr int SORT_THREADS = 512;
 constexpr int SORT_CHUNK = 256;
 
@@ -64,16 +69,158 @@ __device__ __forceinline__ int32_t sort_scan(int32_t v, int32_t* total) {
   return before + incl - v;
 }
 
+// Counts of all pairs by expert: before p0 in base, from p0 on in later. Every thread calls it; ends with a barrier.
+__device__ __forceinline__ void sort_count(const SortArgs& a, int64_t p0, int32_t* base, int32_t* later) {
+  const int64_t pairs = a.tokens * a.k;
+  for (int e = threadIdx.x; e < a.experts; e += SORT_THREADS) base[e] = later[e] = 0;
+  __syncthreads();
+  // 16 ids in flight a thread, by 16 bytes at any alignment
+  for (int64_t q0 = 4 * threadIdx.x; q0 < pairs; q0 += 16 * SORT_THREADS) {
+    int32_t e[4][4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int64_t q = q0 + b * 4 * SORT_THREADS;
+      if (q + 4 <= pairs) {
+        const wm_u32x4 v = load16(a.indices + q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[b][i] = (int32_t)v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[b][i] = q + i < pairs ? a.indices[q + i] : -1;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if ((uint32_t)e[b][i] < (uint32_t)a.experts)
+          atomicAdd(q0 + b * 4 * SORT_THREADS + i < p0 ? &base[e[b][i]] : &later[e[b][i]], 1);
+  }
+  __syncthreads();
+}
+
+// The lists that belong to no pair: offsets, tiles, their number. One workgroup; count and first are LDS of an
+// entry an expert.
+__device__ __forceinline__ void sort_lists(const SortArgs& a, int32_t* count, int32_t* first) {
+  __shared__ int32_t tile_start[PERMUTE_MAX_EXPERTS];
+  const int E = a.experts;
+  sort_count(a, 0, first, count);
+  const int e0 = 2 * threadIdx.x, e1 = e0 + 1;  // two experts a thread
+  const int32_t n0 = e0 < E ? count[e0] : 0, n1 = e1 < E ? count[e1] : 0;
+  int32_t present, tiles;
+  const int32_t row = sort_scan(n0 + n1, &present);
+  const int32_t t0 = (n0 + a.tile_rows - 1) / a.tile_rows, t1 = (n1 + a.tile_rows - 1) / a.tile_rows;
+  const int32_t tile = sort_scan(t0 + t1, &tiles);
+  if (e0 < E) a.offsets[e0] = first[e0] = row, tile_start[e0] = tile;
+  if (e1 < E) a.offsets[e1] = first[e1] = row + n0, tile_start[e1] = tile + t0;
+  if (threadIdx.x == 0) {
+    a.offsets[E] = present;
+    a.tile_count[0] = tiles;
+  }
+  __syncthreads();
+  // Tile i belongs to the last expert whose first tile is <= i: experts without tiles share their start with
+  // the next one that has some, and come before it.
+  for (int64_t i = threadIdx.x; i < a.max_tiles; i += SORT_THREADS) {
+    int2 t = make_int2(-1, -1);
+    if (i < tiles) {
+      int lo = 0, hi = E - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tile_start[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      t = make_int2(lo, first[lo] + ((int32_t)i - tile_start[lo]) * a.tile_rows);
+    }
+    reinterpret_cast<int2*>(a.tiles)[i] = t;
+  }
+}
+
+// One unit of a row: from x's element `at`, to the same place of k rows.
+template <typename Unit>
+__device__ __forceinline__ void sort_store(uint16_t* rows, int64_t length, int64_t at, const int32_t* row, int k,
+                                           typename Unit::Raw v) {
+#pragma unroll 4
+  for (int j = 0; j < k; ++j)
+    if (row[j] >= 0) Unit::store_once(rows + row[j] * length + at, v);
+}
+
+// Zeros in the rows from `present` on, every step-th from the me-th, units c0 .. c1.
+__device__ __forceinline__ void sort_clear(const SortArgs& a, int32_t present, int64_t me, int64_t step, int c0, int c1) {
+  uint16_t* rows = (uint16_t*)a.rows;
+  for (int64_t r = present + me; r < a.tokens * a.k; r += step) {
+    for (int c = c0 + threadIdx.x; c < c1; c += SORT_THREADS) {
+      if (c < a.row.wide) store16_nt(rows + r * a.length + 8 * (int64_t)c, wm_u32x4{0, 0, 0, 0});
+      else rows[r * a.length + 8 * (int64_t)a.row.wide + c - a.row.wide] = 0;
+    }
+  }
+}
+
+// A workgroup a token, and the last one for the lists; columns by SORT_THREADS units.
+__global__ void __launch_bounds__(SORT_THREADS) sort_few_kernel(SortArgs a) {
+  __shared__ int32_t scratch[2][PERMUTE_MAX_EXPERTS];
+  __shared__ int32_t row[SORT_MAX_K], present_;
+  if (blockIdx.x == a.tokens) {
+    if (blockIdx.y == 0) sort_lists(a, scratch[0], scratch[1]);
+    return;
+  }
+  int32_t* key = scratch[0];
+  const int t = blockIdx.x, pairs = (int)a.tokens * a.k, p0 = t * a.k;
+  const int c = blockIdx.y * SORT_THREADS + threadIdx.x;
+  if ((int)threadIdx.x < pairs) {
+    const int32_t e = a.indices[threadIdx.x];
+    key[threadIdx.x] = (uint32_t)e < (uint32_t)a.experts ? e : 0x7fffffff;
+  }
+  const uint16_t* x = (const uint16_t*)a.x + t * a.length;
+  const int64_t at = c < a.row.wide ? 8 * (int64_t)c : 8 * (int64_t)a.row.wide + c - a.row.wide;
+  wm_u32x4 v = {0, 0, 0, 0};
+  uint16_t one = 0;
+  if (c < a.row.wide) v = load16(x + at);
+  else if (c < a.row.units) one = x[at];
+  __syncthreads();
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  for (int j = wave; j < a.k + 1; j += SORT_THREADS / 64) {  // the last one counts the pairs that are there
+    const int p = p0 + j;
+    const int32_t e = j < a.k ? key[p] : 0x7fffffff;
+    int32_t before = 0;
+    for (int q0 = 0; q0 < pairs; q0 += 64) {
+      const int q = q0 + lane;
+      before += __popcll(__ballot(q < pairs && (key[q] < e || (j < a.k && key[q] == e && q < p))));
+    }
+    if (lane == 0) {
+      if (j == a.k) {
+        present_ = before;
+      } else {
+        const int32_t r = e == 0x7fffffff ? -1 : before;
+        row[j] = r;
+        if (blockIdx.y == 0) {
+          a.inverse[p] = r;
+          if (r >= 0) a.order[r] = p;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int32_t present = present_;
+  if (blockIdx.y == 0 && (int)threadIdx.x < a.k && p0 + (int)threadIdx.x >= present) a.order[p0 + threadIdx.x] = -1;
+  uint16_t* rows = (uint16_t*)a.rows;
+  if (c < a.row.wide) sort_store<RowUnit<false, true>>(rows, a.length, at, row, a.k, v);
+  else if (c < a.row.units) sort_store<RowUnit<false, false>>(rows, a.length, at, row, a.k, one);
+  const int c0 = blockIdx.y * SORT_THREADS;
+  sort_clear(a, present, t, a.tokens, c0, min(a.row.units, c0 + SORT_THREADS));
+}
+
 template <bool ONE>
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
-  // base: counts, then the chunk's first row of each expert; later the first row of each expert (offsets)
-  __shared__ int32_t base[PERMUTE_MAX_EXPERTS], later[PERMUTE_MAX_EXPERTS + 1];
-  __shared__ int32_t tile_start[ONE ? PERMUTE_MAX_EXPERTS : 1];
+  // base: the chunk's first row of each expert
+  __shared__ int32_t base[PERMUTE_MAX_EXPERTS], later[PERMUTE_MAX_EXPERTS];
   __shared__ __align__(16) int32_t key[SORT_CHUNK];
   __shared__ int32_t row[SORT_CHUNK];
   const int64_t pairs = a.tokens * a.k;
   const int64_t t0 = (int64_t)blockIdx.x * a.chunk_tokens;
   const int64_t p0 = t0 * a.k;
+  if (ONE && t0 >= a.tokens) {
+    if (blockIdx.y == 0) sort_lists(a, base, later);
+    return;
+  }
   const int tokens = (int)max((int64_t)0, min((int64_t)a.chunk_tokens, a.tokens - t0));
   const int n = tokens * a.k;
   const int E = a.experts;
@@ -83,61 +230,13 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
     key[threadIdx.x] = (uint32_t)e < (uint32_t)E ? e : -1;
   }
   if constexpr (ONE) {
-    for (int e = threadIdx.x; e < E; e += SORT_THREADS) base[e] = later[e] = 0;
-    __syncthreads();
-    // 16 ids in flight a thread, as four 16-byte loads where the list allows them
-    const bool quads = (uintptr_t)a.indices % 16 == 0;
-    for (int64_t q0 = 4 * threadIdx.x; q0 < pairs; q0 += 16 * SORT_THREADS) {
-      int32_t e[4][4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int64_t q = q0 + b * 4 * SORT_THREADS;
-        if (quads && q + 4 <= pairs) {
-          const int4 v = *reinterpret_cast<const int4*>(a.indices + q);
-          e[b][0] = v.x, e[b][1] = v.y, e[b][2] = v.z, e[b][3] = v.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) e[b][i] = q + i < pairs ? a.indices[q + i] : -1;
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if ((uint32_t)e[b][i] < (uint32_t)E)
-            atomicAdd(q0 + b * 4 * SORT_THREADS + i < p0 ? &base[e[b][i]] : &later[e[b][i]], 1);
-    }
-    __syncthreads();
+    sort_count(a, p0, base, later);
     const int e0 = 2 * threadIdx.x, e1 = e0 + 1;  // two experts a thread
     const int32_t b0 = e0 < E ? base[e0] : 0, b1 = e1 < E ? base[e1] : 0;
     const int32_t n0 = e0 < E ? b0 + later[e0] : 0, n1 = e1 < E ? b1 + later[e1] : 0;
     const int32_t first = sort_scan(n0 + n1, &present);
-    if (e0 < E) base[e0] = first + b0, later[e0] = first;
-    if (e1 < E) base[e1] = first + n0 + b1, later[e1] = first + n0;
-    if (blockIdx.x == 0 && blockIdx.y == 0) {  // the lists that have no pair to them
-      if (e0 < E) a.offsets[e0] = first;
-      if (e1 < E) a.offsets[e1] = first + n0;
-      if (threadIdx.x == 0) a.offsets[E] = present;
-      const int32_t t0s = (n0 + a.tile_rows - 1) / a.tile_rows, t1s = (n1 + a.tile_rows - 1) / a.tile_rows;
-      int32_t count;
-      const int32_t tile = sort_scan(t0s + t1s, &count);
-      if (threadIdx.x == 0) a.tile_count[0] = count;
-      if (e0 < E) tile_start[e0] = tile;
-      if (e1 < E) tile_start[e1] = tile + t0s;
-      __syncthreads();
-      // Tile i belongs to the last expert whose first tile is <= i: experts without tiles share their start
-      // with the next one that has some, and come before it.
-      for (int32_t i = threadIdx.x; i < count; i += SORT_THREADS) {
-        int lo = 0, hi = E - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (tile_start[mid] <= i) lo = mid; else hi = mid - 1;
-        }
-        reinterpret_cast<int2*>(a.tiles)[i] = make_int2(lo, later[lo] + (i - tile_start[lo]) * a.tile_rows);
-      }
-      for (int64_t i = count + threadIdx.x; i < a.max_tiles; i += SORT_THREADS)
-        reinterpret_cast<int2*>(a.tiles)[i] = make_int2(-1, -1);
-    }
+    if (e0 < E) base[e0] = first + b0;
+    if (e1 < E) base[e1] = first + n0 + b1;
   } else {
     present = a.offsets[E];
     if (blockIdx.y == 0)
@@ -180,32 +279,20 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
   uint16_t* rows = (uint16_t*)a.rows;
   const int c0 = blockIdx.y * a.split_units, c1 = min(a.row.units, c0 + a.split_units);
   for (int t = threadIdx.x >> a.log2; t < tokens; t += SORT_THREADS >> a.log2) {
+    const uint16_t* from = x + (t0 + t) * a.length;
     for (int c = c0 + (threadIdx.x & ((1 << a.log2) - 1)); c < c1; c += 1 << a.log2) {
-      auto move = [&](auto unit, int64_t at) {
-        typedef decltype(unit) U;
-        const auto v = U::load(x + (t0 + t) * a.length + at);
-#pragma unroll 4
-        for (int j = 0; j < a.k; ++j) {
-          const int32_t r = row[t * a.k + j];
-          if (r >= 0) U::store_once(rows + r * a.length + at, v);
-        }
-      };
-      if (c < a.row.wide) move(RowUnit<false, true>(), 8 * (int64_t)c);
-      else move(RowUnit<false, false>(), 8 * (int64_t)a.row.wide + c - a.row.wide);
+      const int64_t at = c < a.row.wide ? 8 * (int64_t)c : 8 * (int64_t)a.row.wide + c - a.row.wide;
+      if (c < a.row.wide) sort_store<RowUnit<false, true>>(rows, a.length, at, row + t * a.k, a.k, load16(from + at));
+      else sort_store<RowUnit<false, false>>(rows, a.length, at, row + t * a.k, a.k, from[at]);
     }
   }
   // The rows behind the last pair, spread over the workgroups: the few that own the last pairs would take
   // twice as long (4096 tokens x 8, hidden 7168, 2% of the pairs absent: 112 us, spread 103).
-  for (int64_t r = present + (int64_t)blockIdx.x; r < pairs; r += gridDim.x) {
-    for (int c = c0 + threadIdx.x; c < c1; c += SORT_THREADS) {
-      if (c < a.row.wide) store16_nt(rows + r * a.length + 8 * (int64_t)c, wm_u32x4{0, 0, 0, 0});
-      else rows[r * a.length + 8 * (int64_t)a.row.wide + c - a.row.wide] = 0;
-    }
-  }
+  sort_clear(a, present, blockIdx.x, (pairs + (int64_t)a.chunk_tokens * a.k - 1) / ((int64_t)a.chunk_tokens * a.k), c0, c1);
 }
 
-// Up to this many pairs a call is one launch.
-constexpr int64_t SORT_ONE_MAX = 32768;
+// Up to this many pairs each way is taken.
+constexpr int64_t SORT_FEW_MAX = 256, SORT_ONE_MAX = 32768;
 
 static int sort_chunk_tokens(int64_t tokens, int k, bool one) {
   const int most = SORT_CHUNK / k > 0 ? SORT_CHUNK / k : 1;
@@ -214,8 +301,16 @@ static int sort_chunk_tokens(int64_t tokens, int k, bool one) {
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-static void sort_launch(SortArgs a, bool one, hipStream_t s) {
-  const int64_t chunks = a.tokens > 0 ? (a.tokens + a.chunk_tokens - 1) / a.chunk_tokens : 1;
+static void sort_launch(SortArgs a, hipStream_t s) {
+  const int64_t pairs = a.tokens * a.k;
+  if (pairs <= SORT_FEW_MAX) {
+    const dim3 grid((unsigned)a.tokens + 1, (unsigned)((a.row.units + SORT_THREADS - 1) / SORT_THREADS));
+    hipLaunchKernelGGL(sort_few_kernel, grid, dim3(SORT_THREADS), 0, s, a);
+    check_launch("sort_few");
+    return;
+  }
+  const bool one = pairs <= SORT_ONE_MAX;
+  const int64_t chunks = (a.tokens + a.chunk_tokens - 1) / a.chunk_tokens;
   // columns are split until the chip has work for every CU
   const int64_t most = (a.row.units + 255) / 256;
   int64_t splits = chunks >= 512 ? 1 : (511 + chunks) / chunks;
@@ -223,7 +318,7 @@ static void sort_launch(SortArgs a, bool one, hipStream_t s) {
   a.split_units = (int)((a.row.units + splits - 1) / splits);
   a.log2 = 0;
   while (a.log2 < 9 && (1 << a.log2) < a.split_units) ++a.log2;
-  const dim3 grid((unsigned)chunks, (unsigned)splits);
+  const dim3 grid((unsigned)(chunks + one), (unsigned)splits);
   if (one) hipLaunchKernelGGL((sort_kernel<true>), grid, dim3(SORT_THREADS), 0, s, a);
   else hipLaunchKernelGGL((sort_kernel<false>), grid, dim3(SORT_THREADS), 0, s, a);
   check_launch("sort");
@@ -430,7 +525,7 @@ WM_EXPORT int wm_sort_tokens(const void* x, int32_t fp32, int32_t tokens, int32_
     }
     a.length = (int64_t)hidden * (fp32 ? 2 : 1);
     a.row = row_units(a.length, false);
-    sort_launch(a, one, s);
+    sort_launch(a, s);
   });
 }
 
