@@ -88,10 +88,7 @@ void prefill_fp8(const uint16_t* x, int tokens, const int32_t* indices, const fl
 // The one-launch decode layer (decode_layer.hip): shapes with a fused instantiation.
 bool moe_layer_fused_supports(int hidden, int inter, int k);
 
-// The parts of wm_permute on checked arguments. permute_count launches permute_count_block
-// (permute_device.h) alone, over chunks of chunk_pairs pairs; permute_scan turns its counts into each
-// chunk's first row of an expert within the expert, and writes the offsets and tiles; permute_lists is the
-// scan and the scatter after a launch that holds the block with its own chunks. With
+// wm_permute on checked arguments, after permute_count_block's launch (permute_device.h). With
 // cold_rows > 0 the experts of up to that many rows (and more than none) are left out of `tiles` and get
 // one tile each in cold_tiles [experts][2], counted in tile_count[1]. order may be null; row_token (or
 // null): pair / k of every permuted row.
@@ -99,10 +96,6 @@ struct PermuteWorkspace {
   int32_t *counts, *totals, *done;
 };
 PermuteWorkspace permute_workspace(void* workspace, int64_t pairs, int experts);
-void permute_count(const int32_t* indices, int64_t pairs, int experts, int chunk_pairs, const PermuteWorkspace& ws,
-                   hipStream_t s);
-void permute_scan(int64_t chunks, int experts, int tile_rows, int cold_rows, int32_t* offsets, int32_t* tiles,
-                  int32_t* cold_tiles, int32_t* tile_count, const PermuteWorkspace& ws, hipStream_t s);
 void permute_lists(const int32_t* indices, int64_t pairs, int experts, int tile_rows, int cold_rows, int32_t* order,
                    int32_t* inverse, int32_t* row_token, int k, int32_t* offsets, int32_t* tiles, int32_t* cold_tiles,
                    int32_t* tile_count, const PermuteWorkspace& ws, hipStream_t s);

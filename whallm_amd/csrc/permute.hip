@@ -26,8 +26,8 @@ constexpr int SCAN_SEGS = 16;     // chunk segments per expert (one per wave)
 
 __global__ void __launch_bounds__(64 * PERMUTE_COUNT_WAVES)
     permute_count_kernel(const int32_t* __restrict__ idx, int64_t pairs, int experts, int32_t* __restrict__ chunk_counts,
-                         int32_t* __restrict__ done, int chunk_pairs) {
-  permute_count_block(idx, pairs, experts, blockIdx.x, chunk_counts, done, chunk_pairs);
+                         int32_t* __restrict__ done) {
+  permute_count_block(idx, pairs, experts, blockIdx.x, chunk_counts, done);
 }
 
 // Inclusive prefix sum over the 1024 threads of the block (wave shuffles, then the 16
@@ -202,26 +202,14 @@ __global__ void __launch_bounds__(64) permute_scatter_kernel(const int32_t* __re
 }
 
 // See moe_internal.h.
-void permute_count(const int32_t* indices, int64_t pairs, int experts, int chunk_pairs, const PermuteWorkspace& ws,
-                   hipStream_t s) {
-  hipLaunchKernelGGL(permute_count_kernel, dim3((unsigned)permute_count_blocks(pairs, chunk_pairs)),
-                     dim3(64 * PERMUTE_COUNT_WAVES), 0, s, indices, pairs, experts, ws.counts, ws.done, chunk_pairs);
-  check_launch("permute_count");
-}
-
-void permute_scan(int64_t chunks, int experts, int tile_rows, int cold_rows, int32_t* offsets, int32_t* tiles,
-                  int32_t* cold_tiles, int32_t* tile_count, const PermuteWorkspace& ws, hipStream_t s) {
-  hipLaunchKernelGGL(permute_scan_kernel, dim3((unsigned)((experts + SCAN_EXPERTS - 1) / SCAN_EXPERTS)),
-                     dim3(64 * SCAN_SEGS), 0, s, ws.counts, chunks, experts, ws.totals, ws.done, tile_rows, cold_rows, offsets,
-                     tiles, cold_tiles, tile_count);
-  check_launch("permute_scan");
-}
-
 void permute_lists(const int32_t* indices, int64_t pairs, int experts, int tile_rows, int cold_rows, int32_t* order,
                    int32_t* inverse, int32_t* row_token, int k, int32_t* offsets, int32_t* tiles, int32_t* cold_tiles,
                    int32_t* tile_count, const PermuteWorkspace& ws, hipStream_t s) {
   const int64_t chunks = (pairs + PERMUTE_CHUNK - 1) / PERMUTE_CHUNK;
-  permute_scan(chunks, experts, tile_rows, cold_rows, offsets, tiles, cold_tiles, tile_count, ws, s);
+  hipLaunchKernelGGL(permute_scan_kernel, dim3((unsigned)((experts + SCAN_EXPERTS - 1) / SCAN_EXPERTS)),
+                     dim3(64 * SCAN_SEGS), 0, s, ws.counts, chunks, experts, ws.totals, ws.done, tile_rows, cold_rows, offsets,
+                     tiles, cold_tiles, tile_count);
+  check_launch("permute_scan");
   if (chunks > 0) {
     hipLaunchKernelGGL(permute_scatter_kernel, dim3((unsigned)chunks), dim3(64), 0, s, indices, pairs, experts, ws.counts,
                        offsets, order, inverse, row_token, k);
@@ -259,7 +247,9 @@ WM_EXPORT int wm_permute(const int32_t* indices, int64_t pairs, int32_t experts,
     if (!offsets || !tile_count || !workspace || (pairs > 0 && (!indices || !order || !inverse || !tiles)))
       fail("wm_permute: null pointer");
     const PermuteWorkspace ws = permute_workspace(workspace, pairs, experts);
-    permute_count(indices, pairs, experts, PERMUTE_CHUNK, ws, as_stream(stream));
+    hipLaunchKernelGGL(permute_count_kernel, dim3((unsigned)permute_count_blocks(pairs)), dim3(64 * PERMUTE_COUNT_WAVES), 0,
+                       as_stream(stream), indices, pairs, experts, ws.counts, ws.done);
+    check_launch("permute_count");
     permute_lists(indices, pairs, experts, tile_rows, 0, order, inverse, nullptr, 1, offsets, tiles, nullptr, tile_count, ws,
                   as_stream(stream));
   });

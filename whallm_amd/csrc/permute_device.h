@@ -9,20 +9,20 @@ constexpr int PERMUTE_CHUNK = 256;
 constexpr int PERMUTE_MAX_EXPERTS = 1024;
 constexpr int PERMUTE_COUNT_WAVES = 4;  // chunks a block
 
-// Chunks of pairs (PERMUTE_CHUNK, or a caller's own number) counted by block `block`, one a wave; block 0
-// also clears the counter `done` of the scan after it. Every thread of the block calls it.
+// Chunks of pairs counted by block `block`, one a wave; block 0 also clears the counter `done` of the
+// scan after it. Every thread of the block calls it.
 __device__ __forceinline__ void permute_count_block(const int32_t* __restrict__ idx, int64_t pairs, int experts,
                                                     int64_t block, int32_t* __restrict__ chunk_counts,
-                                                    int32_t* __restrict__ done, int chunk_pairs = PERMUTE_CHUNK) {
+                                                    int32_t* __restrict__ done) {
   __shared__ int32_t all_counts[PERMUTE_COUNT_WAVES][PERMUTE_MAX_EXPERTS];
   int32_t* counts = all_counts[threadIdx.x / 64];
   const int lane = threadIdx.x % 64;
-  const int64_t chunks = (pairs + chunk_pairs - 1) / chunk_pairs;
+  const int64_t chunks = (pairs + PERMUTE_CHUNK - 1) / PERMUTE_CHUNK;
   const int64_t chunk = block * PERMUTE_COUNT_WAVES + threadIdx.x / 64;
   if (block == 0 && threadIdx.x == 0) *done = 0;
   for (int e = lane; e < experts; e += 64) counts[e] = 0;
   __syncthreads();
-  const int64_t begin = chunk * chunk_pairs, end = min<int64_t>(pairs, begin + chunk_pairs);
+  const int64_t begin = chunk * PERMUTE_CHUNK, end = min<int64_t>(pairs, begin + PERMUTE_CHUNK);
   for (int64_t p = begin + lane; p < end; p += 64) {
     const int e = idx[p];
     if (e >= 0 && e < experts) atomicAdd(&counts[e], 1);
@@ -33,8 +33,8 @@ __device__ __forceinline__ void permute_count_block(const int32_t* __restrict__ 
 }
 
 // Blocks of permute_count_block for a list of pairs.
-inline int64_t permute_count_blocks(int64_t pairs, int chunk_pairs = PERMUTE_CHUNK) {
-  const int64_t n = (pairs + chunk_pairs * PERMUTE_COUNT_WAVES - 1) / (chunk_pairs * PERMUTE_COUNT_WAVES);
+inline int64_t permute_count_blocks(int64_t pairs) {
+  const int64_t n = (pairs + PERMUTE_CHUNK * PERMUTE_COUNT_WAVES - 1) / (PERMUTE_CHUNK * PERMUTE_COUNT_WAVES);
   return n > 0 ? n : 1;
 }
 
