@@ -440,11 +440,12 @@ static void gather_sum(const void* rows, bool f32, const float* weights, const i
   check_launch("gather_sum");
 }
 
-// ---- the gradients of back: a block per token. Each thread holds the same units of dy for a batch of
-// pairs, so a pair's row is read once, its gradient written, and its dot product summed over the block.
+// ---- the gradients of back: GROUP threads a token, a wave or a workgroup. Each thread holds the same units of dy
+// for a batch of pairs, so a pair's row is read once, its gradient written, and its dot product summed over the
+// group.
 constexpr int BACK_BATCH = 8;
 
-template <bool F32, bool ONCE>
+template <bool F32, bool ONCE, int GROUP>
 __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__ dy_, const void* __restrict__ rows_,
                                                        const float* __restrict__ weights, const int32_t* __restrict__ inverse,
                                                        const int32_t* __restrict__ present_, int64_t tokens, int64_t hidden,
@@ -453,15 +454,16 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
   typedef typename RowUnit<F32, true>::Elem Elem;
   constexpr int N = RowUnit<F32, true>::N;
   __shared__ float part[BACK_BATCH][4];
-  const int64_t t = blockIdx.x;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t t = blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
+  const int me = threadIdx.x % GROUP, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  if (t >= tokens) return;  // a whole wave, where a token has one: no barrier is ahead
   const Elem* dy = (const Elem*)dy_ + t * hidden;
   const Elem* rows = (const Elem*)rows_;
   Elem* drows = (Elem*)drows_;
   const uint32_t pairs = (uint32_t)(tokens * k);
   // the rows without a pair, spread over the tokens
   for (int64_t r = *present_ + t; r < tokens * k; r += tokens) {
-    for (int c = threadIdx.x; c < row.units; c += 256) {
+    for (int c = me; c < row.units; c += GROUP) {
       if (c < row.wide) store16_nt(drows + r * hidden + (int64_t)c * N, wm_u32x4{0, 0, 0, 0});
       else drows[r * hidden + (int64_t)row.wide * N + c - row.wide] = 0;
     }
@@ -497,8 +499,16 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
         }
       }
     };
-    for (int c = threadIdx.x; c < row.wide; c += 256) unit(RowUnit<F32, true>(), (int64_t)c * N);
-    if (threadIdx.x < row.units - row.wide) unit(RowUnit<F32, false>(), (int64_t)row.wide * N + threadIdx.x);
+    for (int c = me; c < row.wide; c += GROUP) unit(RowUnit<F32, true>(), (int64_t)c * N);
+    if (me < row.units - row.wide) unit(RowUnit<F32, false>(), (int64_t)row.wide * N + me);
+    if (GROUP == 64) {
+#pragma unroll
+      for (int q = 0; q < BACK_BATCH; ++q) {
+        const float v = segment_sum<64>(dot[q]);
+        if (lane == q && j0 + q < k) dweights[t * k + j0 + q] = v;
+      }
+      continue;
+    }
 #pragma unroll
     for (int q = 0; q < BACK_BATCH; ++q) {
       const float v = segment_sum<64>(dot[q]);
@@ -511,6 +521,19 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
     }
     __syncthreads();
   }
+}
+
+template <bool F32, bool ONCE>
+static void back_grad(const void* dy, const void* rows, const float* weights, const int32_t* inverse, const int32_t* present,
+                      int64_t tokens, int64_t hidden, int k, void* drows, float* dweights, hipStream_t s) {
+  const RowUnits row = row_units(hidden, F32);
+  if (row.units <= 64)  // 16000 tokens x 8 of 100 in bf16: 39 us, with a workgroup a token 102; of 1000 95 and 92
+    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 64>), dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, dy, rows, weights,
+                       inverse, present, tokens, hidden, row, k, drows, dweights);
+  else
+    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 256>), dim3((unsigned)tokens), dim3(256), 0, s, dy, rows, weights, inverse,
+                       present, tokens, hidden, row, k, drows, dweights);
+  check_launch("back_grad");
 }
 
 static void check_rows(const char* name, int64_t tokens, int k, int64_t hidden, int f32) {
@@ -595,21 +618,17 @@ WM_EXPORT int wm_combine_rows_backward(const void* dy, const void* rows, int32_t
     if (!dy || !rows || !weights || !inverse || !present || !drows || !dweights) fail("wm_combine_rows_backward: null pointer");
     if (((uintptr_t)dy | (uintptr_t)rows | (uintptr_t)drows) % (fp32 ? 4 : 2))
       fail("wm_combine_rows_backward: rows must be aligned to their elements");
-    const RowUnits row = row_units(hidden, fp32 != 0);
     hipStream_t s = as_stream(stream);
     // as for the sort, but the rows that are read go past the cache already: 250 MB 104 us past it, 88 through
     // it; 500 MB 203 and 211
     const bool once = (int64_t)tokens * k * hidden * (fp32 ? 4 : 2) > 384ll << 20;
-#define WM_BACK(F, O)                                                                                                     \
-  hipLaunchKernelGGL((back_grad_kernel<F, O>), dim3((unsigned)tokens), dim3(256), 0, s, dy, rows, weights, inverse, present, \
-                     (int64_t)tokens, (int64_t)hidden, row, k, drows, dweights)
+#define WM_BACK(F, O) back_grad<F, O>(dy, rows, weights, inverse, present, tokens, hidden, k, drows, dweights, s)
     if (fp32) {
       if (once) WM_BACK(true, true); else WM_BACK(true, false);
     } else {
       if (once) WM_BACK(false, true); else WM_BACK(false, false);
     }
 #undef WM_BACK
-    check_launch("back_grad");
   });
 }
 
