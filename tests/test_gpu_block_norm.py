@@ -3,8 +3,9 @@
 
 Bar: the running error of the same steps in fp32 (running_error.py) and one rounding to the
 output's type. x is held against the norm of the residual as the kernel stored it. A row's sums pass
-at most 16 columns of a thread, 6 steps of a wave and 16 waves; a sum over T tokens
-T / 512 + 1 tokens of a workgroup, 32 of 512 workgroups and 16 slices.
+at most 16 columns of a thread, 6 steps of a wave and 16 waves; a sum over T tokens passes the
+tokens of a thread group, at most T / 256 + 1 (with fewer than 256 groups it is one token a group),
+16 groups of a workgroup, 64 of at most 1024 workgroups and 16 slices.
 """
 import numpy as np
 import pytest
@@ -65,7 +66,7 @@ def want_x(residual_out, s, eps):
 def want_grads(s, dx, dres, sigmoid, scale, eps, post_norm):
     """s['residual'] is the residual behind the block."""
     T = s["y"].shape[0]
-    tokens = T // 512 + 1 + 32 + 16
+    tokens = T // 256 + 1 + 16 + 64 + 16
     r, y, dx = Fp32(f64(s["residual"])), Fp32(f64(s["y"])), Fp32(f64(dx))
     wpre, wpost = weight(s["pre_weight"], s["weight_offset"]), weight(s["post_weight"], s["weight_offset"])
     q = ((r * r).mean(ROW) + eps).rsqrt()

@@ -10,12 +10,12 @@
 //   b = s g dr',  c = b (o + w_post)               dy = p c - y p^3 mean(c y)     dw_post = sum_t b y p
 //   dg = s dr' z (by sigmoid'), summed over what g is broadcast over
 //
-// Bound by HBM: every tensor passes once. A workgroup holds a token's row in registers, 8 or 16 columns a
-// thread, sums over the row twice at most, and goes on to the next token with the weights still in
-// registers. Sums over tokens (weight gradients) stay in the threads' registers, go to the workspace once
-// per workgroup and are added up by a second launch in the workgroups' order. All arithmetic is fp32; bf16
-// outputs are rounded once, from values that no earlier rounding touched but r''s own (x is the norm of
-// the residual that the next block reads).
+// Bound by HBM: every tensor passes once. A group of threads holds a token's row in registers, 8 or 16 columns
+// a thread, sums over the row twice at most, and goes on to its next token with the weights still in
+// registers. A group is 16 threads or a wave for short rows, whose sums need no barrier, else a workgroup. Sums
+// over tokens (weight gradients) stay with the group, go to the workspace once per workgroup and are added up
+// by a second launch in the workgroups' order. All arithmetic is fp32; bf16 outputs are rounded once, from values that no
+// earlier rounding touched but r''s own (x is the norm of the residual that the next block reads).
 #include <initializer_list>
 
 #include "row_units.h"
@@ -43,6 +43,8 @@ struct Row8<false> {
     }
   }
   __device__ __forceinline__ void clear() { a = wm_u32x4{0, 0, 0, 0}; }
+  // The compiler must not keep what it unpacked before this: the packed words are half the registers.
+  __device__ __forceinline__ void repack() { asm volatile("" : "+v"(a)); }
   __device__ __forceinline__ float get(int i) const { return __uint_as_float(i % 2 ? a[i / 2] & 0xffff0000u : a[i / 2] << 16); }
 };
 template <>
@@ -63,6 +65,7 @@ struct Row8<true> {
     }
   }
   __device__ __forceinline__ void clear() { a = b = wm_u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void repack() {}
   __device__ __forceinline__ float get(int i) const { return __uint_as_float(i < 4 ? a[i] : b[i - 4]); }
 };
 template <bool WHOLE>
@@ -89,19 +92,30 @@ __device__ __forceinline__ void store8(void* p, bool f32, int64_t i, int n, cons
   }
 }
 
-__device__ __forceinline__ float sigmoid_f32(float v) { return 1.0f / (1.0f + expf(-v)); }
+// 1 / (1 + exp(-v)) to a few units: exp2 of the product with log2 e, whose rounding and the constant's rest come in as
+// a factor. Below -87 the exponential is held at 2^126 (the result is then the smallest normal number), NaN passes.
+__device__ __forceinline__ float sigmoid_f32(float v) {
+  constexpr float LOG2E = 1.44269502162933349609375f, REST = 1.925963033500011079e-8f, LN2 = 0.693147182464599609375f;
+  float h = -v * LOG2E;
+  const float l = fmaf(-v, LOG2E, -h) - v * REST;
+  h = h > 126.0f ? 126.0f : h;
+  float e = __builtin_amdgcn_exp2f(h);
+  e = fmaf(e, l * LN2, e);
+  return __builtin_amdgcn_rcpf(1.0f + e);
+}
 
-// Sums N values over the workgroup (whole waves, 16 at most) in a fixed order; every thread gets them. `part`
-// holds zeros behind the waves, and is written again only behind another sum's barrier: the callers
-// alternate between two or three.
-template <int N>
-__device__ __forceinline__ void block_sums(float v[N], float (*part)[16]) {
+// Sums N values over the group in a fixed order; every thread gets them. GROUP 0 is the workgroup (whole waves,
+// 16 at most): `part` holds zeros behind the waves, and is written again only behind another sum's barrier:
+// the callers alternate between two or three.
+template <int N, int GROUP>
+__device__ __forceinline__ void group_sums(float v[N], float (*part)[16]) {
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    v[n] = segment_sum<64>(v[n]);
-    if (lane == 0) part[n][wave] = v[n];
+    v[n] = segment_sum<GROUP == 16 ? 16 : 64>(v[n]);
+    if (GROUP == 0 && lane == 0) part[n][wave] = v[n];
   }
+  if (GROUP != 0) return;
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < N; ++n) v[n] = segment_sum<16>(part[n][lane % 16]);
@@ -110,6 +124,21 @@ __device__ __forceinline__ void clear_parts(float* part, int n) {
   for (int i = threadIdx.x; i < n; i += blockDim.x) part[i] = 0.0f;
   __syncthreads();
 }
+
+// A thread's place: group g of all has tokens g, g + groups, ..; the thread columns 8 (v size + me) .. + 7 of each,
+// v < V.
+template <int GROUP>
+struct NormGroup {
+  int me, size;
+  int64_t g, groups;
+  __device__ __forceinline__ NormGroup() {
+    size = GROUP == 0 ? (int)blockDim.x : GROUP;
+    me = GROUP == 0 ? (int)threadIdx.x : (int)threadIdx.x % GROUP;
+    g = GROUP == 0 ? blockIdx.x : blockIdx.x * (int64_t)(blockDim.x / GROUP) + threadIdx.x / GROUP;
+    groups = GROUP == 0 ? gridDim.x : gridDim.x * (int64_t)(blockDim.x / GROUP);
+  }
+  __device__ __forceinline__ int column(int v) const { return (v * size + me) * 8; }
+};
 
 struct NormArgs {
   const void* residual;  // forward: r; backward: r' (residual_out)
@@ -140,18 +169,18 @@ __device__ __forceinline__ float gate_value(const NormArgs& a, int64_t i) {
   return a.gate_sigmoid ? sigmoid_f32(g) : g;
 }
 
-// A thread has columns 8 (v blockDim + thread) .. + 7 of every row, v < V.
-template <bool F32, int V, bool WHOLE, int GATE, int THREADS>
+template <bool F32, int V, bool WHOLE, int GATE, int GROUP, int THREADS>
 __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* residual_out, uint16_t* __restrict__ x) {
   __shared__ float part[3][1][16];
-  clear_parts(&part[0][0][0], 48);
+  if (GROUP == 0) clear_parts(&part[0][0][0], 48);
+  const NormGroup<GROUP> at;
   const int H = a.hidden;
   const float opost = a.post ? a.offset : 0.0f, opre = a.pre ? a.offset : 0.0f;
   Weight8 wpost[V], wpre[V];
   float channel[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * 8;
+    const int c = at.column(v);
     if (c < H) {
       wpost[v].template load<WHOLE>(a.post, c, H - c);
       wpre[v].template load<WHOLE>(a.pre, c, H - c);
@@ -162,7 +191,7 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* r
     }
   }
   int odd = 0;
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x, odd ^= 1) {
+  for (int64_t t = at.g; t < a.tokens; t += at.groups, odd ^= 1) {
     Row8<F32> raw[V];
     Row8<false> y[V];
     Row8<GATE == GATE_FULL_F32> gate[V];
@@ -170,7 +199,7 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* r
     float sum[1] = {0.0f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
+      const int c = at.column(v);
       if (c < H) {
         y[v].template load<WHOLE>(a.y, t * H + c, H - c);
         raw[v].template load<WHOLE>(a.residual, t * H + c, H - c);
@@ -182,18 +211,18 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* r
     if (a.post_norm) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if ((int)((v * blockDim.x + threadIdx.x) * 8) < H) {
+        if (at.column(v) < H) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) sum[0] = fmaf(y[v].get(i), y[v].get(i), sum[0]);
         }
       }
-      block_sums<1>(sum, part[0]);
+      group_sums<1, GROUP>(sum, part[0]);
       p = rsqrtf(sum[0] / (float)H + a.eps);
     }
     sum[0] = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
+      const int c = at.column(v);
       if (c < H) {
         float g[8];
 #pragma unroll
@@ -214,11 +243,11 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* r
         store8<WHOLE>(residual_out, F32, t * H + c, H - c, r[v]);
       }
     }
-    block_sums<1>(sum, part[1 + odd]);  // without the post norm no other barrier stands between two of these
+    group_sums<1, GROUP>(sum, part[1 + odd]);  // without the post norm no other barrier stands between two of these
     const float q = rsqrtf(sum[0] / (float)H + a.eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
+      const int c = at.column(v);
       if (c < H) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[v][i] *= q * wpre[v].get(opre, i);
@@ -237,18 +266,21 @@ struct NormGrads {
   float* partial;  // [3][workgroups][H]: post, pre, channel gate
 };
 
-// What a thread loads of a token's row. (Loading the next token's meanwhile takes the registers of a second
-// workgroup a CU and is no faster: 74.0 us for 4001 tokens of 5120 with a full gate, 72.7 without.)
+// What a thread loads of a token's row. A workgroup that has a CU to itself loads the next token's behind the first
+// sums, while it works on this one's: 4001 tokens of 5120 with a full gate 68.9 us, without 70.9. (Workgroups that
+// share one do so for each other; they unpack the weights anew for each token, since more registers make them
+// fewer: 16000 of 2051 with a channel's gate 136 us, with the weights kept 183.)
 template <bool F32, int V, bool WHOLE, int GATE>
 struct NormRow {
   Row8<F32> r[V], dr[V];
   Row8<false> y[V], dx[V];
   Row8<GATE == GATE_FULL_F32> gate[V];
-  __device__ __forceinline__ void load(const NormArgs& a, const NormGrads& d, int64_t t) {
+  template <int GROUP>
+  __device__ __forceinline__ void load(const NormArgs& a, const NormGrads& d, const NormGroup<GROUP>& at, int64_t t) {
     const int H = a.hidden;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
+      const int c = at.column(v);
       if (c < H) {
         r[v].template load<WHOLE>(a.residual, t * H + c, H - c);
         dx[v].template load<WHOLE>(d.dx, t * H + c, H - c);
@@ -260,18 +292,50 @@ struct NormRow {
   }
 };
 
-template <bool F32, int V, bool WHOLE, int GATE, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_norm_grad_kernel(NormArgs a, NormGrads d) {
+// A thread's sums over its tokens, of the post weight (or of what its gradient and a channel gate's have in
+// common) and of the pre weight. With 16 columns they are in LDS: registers would not hold them.
+template <int V, int THREADS>
+struct NormSums {
+  float post_[8], pre_[8];
+  __device__ __forceinline__ void clear(float*) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) post_[i] = pre_[i] = 0.0f;
+  }
+  __device__ __forceinline__ void post(float*, int, int i, float x, float y) { post_[i] = fmaf(x, y, post_[i]); }
+  __device__ __forceinline__ void pre(float*, int, int i, float x, float y) { pre_[i] = fmaf(x, y, pre_[i]); }
+  __device__ __forceinline__ float post(const float*, int, int i) const { return post_[i]; }
+  __device__ __forceinline__ float pre(const float*, int, int i) const { return pre_[i]; }
+};
+template <int THREADS>
+struct NormSums<2, THREADS> {
+  static constexpr int PRE = 16 * THREADS;
+  static __device__ __forceinline__ int place(int v, int i) { return (8 * v + i) * THREADS + threadIdx.x; }
+  __device__ __forceinline__ void clear(float* s) {
+    for (int i = 0; i < 32; ++i) s[i * THREADS + threadIdx.x] = 0.0f;
+  }
+  __device__ __forceinline__ void post(float* s, int v, int i, float x, float y) { s[place(v, i)] = fmaf(x, y, s[place(v, i)]); }
+  __device__ __forceinline__ void pre(float* s, int v, int i, float x, float y) {
+    s[PRE + place(v, i)] = fmaf(x, y, s[PRE + place(v, i)]);
+  }
+  __device__ __forceinline__ float post(const float* s, int v, int i) const { return s[place(v, i)]; }
+  __device__ __forceinline__ float pre(const float* s, int v, int i) const { return s[PRE + place(v, i)]; }
+};
+
+template <bool F32, int V, bool WHOLE, int GATE, int GROUP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a, NormGrads d) {
   __shared__ float part[2][3][16];
-  clear_parts(&part[0][0][0], 96);
+  __shared__ float lds[V == 2 ? 32 * THREADS : GROUP != 0 ? 8 * THREADS : 1];
+  if (GROUP == 0) clear_parts(&part[0][0][0], 96);
+  const NormGroup<GROUP> at;
   const int H = a.hidden;
   const float opost = a.post ? a.offset : 0.0f, opre = a.pre ? a.offset : 0.0f;
   Weight8 wpost[V], wpre[V];
   float channel[V][8];
-  float dpost[V][8], dpre[V][8], dch[V][8];
+  NormSums<V, THREADS> sums;
+  sums.clear(lds);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * 8;
+    const int c = at.column(v);
     if (c < H) {
       wpost[v].template load<WHOLE>(a.post, c, H - c);
       wpre[v].template load<WHOLE>(a.pre, c, H - c);
@@ -280,20 +344,22 @@ __global__ void __launch_bounds__(THREADS) block_norm_grad_kernel(NormArgs a, No
         for (int i = 0; i < 8; ++i) channel[v][i] = WHOLE || i < H - c ? gate_value(a, c + i) : 0.0f;
       }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dpost[v][i] = dpre[v][i] = dch[v][i] = 0.0f;
   }
   const float inv = 1.0f / (float)H;
   NormRow<F32, V, WHOLE, GATE> row;
 #pragma unroll
   for (int v = 0; v < V; ++v) row.dr[v].clear();
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    row.load(a, d, t);
+  constexpr bool AHEAD = THREADS == 1024 && V == 1;
+  NormRow<F32, V, WHOLE, GATE> next = row;
+  if (AHEAD) next.load(a, d, at, at.g);
+  for (int64_t t = at.g; t < a.tokens; t += at.groups) {
+    if (AHEAD) row = next;
+    else row.load(a, d, at, t);
     const float g1 = GATE == GATE_TOKEN ? gate_value(a, t) : 1.0f;
     float sum[3] = {0.0f, 0.0f, 0.0f};  // r'^2, a r', y^2
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if ((int)((v * blockDim.x + threadIdx.x) * 8) < H) {
+      if (at.column(v) < H) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // behind a row's end r', dx and y are 0
           const float r = row.r[v].get(i), y = row.y[v].get(i);
@@ -303,7 +369,15 @@ __global__ void __launch_bounds__(THREADS) block_norm_grad_kernel(NormArgs a, No
         }
       }
     }
-    block_sums<3>(sum, part[0]);
+    group_sums<3, GROUP>(sum, part[0]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      row.r[v].repack();
+      row.dx[v].repack();
+      row.y[v].repack();
+      if (THREADS < 1024 || V == 2) wpre[v].w.repack(), wpost[v].w.repack();
+    }
+    if (AHEAD && t + at.groups < a.tokens) next.load(a, d, at, t + at.groups);
     const float q = rsqrtf(sum[0] * inv + a.eps);
     const float p = a.post_norm ? rsqrtf(sum[2] * inv + a.eps) : 1.0f;
     const float k1 = q * q * q * (sum[1] * inv);
@@ -311,65 +385,87 @@ __global__ void __launch_bounds__(THREADS) block_norm_grad_kernel(NormArgs a, No
     float cc[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
+      const int c = at.column(v);
       if (c < H) {
-        float dr[8], dg[8], g[8];
+        float dr[8], dg[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = GATE == GATE_CHANNEL ? channel[v][i] : GATE >= GATE_FULL ? row.gate[v].get(i) : g1;
-        if (GATE >= GATE_FULL && a.gate_sigmoid) {
+        for (int h = 0; h < 8; h += 4) {
+          float g[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = sigmoid_f32(g[i]);
-        }
+          for (int j = 0; j < 4; ++j)
+            g[j] = GATE == GATE_CHANNEL ? channel[v][h + j] : GATE >= GATE_FULL ? row.gate[v].get(h + j) : g1;
+          if (GATE >= GATE_FULL && a.gate_sigmoid) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float r = row.r[v].get(i), dx = row.dx[v].get(i), n = row.y[v].get(i) * p;
-          dr[i] = row.dr[v].get(i) + fmaf(q * dx, wpre[v].get(opre, i), -r * k1);
-          dpre[v][i] = fmaf(q * dx, r, dpre[v][i]);
-          const float sdr = a.scale * dr[i], w = wpost[v].get(opost, i);
-          const float b = sdr * g[i];
-          dpost[v][i] = fmaf(b, n, dpost[v][i]);
-          if (GATE != GATE_NONE) dg[i] = sdr * (n * w);
-          cc[v][i] = b * w;
-          sum2[0] = fmaf(cc[v][i], row.y[v].get(i), sum2[0]);
+            for (int j = 0; j < 4; ++j) g[j] = sigmoid_f32(g[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = h + j;
+            const float r = row.r[v].get(i), dx = row.dx[v].get(i), n = row.y[v].get(i) * p;
+            dr[i] = row.dr[v].get(i) + fmaf(q * dx, wpre[v].get(opre, i), -r * k1);
+            sums.pre(lds, v, i, q * dx, r);
+            const float sdr = a.scale * dr[i], w = wpost[v].get(opost, i);
+            const float b = sdr * g[j];
+            sums.post(lds, v, i, GATE == GATE_CHANNEL ? sdr : b, n);
+            if (GATE != GATE_NONE && GATE != GATE_CHANNEL) dg[i] = sdr * (n * w);
+            if (GATE >= GATE_FULL && a.gate_sigmoid) dg[i] *= g[j] * (1.0f - g[j]);
+            if (GATE == GATE_TOKEN) sum2[1] += dg[i];
+            cc[v][i] = b * w;
+            sum2[0] = fmaf(cc[v][i], row.y[v].get(i), sum2[0]);
+          }
+          if (V == 2) __builtin_amdgcn_sched_barrier(0);  // fewer values at once: there are no registers for more
         }
         store8<WHOLE>(d.dr, F32, t * H + c, H - c, dr);
-        if (GATE != GATE_NONE) {
-          if (a.gate_sigmoid) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dg[i] *= g[i] * (1.0f - g[i]);
-          }
-          if (GATE >= GATE_FULL) store8<WHOLE>(d.dgate, GATE == GATE_FULL_F32, t * H + c, H - c, dg);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (GATE == GATE_CHANNEL) dch[v][i] += dg[i];
-            if (GATE == GATE_TOKEN) sum2[1] += dg[i];
-          }
-        }
+        if (GATE >= GATE_FULL) store8<WHOLE>(d.dgate, GATE == GATE_FULL_F32, t * H + c, H - c, dg);
       }
     }
-    if (a.post_norm || GATE == GATE_TOKEN) block_sums<GATE == GATE_TOKEN ? 2 : 1>(sum2, part[1]);
+    if (GROUP != 0 || a.post_norm || GATE == GATE_TOKEN) group_sums<GATE == GATE_TOKEN ? 2 : 1, GROUP>(sum2, part[1]);
     else __syncthreads();
     const float k2 = a.post_norm ? p * p * p * (sum2[0] * inv) : 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
+      const int c = at.column(v);
+      row.y[v].repack();
       if (c < H) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) cc[v][i] = fmaf(p, cc[v][i], -row.y[v].get(i) * k2);
         store8<WHOLE>(d.dy, false, t * H + c, H - c, cc[v]);
       }
     }
-    if (GATE == GATE_TOKEN && threadIdx.x == 0) ((float*)d.dgate)[t] = sum2[1];
+    if (GATE == GATE_TOKEN && at.me == 0) ((float*)d.dgate)[t] = a.gate_sigmoid ? sum2[1] * (g1 * (1.0f - g1)) : sum2[1];
   }
+  // A workgroup's row of each sum.
+  auto emit = [&](int which, auto value) {
+    float* out = d.partial + ((int64_t)which * gridDim.x + blockIdx.x) * H;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * 8;
-    if (c < H) {
-      const int64_t at = (int64_t)blockIdx.x * H + c, all = (int64_t)gridDim.x * H;
-      if (a.post) store8<WHOLE>(d.partial, true, at, H - c, dpost[v]);
-      if (a.pre) store8<WHOLE>(d.partial, true, all + at, H - c, dpre[v]);
-      if (GATE == GATE_CHANNEL) store8<WHOLE>(d.partial, true, 2 * all + at, H - c, dch[v]);
+    for (int v = 0; v < V; ++v) {
+      const int c = at.column(v);
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = c < H ? value(v, i) : 0.0f;
+      if (GROUP == 0) {
+        if (c < H) store8<WHOLE>(out, true, c, H - c, f);
+      } else {  // its groups' sums, in their order
+        float* mine = &lds[threadIdx.x * 8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[i] = f[i];
+        __syncthreads();
+        for (int j = threadIdx.x; j < H; j += THREADS) {
+          float sum = 0.0f;
+          for (int g = 0; g < THREADS; g += GROUP) sum += lds[g * 8 + j];
+          out[j] = sum;
+        }
+        __syncthreads();
+      }
     }
+  };
+  if (a.post) emit(0, [&](int v, int i) { return sums.post(lds, v, i) * (GATE == GATE_CHANNEL ? channel[v][i] : 1.0f); });
+  if (a.pre) emit(1, [&](int v, int i) { return sums.pre(lds, v, i); });
+  if (GATE == GATE_CHANNEL) {
+    emit(2, [&](int v, int i) {
+      const float g = channel[v][i];
+      return sums.post(lds, v, i) * wpost[v].get(opost, i) * (a.gate_sigmoid ? g * (1.0f - g) : 1.0f);
+    });
   }
 }
 
@@ -396,28 +492,35 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(const float* __restr
   }
 }
 
-// A workgroup's threads: 8 columns each where 1024 threads suffice, else 16.
+// How a row is held: by `group` threads (0: a workgroup of `threads`), 8 v columns each. Short rows have 16 threads
+// or a wave, four waves a workgroup; rows of more than 8192 columns 16 columns a thread.
 struct NormShape {
-  int v, threads;
+  int group, v, threads;
 };
 static NormShape norm_shape(int hidden) {
-  const int units = (hidden + 7) / 8, v = units <= 1024 ? 1 : 2;
-  return {v, ((units + v - 1) / v + 63) / 64 * 64};
+  const int units = (hidden + 7) / 8;
+  if (units <= 64) return {units <= 16 ? 16 : 64, 1, 256};
+  const int v = units <= 1024 ? 1 : 2;
+  return {0, v, ((units + v - 1) / v + 63) / 64 * 64};
 }
+static int norm_groups_of_block(const NormShape& s) { return s.group ? s.threads / s.group : 1; }
 
-// Workgroups of a pass by the waves a CU gets, two workgroups at least. (The forward pass with 64, twice what a
-// CU holds, 152 us for 16384 tokens of 4096, with 32 157 us, with a workgroup a token 218.)
-static int norm_blocks(int64_t tokens, int hidden, int waves) {
-  const int64_t per_cu = waves * 64 / norm_shape(hidden).threads, want = 256 * (per_cu > 2 ? per_cu : 2);
-  return (int)(tokens < want ? tokens : want);
+// Workgroups of a pass by the waves a CU gets, `least` at least. (The forward pass with 64, twice what a CU holds,
+// 152 us for 16384 tokens of 4096, with 32 157 us, with a workgroup a token 218.)
+static int norm_blocks(int64_t tokens, const NormShape& s, int waves, int least) {
+  const int64_t per_cu = waves * 64 / s.threads, want = 256 * (per_cu > least ? per_cu : least);
+  const int64_t most = (tokens + norm_groups_of_block(s) - 1) / norm_groups_of_block(s);
+  return (int)(most < want ? most : want);
 }
-// The gradient pass adds a row a workgroup to the second launch's work: 8 tokens each or more, unless that
-// leaves CUs without one.
+// The gradient pass has what a CU holds at once, one workgroup of long rows (4001 tokens of 5120: 68.5 us, two in turn
+// 72.8), and adds a row a workgroup to the second launch's work: 8 tokens a group or more, unless that leaves
+// CUs without one.
 static int norm_grad_blocks(int64_t tokens, int hidden) {
-  const int64_t most = tokens / 8 > 512 ? tokens / 8 : 512, blocks = norm_blocks(tokens, hidden, 16);
+  const NormShape s = norm_shape(hidden);
+  const int64_t each = 8 * norm_groups_of_block(s), most = tokens / each > 512 ? tokens / each : 512;
+  const int64_t blocks = norm_blocks(tokens, s, 16, 1);
   return (int)(blocks < most ? blocks : most);
 }
-
 static NormArgs norm_args(const char* name, const wm_block_norm_form* f, const void* residual, const void* y, int tokens,
                           int hidden) {
   const std::string n(name);
@@ -448,36 +551,39 @@ static void norm_aligned(const char* name, const wm_block_norm_form* f, std::ini
     fail(std::string(name) + ": tensors must be aligned to their elements");
 }
 
-// The kernels' instances: the residual's type, 8 columns a thread in up to 512 or 1024 threads or 16 in up to
-// 1024 (fewer threads leave each more registers), whole rows of eights or not, the gate.
-#define WM_NORM_GATES(KERNEL, F, V, W, N, ...)                                                          \
-  switch (gate) {                                                                                      \
-    case GATE_NONE: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_NONE, N>), __VA_ARGS__); break;           \
-    case GATE_TOKEN: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_TOKEN, N>), __VA_ARGS__); break;         \
-    case GATE_CHANNEL: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_CHANNEL, N>), __VA_ARGS__); break;     \
-    case GATE_FULL: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_FULL, N>), __VA_ARGS__); break;           \
-    default: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_FULL_F32, N>), __VA_ARGS__);                     \
+// The kernels' instances: the residual's type, the gate, whole rows of eights or not, and the shapes that
+// norm_shape gives; fewer threads a workgroup leave each more registers.
+#define WM_NORM_GATES(KERNEL, F, V, W, G, N, ...)                                                          \
+  switch (gate) {                                                                                         \
+    case GATE_NONE: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_NONE, G, N>), __VA_ARGS__); break;           \
+    case GATE_TOKEN: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_TOKEN, G, N>), __VA_ARGS__); break;         \
+    case GATE_CHANNEL: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_CHANNEL, G, N>), __VA_ARGS__); break;     \
+    case GATE_FULL: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_FULL, G, N>), __VA_ARGS__); break;           \
+    default: hipLaunchKernelGGL((KERNEL<F, V, W, GATE_FULL_F32, G, N>), __VA_ARGS__);                     \
   }
-#define WM_NORM_WHOLE(KERNEL, F, V, N, ...)                              \
-  if (a.hidden % 8 == 0) { WM_NORM_GATES(KERNEL, F, V, true, N, __VA_ARGS__) } \
-  else { WM_NORM_GATES(KERNEL, F, V, false, N, __VA_ARGS__) }
-#define WM_NORM_SHAPES(KERNEL, F, ...)                                                   \
-  if (shape.v == 2) { WM_NORM_WHOLE(KERNEL, F, 2, 1024, __VA_ARGS__) }                   \
-  else if (shape.threads > 512) { WM_NORM_WHOLE(KERNEL, F, 1, 1024, __VA_ARGS__) }       \
-  else { WM_NORM_WHOLE(KERNEL, F, 1, 512, __VA_ARGS__) }
+#define WM_NORM_WHOLE(KERNEL, F, V, G, N, ...)                                    \
+  if (a.hidden % 8 == 0) { WM_NORM_GATES(KERNEL, F, V, true, G, N, __VA_ARGS__) } \
+  else { WM_NORM_GATES(KERNEL, F, V, false, G, N, __VA_ARGS__) }
+#define WM_NORM_SHAPES(KERNEL, F, ...)                                                     \
+  if (shape.group == 16) { WM_NORM_WHOLE(KERNEL, F, 1, 16, 256, __VA_ARGS__) }             \
+  else if (shape.group == 64) { WM_NORM_WHOLE(KERNEL, F, 1, 64, 256, __VA_ARGS__) }        \
+  else if (shape.v == 2) { WM_NORM_WHOLE(KERNEL, F, 2, 0, 1024, __VA_ARGS__) }             \
+  else if (shape.threads > 512) { WM_NORM_WHOLE(KERNEL, F, 1, 0, 1024, __VA_ARGS__) }      \
+  else { WM_NORM_WHOLE(KERNEL, F, 1, 0, 512, __VA_ARGS__) }
 #define WM_NORM_LAUNCH(KERNEL, ...)                                                       \
-  const NormShape shape = norm_shape(a.hidden);                                           \
   const int gate = a.gate_kind == GATE_FULL && a.gate_f32 ? GATE_FULL_F32 : a.gate_kind;  \
   const dim3 threads(shape.threads);                                                      \
   if (f32) { WM_NORM_SHAPES(KERNEL, true, __VA_ARGS__) } else { WM_NORM_SHAPES(KERNEL, false, __VA_ARGS__) }
 
 static void norm_forward(const NormArgs& a, bool f32, void* residual_out, uint16_t* x, hipStream_t s) {
-  const dim3 blocks((unsigned)norm_blocks(a.tokens, a.hidden, 64));
+  const NormShape shape = norm_shape(a.hidden);
+  const dim3 blocks((unsigned)norm_blocks(a.tokens, shape, 64, 2));
   WM_NORM_LAUNCH(block_norm_kernel, blocks, threads, 0, s, a, residual_out, x)
   check_launch("block_norm");
 }
 
 static void norm_grad(const NormArgs& a, bool f32, const NormGrads& d, int grid, hipStream_t s) {
+  const NormShape shape = norm_shape(a.hidden);
   const dim3 blocks((unsigned)grid);
   WM_NORM_LAUNCH(block_norm_grad_kernel, blocks, threads, 0, s, a, d)
   check_launch("block_norm_grad");
