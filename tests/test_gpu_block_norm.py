@@ -255,3 +255,18 @@ def test_other_stream_and_graph_replays(device):
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
             if k == 0:
                 assert all(torch.equal(a, b) for a, b in zip(outs, first))
+
+
+def test_offsets_past_2_31_elements(device):
+    """Rows far into a tensor give what the same rows give by themselves, bit for bit."""
+    T, H, last = 131100, 16384, 3
+    gen = torch.Generator(device).manual_seed(2)
+    y = torch.randn(T, H, generator=gen, device=device, dtype=torch.bfloat16)
+    w = torch.ones(H, device=device, dtype=torch.bfloat16)
+    x, r = wa.block_norm(y, y, w, w, y)
+    xl, rl = wa.block_norm(y[-last:], y[-last:], w, w, y[-last:])
+    assert torch.equal(x[-last:], xl) and torch.equal(r[-last:], rl)
+    d = wa.block_norm_backward(x, y, r, y, w, w, y)
+    dl = wa.block_norm_backward(xl, y[-last:], rl, y[-last:], w, w, y[-last:])
+    for name in ("residual", "y", "gate"):
+        assert torch.equal(getattr(d, name)[-last:], getattr(dl, name)), name

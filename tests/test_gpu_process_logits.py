@@ -253,3 +253,17 @@ def test_feeds_acceptance(device):
     draft = wa.process_logits(torch.randn(n, V, device=device), log_probs=True)
     out = wa.mtp_verify_rejection(target, draft, drafts, torch.rand(n + 1, device=device)).tolist()
     assert 2 <= out[0] <= n and 0 <= out[1] < V    # the first two drafts are all but certain
+
+
+def test_offsets_past_2_31_elements(device):
+    """The last of so many rows that offsets pass 31 bits, at the largest vocabulary."""
+    R, V = 520, 4194304
+    gen = torch.Generator(device).manual_seed(4)
+    logits = torch.randn(R, V, generator=gen, device=device)
+    kw = dict(history=torch.randint(0, V, (1, 5000), generator=gen, device=device, dtype=torch.int32),
+              mask=torch.randint(-2 ** 31, 2 ** 31 - 1, (1, V // 32), generator=gen, device=device).to(torch.int32))
+    rows = dict(repetition=torch.full((R,), 1.5, device=device), temperature=torch.full((R,), 0.7, device=device))
+    for log_probs in (False, True):
+        out = wa.process_logits(logits, log_probs=log_probs, **kw, **rows)
+        want = want_logits(logits[-1:], log_probs=log_probs, **kw, **{k: v[-1:] for k, v in rows.items()})
+        check("last row", out[-1:], want)

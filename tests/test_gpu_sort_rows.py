@@ -220,3 +220,39 @@ def test_other_stream_and_graph_replays(device):
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
         del eager
+
+
+@pytest.mark.parametrize("T,K,H,dtype", [(9001, 4, 3001, "bf16"),     # rows past 192 MiB, odd rows
+                                         (9000, 4, 3008, "fp32"),     # gradients past 384 MiB, whole lines
+                                         (16400, 8, 16384, "bf16")])  # offsets past 2^31 elements
+def test_large_tensors(device, T, K, H, dtype):
+    """Moved rows exact; the sums of the first and last tokens and of some between against 64 bits."""
+    E, dt = 64, DTYPES[dtype]
+    gen = torch.Generator(device).manual_seed(T)
+    x = torch.randn(T, H, generator=gen, device=device, dtype=torch.float32).to(dt)
+    idx = torch.randint(0, E + 1, (T, K), generator=gen, device=device).to(torch.int32)  # E: no expert
+    rows, p = wa.sort_tokens(x, idx, E)
+    order, inverse, offsets, _, _ = want_lists(idx.cpu().numpy(), E, 128)
+    np.testing.assert_array_equal(p.order.cpu().numpy(), order)
+    np.testing.assert_array_equal(p.inverse.cpu().numpy(), inverse)
+    n = int(offsets[-1])
+    for a in range(0, n, 8192):
+        b = min(a + 8192, n)
+        assert torch.equal(rows[a:b], x[p.order[a:b].long() // K])
+    assert not rows[n:].any()
+    some = [0, 1, T // 3, T // 2, T - 2, T - 1]
+    live = inverse.reshape(T, K)[some] >= 0
+    at = torch.from_numpy(np.maximum(inverse.reshape(T, K)[some], 0)).to(device)
+    w = torch.randn(T, K, generator=gen, device=device)
+    own = f64(rows[at]) * live[..., None]
+    check(wa.sort_tokens_backward(rows, p, K)[some], own.sum(1), K, np.abs(own).sum(1))
+    terms = own * f64(w[some])[..., None]
+    check(wa.combine_rows(rows, w, p)[some], terms.sum(1), K, np.abs(terms).sum(1))
+    drows, dw = wa.combine_rows_backward(x, rows, w, p)
+    assert not drows[n:].any()
+    want = f64(w[some])[..., None] * f64(x[some])[:, None]
+    for t, k in np.ndindex(len(some), K):
+        if live[t, k]:
+            check(drows[at[t, k]], want[t, k], 0, np.abs(want[t, k]))
+    dots = own * f64(x[some])[:, None]
+    check(dw[some], dots.sum(-1), -(-H // 64) + 64, np.abs(dots).sum(-1), torch.float32)
