@@ -19,6 +19,7 @@ def sort_args(**kw):
     ({"tokens": -1}, "negative"), ({"k": 0}, "k must be"), ({"k": 65}, "k must be"), ({"hidden": 0}, "hidden must be"),
     ({"hidden": 1 << 21}, "hidden must be"), ({"fp32": 2}, "fp32 must be"), ({"experts": 0}, "experts must be"),
     ({"experts": 1025}, "experts must be"), ({"tile_rows": 0}, "tile_rows"), ({"tokens": 1 << 30, "k": 2}, "below 2"),
+    ({"tokens": 2 ** 31 - 1, "k": 1}, "too many rows"),
     ({"x": None}, "null pointer"), ({"indices": None}, "null pointer"), ({"rows": None}, "null pointer"),
     ({"offsets": None}, "null pointer"), ({"workspace": None, "tokens": 1 << 20}, "null pointer"),
     ({"workspace_bytes": 8, "tokens": 1 << 20}, "workspace too small"),
@@ -48,6 +49,9 @@ def test_rows_c_refusals():
     for call, kw in ((backward, {"dx": A + 1}), (combine, {"add": A + 1}), (combine, {"fp32": 1, "y": A + 2}), (grads, {"dy": A + 1})):
         with pytest.raises(_lib.WhallmError, match="aligned"):
             call(**kw)
+    for call in (backward, combine, grads):
+        with pytest.raises(_lib.WhallmError, match="too many rows"):
+            call(tokens=1 << 24, k=1, hidden=4096)
     for kw in ({"present": None}, {"drows": None}, {"dweights": None}):
         with pytest.raises(_lib.WhallmError, match="null pointer"):
             grads(**kw)
@@ -180,7 +184,8 @@ def logits_call(logits=A, fp32=1, rows=2, vocab=100, log_probs=1, out=A, ws=A, w
 
 @pytest.mark.parametrize("kw,msg", [
     ({"rows": -1}, "rows must"), ({"vocab": 0}, "vocab must"), ({"vocab": (1 << 22) + 1}, "vocab must"), ({"fp32": 3}, "fp32 must"),
-    ({"rows": 1 << 30, "vocab": 1 << 22}, "too many rows"), ({"history": A, "history_len": 1 << 20}, "history_len"),
+    ({"rows": 1 << 30, "vocab": 1 << 22}, "too many rows"), ({"rows": 1 << 24}, "too many rows"),
+    ({"history": A, "history_len": 1 << 20}, "history_len"),
     ({"history": A, "history_len": -1}, "history_len"), ({"biases": 2048}, "biases must"), ({"biases": -1}, "biases must"),
     ({"history_stride": -1}, "strides"), ({"lengths": A}, "without a history"), ({"prompt_lengths": A}, "without a history"),
     ({"bias_ids": A}, "go together"), ({"bias_values": A}, "go together"), ({"logits": None}, "null pointer"),
@@ -207,6 +212,22 @@ def test_process_logits_python_refusals():
             ((logits,), {"bias_ids": i32(3, 2)}, "go together"), ((logits,), {"bias_ids": i32(3, 2), "bias_values": torch.zeros(3, 3)}, "one shape"),
             ((logits,), {"mask": i32(3, 1)}, "a bit for every token"), ((logits,), {"mask": torch.zeros(3, 2).bool()}, "mask must be"),
             ((logits,), {"out": torch.zeros(3, 40).bfloat16()}, "out must be"), ((logits,), {"out": torch.zeros(40, 3).t()}, "out must be"),
+            ((logits,), {"out": torch.zeros(124)[4:].view(3, 40).requires_grad_()}, "autograd"),
+            ((logits,), {"temperature": torch.ones(3).requires_grad_()}, "autograd"),
             ((logits.clone().requires_grad_(),), {}, "autograd")):
         with pytest.raises(ValueError, match=msg):
             ops.process_logits(*args, **kw)
+
+
+def test_outputs_that_overlap_an_input_partly():
+    buf = torch.zeros(64)
+    rows = lambda at: buf[at:at + 24].view(3, 8)  # noqa: E731
+    y = torch.zeros(3, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.block_norm(rows(0), y, residual_out=rows(4))
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.block_norm(rows(0), buf[30:42].view(torch.bfloat16).view(3, 8), residual_out=rows(24))
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.process_logits(rows(0), out=rows(8))
+    with pytest.raises(ValueError, match="device"):          # the input itself is fine
+        ops.process_logits(rows(0), out=rows(0))

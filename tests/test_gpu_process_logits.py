@@ -267,3 +267,13 @@ def test_offsets_past_2_31_elements(device):
         out = wa.process_logits(logits, log_probs=log_probs, **kw, **rows)
         want = want_logits(logits[-1:], log_probs=log_probs, **kw, **{k: v[-1:] for k, v in rows.items()})
         check("last row", out[-1:], want)
+
+
+def test_autograd_sees_an_output_change(device):
+    x = torch.randn(2, 50, device=device, requires_grad=True)
+    logits = x * 1.0
+    loss = (logits * logits).sum()                           # keeps logits for its backward pass
+    with torch.no_grad():
+        wa.process_logits(logits, out=logits, temperature=torch.full((2,), 0.5, device=device))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

@@ -5,6 +5,7 @@
 //
 // Errors: ValueError for what the call refuses, before anything is allocated or launched; WhallmError with
 // wm_last_error() where the C call does.
+#include <ATen/MemoryOverlap.h>
 #include <torch/extension.h>
 
 #include <initializer_list>
@@ -104,6 +105,18 @@ void checked(const char* name, Call call) {
     PyErr_SetString(error.ptr(), (std::string(name) + ": " + message).c_str());
     throw py::error_already_set();
   }
+}
+
+// The caller's `out` is written where the inputs are read: it may be one of them and must not lie partly over one.
+void own_out(const Maybe& out, const char* name, std::initializer_list<const Tensor*> inputs) {
+  if (!out) return;
+  for (const Tensor* t : inputs)
+    if (t && at::get_overlap_status(*out, *t) == at::MemOverlapStatus::Partial)
+      refuse(std::string(name) + " must be an input itself or share no memory with one");
+}
+// Autograd sees that `out` was written.
+void changed(const Maybe& out) {
+  if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
 }
 
 Tensor empty(at::IntArrayRef shape, at::ScalarType type, c10::Device device) {
@@ -272,17 +285,19 @@ NormForm norm_form(const Tensor& residual, const Tensor& y, const Maybe& post, c
 std::tuple<Tensor, Tensor> block_norm(const Tensor& residual_, const Tensor& y, const Maybe& post, const Maybe& pre,
                                       const Maybe& gate, bool gate_sigmoid, double scale, double eps, double weight_offset,
                                       bool post_norm, const Maybe& out) {
-  no_autograd("block_norm", "its gradients are block_norm_backward's", {&residual_, &y, ptr(post), ptr(pre), ptr(gate)});
+  no_autograd("block_norm", "its gradients are block_norm_backward's", {&residual_, &y, ptr(post), ptr(pre), ptr(gate), ptr(out)});
   const NormForm f = norm_form(residual_, y, post, pre, gate, gate_sigmoid, scale, eps, weight_offset, post_norm);
   if (out && (out->scalar_type() != residual_.scalar_type() || out->sizes() != residual_.sizes() || !out->is_contiguous()))
     refuse("residual_out must be a contiguous tensor shaped and typed like residual");
   const Tensor residual = residual_.contiguous();
+  own_out(out, "residual_out", {&residual, &f.y, ptr(f.post), ptr(f.pre), ptr(f.gate)});
   const c10::Device device = device_of({&residual, &f.y, ptr(f.post), ptr(f.pre), ptr(f.gate), ptr(out)});
   const On on(device);
   const Tensor residual_out = out ? *out : at::empty_like(residual), x = at::empty_like(f.y);
   checked("wm_block_norm", [&] {
     return wm_block_norm(&f.c, at_of(residual), at_of(f.y), (int32_t)f.T, (int32_t)f.H, at_of(residual_out), at_of(x), on.stream);
   });
+  changed(out);
   return {x, residual_out};
 }
 
@@ -339,7 +354,8 @@ Maybe row_lists(const Maybe& t, int64_t rows, at::ScalarType type, const char* n
 Tensor process_logits(const Tensor& logits_, const Maybe& history_, const Maybe& lengths_, const Maybe& prompt_lengths_,
                       const Maybe& repetition_, const Maybe& frequency_, const Maybe& presence_, const Maybe& bias_ids_,
                       const Maybe& bias_values_, const Maybe& mask_, const Maybe& temperature_, bool log_probs, const Maybe& out_) {
-  no_autograd("process_logits", "it has no gradient", {&logits_, ptr(bias_values_)});
+  no_autograd("process_logits", "it has no gradient",
+              {&logits_, ptr(repetition_), ptr(frequency_), ptr(presence_), ptr(bias_values_), ptr(temperature_), ptr(out_)});
   const Tensor logits = rows_of(logits_, "logits");
   if (logits.dim() != 2 || logits.size(1) < 1) refuse("logits must be [rows, vocab]");
   const int64_t R = logits.size(0), V = logits.size(1);
@@ -364,6 +380,7 @@ Tensor process_logits(const Tensor& logits_, const Maybe& history_, const Maybe&
   if (mask && mask->size(1) != (V + 31) / 32) refuse("mask must hold a bit for every token, 32 in a word");
   if (out_ && (out_->scalar_type() != at::kFloat || out_->sizes() != logits.sizes() || !out_->is_contiguous()))
     refuse("out must be a contiguous float32 tensor shaped like logits");
+  own_out(out_, "out", {&logits, ptr(history), ptr(bias_ids), ptr(bias_values), ptr(mask)});
   const c10::Device device = device_of({&logits, ptr(history), ptr(lengths), ptr(prompts), ptr(repetition), ptr(frequency),
                                         ptr(presence), ptr(bias_ids), ptr(bias_values), ptr(mask), ptr(temperature), ptr(out_)});
   const On on(device);
@@ -387,6 +404,7 @@ Tensor process_logits(const Tensor& logits_, const Maybe& history_, const Maybe&
     return wm_process_logits(at_of(logits), is_f32(logits), (int32_t)R, (int32_t)V, &r, log_probs, static_cast<float*>(at_of(out)),
                              at_of(ws), ws_bytes, on.stream);
   });
+  changed(out_);
   return out;
 }
 

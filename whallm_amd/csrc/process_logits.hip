@@ -399,7 +399,7 @@ WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, 
     if (!rules) fail("wm_process_logits: null rules");
     if (rows < 0) fail("wm_process_logits: rows must not be negative");
     if (vocab < 1 || vocab > 1 << 22) fail("wm_process_logits: vocab must be in 1..4194304");
-    if (rows * logit_chunks(rows, vocab) > (int64_t)0x7fffffff) fail("wm_process_logits: too many rows");
+    grid_of("wm_process_logits", rows * logit_chunks(rows, vocab), LOGIT_THREADS);
     if (fp32 != 0 && fp32 != 1) fail("wm_process_logits: fp32 must be 0 (bf16 logits) or 1");
     const wm_logit_rules& r = *rules;
     if (r.history_len < 0 || r.history_len > LOGIT_MAX_HISTORY) fail("wm_process_logits: history_len must be in 0..1048575");

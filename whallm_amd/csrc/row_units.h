@@ -129,11 +129,16 @@ struct RowGrid {
   int log2;
   dim3 grid;
 };
-inline RowGrid row_grid(int64_t rows, int64_t units) {
+// Workgroups of one launch dimension, whose threads HIP counts in 32 bits.
+inline unsigned grid_of(const char* name, int64_t blocks, int threads) {
+  if (blocks * threads > 0xffffffffll) fail(std::string(name) + ": too many rows for one launch");
+  return (unsigned)blocks;
+}
+inline RowGrid row_grid(const char* name, int64_t rows, int64_t units) {
   int log2 = 0;
   while (log2 < 8 && (1 << log2) < units) ++log2;
   const int64_t per = 256 >> log2;
-  return {log2, dim3((unsigned)((rows + per - 1) / per), (unsigned)((units + (1 << log2) - 1) >> log2))};
+  return {log2, dim3(grid_of(name, (rows + per - 1) / per, 256), (unsigned)((units + (1 << log2) - 1) >> log2))};
 }
 
 }  // namespace wm

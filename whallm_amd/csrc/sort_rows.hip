@@ -151,7 +151,8 @@ __device__ __forceinline__ void sort_lists(const SortArgs& a, int32_t* count, in
   const int32_t n0 = e0 < E ? count[e0] : 0, n1 = e1 < E ? count[e1] : 0;
   int32_t present, tiles;
   const int32_t row = sort_scan(n0 + n1, &present);
-  const int32_t t0 = (n0 + a.tile_rows - 1) / a.tile_rows, t1 = (n1 + a.tile_rows - 1) / a.tile_rows;
+  const uint32_t per = a.tile_rows;  // the sums below pass 31 bits
+  const int32_t t0 = (int32_t)((n0 + per - 1) / per), t1 = (int32_t)((n1 + per - 1) / per);
   const int32_t tile = sort_scan(t0 + t1, &tiles);
   if (e0 < E) a.offsets[e0] = first[e0] = row, tile_start[e0] = tile;
   if (e1 < E) a.offsets[e1] = first[e1] = row + n0, tile_start[e1] = tile + t0;
@@ -352,18 +353,19 @@ static void sort_launch(SortArgs a, int32_t* workspace, hipStream_t s) {
     check_launch("sort_few");
     return;
   }
+  const int64_t chunks = (a.tokens + a.chunk_tokens - 1) / a.chunk_tokens;
+  const unsigned blocks = grid_of("sort", chunks + 1, SORT_THREADS);
   if (a.spans > 1) {
     hipLaunchKernelGGL(sort_spans_kernel, dim3(a.spans), dim3(SORT_THREADS), 0, s, a, workspace);
     check_launch("sort_spans");
     a.span_counts = workspace;
   }
-  const int64_t chunks = (a.tokens + a.chunk_tokens - 1) / a.chunk_tokens;
   // columns are split, by whole waves, until the chip has work for every CU
   const int64_t most = (a.row.units + 255) / 256;
   int64_t splits = chunks >= 512 ? 1 : (511 + chunks) / chunks;
   if (splits > most) splits = most;
   a.split_units = (int)(((a.row.units + splits - 1) / splits + 63) / 64 * 64);
-  const dim3 grid((unsigned)chunks + 1, (unsigned)((a.row.units + a.split_units - 1) / a.split_units));
+  const dim3 grid(blocks, (unsigned)((a.row.units + a.split_units - 1) / a.split_units));
   // Rows of more than the 256 MB cache keeps beside the rest are stored past it, where they are whole 128-byte
   // lines: 250 MB of 8 KB rows 62 us, through the cache 77; 128 MB 34 and 31; 244 MB of 2000-byte rows 90 and 77.
   const bool once = pairs * a.length * 2 > 192ll << 20 && a.length % 64 == 0;
@@ -430,7 +432,7 @@ template <bool WEIGHTED>
 static void gather_sum(const void* rows, bool f32, const float* weights, const int32_t* inverse, int64_t tokens, int k,
                        int64_t hidden, const void* add, void* y, hipStream_t s) {
   const RowUnits row = row_units(hidden, f32);
-  const RowGrid g = row_grid(tokens, row.units);
+  const RowGrid g = row_grid("gather_sum", tokens, row.units);
   if (f32)
     hipLaunchKernelGGL((gather_sum_kernel<true, WEIGHTED>), g.grid, dim3(256), 0, s, rows, weights, inverse, tokens, hidden, row,
                        g.log2, k, add, y);
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
   Elem* drows = (Elem*)drows_;
   const uint32_t pairs = (uint32_t)(tokens * k);
   // the rows without a pair, spread over the tokens
-  for (int64_t r = *present_ + t; r < tokens * k; r += tokens) {
+  for (int64_t r = max(*present_, 0) + t; r < tokens * k; r += tokens) {
     for (int c = me; c < row.units; c += GROUP) {
       if (c < row.wide) store16_nt(drows + r * hidden + (int64_t)c * N, wm_u32x4{0, 0, 0, 0});
       else drows[r * hidden + (int64_t)row.wide * N + c - row.wide] = 0;
@@ -528,10 +530,10 @@ static void back_grad(const void* dy, const void* rows, const float* weights, co
                       int64_t tokens, int64_t hidden, int k, void* drows, float* dweights, hipStream_t s) {
   const RowUnits row = row_units(hidden, F32);
   if (row.units <= 64)  // 16000 tokens x 8 of 100 in bf16: 39 us, with a workgroup a token 102; of 1000 95 and 92
-    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 64>), dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, dy, rows, weights,
+    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 64>), dim3(grid_of("back_grad", (tokens + 3) / 4, 256)), dim3(256), 0, s, dy, rows, weights,
                        inverse, present, tokens, hidden, row, k, drows, dweights);
   else
-    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 256>), dim3((unsigned)tokens), dim3(256), 0, s, dy, rows, weights, inverse,
+    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 256>), dim3(grid_of("back_grad", tokens, 256)), dim3(256), 0, s, dy, rows, weights, inverse,
                        present, tokens, hidden, row, k, drows, dweights);
   check_launch("back_grad");
 }
