@@ -513,11 +513,12 @@ static int norm_blocks(int64_t tokens, const NormShape& s, int waves, int least)
   return (int)(most < want ? most : want);
 }
 // The gradient pass has what a CU holds at once, one workgroup of long rows (4001 tokens of 5120: 68.5 us, two in turn
-// 72.8), and adds a row a workgroup to the second launch's work: 8 tokens a group or more, unless that leaves
-// CUs without one.
+// 72.8), and adds a row a workgroup to the second launch's work: 8 tokens a group or more, 4 where rows are
+// short and no eights (their loads take longer), unless that leaves CUs without one: 18775 tokens of 479 with 8
+// 59.6 us, with 4 44.6; 16000 of 512 24.9 and 28.3.
 static int norm_grad_blocks(int64_t tokens, int hidden) {
   const NormShape s = norm_shape(hidden);
-  const int64_t each = 8 * norm_groups_of_block(s), most = tokens / each > 512 ? tokens / each : 512;
+  const int64_t each = (s.group && hidden % 8 ? 4 : 8) * norm_groups_of_block(s), most = tokens / each > 512 ? tokens / each : 512;
   const int64_t blocks = norm_blocks(tokens, s, 16, 1);
   return (int)(blocks < most ? blocks : most);
 }
