@@ -123,6 +123,14 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, c10::Device device) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
 
+// `n` elements of a new 1-d tensor from `first` on: a view without the dispatcher's way (0.1 us, narrow 0.5).
+Tensor part(const Tensor& whole, int64_t first, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(whole.storage_offset() + first);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 // ---------------------------------------------------------------- token rows to experts and back
 
 // The tokens of rows [T * k, H] in the order of `inverse`.
@@ -162,8 +170,8 @@ py::tuple sort_tokens(const Tensor& x_, const Tensor& indices_, int64_t experts,
                           (int32_t)experts, (int32_t)tile_rows, at_of(rows), order, inverse, offsets,
                           static_cast<int32_t*>(at_of(tiles)), count, count + 1, ws_bytes, on.stream);
   });
-  return py::make_tuple(rows, lists.narrow(0, 0, P), lists.narrow(0, P, P), lists.narrow(0, 2 * P, experts + 1), tiles,
-                        lists.narrow(0, 2 * P + experts + 1, 1));
+  return py::make_tuple(rows, part(lists, 0, P), part(lists, P, P), part(lists, 2 * P, experts + 1), tiles,
+                        part(lists, 2 * P + experts + 1, 1));
 }
 
 Tensor sort_tokens_backward(const Tensor& drows_, const Tensor& inverse, int64_t k) {
