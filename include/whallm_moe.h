@@ -153,9 +153,10 @@ WM_EXPORT int wm_permute(const int32_t* indices, int64_t pairs, int32_t experts,
  * of a batch sorted by expert, the products' rows back to their tokens, and the gradients of both
  * (the gather, inverse gather and weighted sum of qwen4_exp.py:865-904, :1048-1051; the reference
  * has no gradients). rows [tokens * k, hidden], x, y, dx, dy, add [tokens, hidden] hold bf16, or
- * fp32 where `fp32` is 1, aligned to their elements (16-byte aligned rows of a multiple of 16
- * bytes are moved 16 bytes at a time). hidden 1..1048576, k 1..64, tokens * k below 2^31. inverse
- * [tokens * k] is the row of each pair, -1 for a pair without one (wm_sort_tokens, wm_permute).
+ * fp32 where `fp32` is 1, aligned to their elements (they are moved 16 bytes at a time at any
+ * alignment). hidden 1..1048576, k 1..64, tokens * k below 2^31; a call of more rows than one launch
+ * holds (about 16 million workgroups) is refused. inverse [tokens * k] is the row of each pair, -1
+ * for a pair without one (wm_sort_tokens, wm_permute).
  * Outputs must not overlap inputs, except that y may be add. */
 /* Sorts the pairs as wm_permute does (experts 1..1024) and copies x[t] to the rows of t's pairs;
  * the lists as wm_permute's, and behind their ends: order -1, tiles (-1, -1), rows zero.
@@ -341,8 +342,7 @@ WM_EXPORT int wm_repack_router(const void* router, const void* shared_gate, int3
  * over rows of hidden values, fp32 inside, x from residual_out as it is stored. y and x bf16,
  * residual and residual_out bf16 or fp32 [tokens, hidden], weights bf16 [hidden] (null: the norm
  * alone, no offset), the gate g bf16 or fp32, through a sigmoid with gate_sigmoid. hidden 1..16384;
- * rows of a multiple of 8 values at 16-byte aligned addresses are read 16 bytes at a time, others
- * value by value. */
+ * tensors aligned to their elements. */
 typedef struct wm_block_norm_form {
   const void* post_weight;
   const void* pre_weight;
@@ -641,7 +641,8 @@ WM_EXPORT int wm_slot_cache_route_state(wm_slot_cache* cache, double* scores, in
  *                                                  hides makes its row's other values NaN
  * Every pointer of the rules is nullable (the step is left out) and every per-row value is on the
  * device, so a captured call follows them. out may be logits where they are fp32; it overlaps no
- * other input. vocab up to 4194304. workspace (log_probs only):
+ * other input. vocab up to 4194304, rows as many as one launch holds (about 8 million workgroups of
+ * 4096 tokens). workspace (log_probs only):
  * wm_process_logits_workspace_size bytes, 8-byte aligned. */
 typedef struct wm_logit_rules {
   const int32_t* history;        /* token ids, row r at history + r * history_stride (0: one

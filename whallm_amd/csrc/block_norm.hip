@@ -14,8 +14,10 @@
 // a thread, sums over the row twice at most, and goes on to its next token with the weights still in
 // registers. A group is 16 threads or a wave for short rows, whose sums need no barrier, else a workgroup. Sums
 // over tokens (weight gradients) stay with the group, go to the workspace once per workgroup and are added up
-// by a second launch in the workgroups' order. All arithmetic is fp32; bf16 outputs are rounded once, from values that no
-// earlier rounding touched but r''s own (x is the norm of the residual that the next block reads).
+// by a second launch in the workgroups' order. All arithmetic is fp32; bf16 outputs are rounded once, from
+// values that no earlier rounding touched but r''s own (x is the norm of the residual that the next block
+// reads). 16384 tokens of 4096 in fp32 take 152 us (805 MB, 5.3 TB/s), the gradients of 4001 tokens of 5120 in
+// bf16 with a full gate 67 + 5 us (328 MB, 4.9 TB/s in the first launch).
 #include <initializer_list>
 
 #include "row_units.h"
@@ -493,7 +495,8 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(const float* __restr
 }
 
 // How a row is held: by `group` threads (0: a workgroup of `threads`), 8 v columns each. Short rows have 16 threads
-// or a wave, four waves a workgroup; rows of more than 8192 columns 16 columns a thread.
+// or a wave, four waves a workgroup (16000 tokens of 100 10 us and the gradients 17, with a workgroup a row 17 and
+// 40); rows of more than 8192 columns 16 columns a thread, since a workgroup has 1024.
 struct NormShape {
   int group, v, threads;
 };

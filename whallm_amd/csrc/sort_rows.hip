@@ -10,7 +10,8 @@
 //
 // All four are bound by HBM and walk the tokens, not the permuted rows: a token's row is read or written
 // once and its k permuted rows once each. Sums are fp32 in j order, so a result does not depend on the
-// grid, and are rounded once.
+// grid, and are rounded once. 4096 tokens x 8 of 7168 in bf16: the sort 102 us (529 MB, 5.2 TB/s), back 107 us
+// (578 MB, 5.4 TB/s); 2048 x 6 of 5120 in fp32: the gradients of back 113 us (545 MB, 4.8 TB/s).
 #include "permute_device.h"
 #include "row_units.h"
 
@@ -325,7 +326,9 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
   sort_clear(a, present, blockIdx.x, (a.tokens + a.chunk_tokens - 1) / a.chunk_tokens, c0, c1);
 }
 
-// Up to this many pairs each way is taken.
+// Up to this many pairs each way is taken. 8 tokens x 10 of 2560, captured: a workgroup a token 4.3 us, the
+// counting workgroups 7.3. 32768 pairs of 136 and 1000 columns: one launch 19.2 and 30.5 us, with the spans' launch 16.2 and 26.0;
+// 16384 pairs 10.3 and 12.7.
 constexpr int64_t SORT_FEW_MAX = 256, SORT_ONE_MAX = 16384;
 
 // Spans that are counted apart: each a multiple of the chunk, of 2048 pairs or more.
@@ -375,6 +378,7 @@ static void sort_launch(SortArgs a, int32_t* workspace, hipStream_t s) {
 }
 
 // ---- back (WEIGHTED) and the sort's gradient: a thread owns one unit of a token, sums its k rows.
+// A row is read once and not again, so past the cache.
 constexpr int GATHER_BATCH = 8;  // rows in flight
 
 template <typename U, bool WEIGHTED>
