@@ -234,3 +234,32 @@ def test_two_captured_runs(device):
             for i, (a, b) in enumerate(zip(outs, want)):
                 assert torch.equal(a, b), (step, i)
         torch.cuda.synchronize(device)
+
+
+def test_inference_mode_and_grad_mode(device):
+    """The same results under inference mode, where outputs are inference tensors, and for leaves under no_grad."""
+    s = layer(device, 6, 128, 32, 5, 100, 2)
+
+    def run():
+        x, r = wa.block_norm(s["residual"].clone(), s["y"], s["post"], s["pre"], s["channel"])
+        again = r.clone()
+        wa.block_norm(again, s["y"], residual_out=again)
+        idx = (torch.arange(18, device=device, dtype=torch.int32) % 6 - 1).view(6, 3)
+        rows, p = wa.sort_tokens(x, idx, 5)
+        y = wa.combine_rows(rows, torch.ones(6, 3, device=device), p, add=x)
+        logits = wa.process_logits(wa.linear_bf16(y, s["head"]), **rules(s))
+        wa.process_logits(logits, out=logits, log_probs=True)
+        d = wa.block_norm_backward(y, r, again, s["y"], s["post"], s["pre"], s["channel"])
+        return [x, r, again, p.order, p.inverse, p.offsets, p.tile_count, y, logits, d.post_weight, d.pre_weight, d.gate]
+
+    want = run()
+    with torch.inference_mode():
+        got = run()
+        assert all(t.is_inference() for t in got)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for t in (s["residual"], s["post"], s["channel"]):
+        t.requires_grad_()
+    with pytest.raises(ValueError, match="autograd"):
+        wa.block_norm(s["residual"], s["y"], s["post"], s["pre"], s["channel"])
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(want, run()))

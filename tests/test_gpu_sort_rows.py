@@ -78,6 +78,7 @@ CASES = [
     (1000, 10, 512, 264, 128, "some"),
     (2300, 8, 128, 136, 128, "one expert"),
     (700, 64, 256, 33, 100, "some"),
+    (250, 9, 100, 4104, 128, "some"),    # a workgroup of 1024 a token
     (6, 4, 5, 16, 2 ** 31 - 1, None),    # one tile an expert, whose rows' sum passes 31 bits
     (5000, 4, 5, 16, 2 ** 31 - 1, "some"),
 ]

@@ -327,9 +327,16 @@ py::tuple block_norm_backward(const Tensor& dx_, const Maybe& dresidual_, const 
   const On on(device);
   const Tensor dr = at::empty_like(residual_out), dy = at::empty_like(f.y);
   Maybe dpost, dpre, dgate;
-  if (f.post) dpost = empty({f.H}, at::kFloat, device);
-  if (f.pre) dpre = empty({f.H}, at::kFloat, device);
-  if (f.gate) dgate = empty(f.gate->sizes(), f.c.gate_kind == 3 ? f.gate->scalar_type() : at::kFloat, device);
+  const bool channel = f.c.gate_kind == 2;
+  const int64_t columns = (f.post ? 1 : 0) + (f.pre ? 1 : 0) + channel;  // fp32 [H] each, in one allocation
+  if (columns) {
+    const Tensor sums = empty({columns * f.H}, at::kFloat, device);
+    int64_t at = 0;
+    if (f.post) dpost = part(sums, at, f.H), at += f.H;
+    if (f.pre) dpre = part(sums, at, f.H), at += f.H;
+    if (channel) dgate = part(sums, at, f.H);
+  }
+  if (f.gate && !channel) dgate = empty(f.gate->sizes(), f.c.gate_kind == 3 ? f.gate->scalar_type() : at::kFloat, device);
   const size_t ws_bytes = wm_block_norm_backward_workspace_size((int32_t)f.T, (int32_t)f.H);
   const Tensor ws = empty({(int64_t)ws_bytes}, at::kByte, device);
   checked("wm_block_norm_backward", [&] {

@@ -446,21 +446,21 @@ static void gather_sum(const void* rows, bool f32, const float* weights, const i
   check_launch("gather_sum");
 }
 
-// ---- the gradients of back: GROUP threads a token, a wave or a workgroup. Each thread holds the same units of dy
+// ---- the gradients of back: GROUP threads a token, a wave or a workgroup of 256 or 1024. Each thread holds the same units of dy
 // for a batch of pairs, so a pair's row is read once, its gradient written, and its dot product summed over the
 // group.
 constexpr int BACK_BATCH = 8;
 
-template <bool F32, bool ONCE, int GROUP>
-__global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__ dy_, const void* __restrict__ rows_,
+template <bool F32, bool ONCE, int GROUP, int THREADS>
+__global__ void __launch_bounds__(THREADS) back_grad_kernel(const void* __restrict__ dy_, const void* __restrict__ rows_,
                                                        const float* __restrict__ weights, const int32_t* __restrict__ inverse,
                                                        const int32_t* __restrict__ present_, int64_t tokens, int64_t hidden,
                                                        RowUnits row, int k, void* __restrict__ drows_,
                                                        float* __restrict__ dweights) {
   typedef typename RowUnit<F32, true>::Elem Elem;
   constexpr int N = RowUnit<F32, true>::N;
-  __shared__ float part[BACK_BATCH][4];
-  const int64_t t = blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
+  __shared__ float part[BACK_BATCH][GROUP / 64];
+  const int64_t t = blockIdx.x * (THREADS / GROUP) + threadIdx.x / GROUP;
   const int me = threadIdx.x % GROUP, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   if (t >= tokens) return;  // a whole wave, where a token has one: no barrier is ahead
   const Elem* dy = (const Elem*)dy_ + t * hidden;
@@ -523,7 +523,10 @@ __global__ void __launch_bounds__(256) back_grad_kernel(const void* __restrict__
     __syncthreads();
     if (threadIdx.x < BACK_BATCH && j0 + (int)threadIdx.x < k) {
       const float* v = part[threadIdx.x];
-      dweights[t * k + j0 + threadIdx.x] = (v[0] + v[1]) + (v[2] + v[3]);
+      float sum = 0.0f;
+#pragma unroll
+      for (int q = 0; q + 4 <= GROUP / 64; q += 4) sum += (v[q] + v[q + 1]) + (v[q + 2] + v[q + 3]);
+      dweights[t * k + j0 + threadIdx.x] = sum;
     }
     __syncthreads();
   }
@@ -534,10 +537,13 @@ static void back_grad(const void* dy, const void* rows, const float* weights, co
                       int64_t tokens, int64_t hidden, int k, void* drows, float* dweights, hipStream_t s) {
   const RowUnits row = row_units(hidden, F32);
   if (row.units <= 64)  // 16000 tokens x 8 of 100 in bf16: 39 us, with a workgroup a token 102; of 1000 95 and 92
-    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 64>), dim3(grid_of("back_grad", (tokens + 3) / 4, 256)), dim3(256), 0, s, dy, rows, weights,
+    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 64, 256>), dim3(grid_of("back_grad", (tokens + 3) / 4, 256)), dim3(256), 0, s, dy, rows, weights,
                        inverse, present, tokens, hidden, row, k, drows, dweights);
+  else if (tokens <= 256 && row.units > 256)  // a CU a token: 11 x 7 of 6016 in fp32 7.2 us, with 256 threads 10.7
+    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 1024, 1024>), dim3((unsigned)tokens), dim3(1024), 0, s, dy, rows, weights, inverse,
+                       present, tokens, hidden, row, k, drows, dweights);
   else
-    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 256>), dim3(grid_of("back_grad", tokens, 256)), dim3(256), 0, s, dy, rows, weights, inverse,
+    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 256, 256>), dim3(grid_of("back_grad", tokens, 256)), dim3(256), 0, s, dy, rows, weights, inverse,
                        present, tokens, hidden, row, k, drows, dweights);
   check_launch("back_grad");
 }
