@@ -126,6 +126,10 @@ def make(rng, R, V, L, device, dtype=torch.float32, shared=False, biases=0, mask
     (40, 1000, 257, False, 16, "none"),
     (300, 64, 17, False, 5, "one"),
     (4, 129280, 4096, True, 300, "some"),
+    (3, 20003, 9001, False, 700, "some"),     # more ids than a round of them
+    (2, 50, 20000, True, 3, None),
+    (1, 8192, 8193, False, 0, "some"),
+    (40, 130001, 8200, False, 1, None),       # and more tokens than are kept
 ])
 def test_matches_the_formula(device, R, V, L, shared, biases, mask, dtype):
     rng = np.random.default_rng(R + V + L)

@@ -15,7 +15,7 @@
 // log-probabilities with 2000 ids, 64 biases and a mask each take 49 us: 24 for the maxima, 27 to write (99 MB,
 // with 50 MB read twice). A workgroup counts its row's whole history (a few thousand tokens, from L2 after the
 // first workgroup) into one LDS word per token of the chunk, so no count table exists in memory and nothing is
-// left to clear. A word holds the answer's count (20 bits), whether a prompt holds the token (1) and the place
+// left to clear; only for long histories of few rows the first launch keeps the words for the second. A word holds the answer's count (20 bits), whether a prompt holds the token (1) and the place
 // of its bias in the list (11, the last one where a token is listed twice): integer additions and maxima, so
 // the result does not depend on their order.
 //
@@ -186,8 +186,7 @@ __device__ __forceinline__ void count_words(LogitIds& f, int lo, int n, LogitWor
 }
 
 // Penalties and bias of a unit's logits, by their words.
-__device__ __forceinline__ void apply_words(const uint32_t* words, const float* biases, const LogitRow& r, float l[LOGIT_UNIT]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(words);
+__device__ __forceinline__ void apply_words(const uint4& a, const float* biases, const LogitRow& r, float l[LOGIT_UNIT]) {
   if ((a.x | a.y | a.z | a.w) == 0) return;
   const uint32_t w[LOGIT_UNIT] = {a.x, a.y, a.z, a.w};
 #pragma unroll
@@ -196,7 +195,7 @@ __device__ __forceinline__ void apply_words(const uint32_t* words, const float* 
     if (w[e] & (LOGIT_COUNT | LOGIT_PROMPT)) l[e] *= l[e] > 0.0f ? r.inv_rep : r.rep;
     if (count) l[e] = l[e] - r.freq * (float)count - r.pres;
     const uint32_t j = w[e] >> LOGIT_BIAS_SHIFT;
-    if (j) l[e] += j <= LOGIT_THREADS ? biases[j - 1] : r.bias[j - 1];
+    if (j) l[e] += biases && j <= LOGIT_THREADS ? biases[j - 1] : r.bias[j - 1];
   }
 }
 
@@ -245,19 +244,24 @@ struct LogitChunk {
       else if (i < n) raw[k].load_part(logits, base + i, n - i);
     }
   }
-  // Logits of unit k after the rules; words null: without lists.
-  __device__ __forceinline__ void apply(int k, const uint32_t* words, const float* biases, const LogitRow& r,
+  // The words of unit k.
+  static __device__ __forceinline__ uint4 words_of(const uint32_t* words, int k) {
+    return *reinterpret_cast<const uint4*>(words + k * STEP + threadIdx.x * LOGIT_UNIT);
+  }
+  // Logits of unit k after the rules, by its words; biases null: not in LDS.
+  __device__ __forceinline__ void apply(int k, const uint4& words, const float* biases, const LogitRow& r,
                                         float l[LOGIT_UNIT]) const {
     raw[k].unpack(l);
-    if (words) apply_words(words + k * STEP + threadIdx.x * LOGIT_UNIT, biases, r, l);
+    apply_words(words, biases, r, l);
     mask_and_scale((uint32_t)mask[k] >> (threadIdx.x % 2 * LOGIT_UNIT), r.mask != nullptr, r.inv_temp, l);
   }
 };
 
 // The maximum and the sum of a chunk: in part[0] .. of the waves.
-template <bool F32, int PER, bool WHOLE>
+template <bool F32, int PER, bool WHOLE, bool KEPT>
 __device__ __forceinline__ void chunk_stats(const void* logits, int vocab, const wm_logit_rules& r, int row, int lo, int n,
-                                            LogitWords<LOGIT_THREADS * LOGIT_UNIT * PER>& s, LogitPart* part) {
+                                            LogitWords<LOGIT_THREADS * LOGIT_UNIT * PER>& s, LogitPart* part,
+                                            uint32_t* __restrict__ kept) {
   const bool lists = r.history || r.bias_ids;
   const LogitRow lr = logit_row(r, row);
   LogitIds f;
@@ -271,7 +275,9 @@ __device__ __forceinline__ void chunk_stats(const void* logits, int vocab, const
   for (int k = 0; k < PER; ++k) {
     const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
     if (WHOLE || i < n) {
-      c.apply(k, lists ? s.word : nullptr, s.bias, lr, l[k]);
+      const uint4 w = lists ? c.words_of(s.word, k) : make_uint4(0, 0, 0, 0);
+      if (KEPT) *reinterpret_cast<uint4*>(kept + i) = w;
+      c.apply(k, w, s.bias, lr, l[k]);
 #pragma unroll
       for (int e = 0; e < LOGIT_UNIT; ++e) {
         if (!WHOLE && i + e >= n) l[k][e] = -INFINITY;
@@ -291,16 +297,18 @@ __device__ __forceinline__ void chunk_stats(const void* logits, int vocab, const
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = p;
 }
 
-// The chunks' maxima and sums.
-template <bool F32, int PER>
+// The chunks' maxima and sums, and their words where the write kernel takes them (KEPT).
+template <bool F32, int PER, bool KEPT>
 __global__ void __launch_bounds__(LOGIT_THREADS) logit_stats_kernel(const void* __restrict__ logits, int vocab, int chunks,
-                                                                   wm_logit_rules r, LogitPart* __restrict__ parts) {
+                                                                   wm_logit_rules r, LogitPart* __restrict__ parts,
+                                                                   uint32_t* kept) {
   constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
   __shared__ __align__(16) LogitWords<CHUNK> s;
   __shared__ LogitPart part[LOGIT_THREADS / 64];
   const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
-  if (n == CHUNK) chunk_stats<F32, PER, true>(logits, vocab, r, row, lo, n, s, part);
-  else chunk_stats<F32, PER, false>(logits, vocab, r, row, lo, n, s, part);
+  if (KEPT) kept += (int64_t)blockIdx.x * CHUNK;
+  if (n == CHUNK) chunk_stats<F32, PER, true, KEPT>(logits, vocab, r, row, lo, n, s, part, kept);
+  else chunk_stats<F32, PER, false, KEPT>(logits, vocab, r, row, lo, n, s, part, kept);
   __syncthreads();
   if (threadIdx.x < 64) {
     LogitPart p = threadIdx.x < LOGIT_THREADS / 64 ? part[threadIdx.x] : LogitPart{-INFINITY, 0.0f};
@@ -309,19 +317,25 @@ __global__ void __launch_bounds__(LOGIT_THREADS) logit_stats_kernel(const void* 
   }
 }
 
-// A chunk's results. parts (nullable): the row's chunks, for log-probabilities.
-template <bool F32, int PER, bool WHOLE>
+// A chunk's results. parts (nullable): the row's chunks, for log-probabilities. KEPT: the words are in memory.
+template <bool F32, int PER, bool WHOLE, bool KEPT>
 __device__ __forceinline__ void chunk_write(const void* logits, int vocab, int chunks, const wm_logit_rules& r, int row, int lo,
                                             int n, const LogitPart* __restrict__ parts, float* out,
-                                            LogitWords<LOGIT_THREADS * LOGIT_UNIT * PER>& s, LogitPart* whole) {
+                                            LogitWords<LOGIT_THREADS * LOGIT_UNIT * PER>& s, LogitPart* whole, const uint32_t* kept) {
   const int64_t base = (int64_t)row * vocab + lo;
   const bool lists = r.history || r.bias_ids;
   const LogitRow lr = logit_row(r, row);
   LogitIds f;
-  if (lists) f.load(r, row);
+  if (!KEPT && lists) f.load(r, row);
   LogitPart o = {-INFINITY, 0.0f};
   if (parts && threadIdx.x < 64 && (int)threadIdx.x < chunks) o = parts[threadIdx.x];
   LogitChunk<F32, PER, WHOLE> c;
+  uint4 words[PER];
+  if (KEPT) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (WHOLE || (k * LOGIT_THREADS + (int)threadIdx.x) * LOGIT_UNIT < n) words[k] = c.words_of(kept, k);
+  }
   c.load(logits, base, lo, n, lr.mask);
   if (parts && threadIdx.x < 64) {
     LogitPart p = o;
@@ -335,7 +349,7 @@ __device__ __forceinline__ void chunk_write(const void* logits, int vocab, int c
     p = wave_part(p);
     if (threadIdx.x == 0) *whole = p;
   }
-  if (lists) count_words(f, lo, n, s);
+  if (!KEPT && lists) count_words(f, lo, n, s);
   else __syncthreads();
   const float top = parts ? finite_top(whole->top) : 0.0f, log_sum = parts ? logf(whole->sum) : 0.0f;
 #pragma unroll
@@ -343,7 +357,8 @@ __device__ __forceinline__ void chunk_write(const void* logits, int vocab, int c
     const int i = (k * LOGIT_THREADS + threadIdx.x) * LOGIT_UNIT;
     if (!WHOLE && i >= n) break;
     float l[LOGIT_UNIT];
-    c.apply(k, lists ? s.word : nullptr, s.bias, lr, l);
+    if (!KEPT) words[k] = lists ? c.words_of(s.word, k) : make_uint4(0, 0, 0, 0);
+    c.apply(k, words[k], KEPT ? nullptr : s.bias, lr, l);
     if (parts) {
 #pragma unroll
       for (int e = 0; e < LOGIT_UNIT; ++e) l[e] = l[e] == -INFINITY ? l[e] : (l[e] - top) - log_sum;
@@ -352,16 +367,18 @@ __device__ __forceinline__ void chunk_write(const void* logits, int vocab, int c
   }
 }
 
-template <bool F32, int PER>
+template <bool F32, int PER, bool KEPT>
 __global__ void __launch_bounds__(LOGIT_THREADS) logit_write_kernel(const void* logits, int vocab, int chunks, wm_logit_rules r,
-                                                                   const LogitPart* __restrict__ parts, float* out) {
+                                                                   const LogitPart* __restrict__ parts, float* out,
+                                                                   const uint32_t* __restrict__ kept) {
   constexpr int CHUNK = LOGIT_THREADS * LOGIT_UNIT * PER;
   __shared__ __align__(16) LogitWords<CHUNK> s;
   __shared__ LogitPart whole;
   const int row = blockIdx.x / chunks, lo = blockIdx.x % chunks * CHUNK, n = min(CHUNK, vocab - lo);
   const LogitPart* mine = parts ? parts + (int64_t)row * chunks : nullptr;
-  if (n == CHUNK) chunk_write<F32, PER, true>(logits, vocab, chunks, r, row, lo, n, mine, out, s, &whole);
-  else chunk_write<F32, PER, false>(logits, vocab, chunks, r, row, lo, n, mine, out, s, &whole);
+  if (KEPT) kept += (int64_t)blockIdx.x * CHUNK;
+  if (n == CHUNK) chunk_write<F32, PER, true, KEPT>(logits, vocab, chunks, r, row, lo, n, mine, out, s, &whole, kept);
+  else chunk_write<F32, PER, false, KEPT>(logits, vocab, chunks, r, row, lo, n, mine, out, s, &whole, kept);
 }
 
 // Units of a thread, by how many workgroups the rows make: 64 rows of 129,280 23.2 us with four, 26.0 with two; one row
@@ -374,16 +391,33 @@ static int64_t logit_chunks(int64_t rows, int64_t vocab) {
   return (vocab + chunk - 1) / chunk;
 }
 
+// Words that the chunks' statistics keep for the write kernel, which then reads no list: where a history is longer
+// than a round of ids and the words are few. Log-probabilities of 4 rows with 32768 ids 12.4 us, counted twice 16.6;
+// 15 rows of 18000 13.3 and 15.3, of 4000 11.9 and 11.7; 64 rows of 4096 32.9 and 27.7.
+constexpr int LOGIT_KEEP_HISTORY = 16 * LOGIT_THREADS;
+static int64_t logit_kept(int64_t rows, int64_t vocab) {
+  const int64_t words = logit_chunks(rows, vocab) * rows * LOGIT_THREADS * LOGIT_UNIT * logit_per(rows, vocab);
+  return words <= 1 << 22 ? words : 0;
+}
+
 template <bool F32, int PER>
 static void process_logits(const void* logits, int rows, int vocab, const wm_logit_rules& r, float* out, LogitPart* parts,
-                           hipStream_t s) {
+                           uint32_t* kept, hipStream_t s) {
   const int chunks = (int)logit_chunks(rows, vocab);
   const dim3 grid((unsigned)(rows * chunks));
   if (parts) {
-    hipLaunchKernelGGL((logit_stats_kernel<F32, PER>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts);
+    if (kept)
+      hipLaunchKernelGGL((logit_stats_kernel<F32, PER, true>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts, kept);
+    else
+      hipLaunchKernelGGL((logit_stats_kernel<F32, PER, false>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts, kept);
     check_launch("logit_stats");
   }
-  hipLaunchKernelGGL((logit_write_kernel<F32, PER>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts, out);
+  if (kept)
+    hipLaunchKernelGGL((logit_write_kernel<F32, PER, true>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts, out,
+                       kept);
+  else
+    hipLaunchKernelGGL((logit_write_kernel<F32, PER, false>), grid, dim3(LOGIT_THREADS), 0, s, logits, vocab, chunks, r, parts,
+                       out, kept);
   check_launch("logit_write");
 }
 
@@ -395,7 +429,7 @@ extern "C" {
 
 WM_EXPORT size_t wm_process_logits_workspace_size(int32_t rows, int32_t vocab) {
   if (rows < 0 || vocab < 1) return 0;
-  return (size_t)(rows * logit_chunks(rows, vocab)) * sizeof(LogitPart);
+  return (size_t)(rows * logit_chunks(rows, vocab)) * sizeof(LogitPart) + 8 + logit_kept(rows, vocab) * sizeof(uint32_t);
 }
 
 WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab, const wm_logit_rules* rules,
@@ -419,9 +453,12 @@ WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, 
     if (log_probs && (!workspace || workspace_bytes < wm_process_logits_workspace_size(rows, vocab) || (uintptr_t)workspace % 8))
       fail("wm_process_logits: workspace too small or misaligned");
     LogitPart* parts = log_probs ? (LogitPart*)workspace : nullptr;
+    uint32_t* kept = nullptr;  // behind the parts, at 16 bytes
+    if (log_probs && r.history && r.history_len > LOGIT_KEEP_HISTORY && logit_kept(rows, vocab) > 0)
+      kept = (uint32_t*)(((uintptr_t)(parts + rows * logit_chunks(rows, vocab)) + 15) / 16 * 16);
     hipStream_t s = as_stream(stream);
     const int per = logit_per(rows, vocab);
-#define WM_LOGITS(F, P) process_logits<F, P>(logits, rows, vocab, r, out, parts, s)
+#define WM_LOGITS(F, P) process_logits<F, P>(logits, rows, vocab, r, out, parts, kept, s)
     if (fp32) {
       if (per == 4) WM_LOGITS(true, 4); else WM_LOGITS(true, 2);
     } else {
