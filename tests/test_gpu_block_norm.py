@@ -270,3 +270,23 @@ def test_offsets_past_2_31_elements(device):
     dl = wa.block_norm_backward(xl, y[-last:], rl, y[-last:], w, w, y[-last:])
     for name in ("residual", "y", "gate"):
         assert torch.equal(getattr(d, name)[-last:], getattr(dl, name)), name
+
+
+@pytest.mark.parametrize("T,H,residual", [(5, 96, "fp32"), (300, 1000, "bf16"), (700, 6152, "bf16"), (3, 9000, "fp32")])
+def test_gradients_written_over_what_came_in(device, T, H, residual):
+    """The C call's dresidual may be dresidual_out and its dy may be dx."""
+    from whallm_amd import _lib
+    rng = np.random.default_rng(H)
+    s = make(rng, T, H, device, residual, gate="full", gate_type="bf16")
+    dx, dres = randn(rng, (T, H), torch.bfloat16, device), randn(rng, (T, H), TYPES[residual], device)
+    r_out = s.pop("residual")
+    want = wa.block_norm_backward(dx, dres, r_out, **s)
+    dpost, dpre, dgate = torch.empty(H, device=device), torch.empty(H, device=device), torch.empty_like(s["gate"])
+    form = _lib.BlockNormFormC(s["post_weight"].data_ptr(), s["pre_weight"].data_ptr(), s["gate"].data_ptr(), 0.0, 1.0, 1e-6, 1, 3, 0,
+                               0, int(residual == "fp32"))
+    ws = torch.empty(_lib.load().wm_block_norm_backward_workspace_size(T, H), dtype=torch.uint8, device=device)
+    _lib.call("wm_block_norm_backward", form, dx.data_ptr(), dres.data_ptr(), r_out.data_ptr(), s["y"].data_ptr(), T, H, dres.data_ptr(),
+              dx.data_ptr(), dpost.data_ptr(), dpre.data_ptr(), dgate.data_ptr(), ws.data_ptr(), ws.numel(),
+              torch.cuda.current_stream(device).cuda_stream)
+    for got, name in ((dres, "residual"), (dx, "y"), (dpost, "post_weight"), (dpre, "pre_weight"), (dgate, "gate")):
+        assert torch.equal(got, getattr(want, name)), name

@@ -259,3 +259,18 @@ def test_large_tensors(device, T, K, H, dtype):
             check(drows[at[t, k]], want[t, k], 0, np.abs(want[t, k]))
     dots = own * f64(x[some])[:, None]
     check(dw[some], dots.sum(-1), -(-H // 64) + 64, np.abs(dots).sum(-1), torch.float32)
+
+
+@pytest.mark.parametrize("H,dtype", [(24, "bf16"), (257, "fp32"), (4099, "bf16")])
+def test_back_over_what_it_adds_to(device, H, dtype):
+    """The C call's y may be add."""
+    from whallm_amd import _lib
+    rng = np.random.default_rng(H)
+    T, K, E = 70, 5, 9
+    idx = torch.from_numpy(make_indices(rng, T, K, E, "some")).to(device)
+    rows, p = wa.sort_tokens(rows_tensor(rng, (T, H), DTYPES[dtype], device), idx, E)
+    w, add = torch.rand(T, K, device=device), rows_tensor(rng, (T, H), DTYPES[dtype], device)
+    want = wa.combine_rows(rows, w, p, add)
+    _lib.call("wm_combine_rows", rows.data_ptr(), int(dtype == "fp32"), w.data_ptr(), p.inverse.data_ptr(), T, K, H, add.data_ptr(),
+              add.data_ptr(), torch.cuda.current_stream(device).cuda_stream)
+    assert torch.equal(add, want)

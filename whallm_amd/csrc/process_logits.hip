@@ -15,9 +15,10 @@
 // log-probabilities with 2000 ids, 64 biases and a mask each take 49 us: 24 for the maxima, 27 to write (99 MB,
 // with 50 MB read twice). A workgroup counts its row's whole history (a few thousand tokens, from L2 after the
 // first workgroup) into one LDS word per token of the chunk, so no count table exists in memory and nothing is
-// left to clear; only for long histories of few rows the first launch keeps the words for the second. A word holds the answer's count (20 bits), whether a prompt holds the token (1) and the place
-// of its bias in the list (11, the last one where a token is listed twice): integer additions and maxima, so
-// the result does not depend on their order.
+// left to clear; only for long histories of few rows the first launch keeps the words for the second. A word
+// holds the answer's count (20 bits), whether a prompt holds the token (1) and the place of its bias in the list
+// (11, the last one where a token is listed twice): integer additions and maxima, so the result does not depend
+// on their order.
 //
 // The lists cost latency, not work: the ids' way from memory, three barriers, then the logits'. So the chunk's
 // logits, the first ids of the history and the biases are all loaded before the first barrier. A history
