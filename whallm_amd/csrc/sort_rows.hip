@@ -19,6 +19,15 @@ namespace wm {
 
 constexpr int SORT_MAX_K = 64;
 
+// Whether permuted rows are stored past the 256 MB cache: where it would not hold them for their reader beside the
+// rest, but for short rows that are no whole 128-byte lines. Sort: 256 MB of 4 KB rows 64 us past it, 82 through
+// it; 229 MB of 2002 bytes 94 and 110; 458 MB of 500 bytes 246 and 239. The gradients of back: 240 MB of 20 KB
+// 104 and 115; 458 MB of 500 bytes 437 and 395. (A call by itself after a pause 115 and 102 at 240 MB; smaller
+// ones gain as much, 128 MB of the sort 38 and 46, but their reader would lose it again.)
+static bool past_cache(int64_t pairs, int64_t row_bytes) {
+  return pairs * row_bytes > 192ll << 20 && (row_bytes > 512 || row_bytes % 128 == 0);
+}
+
 // ---- sort. A workgroup owns a chunk of tokens (256 pairs at most) and a range of units. It finds its
 // pairs' rows in LDS, and moves the tokens' units to them. Three ways to the rows, by the number of pairs:
 //   up to 256     (sort_few_kernel) a workgroup a token; each has all ids in LDS and counts, for each of its
@@ -369,9 +378,7 @@ static void sort_launch(SortArgs a, int32_t* workspace, hipStream_t s) {
   if (splits > most) splits = most;
   a.split_units = (int)(((a.row.units + splits - 1) / splits + 63) / 64 * 64);
   const dim3 grid(blocks, (unsigned)((a.row.units + a.split_units - 1) / a.split_units));
-  // Rows of more than the 256 MB cache keeps beside the rest are stored past it, where they are whole 128-byte
-  // lines: 250 MB of 8 KB rows 62 us, through the cache 77; 128 MB 34 and 31; 244 MB of 2000-byte rows 90 and 77.
-  const bool once = pairs * a.length * 2 > 192ll << 20 && a.length % 64 == 0;
+  const bool once = past_cache(pairs, a.length * 2);
   if (once) hipLaunchKernelGGL(sort_kernel<true>, grid, dim3(SORT_THREADS), 0, s, a);
   else hipLaunchKernelGGL(sort_kernel<false>, grid, dim3(SORT_THREADS), 0, s, a);
   check_launch("sort");
@@ -631,9 +638,7 @@ WM_EXPORT int wm_combine_rows_backward(const void* dy, const void* rows, int32_t
     if (((uintptr_t)dy | (uintptr_t)rows | (uintptr_t)drows) % (fp32 ? 4 : 2))
       fail("wm_combine_rows_backward: rows must be aligned to their elements");
     hipStream_t s = as_stream(stream);
-    // as for the sort, but the rows that are read go past the cache already: 250 MB 104 us past it, 88 through
-    // it; 500 MB 203 and 211
-    const bool once = (int64_t)tokens * k * hidden * (fp32 ? 4 : 2) > 384ll << 20;
+    const bool once = past_cache((int64_t)tokens * k, (int64_t)hidden * (fp32 ? 4 : 2));
 #define WM_BACK(F, O) back_grad<F, O>(dy, rows, weights, inverse, present, tokens, hidden, k, drows, dweights, s)
     if (fp32) {
       if (once) WM_BACK(true, true); else WM_BACK(true, false);
