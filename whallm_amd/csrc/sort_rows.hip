@@ -11,7 +11,7 @@
 // All four are bound by HBM and walk the tokens, not the permuted rows: a token's row is read or written
 // once and its k permuted rows once each. Sums are fp32 in j order, so a result does not depend on the
 // grid, and are rounded once. 4096 tokens x 8 of 7168 in bf16: the sort 102 us (529 MB, 5.2 TB/s), back 107 us
-// (578 MB, 5.4 TB/s); 2048 x 6 of 5120 in fp32: the gradients of back 113 us (545 MB, 4.8 TB/s).
+// (578 MB, 5.4 TB/s); 2048 x 6 of 5120 in fp32: the gradients of back 101 us (545 MB, 5.4 TB/s).
 #include "permute_device.h"
 #include "row_units.h"
 
