@@ -95,12 +95,14 @@ __device__ __forceinline__ void store8(void* p, bool f32, int64_t i, int n, cons
 }
 
 // 1 / (1 + exp(-v)) to a few units: exp2 of the product with log2 e, whose rounding and the constant's rest come in as
-// a factor. Below -87 the exponential is held at 2^126 (the result is then the smallest normal number), NaN passes.
+// a factor. v is held between the ends first, so that product and rest are finite for infinite v and the types'
+// largest values, too; NaN passes. From 88 on the result is 1; below -87.34 it would be less than the smallest normal
+// number, and the reciprocal makes it 0.
 __device__ __forceinline__ float sigmoid_f32(float v) {
   constexpr float LOG2E = 1.44269502162933349609375f, REST = 1.925963033500011079e-8f, LN2 = 0.693147182464599609375f;
-  float h = -v * LOG2E;
-  const float l = fmaf(-v, LOG2E, -h) - v * REST;
-  h = h > 126.0f ? 126.0f : h;
+  const float c = __builtin_elementwise_maximum(__builtin_elementwise_minimum(v, 88.0f), -88.7f);  // e below 2^128
+  const float h = -c * LOG2E;
+  const float l = fmaf(-c, LOG2E, -h) - c * REST;
   float e = __builtin_amdgcn_exp2f(h);
   e = fmaf(e, l * LN2, e);
   return __builtin_amdgcn_rcpf(1.0f + e);
