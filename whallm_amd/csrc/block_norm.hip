@@ -129,6 +129,16 @@ __device__ __forceinline__ void clear_parts(float* part, int n) {
   __syncthreads();
 }
 
+// A row's mean from its threads' sums. They are added as parts of 2^-k, 2^k the power of two from `hidden` on: exact, and
+// the row's sum is then not past fp32 where the mean is not.
+struct RowMean {
+  float part, n;  // n: hidden 2^-k
+  __device__ __forceinline__ explicit RowMean(int hidden) {
+    part = __uint_as_float((uint32_t)(127 - (hidden > 1 ? 32 - __clz(hidden - 1) : 0)) << 23);
+    n = (float)hidden * part;
+  }
+};
+
 // A thread's place: group g of all has tokens g, g + groups, ..; the thread columns 8 (v size + me) .. + 7 of each,
 // v < V.
 template <int GROUP>
@@ -179,6 +189,7 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* r
   if (GROUP == 0) clear_parts(&part[0][0][0], 48);
   const NormGroup<GROUP> at;
   const int H = a.hidden;
+  const RowMean mean(H);
   const float opost = a.post ? a.offset : 0.0f, opre = a.pre ? a.offset : 0.0f;
   Weight8 wpost[V], wpre[V];
   float channel[V][8];
@@ -220,8 +231,9 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* r
           for (int i = 0; i < 8; ++i) sum[0] = fmaf(y[v].get(i), y[v].get(i), sum[0]);
         }
       }
+      sum[0] *= mean.part;
       group_sums<1, GROUP>(sum, part[0]);
-      p = rsqrtf(sum[0] / (float)H + a.eps);
+      p = rsqrtf(sum[0] / mean.n + a.eps);
     }
     sum[0] = 0.0f;
 #pragma unroll
@@ -247,8 +259,9 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(NormArgs a, void* r
         store8<WHOLE>(residual_out, F32, t * H + c, H - c, r[v]);
       }
     }
+    sum[0] *= mean.part;
     group_sums<1, GROUP>(sum, part[1 + odd]);  // without the post norm no other barrier stands between two of these
-    const float q = rsqrtf(sum[0] / (float)H + a.eps);
+    const float q = rsqrtf(sum[0] / mean.n + a.eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = at.column(v);
@@ -349,7 +362,8 @@ __global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a,
       }
     }
   }
-  const float inv = 1.0f / (float)H;
+  const RowMean mean(H);
+  const float inv = 1.0f / mean.n;
   NormRow<F32, V, WHOLE, GATE> row;
 #pragma unroll
   for (int v = 0; v < V; ++v) row.dr[v].clear();
@@ -373,6 +387,8 @@ __global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a,
         }
       }
     }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) sum[n] *= mean.part;
     group_sums<3, GROUP>(sum, part[0]);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -423,6 +439,7 @@ __global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a,
         if (GATE >= GATE_FULL) store8<WHOLE>(d.dgate, GATE == GATE_FULL_F32, t * H + c, H - c, dg);
       }
     }
+    sum2[0] *= mean.part;
     if (GROUP != 0 || a.post_norm || GATE == GATE_TOKEN) group_sums<GATE == GATE_TOKEN ? 2 : 1, GROUP>(sum2, part[1]);
     else __syncthreads();
     const float k2 = a.post_norm ? p * p * p * (sum2[0] * inv) : 0.0f;
