@@ -6,8 +6,8 @@
 // the residual add and norm of a decoder layer (DecoderLayer.feed_forward, qwen4_exp.py:1127-1149) for
 // layers that also norm, gate or scale what a block adds. With q and p the two reciprocal roots and
 // a = dx (o + w_pre):
-//   dr' = dr_out + q a - r' q^3 mean(a r')         dr = dr'         dw_pre = sum_t dx r' q
-//   b = s g dr',  c = b (o + w_post)               dy = p c - y p^3 mean(c y)     dw_post = sum_t b y p
+//   dr' = dr_out + q (a - r' q^2 mean(a r'))       dr = dr'         dw_pre = sum_t dx r' q
+//   b = s g dr',  c = b (o + w_post)               dy = p c - y p p mean(c y p)   dw_post = sum_t b y p
 //   dg = s dr' z (by sigmoid'), summed over what g is broadcast over
 //
 // Bound by HBM: every tensor passes once. A group of threads holds a token's row in registers, 8 or 16 columns
@@ -400,8 +400,8 @@ __global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a,
     if (AHEAD && t + at.groups < a.tokens) next.load(a, d, at, t + at.groups);
     const float q = rsqrtf(sum[0] * inv + a.eps);
     const float p = a.post_norm ? rsqrtf(sum[2] * inv + a.eps) : 1.0f;
-    const float k1 = q * q * q * (sum[1] * inv);
-    float sum2[2] = {0.0f, 0.0f};  // c y, the token's gate gradient
+    const float k1 = q * (q * (sum[1] * inv));  // the third q comes last: q^3 leaves fp32 for rows of 1e13 or 1e-13
+    float sum2[2] = {0.0f, 0.0f};  // c y p, the token's gate gradient
     float cc[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a,
           for (int j = 0; j < 4; ++j) {
             const int i = h + j;
             const float r = row.r[v].get(i), dx = row.dx[v].get(i), n = row.y[v].get(i) * p;
-            dr[i] = row.dr[v].get(i) + fmaf(q * dx, wpre[v].get(opre, i), -r * k1);
+            dr[i] = fmaf(q, fmaf(dx, wpre[v].get(opre, i), -r * k1), row.dr[v].get(i));
             sums.pre(lds, v, i, q * dx, r);
             const float sdr = a.scale * dr[i], w = wpost[v].get(opost, i);
             const float b = sdr * g[j];
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a,
             if (GATE >= GATE_FULL && a.gate_sigmoid) dg[i] *= g[j] * (1.0f - g[j]);
             if (GATE == GATE_TOKEN) sum2[1] += dg[i];
             cc[v][i] = b * w;
-            sum2[0] = fmaf(cc[v][i], row.y[v].get(i), sum2[0]);
+            sum2[0] = fmaf(cc[v][i], n, sum2[0]);
           }
           if (V == 2) __builtin_amdgcn_sched_barrier(0);  // fewer values at once: there are no registers for more
         }
@@ -442,14 +442,14 @@ __global__ void __launch_bounds__(THREADS, 4) block_norm_grad_kernel(NormArgs a,
     sum2[0] *= mean.part;
     if (GROUP != 0 || a.post_norm || GATE == GATE_TOKEN) group_sums<GATE == GATE_TOKEN ? 2 : 1, GROUP>(sum2, part[1]);
     else __syncthreads();
-    const float k2 = a.post_norm ? p * p * p * (sum2[0] * inv) : 0.0f;
+    const float k2 = a.post_norm ? p * (sum2[0] * inv) : 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = at.column(v);
       row.y[v].repack();
       if (c < H) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cc[v][i] = fmaf(p, cc[v][i], -row.y[v].get(i) * k2);
+        for (int i = 0; i < 8; ++i) cc[v][i] = fmaf(p, cc[v][i], -(row.y[v].get(i) * p) * k2);
         store8<WHOLE>(d.dy, false, t * H + c, H - c, cc[v]);
       }
     }
