@@ -5,7 +5,6 @@
 //
 // Errors: ValueError for what the call refuses, before anything is allocated or launched; WhallmError with
 // wm_last_error() where the C call does.
-#include <ATen/MemoryOverlap.h>
 #include <torch/extension.h>
 
 #include <initializer_list>
@@ -107,12 +106,20 @@ void checked(const char* name, Call call) {
   }
 }
 
-// The caller's `out` is written where the inputs are read: it may be one of them and must not lie partly over one.
-void own_out(const Maybe& out, const char* name, std::initializer_list<const Tensor*> inputs) {
+// Whether two contiguous tensors have a byte in common, whichever storages hold them.
+bool meet(const Tensor& a, const Tensor& b) {
+  const char *p = static_cast<const char*>(a.const_data_ptr()), *q = static_cast<const char*>(b.const_data_ptr());
+  return a.nbytes() > 0 && b.nbytes() > 0 && p < q + b.nbytes() && q < p + a.nbytes();
+}
+// The caller's `out` is written while other workgroups still read the inputs: it may be `same`, element for element, and
+// lies over no other.
+void own_out(const Maybe& out, const char* name, const Tensor& same, const char* same_name,
+             std::initializer_list<const Tensor*> others) {
   if (!out) return;
-  for (const Tensor* t : inputs)
-    if (t && at::get_overlap_status(*out, *t) == at::MemOverlapStatus::Partial)
-      refuse(std::string(name) + " must be an input itself or share no memory with one");
+  const bool itself = out->const_data_ptr() == same.const_data_ptr() && out->scalar_type() == same.scalar_type();
+  bool apart = itself || !meet(*out, same);
+  for (const Tensor* t : others) apart = apart && !(t && meet(*out, *t));
+  if (!apart) refuse(std::string(name) + " must be " + same_name + " itself or share no memory with it, and none with another input");
 }
 // Autograd sees that `out` was written.
 void changed(const Maybe& out) {
@@ -298,7 +305,7 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& residual_, const Tensor& y, 
   if (out && (out->scalar_type() != residual_.scalar_type() || out->sizes() != residual_.sizes() || !out->is_contiguous()))
     refuse("residual_out must be a contiguous tensor shaped and typed like residual");
   const Tensor residual = residual_.contiguous();
-  own_out(out, "residual_out", {&residual, &f.y, ptr(f.post), ptr(f.pre), ptr(f.gate)});
+  own_out(out, "residual_out", residual, "residual", {&f.y, ptr(f.post), ptr(f.pre), ptr(f.gate)});
   const c10::Device device = device_of({&residual, &f.y, ptr(f.post), ptr(f.pre), ptr(f.gate), ptr(out)});
   const On on(device);
   const Tensor residual_out = out ? *out : at::empty_like(residual), x = at::empty_like(f.y);
@@ -395,7 +402,9 @@ Tensor process_logits(const Tensor& logits_, const Maybe& history_, const Maybe&
   if (mask && mask->size(1) != (V + 31) / 32) refuse("mask must hold a bit for every token, 32 in a word");
   if (out_ && (out_->scalar_type() != at::kFloat || out_->sizes() != logits.sizes() || !out_->is_contiguous()))
     refuse("out must be a contiguous float32 tensor shaped like logits");
-  own_out(out_, "out", {&logits, ptr(history), ptr(bias_ids), ptr(bias_values), ptr(mask)});
+  own_out(out_, "out", logits, "logits",
+          {ptr(history), ptr(lengths), ptr(prompts), ptr(repetition), ptr(frequency), ptr(presence), ptr(bias_ids),
+           ptr(bias_values), ptr(mask), ptr(temperature)});
   const c10::Device device = device_of({&logits, ptr(history), ptr(lengths), ptr(prompts), ptr(repetition), ptr(frequency),
                                         ptr(presence), ptr(bias_ids), ptr(bias_values), ptr(mask), ptr(temperature), ptr(out_)});
   const On on(device);
