@@ -143,6 +143,9 @@ Tensor part(const Tensor& whole, int64_t first, int64_t n) {
 // The tokens of rows [T * k, H] in the order of `inverse`.
 int64_t pair_rows(const Tensor& rows, const Tensor& inverse, int64_t k) {
   if (rows.dim() != 2 || rows.size(1) < 1) refuse("rows must be [tokens * k, hidden]");
+  if (rows.size(1) > 1 << 20) refuse("hidden must be at most 1048576");
+  if (rows.size(0) > INT32_MAX) refuse("tokens * k must be below 2^31");
+  if (k > 64) refuse("k must be at most 64");
   if (k < 1 || rows.size(0) % k) refuse("rows must hold k rows of every token");
   if (inverse.scalar_type() != at::kInt || !inverse.is_contiguous() || inverse.numel() != rows.size(0))
     refuse("the permutation is not that of these rows");
@@ -381,7 +384,7 @@ Tensor process_logits(const Tensor& logits_, const Maybe& history_, const Maybe&
   const Tensor logits = rows_of(logits_, "logits");
   if (logits.dim() != 2 || logits.size(1) < 1) refuse("logits must be [rows, vocab]");
   const int64_t R = logits.size(0), V = logits.size(1);
-  if (R > INT32_MAX || V > 1 << 22) refuse("logits must have at most 4194304 values a row");
+  if (R > INT32_MAX || V > 1 << 22) refuse("logits must have at most 2147483647 rows of at most 4194304 values");
   wm_logit_rules r = {};
   Maybe lengths = row_values(lengths_, R, at::kInt, "lengths"), prompts = row_values(prompt_lengths_, R, at::kInt, "prompt_lengths");
   const Maybe repetition = row_values(repetition_, R, at::kFloat, "repetition"),
