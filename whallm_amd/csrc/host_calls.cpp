@@ -60,12 +60,16 @@ int is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
 const Tensor* ptr(const Tensor& t) { return &t; }
 const Tensor* ptr(const Maybe& t) { return t ? &*t : nullptr; }
 
-// Refuses inputs whose gradient would be lost: these calls are not recorded by autograd.
+// Refuses inputs whose gradient or tangent would be lost: these calls are not recorded by autograd. Forward mode is a
+// mode of its own, on under torch.no_grad() and off in inference mode.
 void no_autograd(const char* name, const char* gradients, std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : tensors)
-    if (t && t->requires_grad())
+  const bool reverse = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : tensors) {
+    if (!t) continue;
+    if (reverse && t->requires_grad())
       refuse(std::string(name) + " is not recorded by autograd (" + gradients + "): call it under torch.no_grad()");
+    if (forward && t->_fw_grad(0).defined()) refuse(std::string(name) + " has no forward-mode derivative: pass the tensor without its tangent");
+  }
 }
 
 c10::Device device_of(std::initializer_list<const Tensor*> tensors) {
