@@ -36,8 +36,10 @@ static bool past_cache(int64_t pairs, int64_t row_bytes) {
 //                 knows the first row of each expert for this chunk; a pair's row is that plus its place
 //                 among the chunk's earlier pairs of its expert. One launch and no workspace, the counting
 //                 repeated by every workgroup.
-//   more          a launch before counts the pairs of up to 64 spans (sort_spans_kernel); a workgroup adds up
-//                 the spans' counts and counts only the pairs of its own span before its chunk.
+//   more          a launch before counts the pairs of spans (sort_spans_kernel); a workgroup adds up the spans'
+//                 counts and counts only the pairs of its own span before its chunk. Past 64 spans of 8192 pairs
+//                 a second launch adds them up for all (sort_bases_kernel), so that a workgroup's counting has
+//                 an end however many pairs there are.
 // Each has one workgroup more, for the lists that belong to no pair.
 constexpr int SORT_THREADS = 512;
 constexpr int SORT_CHUNK = 256;
@@ -53,6 +55,7 @@ struct SortArgs {
   int32_t *order, *inverse, *offsets, *tiles, *tile_count;
   int64_t max_tiles;
   const int32_t* span_counts;  // [spans][experts], null where there is one span
+  const int32_t* totals;       // [experts], where span_counts are those of the spans before; else null
   int64_t span_pairs;
   int spans;
 };
@@ -114,6 +117,14 @@ __device__ __forceinline__ void sort_count(const SortArgs& a, int64_t q0, int64_
 // ends with a barrier.
 __device__ __forceinline__ void sort_counts(const SortArgs& a, int64_t p0, int32_t* before, int32_t* all) {
   const int E = a.experts;
+  if (a.totals) {
+    const int64_t span = p0 / a.span_pairs;
+    for (int e = threadIdx.x; e < E; e += SORT_THREADS) before[e] = a.span_counts[span * E + e], all[e] = a.totals[e];
+    __syncthreads();
+    sort_count(a, span * a.span_pairs, p0, p0, before, nullptr);
+    __syncthreads();
+    return;
+  }
   for (int e = threadIdx.x; e < E; e += SORT_THREADS) before[e] = all[e] = 0;
   __syncthreads();
   if (!a.span_counts) {
@@ -149,6 +160,38 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_spans_kernel(SortArgs a, in
   sort_count(a, q0, q1, q1, count, nullptr);
   __syncthreads();
   for (int e = threadIdx.x; e < a.experts; e += SORT_THREADS) counts[(int64_t)blockIdx.x * a.experts + e] = count[e];
+}
+
+// The spans' counts [spans][experts] become those of the spans before, and the row behind them the totals. A lane has an
+// expert, the waves slices of the spans in order; 64 experts a workgroup.
+constexpr int BASES_WAVES = 16;
+__global__ void __launch_bounds__(64 * BASES_WAVES) sort_bases_kernel(int32_t* counts, int spans, int experts) {
+  __shared__ int32_t slice_sum[BASES_WAVES][64];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, e = blockIdx.x * 64 + lane;
+  const int per = (spans + BASES_WAVES - 1) / BASES_WAVES;
+  const int64_t s0 = min((int64_t)spans, (int64_t)wave * per), s1 = min((int64_t)spans, s0 + per);
+  int32_t sum = 0;
+  if (e < experts) {
+#pragma unroll 8
+    for (int64_t s = s0; s < s1; ++s) sum += counts[s * experts + e];
+  }
+  slice_sum[wave][lane] = sum;
+  __syncthreads();
+  int32_t at = 0;
+  for (int w = 0; w < wave; ++w) at += slice_sum[w][lane];
+  if (e >= experts) return;
+  constexpr int BATCH = 8;  // loaded before any is written
+  for (int64_t s = s0; s < s1; s += BATCH) {
+    int32_t n[BATCH];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) n[b] = s + b < s1 ? counts[(s + b) * experts + e] : 0;
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      if (s + b < s1) counts[(s + b) * experts + e] = at;
+      at += n[b];
+    }
+  }
+  if (wave == BASES_WAVES - 1) counts[(int64_t)spans * experts + e] = at;
 }
 
 // The lists that belong to no pair: offsets, tiles, their number. One workgroup; count and first are LDS of an
@@ -340,7 +383,9 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
 // 16384 pairs 10.3 and 12.7.
 constexpr int64_t SORT_FEW_MAX = 256, SORT_ONE_MAX = 16384;
 
-// Spans that are counted apart: each a multiple of the chunk, of 2048 pairs or more.
+// Spans that are counted apart: each a multiple of the chunk, of 2048 to 8192 pairs (and less than a chunk more).
+// Up to SORT_SPANS_ADDED of them every workgroup adds up itself.
+constexpr int SORT_SPANS_ADDED = 64;
 struct SortSpans {
   int64_t pairs;
   int spans;
@@ -353,7 +398,8 @@ static int sort_chunk_tokens(int64_t tokens, int k) {
 static SortSpans sort_spans(int64_t tokens, int k) {
   const int64_t pairs = tokens * k, chunk = (int64_t)sort_chunk_tokens(tokens, k) * k;
   if (pairs <= SORT_ONE_MAX) return {pairs, 1};
-  const int64_t least = pairs / 64 > 2048 ? (pairs + 63) / 64 : 2048, span = (least + chunk - 1) / chunk * chunk;
+  const int64_t part = (pairs + SORT_SPANS_ADDED - 1) / SORT_SPANS_ADDED;
+  const int64_t least = part < 2048 ? 2048 : part > 8192 ? 8192 : part, span = (least + chunk - 1) / chunk * chunk;
   return {span, (int)((pairs + span - 1) / span)};
 }
 
@@ -371,6 +417,11 @@ static void sort_launch(SortArgs a, int32_t* workspace, hipStream_t s) {
     hipLaunchKernelGGL(sort_spans_kernel, dim3(a.spans), dim3(SORT_THREADS), 0, s, a, workspace);
     check_launch("sort_spans");
     a.span_counts = workspace;
+    if (a.spans > SORT_SPANS_ADDED) {
+      hipLaunchKernelGGL(sort_bases_kernel, dim3((a.experts + 63) / 64), dim3(64 * BASES_WAVES), 0, s, workspace, a.spans, a.experts);
+      check_launch("sort_bases");
+      a.totals = workspace + (int64_t)a.spans * a.experts;
+    }
   }
   // columns are split, by whole waves, until the chip has work for every CU
   const int64_t most = (a.row.units + 255) / 256;
@@ -573,7 +624,8 @@ extern "C" {
 WM_EXPORT size_t wm_sort_tokens_workspace_size(int32_t tokens, int32_t k, int32_t experts) {
   const int64_t pairs = (int64_t)tokens * k;
   if (tokens < 0 || k < 1 || k > SORT_MAX_K || experts < 1 || pairs <= SORT_ONE_MAX) return 0;
-  return (size_t)sort_spans(tokens, k).spans * experts * sizeof(int32_t);
+  const int spans = sort_spans(tokens, k).spans;
+  return (size_t)(spans + (spans > SORT_SPANS_ADDED)) * experts * sizeof(int32_t);
 }
 
 WM_EXPORT int wm_sort_tokens(const void* x, int32_t fp32, int32_t tokens, int32_t hidden, const int32_t* indices, int32_t k,
