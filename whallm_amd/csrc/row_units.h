@@ -46,10 +46,7 @@ struct RowUnit<false, true> {
   static __device__ __forceinline__ Raw load(const Elem* p) { return load16(p); }
   static __device__ __forceinline__ Raw load_once(const Elem* p) { return load16_nt(p); }
   static __device__ __forceinline__ void store(Elem* p, Raw v) { store16(p, v); }
-  template <bool ONCE>
-  static __device__ __forceinline__ void store_as(Elem* p, Raw v) {
-    if (ONCE) store16_nt(p, v); else store16(p, v);
-  }
+  static __device__ __forceinline__ void store_once(Elem* p, Raw v) { store16_nt(p, v); }
   static __device__ __forceinline__ void unpack(Raw v, float f[N]) {
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
@@ -71,8 +68,7 @@ struct RowUnit<false, false> {
   static __device__ __forceinline__ Raw load(const Elem* p) { return *p; }
   static __device__ __forceinline__ Raw load_once(const Elem* p) { return *p; }
   static __device__ __forceinline__ void store(Elem* p, Raw v) { *p = v; }
-  template <bool ONCE>
-  static __device__ __forceinline__ void store_as(Elem* p, Raw v) { *p = v; }
+  static __device__ __forceinline__ void store_once(Elem* p, Raw v) { *p = v; }
   static __device__ __forceinline__ void unpack(Raw v, float f[N]) { f[0] = bf16_bits_to_f32(v); }
   static __device__ __forceinline__ Raw pack(const float f[N]) { return (Raw)pack_bf16(f[0], 0.0f); }
 };
@@ -85,10 +81,7 @@ struct RowUnit<true, true> {
   static __device__ __forceinline__ Raw load(const Elem* p) { return load16(p); }
   static __device__ __forceinline__ Raw load_once(const Elem* p) { return load16_nt(p); }
   static __device__ __forceinline__ void store(Elem* p, Raw v) { store16(p, v); }
-  template <bool ONCE>
-  static __device__ __forceinline__ void store_as(Elem* p, Raw v) {
-    if (ONCE) store16_nt(p, v); else store16(p, v);
-  }
+  static __device__ __forceinline__ void store_once(Elem* p, Raw v) { store16_nt(p, v); }
   static __device__ __forceinline__ void unpack(Raw v, float f[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = __uint_as_float(v[i]);
@@ -107,8 +100,7 @@ struct RowUnit<true, false> {
   static __device__ __forceinline__ Raw load(const Elem* p) { return *p; }
   static __device__ __forceinline__ Raw load_once(const Elem* p) { return *p; }
   static __device__ __forceinline__ void store(Elem* p, Raw v) { *p = v; }
-  template <bool ONCE>
-  static __device__ __forceinline__ void store_as(Elem* p, Raw v) { *p = v; }
+  static __device__ __forceinline__ void store_once(Elem* p, Raw v) { *p = v; }
   static __device__ __forceinline__ void unpack(Raw v, float f[N]) { f[0] = v; }
   static __device__ __forceinline__ Raw pack(const float f[N]) { return f[0]; }
 };

@@ -19,13 +19,50 @@ namespace wm {
 
 constexpr int SORT_MAX_K = 64;
 
-// Whether permuted rows are stored past the 256 MB cache: where it would not hold them for their reader beside the
-// rest, but for short rows that are no whole 128-byte lines. Sort: 256 MB of 4 KB rows 64 us past it, 82 through
-// it; 229 MB of 2002 bytes 94 and 110; 458 MB of 500 bytes 246 and 239. The gradients of back: 240 MB of 20 KB
-// 104 and 115; 458 MB of 500 bytes 437 and 395. (A call by itself after a pause 115 and 102 at 240 MB; smaller
-// ones gain as much, 128 MB of the sort 38 and 46, but their reader would lose it again.)
-static bool past_cache(int64_t pairs, int64_t row_bytes) {
-  return pairs * row_bytes > 192ll << 20 && (row_bytes > 512 || row_bytes % 128 == 0);
+// How permuted rows are stored: through the 256 MB cache, past it, or the first `through` rows through it and the others
+// past it. Their reader starts with the first; what a call leaves in the cache, the next work has to write back.
+//
+// Up to 192 MB all stay for the reader. Up to 256 MB the first 96 MB do. Call and a pass that reads its rows, behind a
+// pass over other memory (in brackets one of many calls in a row), us, with none / 96 MB / all through:
+//   sort       200 MB of 14 KB rows   131 (48)    121 (42)    94 (60)
+//              240 MB of 20 KB        151 (57)    118 (57)   115 (65)
+//              240 MB of 2002 bytes   212 (94)    188 (82)   171 (108)
+//   gradients  200 MB of 14 KB        165 (87)    151 (74)   118 (95)
+//              240 MB of 20 KB        198 (108)   164 (97)   151 (118)
+//              240 MB of 2002 bytes   286 (170)   269 (170)  254 (174)
+// Larger ones go past it: with 64 or 96 MB through, calls in a row of more than two sets of tensors evict each other's
+// (sort of 470 MB 101 us, with 64 MB 119), and for the reader there is less to win:
+//   sort       448 MB of 14 KB        244 (101)   242 (119)  246 (120)
+//              640 MB of 20 KB        315 (142)   308 (168)  338 (167)
+//   gradients  448 MB of 14 KB        333 (194)   324 (198)  315 (209)
+//              640 MB of 20 KB        437 (268)   429 (284)  443 (292)
+// Short rows that are no whole 128-byte lines always stay, since their lines are written in parts: 256 MB of 500-byte
+// rows sorted and read 242, past the cache 265, their gradients 340 and 382; of 384 MB 384 and 393, 518 and 574.
+enum RowStore { THROUGH, PAST, SPLIT };
+struct RowStores {
+  RowStore how;
+  int64_t through;
+};
+static RowStores row_stores(int64_t pairs, int64_t row_bytes) {
+  const int64_t bytes = pairs * row_bytes;
+  if (bytes <= 192ll << 20 || (row_bytes <= 512 && row_bytes % 128 != 0)) return {THROUGH, pairs};
+  if (bytes <= 256ll << 20) return {SPLIT, (96ll << 20) / row_bytes};
+  return {PAST, 0};
+}
+
+// A unit of a permuted row; `past` where the call splits them. The empty statements keep the two stores apart, of
+// which the compiler would make one that goes through the cache.
+template <typename Unit, int STORE>
+__device__ __forceinline__ void store_row_unit(typename Unit::Elem* p, typename Unit::Raw v, bool past) {
+  if (STORE == PAST) {
+    Unit::store_once(p, v);
+  } else if (STORE == SPLIT && past) {
+    asm volatile("");
+    Unit::store_once(p, v);
+    asm volatile("");
+  } else {
+    Unit::store(p, v);
+  }
 }
 
 // ---- sort. A workgroup owns a chunk of tokens (256 pairs at most) and a range of units. It finds its
@@ -54,6 +91,7 @@ struct SortArgs {
   void* rows;
   int32_t *order, *inverse, *offsets, *tiles, *tile_count;
   int64_t max_tiles;
+  int64_t through;             // of SPLIT
   const int32_t* span_counts;  // [spans][experts], null where there is one span
   const int32_t* totals;       // [experts], where span_counts are those of the spans before; else null
   int64_t span_pairs;
@@ -230,13 +268,13 @@ __device__ __forceinline__ void sort_lists(const SortArgs& a, int32_t* count, in
   }
 }
 
-// One unit of a row: from x's element `at`, to the same place of k rows.
-template <typename Unit, bool ONCE>
-__device__ __forceinline__ void sort_store(uint16_t* rows, int64_t length, int64_t at, const int32_t* row, int k,
-                                           typename Unit::Raw v) {
+// One unit of a row: from x's element `at`, to the same place of a token's k rows.
+template <typename Unit, int STORE>
+__device__ __forceinline__ void sort_store(const SortArgs& a, int64_t at, const int32_t* row, typename Unit::Raw v) {
+  uint16_t* rows = (uint16_t*)a.rows;
 #pragma unroll 4
-  for (int j = 0; j < k; ++j)
-    if (row[j] >= 0) Unit::template store_as<ONCE>(rows + row[j] * length + at, v);
+  for (int j = 0; j < a.k; ++j)
+    if (row[j] >= 0) store_row_unit<Unit, STORE>(rows + row[j] * a.length + at, v, row[j] >= a.through);
 }
 
 // Zeros in the rows from `present` on, every step-th from the me-th, units c0 .. c1.
@@ -297,14 +335,13 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_few_kernel(SortArgs a) {
   __syncthreads();
   const int32_t present = present_;
   if (blockIdx.y == 0 && (int)threadIdx.x < a.k && p0 + (int)threadIdx.x >= present) a.order[p0 + threadIdx.x] = -1;
-  uint16_t* rows = (uint16_t*)a.rows;
-  if (c < a.row.wide) sort_store<RowUnit<false, true>, false>(rows, a.length, at, row, a.k, v);
-  else if (c < a.row.units) sort_store<RowUnit<false, false>, false>(rows, a.length, at, row, a.k, one);
+  if (c < a.row.wide) sort_store<RowUnit<false, true>, THROUGH>(a, at, row, v);
+  else if (c < a.row.units) sort_store<RowUnit<false, false>, THROUGH>(a, at, row, one);
   const int c0 = blockIdx.y * SORT_THREADS;
   sort_clear(a, present, t, a.tokens, c0, min(a.row.units, c0 + SORT_THREADS));
 }
 
-template <bool ONCE>
+template <int STORE>
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
   // base: the chunk's first row of each expert
   __shared__ int32_t base[PERMUTE_MAX_EXPERTS], all[PERMUTE_MAX_EXPERTS];
@@ -362,7 +399,6 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
   }
   __syncthreads();
   const uint16_t* x = (const uint16_t*)a.x;
-  uint16_t* rows = (uint16_t*)a.rows;
   const int c0 = blockIdx.y * a.split_units, c1 = min(a.row.units, c0 + a.split_units);
   // Units of all the chunk's tokens one behind the other: no thread without one but at the end.
   const int width = c1 - c0;
@@ -370,8 +406,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
     const int t = (int)((uint32_t)i / (uint32_t)width), c = c0 + i - t * width;
     const uint16_t* from = x + (t0 + t) * a.length;
     const int64_t at = c < a.row.wide ? 8 * (int64_t)c : 8 * (int64_t)a.row.wide + c - a.row.wide;
-    if (c < a.row.wide) sort_store<RowUnit<false, true>, ONCE>(rows, a.length, at, row + t * a.k, a.k, load16(from + at));
-    else sort_store<RowUnit<false, false>, ONCE>(rows, a.length, at, row + t * a.k, a.k, from[at]);
+    if (c < a.row.wide) sort_store<RowUnit<false, true>, STORE>(a, at, row + t * a.k, load16(from + at));
+    else sort_store<RowUnit<false, false>, STORE>(a, at, row + t * a.k, from[at]);
   }
   // The rows behind the last pair, spread over the workgroups: the few that own the last pairs would take
   // twice as long (4096 tokens x 8, hidden 7168, 2% of the pairs absent: 112 us, spread 103).
@@ -429,9 +465,11 @@ static void sort_launch(SortArgs a, int32_t* workspace, hipStream_t s) {
   if (splits > most) splits = most;
   a.split_units = (int)(((a.row.units + splits - 1) / splits + 63) / 64 * 64);
   const dim3 grid(blocks, (unsigned)((a.row.units + a.split_units - 1) / a.split_units));
-  const bool once = past_cache(pairs, a.length * 2);
-  if (once) hipLaunchKernelGGL(sort_kernel<true>, grid, dim3(SORT_THREADS), 0, s, a);
-  else hipLaunchKernelGGL(sort_kernel<false>, grid, dim3(SORT_THREADS), 0, s, a);
+  const RowStores stores = row_stores(pairs, a.length * 2);
+  a.through = stores.through;
+  if (stores.how == THROUGH) hipLaunchKernelGGL(sort_kernel<THROUGH>, grid, dim3(SORT_THREADS), 0, s, a);
+  else if (stores.how == PAST) hipLaunchKernelGGL(sort_kernel<PAST>, grid, dim3(SORT_THREADS), 0, s, a);
+  else hipLaunchKernelGGL(sort_kernel<SPLIT>, grid, dim3(SORT_THREADS), 0, s, a);
   check_launch("sort");
 }
 
@@ -509,11 +547,11 @@ static void gather_sum(const void* rows, bool f32, const float* weights, const i
 // group.
 constexpr int BACK_BATCH = 8;
 
-template <bool F32, bool ONCE, int GROUP, int THREADS>
+template <bool F32, int STORE, int GROUP, int THREADS>
 __global__ void __launch_bounds__(THREADS) back_grad_kernel(const void* __restrict__ dy_, const void* __restrict__ rows_,
                                                        const float* __restrict__ weights, const int32_t* __restrict__ inverse,
                                                        const int32_t* __restrict__ present_, int64_t tokens, int64_t hidden,
-                                                       RowUnits row, int k, void* __restrict__ drows_,
+                                                       RowUnits row, int k, int64_t through, void* __restrict__ drows_,
                                                        float* __restrict__ dweights) {
   typedef typename RowUnit<F32, true>::Elem Elem;
   constexpr int N = RowUnit<F32, true>::N;
@@ -559,7 +597,7 @@ __global__ void __launch_bounds__(THREADS) back_grad_kernel(const void* __restri
             dot[q] = fmaf(d[i], f[i], dot[q]);
             o[i] = w[q] * d[i];
           }
-          U::template store_as<ONCE>(drows + r[q] * hidden + at, U::pack(o));
+          store_row_unit<U, STORE>(drows + r[q] * hidden + at, U::pack(o), r[q] >= through);
         }
       }
     };
@@ -590,19 +628,19 @@ __global__ void __launch_bounds__(THREADS) back_grad_kernel(const void* __restri
   }
 }
 
-template <bool F32, bool ONCE>
+template <bool F32, int STORE>
 static void back_grad(const void* dy, const void* rows, const float* weights, const int32_t* inverse, const int32_t* present,
-                      int64_t tokens, int64_t hidden, int k, void* drows, float* dweights, hipStream_t s) {
+                      int64_t tokens, int64_t hidden, int k, int64_t through, void* drows, float* dweights, hipStream_t s) {
   const RowUnits row = row_units(hidden, F32);
   if (row.units <= 64)  // 16000 tokens x 8 of 100 in bf16: 39 us, with a workgroup a token 102; of 1000 95 and 92
-    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 64, 256>), dim3(grid_of("back_grad", (tokens + 3) / 4, 256)), dim3(256), 0, s, dy, rows, weights,
-                       inverse, present, tokens, hidden, row, k, drows, dweights);
+    hipLaunchKernelGGL((back_grad_kernel<F32, STORE, 64, 256>), dim3(grid_of("back_grad", (tokens + 3) / 4, 256)), dim3(256), 0, s, dy, rows, weights,
+                       inverse, present, tokens, hidden, row, k, through, drows, dweights);
   else if (tokens <= 256 && row.units > 256)  // a CU a token: 11 x 7 of 6016 in fp32 7.2 us, with 256 threads 10.7
-    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 1024, 1024>), dim3((unsigned)tokens), dim3(1024), 0, s, dy, rows, weights, inverse,
-                       present, tokens, hidden, row, k, drows, dweights);
+    hipLaunchKernelGGL((back_grad_kernel<F32, STORE, 1024, 1024>), dim3((unsigned)tokens), dim3(1024), 0, s, dy, rows, weights, inverse,
+                       present, tokens, hidden, row, k, through, drows, dweights);
   else
-    hipLaunchKernelGGL((back_grad_kernel<F32, ONCE, 256, 256>), dim3(grid_of("back_grad", tokens, 256)), dim3(256), 0, s, dy, rows, weights, inverse,
-                       present, tokens, hidden, row, k, drows, dweights);
+    hipLaunchKernelGGL((back_grad_kernel<F32, STORE, 256, 256>), dim3(grid_of("back_grad", tokens, 256)), dim3(256), 0, s, dy, rows, weights, inverse,
+                       present, tokens, hidden, row, k, through, drows, dweights);
   check_launch("back_grad");
 }
 
@@ -690,13 +728,14 @@ WM_EXPORT int wm_combine_rows_backward(const void* dy, const void* rows, int32_t
     if (((uintptr_t)dy | (uintptr_t)rows | (uintptr_t)drows) % (fp32 ? 4 : 2))
       fail("wm_combine_rows_backward: rows must be aligned to their elements");
     hipStream_t s = as_stream(stream);
-    const bool once = past_cache((int64_t)tokens * k, (int64_t)hidden * (fp32 ? 4 : 2));
-#define WM_BACK(F, O) back_grad<F, O>(dy, rows, weights, inverse, present, tokens, hidden, k, drows, dweights, s)
-    if (fp32) {
-      if (once) WM_BACK(true, true); else WM_BACK(true, false);
-    } else {
-      if (once) WM_BACK(false, true); else WM_BACK(false, false);
-    }
+    const RowStores stores = row_stores((int64_t)tokens * k, (int64_t)hidden * (fp32 ? 4 : 2));
+#define WM_BACK(F, S) back_grad<F, S>(dy, rows, weights, inverse, present, tokens, hidden, k, stores.through, drows, dweights, s)
+#define WM_BACKS(F)                                     \
+  if (stores.how == THROUGH) WM_BACK(F, THROUGH);       \
+  else if (stores.how == PAST) WM_BACK(F, PAST);        \
+  else WM_BACK(F, SPLIT);
+    if (fp32) { WM_BACKS(true) } else { WM_BACKS(false) }
+#undef WM_BACKS
 #undef WM_BACK
   });
 }
