@@ -84,7 +84,6 @@ struct LogitRaw<true> {
     for (int e = 0; e < 4; ++e) a[e] = e < n ? ((const uint32_t*)logits)[at + e] : 0u;
   }
   __device__ __forceinline__ void unpack(float l[LOGIT_UNIT]) const { RowUnit<true, true>::unpack(a, l); }
-  static __device__ __forceinline__ float one(const void* logits, int64_t at) { return ((const float*)logits)[at]; }
 };
 template <>
 struct LogitRaw<false> {
@@ -101,9 +100,6 @@ struct LogitRaw<false> {
       l[2 * m] = __uint_as_float(a[m] << 16);
       l[2 * m + 1] = __uint_as_float(a[m] & 0xffff0000u);
     }
-  }
-  static __device__ __forceinline__ float one(const void* logits, int64_t at) {
-    return bf16_bits_to_f32(((const uint16_t*)logits)[at]);
   }
 };
 
