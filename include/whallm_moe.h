@@ -341,8 +341,10 @@ WM_EXPORT int wm_repack_router(const void* router, const void* shared_gate, int3
  *   x = residual_out * rsqrt(mean(residual_out^2) + eps) * (weight_offset + pre_weight)
  * over rows of hidden values, fp32 inside, x from residual_out as it is stored. y and x bf16,
  * residual and residual_out bf16 or fp32 [tokens, hidden], weights bf16 [hidden] (null: the norm
- * alone, no offset), the gate g bf16 or fp32, through a sigmoid with gate_sigmoid. hidden 1..16384;
- * tensors aligned to their elements. */
+ * alone, no offset), the gate g bf16 or fp32, through a sigmoid with gate_sigmoid (0 and 1 for
+ * infinite gates; 0 where it would be less than the smallest normal number). hidden 1..16384;
+ * tensors aligned to their elements. A row's squares are taken in fp32: its values may be up to about
+ * 1e18 (x is 0 for a row of 2e19 and more), and with eps 0 as small as 1e-18. */
 typedef struct wm_block_norm_form {
   const void* post_weight;
   const void* pre_weight;

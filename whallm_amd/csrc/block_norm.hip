@@ -16,8 +16,8 @@
 // over tokens (weight gradients) stay with the group, go to the workspace once per workgroup and are added up
 // by a second launch in the workgroups' order. All arithmetic is fp32; bf16 outputs are rounded once, from
 // values that no earlier rounding touched but r''s own (x is the norm of the residual that the next block
-// reads). 16384 tokens of 4096 in fp32 take 152 us (805 MB, 5.3 TB/s), the gradients of 4001 tokens of 5120 in
-// bf16 with a full gate 67 + 5 us (328 MB, 4.9 TB/s in the first launch).
+// reads). Rows may have any magnitude whose squares fp32 holds (about 1e-18 to 1e18). 16384 tokens of 4096 in fp32 take 152 us (805 MB, 5.3 TB/s), the gradients of 4001 tokens of 5120 in
+// bf16 with a full gate 68 + 5 us (328 MB, 4.8 TB/s in the first launch).
 #include <initializer_list>
 
 #include "row_units.h"
@@ -284,7 +284,7 @@ struct NormGrads {
 };
 
 // What a thread loads of a token's row. A workgroup that has a CU to itself loads the next token's behind the first
-// sums, while it works on this one's: 4001 tokens of 5120 with a full gate 68.9 us, without 70.9. (Workgroups that
+// sums, while it works on this one's: 4001 tokens of 5120 with a full gate 69.7 us, without 72.4. (Workgroups that
 // share one do so for each other; they unpack the weights anew for each token, since more registers make them
 // fewer: 16000 of 2051 with a channel's gate 136 us, with the weights kept 183.)
 template <bool F32, int V, bool WHOLE, int GATE>
@@ -514,8 +514,8 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(const float* __restr
 }
 
 // How a row is held: by `group` threads (0: a workgroup of `threads`), 8 v columns each. Short rows have 16 threads
-// or a wave, four waves a workgroup (16000 tokens of 100 10 us and the gradients 17, with a workgroup a row 17 and
-// 40); rows of more than 8192 columns 16 columns a thread, since a workgroup has 1024.
+// or a wave, four waves a workgroup (16000 tokens of 100, captured, 5.5 us and the gradients 12.6, with a workgroup a
+// row 12.0 and 42); rows of more than 8192 columns 16 columns a thread, since a workgroup has 1024.
 struct NormShape {
   int group, v, threads;
 };
@@ -534,10 +534,10 @@ static int norm_blocks(int64_t tokens, const NormShape& s, int waves, int least)
   const int64_t most = (tokens + norm_groups_of_block(s) - 1) / norm_groups_of_block(s);
   return (int)(most < want ? most : want);
 }
-// The gradient pass has what a CU holds at once, one workgroup of long rows (4001 tokens of 5120: 68.5 us, two in turn
-// 72.8), and adds a row a workgroup to the second launch's work: 8 tokens a group or more, 4 where rows are
-// short and no eights (their loads take longer), unless that leaves CUs without one: 18775 tokens of 479 with 8
-// 59.6 us, with 4 44.6; 16000 of 512 24.9 and 28.3.
+// The gradient pass has what a CU holds at once, one workgroup of long rows (4001 tokens of 5120: 69.7 us, two in turn
+// 74.8), and adds a row a workgroup to the second launch's work: 8 tokens a group or more, 4 where rows are
+// short and no eights (their loads take longer), unless that leaves CUs without one: 18775 tokens of 479 with a
+// channel's gate 60 us with 8, 46 with 4; 16000 of 512 in fp32 28 and 32.
 static int norm_grad_blocks(int64_t tokens, int hidden) {
   const NormShape s = norm_shape(hidden);
   const int64_t each = (s.group && hidden % 8 ? 4 : 8) * norm_groups_of_block(s), most = tokens / each > 512 ? tokens / each : 512;

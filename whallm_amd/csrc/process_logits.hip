@@ -7,18 +7,21 @@
 //   l = allowed[v] ? l / temperature : -inf
 //   log-probabilities: l - max l - log sum exp(l - max l), where -inf stays -inf
 //
-// Bound by HBM: the logits are read and the results written; log-probabilities read the logits twice, once
-// for the rows' maxima and sums (a chunk's go to the workspace) and once to write, which is less than
-// writing the processed logits and going over them again. A workgroup owns a chunk of a row's vocabulary, a
-// thread units of 4 tokens, so that a wave's stores are 1 KB without a gap (with 8 tokens a thread, 16 bytes
-// in every 32 a store, 192 rows of 129,280 take 34 us to write, so 23). 192 rows of bf16 logits to
-// log-probabilities with 2000 ids, 64 biases and a mask each take 49 us: 24 for the maxima, 27 to write (99 MB,
-// with 50 MB read twice). A workgroup counts its row's whole history (a few thousand tokens, from L2 after the
-// first workgroup) into one LDS word per token of the chunk, so no count table exists in memory and nothing is
-// left to clear; only for long histories of few rows the first launch keeps the words for the second. A word
-// holds the answer's count (20 bits), whether a prompt holds the token (1) and the place of its bias in the list
-// (11, the last one where a token is listed twice): integer additions and maxima, so the result does not depend
-// on their order.
+// The launch that writes is bound by HBM: the logits are read and the results written. Log-probabilities read the
+// logits twice, once for the rows' maxima and sums (a chunk's go to the workspace) and once to write, which is
+// less than writing the processed logits and going over them again. A workgroup owns a chunk of a row's
+// vocabulary, a thread units of 4 tokens, so that a wave's stores are 1 KB without a gap (with 8 tokens a thread,
+// 16 bytes in every 32 a store, 192 rows of 129,280 take 34 us to write, so 23). 192 rows of bf16 logits to
+// log-probabilities with 2000 ids, 64 biases and a mask each take 49 us: 28 to write (50 MB read, 99 written; 22.5
+// without lists and mask) and 24 for the maxima, which is no HBM time (50 MB, 2.1 TB/s): 15 are the chunks' own,
+// each workgroup waiting for its 16 KB and then reducing them, three workgroups in turn a place, 2 the mask, and
+// 8 the counting of 2000 ids by each of a row's 16 chunks.
+//
+// A workgroup counts its row's whole history (a few thousand tokens, from L2 after the first workgroup) into one
+// LDS word per token of the chunk, so no count table exists in memory and nothing is left to clear; only for long
+// histories of few rows the first launch keeps the words for the second. A word holds the answer's count (20 bits),
+// whether a prompt holds the token (1) and the place of its bias in the list (11, the last one where a token is
+// listed twice): integer additions and maxima, so the result does not depend on their order.
 //
 // The lists cost latency, not work: the ids' way from memory, three barriers, then the logits'. So the chunk's
 // logits, the first ids of the history and the biases are all loaded before the first barrier. A history

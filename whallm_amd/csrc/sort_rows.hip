@@ -11,7 +11,9 @@
 // All four are bound by HBM and walk the tokens, not the permuted rows: a token's row is read or written
 // once and its k permuted rows once each. Sums are fp32 in j order, so a result does not depend on the
 // grid, and are rounded once. 4096 tokens x 8 of 7168 in bf16: the sort 102 us (529 MB, 5.2 TB/s), back 107 us
-// (578 MB, 5.4 TB/s); 2048 x 6 of 5120 in fp32: the gradients of back 101 us (545 MB, 5.4 TB/s).
+// (578 MB, 5.4 TB/s); 2048 x 6 of 5120 in fp32: the gradients of back 98 us (545 MB, 5.6 TB/s). Rows of 512 bytes and
+// less are two to four times their bytes' time: neighbouring tokens write parts of one 128-byte line, and the
+// gradients of back leave most lanes of a wave without a unit.
 #include "permute_device.h"
 #include "row_units.h"
 
@@ -415,8 +417,9 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
 }
 
 // Up to this many pairs each way is taken. 8 tokens x 10 of 2560, captured: a workgroup a token 4.3 us, the
-// counting workgroups 7.3. 32768 pairs of 136 and 1000 columns: one launch 19.2 and 30.5 us, with the spans' launch 16.2 and 26.0;
-// 16384 pairs 10.3 and 12.7.
+// counting workgroups 7.3. Captured, 8 of 256 experts a token, some far busier than others, of 136 and of 1000 columns:
+// 16384 pairs in one launch 10.4 and 14.1 us, with the spans' launch 11.6 and 16.4; 32768 pairs 14.7 and 23.3, with it
+// 12.7 and 22.4 (evenly routed 11.5 and 21.4, with it 12.8 and 22.7).
 constexpr int64_t SORT_FEW_MAX = 256, SORT_ONE_MAX = 16384;
 
 // Spans that are counted apart: each a multiple of the chunk, of 2048 to 8192 pairs (and less than a chunk more).

@@ -309,7 +309,8 @@ def permute(indices: torch.Tensor, experts: int, tile_rows: int = 128) -> Permut
 # These calls, the block norms and process_logits take a few microseconds on the GPU: their checks, outputs and
 # launches are compiled (csrc/host_calls.cpp). They run on the tensors' device, whatever the current one is, and
 # on its current stream. None is recorded by autograd: inputs that require gradients are refused outside
-# torch.no_grad(), and each backward function gives the gradients.
+# torch.no_grad(), inputs with a forward-mode tangent outside torch.inference_mode(), and each backward function
+# gives the gradients.
 
 def sort_tokens(x: torch.Tensor, indices: torch.Tensor, experts: int,
                 tile_rows: int = 128) -> tuple[torch.Tensor, Permutation]:
@@ -590,7 +591,8 @@ def block_norm(residual: torch.Tensor, y: torch.Tensor, post_weight: torch.Tenso
 
     residual [.., H] fp32 or bf16, y [.., H] bf16, weights bf16 [H] (None: the norm alone); ``gate`` fp32 or bf16:
     [H], one value a token [.., 1], or [.., H], through a sigmoid with ``gate_sigmoid`` (norm_router's shared
-    logit as [.., 1]). ``residual_out`` receives residual' and may be the residual itself."""
+    logit as [.., 1]). ``residual_out`` receives residual' and may be the residual itself; it shares no memory with
+    another input."""
     return _lib.host_calls().block_norm(residual, y, post_weight, pre_weight, gate, gate_sigmoid, scale, eps, weight_offset,
                                         post_norm, residual_out)
 
@@ -932,7 +934,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
     ``prompt_lengths`` int32 [rows] say how many count and how many of these are prompt, which only
     ``repetition`` sees. repetition, frequency, presence and temperature are fp32 [rows]; bias_ids int32 and
     bias_values fp32 [rows, n] or [1, n]; mask int32 [rows, ceil(V / 32)] or [1, ..], a set bit allows its token.
-    Returns fp32 [rows, V]; ``out`` may be fp32 logits themselves."""
+    Returns fp32 [rows, V]; ``out`` may be fp32 logits themselves and shares no memory with another input."""
     return _lib.host_calls().process_logits(logits, history, lengths, prompt_lengths, repetition, frequency, presence, bias_ids,
                                             bias_values, mask, temperature, log_probs, out)
 
