@@ -344,7 +344,7 @@ WM_EXPORT int wm_repack_router(const void* router, const void* shared_gate, int3
  * alone, no offset), the gate g bf16 or fp32, through a sigmoid with gate_sigmoid (0 and 1 for
  * infinite gates; 0 where it would be less than the smallest normal number). hidden 1..16384;
  * tensors aligned to their elements. A row's squares are taken in fp32: its values may be up to about
- * 1e18 (x is 0 for a row of 2e19 and more), and with eps 0 as small as 1e-18. */
+ * 1e18 (x of a row of 4e18 and more may be 0), and with eps 0 as small as 1e-17. */
 typedef struct wm_block_norm_form {
   const void* post_weight;
   const void* pre_weight;
