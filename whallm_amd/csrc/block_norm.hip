@@ -16,8 +16,9 @@
 // over tokens (weight gradients) stay with the group, go to the workspace once per workgroup and are added up
 // by a second launch in the workgroups' order. All arithmetic is fp32; bf16 outputs are rounded once, from
 // values that no earlier rounding touched but r''s own (x is the norm of the residual that the next block
-// reads). Rows may have any magnitude whose squares fp32 holds (about 1e-17 to 1e18). 16384 tokens of 4096 in fp32 take 152 us (805 MB, 5.3 TB/s), the gradients of 4001 tokens of 5120 in
-// bf16 with a full gate 68 + 5 us (328 MB, 4.8 TB/s in the first launch).
+// reads). Rows may have any magnitude whose squares fp32 holds (about 1e-17 to 1e18). 16384 tokens of 4096 in fp32
+// take 152 us (805 MB, 5.3 TB/s), the gradients of 4001 tokens of 5120 in bf16 with a full gate 68 + 5 us (328 MB,
+// 4.8 TB/s in the first launch).
 #include <initializer_list>
 
 #include "row_units.h"
