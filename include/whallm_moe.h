@@ -627,6 +627,32 @@ WM_EXPORT int wm_slot_cache_route_rebalance(wm_slot_cache* cache);
 WM_EXPORT int wm_slot_cache_route_state(wm_slot_cache* cache, double* scores, int32_t* quotas, double* short_rates,
                                         double* long_rates, int64_t* tokens, double* read_cost, int64_t* counters);
 
+/* ---- 8-bit rows -----------------------------------------------------------------
+ * Rows in E4M3 with an fp32 scale for each 128 values of a row, what wm_linear_fp8 multiplies: for a
+ * block of values v, s = max(max |v| / 448, 2^-126), with pow2 the next power of two from that on,
+ * and q = e4m3(v / s) to nearest even. A block with an infinity or a NaN has that scale, and its
+ * values' products are NaN. q [rows, width] bytes, scales [rows, ceil(width / 128)]; the last block of
+ * a row may be shorter. Values are computed in fp32 and rounded once. Tensors aligned to their
+ * elements; no output overlaps an input but where it is said. The reference holds its activations in
+ * bf16 and has none of these.
+ *
+ * wm_norm_fp8: the residual's addition and norm of a decoder layer (DecoderLayer.feed_forward,
+ * qwen4_exp.py:1127-1149) with its result in 8 bits:
+ *   r = residual + y                        (y nullable; stored to residual_out where that is given)
+ *   v = r * rsqrt(mean(r^2) + eps) * (weight_offset + weight)
+ * from r as it is stored. residual and residual_out bf16, or fp32 where `fp32` is 1, [tokens, hidden];
+ * y bf16; weight bf16 [hidden] (null: the norm alone, no offset); x (nullable) receives v in bf16.
+ * residual_out may be residual. hidden 1..16384; a row's squares are taken in fp32, as wm_block_norm's.
+ *
+ * wm_fp8_rows: v = the rows of x, bf16 or fp32 [rows, width]; with swiglu x is [rows, 2 width] and
+ * v = silu(gate) * up, the gate's half first (the other one with up_first), clamped as the experts'
+ * are where limit is above 0: gate to at most limit, up to -limit..limit. width 1..1048576. */
+WM_EXPORT int wm_norm_fp8(const void* residual, int32_t fp32, const void* y, const void* weight, float weight_offset,
+                          float eps, int32_t tokens, int32_t hidden, int32_t pow2, void* residual_out, void* q,
+                          float* scales, void* x, void* stream);
+WM_EXPORT int wm_fp8_rows(const void* x, int32_t fp32, int32_t rows, int32_t width, int32_t swiglu, int32_t up_first,
+                          float limit, int32_t pow2, void* q, float* scales, void* stream);
+
 /* ---- logits to acceptance ------------------------------------------------------
  * The steps between a head's logits and sampling or acceptance (wm_mtp_verify_greedy takes logits,
  * wm_mtp_verify_rejection log-probabilities): penalties for tokens already said, biases, a

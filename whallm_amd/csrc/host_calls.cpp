@@ -1,5 +1,5 @@
 // Host side of the calls whose kernels take a few microseconds: the token rows' sort and combine, the block
-// norms and the logit steps (whallm_amd/ops.py documents them). A CPython extension against torch, host code
+// norms, the 8-bit rows and their products and the logit steps (whallm_amd/ops.py documents them). A CPython extension against torch, host code
 // only: it checks the arguments, allocates the outputs and calls the C ABI of libwhallm_moe.so. In Python
 // these steps took 5 to 10 us a call, more than the kernels of a decode step.
 //
@@ -361,6 +361,80 @@ py::tuple block_norm_backward(const Tensor& dx_, const Maybe& dresidual_, const 
   return py::make_tuple(dr, dy, dpost, dpre, dgate);
 }
 
+// ---------------------------------------------------------------- 8-bit rows and their products
+
+constexpr int64_t FP8_BLOCK = 128;
+
+// The outputs of rows [.., width] in FP8.
+struct Fp8Rows {
+  Tensor q, scales;
+  Fp8Rows(at::IntArrayRef sizes, int64_t width, c10::Device device) {
+    at::DimVector shape(sizes.begin(), sizes.end());
+    shape.back() = width;
+    q = empty(shape, at::kFloat8_e4m3fn, device);
+    shape.back() = (width + FP8_BLOCK - 1) / FP8_BLOCK;
+    scales = empty(shape, at::kFloat, device);
+  }
+};
+
+py::tuple norm_fp8(const Tensor& residual_, const Maybe& y_, const Maybe& weight_, double eps, double weight_offset, bool pow2_scales,
+                   bool with_x, const Maybe& out) {
+  no_autograd("norm_fp8", "block_norm_backward has the norm's gradients", {&residual_, ptr(y_), ptr(weight_), ptr(out)});
+  if (!is_rows(residual_.scalar_type()))
+    refuse("residual must be float32 or bfloat16, got " + type_name(residual_.scalar_type()));
+  if (residual_.dim() < 1 || residual_.size(-1) < 1 || residual_.size(-1) > 16384)
+    refuse("residual must be [.., H] with H from 1 to 16384");
+  const int64_t H = residual_.size(-1), T = residual_.numel() / H;
+  if (T > INT32_MAX) refuse("tokens must be below 2^31");
+  if (!(eps >= 0)) refuse("eps must not be negative");
+  const Maybe y = of_type(y_, at::kBFloat16, "y"), weight = of_type(weight_, at::kBFloat16, "weight");
+  if (y && y->sizes() != residual_.sizes()) refuse("y must match residual");
+  if (weight && (weight->dim() != 1 || weight->size(0) != H)) refuse("weight must be [H]");
+  if (out && !y) refuse("residual_out needs y: without it the residual stays as it is");
+  if (out && (out->scalar_type() != residual_.scalar_type() || out->sizes() != residual_.sizes() || !out->is_contiguous()))
+    refuse("residual_out must be a contiguous tensor shaped and typed like residual");
+  const Tensor residual = residual_.contiguous();
+  own_out(out, "residual_out", residual, "residual", {ptr(y), ptr(weight)});
+  const c10::Device device = device_of({&residual, ptr(y), ptr(weight), ptr(out)});
+  const On on(device);
+  const Tensor residual_out = !y ? residual_ : out ? *out : at::empty_like(residual);
+  const Fp8Rows o(residual.sizes(), H, device);
+  Maybe x;
+  if (with_x) x = empty(residual.sizes(), at::kBFloat16, device);
+  checked("wm_norm_fp8", [&] {
+    return wm_norm_fp8(at_of(residual), is_f32(residual), at_of(y), at_of(weight), (float)weight_offset, (float)eps, (int32_t)T,
+                       (int32_t)H, pow2_scales, y ? at_of(residual_out) : nullptr, at_of(o.q), static_cast<float*>(at_of(o.scales)),
+                       at_of(x), on.stream);
+  });
+  changed(out);
+  return with_x ? py::make_tuple(o.q, o.scales, residual_out, *x) : py::make_tuple(o.q, o.scales, residual_out);
+}
+
+std::tuple<Tensor, Tensor> fp8_rows(const char* name, const Tensor& x_, bool swiglu, bool up_first, double limit, bool pow2_scales) {
+  no_autograd(name, "it has no gradient", {&x_});
+  const Tensor x = rows_of(x_, swiglu ? "gate_up" : "x");
+  if (x.dim() < 1 || x.size(-1) < 1) refuse(swiglu ? "gate_up must be [.., 2 I]" : "x must be [.., K]");
+  if (swiglu && x.size(-1) % 2) refuse("gate_up must be [.., 2 I]");
+  const int64_t W = x.size(-1) / (swiglu ? 2 : 1), T = x.numel() / x.size(-1);
+  if (W > 1 << 20) refuse("rows must have at most 1048576 values");
+  if (T > INT32_MAX) refuse("rows must be below 2^31");
+  if (!(limit >= 0)) refuse("limit must not be negative");
+  const c10::Device device = device_of({&x});
+  const On on(device);
+  const Fp8Rows o(x.sizes(), W, device);
+  checked("wm_fp8_rows", [&] {
+    return wm_fp8_rows(at_of(x), is_f32(x), (int32_t)T, (int32_t)W, swiglu, up_first, (float)limit, pow2_scales, at_of(o.q),
+                       static_cast<float*>(at_of(o.scales)), on.stream);
+  });
+  return {o.q, o.scales};
+}
+std::tuple<Tensor, Tensor> quantize_fp8(const Tensor& x, bool pow2_scales) {
+  return fp8_rows("quantize_fp8", x, false, false, 0.0, pow2_scales);
+}
+std::tuple<Tensor, Tensor> swiglu_fp8(const Tensor& gate_up, bool up_first, double limit, bool pow2_scales) {
+  return fp8_rows("swiglu_fp8", gate_up, true, up_first, limit, pow2_scales);
+}
+
 // ---------------------------------------------------------------- logits to acceptance
 
 Maybe row_values(const Maybe& t, int64_t rows, at::ScalarType type, const char* name) {
@@ -448,5 +522,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("combine_rows_backward", &combine_rows_backward);
   m.def("block_norm", &block_norm);
   m.def("block_norm_backward", &block_norm_backward);
+  m.def("norm_fp8", &norm_fp8);
+  m.def("quantize_fp8", &quantize_fp8);
+  m.def("swiglu_fp8", &swiglu_fp8);
   m.def("process_logits", &process_logits);
 }

@@ -918,6 +918,37 @@ class PersistentDecodeStack:
         return bool(r)
 
 
+# ----------------------------------------------------------------------------- 8-bit rows and their products
+
+def norm_fp8(residual: torch.Tensor, y: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6,
+             weight_offset: float = 0.0, pow2_scales: bool = False, with_x: bool = False,
+             residual_out: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
+    """The residual's addition and the norm before a projection, with the result in 8 bits (wm_norm_fp8):
+    residual' = residual + y, v = rmsnorm(residual') * (weight_offset + weight) -> (q, scales, residual'): q
+    float8_e4m3fn [.., H] and scales fp32 [.., ceil(H / 128)] with v = q * scales by blocks of 128 values.
+
+    residual [.., H] fp32 or bf16, y [.., H] bf16 (None: residual' is the residual), weight bf16 [H].
+    ``pow2_scales`` makes the scales powers of two; ``with_x`` adds v in bf16 to the results, for readers that take
+    that (a router). ``residual_out`` receives residual' and may be the residual itself; it shares no memory with another
+    input. block_norm_backward gives the gradients of v and residual'."""
+    return _lib.host_calls().norm_fp8(residual, y, weight, eps, weight_offset, pow2_scales, with_x, residual_out)
+
+
+def quantize_fp8(x: torch.Tensor, pow2_scales: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows [.., K] (bf16 or fp32) -> (q float8_e4m3fn [.., K], scales fp32 [.., ceil(K / 128)]): by blocks of 128
+    values, scale = max |x| / 448 (at least 2^-126; with ``pow2_scales`` the next power of two) and q = x / scale
+    to nearest even (wm_fp8_rows). What linear_fp8 takes."""
+    return _lib.host_calls().quantize_fp8(x, pow2_scales)
+
+
+def swiglu_fp8(gate_up: torch.Tensor, up_first: bool = False, limit: float = 0.0,
+               pow2_scales: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """quantize_fp8 of silu(gate) * up for rows [.., 2 I] (bf16 or fp32), the gate's half first unless ``up_first``:
+    the step between an MLP's products, rounded once. ``limit`` above 0 clamps gate and up as the experts'
+    ``swiglu_limit`` does."""
+    return _lib.host_calls().swiglu_fp8(gate_up, up_first, limit, pow2_scales)
+
+
 # ----------------------------------------------------------------------------- logits to acceptance
 
 def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
