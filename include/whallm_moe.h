@@ -653,6 +653,19 @@ WM_EXPORT int wm_norm_fp8(const void* residual, int32_t fp32, const void* y, con
 WM_EXPORT int wm_fp8_rows(const void* x, int32_t fp32, int32_t rows, int32_t width, int32_t swiglu, int32_t up_first,
                           float limit, int32_t pow2, void* q, float* scales, void* stream);
 
+/* Their product with FP8 weights (E4M3 with the 128 x 128 block scales of mimo/weights.py:17-43):
+ *   out[t, n] = add[t, n] + sum over blocks b of 128 values of K of
+ *               x_scales[t, b] * weight_scales[n / 128, b] * sum_{k in b} x[t, k] * weight[n, k]
+ * x [tokens, k] and weight [n, k] bytes, 16-byte aligned, k a multiple of 16 up to 1048576; x_scales
+ * [tokens, ceil(k / 128)], weight_scales [ceil(n / 128), ceil(k / 128)]; add (nullable) and out
+ * [tokens, n] bf16, or fp32 where out_fp32 is 1, aligned to their elements. out may be add; it
+ * overlaps no other input. Blocks are added up in fp32. Within a block the FP8 matrix
+ * instructions drop what is below about 2^-13 of the sum's largest products; with fp32 outputs the
+ * bytes are multiplied as bf16, whose sums are fp32's. */
+WM_EXPORT int wm_linear_fp8(const void* x, const float* x_scales, int32_t tokens, int32_t k, const void* weight,
+                            const float* weight_scales, int32_t n, const void* add, int32_t out_fp32, void* out,
+                            void* stream);
+
 /* ---- logits to acceptance ------------------------------------------------------
  * The steps between a head's logits and sampling or acceptance (wm_mtp_verify_greedy takes logits,
  * wm_mtp_verify_rejection log-probabilities): penalties for tokens already said, biases, a

@@ -104,6 +104,7 @@ _SIGNATURES = {
                                        c_size_t, _P]),
     "wm_norm_fp8": (c_int, [_P, c_int32, _P, _P, c_float, c_float, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P]),
     "wm_fp8_rows": (c_int, [_P, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, _P, _P, _P]),
+    "wm_linear_fp8": (c_int, [_P, _P, c_int32, c_int32, _P, _P, c_int32, _P, c_int32, _P, _P]),
     "wm_norm_router": (c_int, [_P, _P, _P, c_int32, c_int32, c_float, _P, c_int32, _P, _P, c_size_t, _P, _P, _P, _P,
                                _P]),
     "wm_router_packed_bytes": (c_size_t, [c_int32, c_int32, c_int32]),

@@ -365,6 +365,13 @@ py::tuple block_norm_backward(const Tensor& dx_, const Maybe& dresidual_, const 
 
 constexpr int64_t FP8_BLOCK = 128;
 
+// E4M3 bytes as torch's float8_e4m3fn or, as the expert tables hold them, uint8.
+Tensor fp8_of(const Tensor& t, const char* name) {
+  if (t.scalar_type() != at::kFloat8_e4m3fn && t.scalar_type() != at::kByte)
+    refuse(std::string(name) + " must be float8_e4m3fn or uint8, got " + type_name(t.scalar_type()));
+  return t.contiguous();
+}
+
 // The outputs of rows [.., width] in FP8.
 struct Fp8Rows {
   Tensor q, scales;
@@ -433,6 +440,46 @@ std::tuple<Tensor, Tensor> quantize_fp8(const Tensor& x, bool pow2_scales) {
 }
 std::tuple<Tensor, Tensor> swiglu_fp8(const Tensor& gate_up, bool up_first, double limit, bool pow2_scales) {
   return fp8_rows("swiglu_fp8", gate_up, true, up_first, limit, pow2_scales);
+}
+
+Tensor linear_fp8(const Tensor& x_, const Tensor& x_scales_, const Tensor& weight_, const Tensor& weight_scales_, const py::object& out_dtype,
+                  const Maybe& add_) {
+  if (!THPDtype_Check(out_dtype.ptr())) refuse("out_dtype must be a torch.dtype");
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(out_dtype.ptr())->scalar_type;
+  if (!is_rows(type)) refuse("out_dtype must be bfloat16 or float32, got " + type_name(type));
+  no_autograd("linear_fp8", "it has no gradient", {&x_, &x_scales_, &weight_, &weight_scales_, ptr(add_)});
+  const Tensor x = fp8_of(x_, "x"), weight = fp8_of(weight_, "weight");
+  const Tensor x_scales = of_type(x_scales_, at::kFloat, "x_scales"), weight_scales = of_type(weight_scales_, at::kFloat, "weight_scales");
+  if (x.dim() < 1 || weight.dim() != 2 || x.size(-1) != weight.size(1)) refuse("x must be [.., K] and weight [N, K]");
+  const int64_t K = weight.size(1), N = weight.size(0);
+  if (K < 1 || K % 16 || K > 1 << 20) refuse("K must be a multiple of 16 up to 1048576");
+  if (N < 1 || N > INT32_MAX - 65535) refuse("N must be from 1 to 2147418112");
+  const int64_t T = x.numel() / K, blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+  if (T > INT32_MAX - 65535) refuse("tokens must be at most 2147418112");
+  bool fit = x_scales.dim() == x.dim() && x_scales.size(-1) == blocks;
+  for (int64_t i = 0; fit && i < x.dim() - 1; ++i) fit = x_scales.size(i) == x.size(i);
+  if (!fit) refuse("x_scales must be [.., ceil(K / 128)] for x [.., K]");
+  if (weight_scales.dim() != 2 || weight_scales.size(0) != (N + FP8_BLOCK - 1) / FP8_BLOCK || weight_scales.size(1) != blocks)
+    refuse("weight_scales must be [ceil(N / 128), ceil(K / 128)]");
+  at::DimVector shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  Maybe add;
+  if (add_) {
+    if (add_->scalar_type() != type) refuse("add must be " + type_name(type) + " like the output, got " + type_name(add_->scalar_type()));
+    if (add_->sizes() != at::IntArrayRef(shape)) refuse("add must be [.., N] matching x");
+    add = add_->contiguous();
+  }
+  const c10::Device device = device_of({&x, &x_scales, &weight, &weight_scales, ptr(add)});
+  const On on(device);
+  const Tensor y = empty(shape, type, device);
+  // rows of 16 bytes: a view that starts elsewhere is copied
+  const Tensor xa = reinterpret_cast<uintptr_t>(at_of(x)) % 16 ? x.clone() : x;
+  const Tensor wa = reinterpret_cast<uintptr_t>(at_of(weight)) % 16 ? weight.clone() : weight;
+  checked("wm_linear_fp8", [&] {
+    return wm_linear_fp8(at_of(xa), static_cast<float*>(at_of(x_scales)), (int32_t)T, (int32_t)K, at_of(wa),
+                         static_cast<float*>(at_of(weight_scales)), (int32_t)N, at_of(add), type == at::kFloat, at_of(y), on.stream);
+  });
+  return y;
 }
 
 // ---------------------------------------------------------------- logits to acceptance
@@ -525,5 +572,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_fp8", &norm_fp8);
   m.def("quantize_fp8", &quantize_fp8);
   m.def("swiglu_fp8", &swiglu_fp8);
+  m.def("linear_fp8", &linear_fp8);
   m.def("process_logits", &process_logits);
 }

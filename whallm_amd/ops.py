@@ -949,6 +949,18 @@ def swiglu_fp8(gate_up: torch.Tensor, up_first: bool = False, limit: float = 0.0
     return _lib.host_calls().swiglu_fp8(gate_up, up_first, limit, pow2_scales)
 
 
+def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+               out_dtype: torch.dtype = torch.bfloat16, add: torch.Tensor | None = None) -> torch.Tensor:
+    """The product of 8-bit rows and weights with their block scales (wm_linear_fp8): x [.., K] with x_scales
+    [.., ceil(K / 128)] as quantize_fp8, swiglu_fp8 and norm_fp8 give them, weight [N, K] with weight_scales
+    [ceil(N / 128), ceil(K / 128)] (dequant_fp8_blocks' form), both float8_e4m3fn or uint8, K a multiple of 16
+    -> [.., N] in ``out_dtype`` (bf16 or fp32), plus ``add`` of that shape and type.
+
+    fp32 results are exact to fp32's rounding (a head's logits); bf16 ones take the FP8 matrix instructions at twice
+    the rate. The gradient of x before its rounding is linear_fp8 of dy and the transposed weights and scales."""
+    return _lib.host_calls().linear_fp8(x, x_scales, weight, weight_scales, out_dtype, add)
+
+
 # ----------------------------------------------------------------------------- logits to acceptance
 
 def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
