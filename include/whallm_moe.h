@@ -711,6 +711,30 @@ WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, 
                                 const wm_logit_rules* rules, int32_t log_probs, float* out, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
+/* The draw of each row's next token from logits [rows, vocab] (bf16, or fp32 where `fp32` is 1), the
+ * step of the reference's sampler behind the rules above (native_qwen.py:389-408 draws from the whole
+ * row; the cuts are this library's). With L a row's largest logit and e[v] = exp((l[v] - L) /
+ * temperature):
+ *   top-k   the k tokens of the largest logits stay; of equal ones those of the lower ids
+ *   top-p   of these, in that order, each token stays before which less than p of their weights e
+ *           lies (the first always)
+ *   min-p   of these, each token with e >= min_p stays
+ *   token   the lowest id whose running sum of e over the tokens left, in the order of their ids,
+ *           is above uniform times the whole sum
+ *   logp    log(e[token] / that sum)
+ * uniforms [rows] in [0, 1) (below, or NaN, counts as 0, from 1 on as the largest below 1). temperature, top_k,
+ * top_p and min_p [rows] are nullable and, like the uniforms, on the device. temperature 0 or below (or NaN):
+ * the largest logit, of equal ones the lowest id. A rule is off for a row with top_k 0, below, or vocab and more;
+ * top_p 1 and more; min_p 0 and below (above 1 counts as 1); NaN. Logits of -inf (masked) are never
+ * drawn; the largest may be +inf, which then shares with its equals alone. A row with a NaN or with nothing
+ * but -inf gives token -1 and logp NaN. Weights are fixed point (2^-46 of the largest for vocabularies
+ * around 131072), so that no result depends on an order of sums. tokens int32 [rows], logp fp32 [rows].
+ * vocab up to 4194304. workspace: wm_sample_logits_workspace_size bytes, 16-byte aligned. */
+WM_EXPORT size_t wm_sample_logits_workspace_size(int32_t rows, int32_t vocab);
+WM_EXPORT int wm_sample_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab, const float* uniforms,
+                               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                               int32_t* tokens, float* logp, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- MTP acceptance ----------------------------------------------------------
  * Verify n draft tokens (n <= 15) against n + 1 target rows [n + 1, vocab] fp32.
  * out: device int32[2] = (accepted drafts, next token).

@@ -150,6 +150,8 @@ _SIGNATURES = {
     "wm_experts_fp8": (c_int, [_P, c_int32, _P, c_int32, POINTER(FP8ExpertsC), _P, _P, c_size_t, _P]),
     "wm_process_logits_workspace_size": (c_size_t, [c_int32, c_int32]),
     "wm_process_logits": (c_int, [_P, c_int32, c_int32, c_int32, POINTER(LogitRulesC), c_int32, _P, _P, c_size_t, _P]),
+    "wm_sample_logits_workspace_size": (c_size_t, [c_int32, c_int32]),
+    "wm_sample_logits": (c_int, [_P, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
     "wm_mtp_workspace_size": (c_size_t, [c_int32, c_int32]),
     "wm_mtp_verify_greedy": (c_int, [_P, _P, c_int32, c_int32, _P, _P, c_size_t, _P]),
     "wm_verify_step_fp8_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, _P]),

@@ -560,6 +560,30 @@ Tensor process_logits(const Tensor& logits_, const Maybe& history_, const Maybe&
   return out;
 }
 
+std::tuple<Tensor, Tensor> sample_logits(const Tensor& logits_, const Tensor& uniforms_, const Maybe& temperature_, const Maybe& top_k_,
+                                         const Maybe& top_p_, const Maybe& min_p_) {
+  no_autograd("sample_logits", "it has no gradient", {&logits_, &uniforms_, ptr(temperature_), ptr(top_p_), ptr(min_p_)});
+  const Tensor logits = rows_of(logits_, "logits");
+  if (logits.dim() != 2 || logits.size(1) < 1) refuse("logits must be [rows, vocab]");
+  const int64_t R = logits.size(0), V = logits.size(1);
+  if (R > INT32_MAX || V > 1 << 22) refuse("logits must have at most 2147483647 rows of at most 4194304 values");
+  const Tensor uniforms = *row_values(Maybe(uniforms_), R, at::kFloat, "uniforms");
+  const Maybe temperature = row_values(temperature_, R, at::kFloat, "temperature"), top_k = row_values(top_k_, R, at::kInt, "top_k"),
+              top_p = row_values(top_p_, R, at::kFloat, "top_p"), min_p = row_values(min_p_, R, at::kFloat, "min_p");
+  const c10::Device device = device_of({&logits, &uniforms, ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p)});
+  const On on(device);
+  const Tensor tokens = empty({R}, at::kInt, device), logp = empty({R}, at::kFloat, device);
+  const size_t ws_bytes = wm_sample_logits_workspace_size((int32_t)R, (int32_t)V);
+  const Tensor ws = empty({(int64_t)ws_bytes}, at::kByte, device);
+  checked("wm_sample_logits", [&] {
+    return wm_sample_logits(at_of(logits), is_f32(logits), (int32_t)R, (int32_t)V, static_cast<float*>(at_of(uniforms)),
+                            static_cast<float*>(at_of(temperature)), static_cast<int32_t*>(at_of(top_k)),
+                            static_cast<float*>(at_of(top_p)), static_cast<float*>(at_of(min_p)), static_cast<int32_t*>(at_of(tokens)),
+                            static_cast<float*>(at_of(logp)), at_of(ws), ws_bytes, on.stream);
+  });
+  return {tokens, logp};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -574,4 +598,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_fp8", &swiglu_fp8);
   m.def("linear_fp8", &linear_fp8);
   m.def("process_logits", &process_logits);
+  m.def("sample_logits", &sample_logits);
 }

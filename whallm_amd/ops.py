@@ -982,6 +982,17 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
                                             bias_values, mask, temperature, log_probs, out)
 
 
+def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tensor | None = None,
+                  top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+                  min_p: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Each row's next token (wm_sample_logits has the rules): logits [rows, V] (fp32 or bf16; process_logits' result,
+    say), one number of [0, 1) a row in ``uniforms``, and per row temperature, top_k (int32), top_p and min_p, fp32
+    [rows], applied in this order. Returns (tokens int32 [rows], log-probabilities fp32 [rows] of the drawn tokens among
+    those left). A temperature of 0 takes the largest logit, top_k 0, top_p 1 and min_p 0 are off; a row with a NaN
+    or nothing to draw gives token -1. Everything is on the device, so a captured call follows its values."""
+    return _lib.host_calls().sample_logits(logits, uniforms, temperature, top_k, top_p, min_p)
+
+
 # ----------------------------------------------------------------------------- MTP acceptance
 
 def _mtp_rows(t: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int]:
