@@ -11,14 +11,14 @@
 // is off by at most 2^-(s + 1) of the largest one's weight (2^-46 for 129,280 tokens).
 #include <cmath>
 
-#include "row_units.h"
+#include "norm_rows.h"
 
 namespace wm {
 namespace smp {
 
 constexpr int MAX_VOCAB = 1 << 22;
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
-constexpr int CHUNK = 8192;  // tokens whose weights are added up before the draw looks for its place
+constexpr int SMALL = 8192;  // tokens of a vocabulary that one workgroup takes
 
 struct Args {
   const void* logits;
@@ -113,7 +113,7 @@ struct Shared {
   uint32_t counts[256];
   uint64_t part[WAVES];
   float top[WAVES];
-  uint64_t chunk[MAX_VOCAB / CHUNK];
+  uint64_t chunk[THREADS];  // the chunks' sums
   uint64_t bcast[3];
 };
 
@@ -246,13 +246,68 @@ __device__ Cut row_cut(const Args& a, const void* row, const Rules& r, Shared& s
 }
 
 // ---------------------------------------------------------------------------------- the draw
+//
+// floor(u whole), below the whole.
+__device__ __forceinline__ uint64_t place_of(float u, uint64_t whole) {
+  return __umul64hi((uint64_t)((u > 0.0f ? fminf(u, 1.0f - 0x1p-24f) : 0.0f) * 0x1p64f), whole);
+}
 
+// Writes the token whose running sum passes `want`, given the chunks' sums in s.chunk. left(l, i): the weight of
+// logit l with id i, 0 if it goes. `size` is a chunk's tokens, a multiple of THREADS. Every thread calls it.
+template <bool F32, typename Left>
+__device__ void draw(const Args& a, const void* p, int row, const Rules& r, Shared& s, int chunks, int size, Left left) {
+  uint64_t whole;
+  __syncthreads();
+  const uint64_t of_chunk = (int)threadIdx.x < chunks ? s.chunk[threadIdx.x] : 0;
+  const uint64_t first_of = block_scan(of_chunk, s.part, whole);
+  uint64_t want = place_of(a.uniforms[row], whole);
+  if (want >= first_of && want < first_of + of_chunk) {
+    s.bcast[0] = threadIdx.x;
+    s.bcast[1] = want - first_of;
+  }
+  __syncthreads();
+  const int c = (int)s.bcast[0], each = size / THREADS;
+  want = s.bcast[1];
+  const int first = c * size + (int)threadIdx.x * each, end = min(first + each, a.vocab);
+  uint64_t mine = 0, total;
+  for (int i = first; i < end; ++i) mine += left(logit<F32>(p, i), i);
+  uint64_t before = block_scan(mine, s.part, total);
+  if (want >= before && want < before + mine) {
+    int i = first;
+    float l = logit<F32>(p, i);
+    for (uint64_t w; want >= before + (w = left(l, i)); l = logit<F32>(p, i)) before += w, ++i;
+    const double t = l == r.top ? 0.0 : ((double)l - (double)r.top) * r.scale;
+    a.tokens[row] = i;
+    a.logp[row] = (float)((t - log2(ldexp((double)whole, -a.shift))) * 0.6931471805599453);
+  }
+}
+
+// The weight of a logit that a row's cut keeps, if min-p does.
+__device__ __forceinline__ uint64_t left_of(const Args& a, const Rules& r, float l) {
+  const double e = weight_of(l, r);
+  return e >= (double)r.m ? fixed_of(e, a.shift) : 0;
+}
+
+// The draw of a row from its cut, which is found here, and the chunks' sums.
 template <bool F32>
-__global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
+__device__ void draw_cut(const Args& a, const void* p, int row, const Rules& r, Shared& s, int chunks, int size) {
+  const Cut cut = row_cut<F32>(a, p, r, s);
+  auto left = [&](float l, int i) -> uint64_t { return cut.keeps(key_of(l), i) ? left_of(a, r, l) : 0; };
+  for (int c = 0; c < chunks; ++c) {
+    uint64_t v = 0, total;
+    for (int i = c * size + threadIdx.x; i < min((c + 1) * size, a.vocab); i += THREADS) v += left(logit<F32>(p, i), i);
+    block_scan(v, s.part, total);
+    if (threadIdx.x == 0) s.chunk[c] = total;
+  }
+  draw<F32>(a, p, row, r, s, chunks, size, left);
+}
+
+// Vocabularies of one chunk: a workgroup a row does all of it.
+template <bool F32>
+__global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
   __shared__ Shared s;
   const int row = blockIdx.x;
   const void* p = (const uint8_t*)a.logits + (int64_t)row * a.vocab * (F32 ? 4 : 2);
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   // the largest logit; a NaN's key is the largest or the smallest
   uint32_t high = 0;
   bool nan = false;
@@ -262,7 +317,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
     nan |= l != l;
   }
   for (int d = 32; d > 0; d /= 2) high = max(high, (uint32_t)__shfl_xor((int)high, d, 64));
-  if (lane == 0) s.part[wave] = high;
+  if (threadIdx.x % 64 == 0) s.part[threadIdx.x / 64] = high;
   const bool any = __syncthreads_or(nan);
   for (int w = 0; w < WAVES; ++w) high = max(high, (uint32_t)s.part[w]);
   const float top = value_of(high);
@@ -270,44 +325,403 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
     if (threadIdx.x == 0) a.tokens[row] = -1, a.logp[row] = NAN;
     return;
   }
-  const Rules r(a, row, top);
-  const Cut cut = row_cut<F32>(a, p, r, s);
-  auto kept = [&](int i) -> uint64_t {
-    const float l = logit<F32>(p, i);
-    if (!cut.keeps(key_of(l), i)) return 0;
-    const double e = weight_of(l, r);
-    return e >= (double)r.m ? fixed_of(e, a.shift) : 0;
-  };
-  const int chunks = (a.vocab + CHUNK - 1) / CHUNK;
-  uint64_t whole = 0;
-  for (int c = 0; c < chunks; ++c) {
-    uint64_t v = 0, total;
-    for (int i = c * CHUNK + threadIdx.x; i < min((c + 1) * CHUNK, a.vocab); i += THREADS) v += kept(i);
-    block_scan(v, s.part, total);
-    if (threadIdx.x == 0) s.chunk[c] = total;
-    whole += total;
+  draw_cut<F32>(a, p, row, Rules(a, row, top), s, 1, SMALL);
+}
+
+// ---------------------------------------------------------------------------------- larger vocabularies
+//
+// Four launches over chunks of the rows: each chunk's largest logit; weights and counts by bins of the distance from the
+// row's largest; the tokens in the bins that a cut may fall into (candidates), and the chunks' sums of those above;
+// the cut among the candidates and the draw, a workgroup a row. A bin is 1/32 of a factor of 2, so that a cut has some
+// hundreds of candidates where it falls among the bulk of the tokens and a few where it does not. Rows of more
+// candidates than there is room for (a cut among thousands of nearly equal logits) are cut by radix selection as above.
+constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048;
+
+struct RowInfo {
+  uint64_t below_lo, between;  // weights of the bins below lo, and of those between hi and kbin
+  int32_t lo, hi;              // bins below lo stay, bins above hi go by top-p
+  int32_t kbin, kleft;         // top-k ends in kbin, which has kleft tokens that stay (BINS: nowhere)
+};
+
+struct Work {
+  float* tops;          // [rows][chunks]; NaN where the chunk has one
+  uint64_t* sums;       // [rows][chunks]
+  RowInfo* info;        // [rows]
+  uint64_t* weights;    // [rows][BINS]
+  uint32_t* counts;     // [rows][BINS]
+  uint64_t* list;       // [rows][CANDIDATES]: key and the complement of the id
+  uint32_t* listed;     // [rows]
+  int chunks, size;
+};
+
+__device__ __forceinline__ uint64_t entry_of(float l, int i) { return (uint64_t)key_of(l) << 32 | (uint32_t)~i; }
+
+// A row's bins: monotone in the logit, BINS - 1 where the weight is 0 (from 2^-63.9 on).
+struct Bins {
+  float top, scale;
+  __device__ __forceinline__ explicit Bins(const Rules& r) : top(r.top), scale((float)(32.0 * r.scale)) {}
+  __device__ __forceinline__ int of(float l) const { return l == top ? 0 : (int)fminf((top - l) * scale, (float)(BINS - 1)); }
+};
+
+// The row's largest logit from its chunks'; false for a row that has nothing to draw. Every thread calls it.
+template <int N>
+__device__ __forceinline__ bool row_top(const float* tops, int chunks, float* part, float& top) {
+  float t = -INFINITY;
+  bool nan = false;
+  for (int c = threadIdx.x; c < chunks; c += N) {
+    const float v = tops[c];
+    nan |= v != v;
+    t = fmaxf(t, v);
   }
-  const float u = a.uniforms[row];
-  const uint64_t f = (uint64_t)((u > 0.0f ? fminf(u, 1.0f - 0x1p-24f) : 0.0f) * 0x1p64f);
-  uint64_t want = __umul64hi(f, whole);  // floor(u whole), below the whole
+  t = segment_max<64>(t);
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = t;
+  nan = __syncthreads_or(nan);
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) t = fmaxf(t, part[w]);
+  top = t;
+  return !nan && t != -INFINITY;
+}
+
+// Eight logits of a chunk from token i on, `n` of them there; the others are -inf.
+template <bool F32>
+struct Eight {
+  Row8<F32> raw;
+  __device__ __forceinline__ void load(const void* logits, int64_t base, int i, int n) {
+    raw.clear();
+    if (n > 0) raw.template load<false>(logits, base + i, n);
+  }
+  __device__ __forceinline__ float get(int e, int n) const { return e < n ? raw.get(e) + 0.0f : -INFINITY; }
+};
+
+template <bool F32>
+__global__ void __launch_bounds__(BIN_THREADS) sample_tops_kernel(Args a, Work w) {
+  __shared__ float part[BIN_THREADS / 64];
+  const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
+  const int64_t base = (int64_t)row * a.vocab;
+  const int lo = c * w.size, end = min(lo + w.size, a.vocab);
+  for (int i = c * BIN_THREADS + threadIdx.x; i < BINS; i += w.chunks * BIN_THREADS) {
+    w.weights[(int64_t)row * BINS + i] = 0;
+    w.counts[(int64_t)row * BINS + i] = 0;
+  }
+  if (c == 0 && threadIdx.x == 0) w.listed[row] = 0;
+  float t = -INFINITY;
+  bool nan = false;
+  for (int i = lo + 8 * threadIdx.x; i < end; i += UNIT) {
+    Eight<F32> l;
+    l.load(a.logits, base, i, end - i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = l.get(e, end - i);
+      nan |= v != v;
+      t = fmaxf(t, v);
+    }
+  }
+  t = segment_max<64>(t);
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = t;
+  nan = __syncthreads_or(nan);
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int q = 1; q < BIN_THREADS / 64; ++q) t = fmaxf(t, part[q]);
+    w.tops[blockIdx.x] = nan ? NAN : t;
+  }
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(BIN_THREADS) sample_bins_kernel(Args a, Work w) {
+  __shared__ uint64_t weights[BINS];
+  __shared__ uint32_t counts[BINS];
+  __shared__ float part[BIN_THREADS / 64];
+  const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
+  float top;
+  if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, part, top)) return;
+  const Rules r(a, row, top);
+  const bool by_weight = r.p < 1.0f, by_count = r.k > 0;
+  if (!by_weight && !by_count) return;
+  const Bins bins(r);
+  for (int i = threadIdx.x; i < BINS; i += BIN_THREADS) weights[i] = 0, counts[i] = 0;
   __syncthreads();
-  int c = 0;
-  while (want >= s.chunk[c]) want -= s.chunk[c++];
-  constexpr int EACH = CHUNK / THREADS;
-  const int first = c * CHUNK + (int)threadIdx.x * EACH;
-  uint64_t v[EACH], mine = 0, total;
+  const int64_t base = (int64_t)row * a.vocab;
+  const int lo = c * w.size, end = min(lo + w.size, a.vocab);
+  for (int i = lo + 8 * threadIdx.x; i < end; i += UNIT) {
+    Eight<F32> l;
+    l.load(a.logits, base, i, end - i);
 #pragma unroll
-  for (int j = 0; j < EACH; ++j) mine += v[j] = first + j < a.vocab ? kept(first + j) : 0;
-  uint64_t before = block_scan(mine, s.part, total);
-  if (want >= before && want < before + mine) {
-    int j = 0;
+    for (int e = 0; e < 8; ++e) {
+      const float v = l.get(e, end - i);
+      const int b = bins.of(v);
+      if (b == BINS - 1) continue;
+      if (by_count) atomicAdd(&counts[b], 1u);
+      if (by_weight) atomicAdd((unsigned long long*)&weights[b], (unsigned long long)fixed_of(weight_of(v, r), a.shift));
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += BIN_THREADS) {
+    if (weights[i]) atomicAdd((unsigned long long*)&w.weights[(int64_t)row * BINS + i], (unsigned long long)weights[i]);
+    if (counts[i]) atomicAdd(&w.counts[(int64_t)row * BINS + i], counts[i]);
+  }
+}
+
+// Sum of the threads before this one over a workgroup of N threads.
+template <int N>
+__device__ __forceinline__ uint64_t scan_of(uint64_t v, uint64_t* part, uint64_t& total) {
+  const uint64_t s = wave_scan(v);
+  __syncthreads();
+  if (threadIdx.x % 64 == 63) part[threadIdx.x / 64] = s;
+  __syncthreads();
+  uint64_t before = 0;
+  total = 0;
 #pragma unroll
-    for (int q = 0; q < EACH; ++q)
-      if (want >= before + v[q] && j == q) before += v[q], j = q + 1;
-    a.tokens[row] = first + j;
-    const float l = logit<F32>(p, first + j);
-    const double t = l == top ? 0.0 : ((double)l - (double)top) * r.scale;
-    a.logp[row] = (float)((t - log2(ldexp((double)whole, -a.shift))) * 0.6931471805599453);
+  for (int q = 0; q < N / 64; ++q) {
+    if (q < (int)threadIdx.x / 64) before += part[q];
+    total += part[q];
+  }
+  return before + s - v;
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work w) {
+  constexpr int EACH = BINS / BIN_THREADS;
+  __shared__ uint64_t part[BIN_THREADS / 64];
+  __shared__ float top_part[BIN_THREADS / 64];
+  __shared__ RowInfo info;
+  __shared__ uint64_t k_below, k_in;  // weights below kbin, and in it
+  const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
+  float top;
+  if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, top_part, top)) return;
+  const Rules r(a, row, top);
+  const Bins bins(r);
+  if (threadIdx.x == 0) info = {0, 0, BINS, BINS, BINS, 0};
+  if (r.k > 0 || r.p < 1.0f) {
+    uint64_t weight[EACH], sum = 0, total, before;
+    uint32_t count[EACH], n = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int64_t at = (int64_t)row * BINS + threadIdx.x * EACH + j;
+      sum += weight[j] = w.weights[at];
+      n += count[j] = w.counts[at];
+    }
+    before = scan_of<BIN_THREADS>(sum, part, total);
+    if (threadIdx.x == 0) k_below = total, k_in = 0;
+    if (r.k > 0) {
+      uint64_t counted;
+      uint64_t at = scan_of<BIN_THREADS>(n, part, counted), below = before;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        if (at < (uint64_t)r.k && at + count[j] >= (uint64_t)r.k) {
+          info.kbin = threadIdx.x * EACH + j;
+          info.kleft = r.k - (int)at;
+          k_below = below;
+          k_in = info.kleft == (int)count[j] ? 0 : weight[j];
+          if (!k_in) k_below += weight[j];
+        }
+        at += count[j];
+        below += weight[j];
+      }
+    }
+    __syncthreads();
+    if (r.p < 1.0f) {
+      // the weights that top-k leaves are k_below to k_below + k_in
+      const uint64_t least = part_of(r.p, k_below > 0 ? k_below : 1), most = part_of(r.p, k_below + k_in);
+      uint64_t at = before;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int b = threadIdx.x * EACH + j;
+        if (at < least && at + weight[j] >= least) info.lo = b, info.below_lo = at;
+        if (at < most && at + weight[j] >= most) info.hi = b;
+        at += weight[j];
+      }
+      __syncthreads();
+      const int hi = info.hi, kbin = info.kbin;
+      uint64_t v = 0;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int b = threadIdx.x * EACH + j;
+        if (b > hi && b < kbin) v += weight[j];
+      }
+      scan_of<BIN_THREADS>(v, part, total);
+      if (threadIdx.x == 0) info.between = total;
+    } else if (threadIdx.x == 0) {
+      info.lo = info.hi = info.kbin;
+    }
+  }
+  __syncthreads();
+  if (c == 0 && threadIdx.x == 0) w.info[row] = info;
+  const int stay = info.lo, hi = info.hi, kbin = info.kbin;
+  uint64_t sum = 0;
+  const int64_t base = (int64_t)row * a.vocab;
+  const int lo = c * w.size, end = min(lo + w.size, a.vocab);
+  for (int i = lo + 8 * threadIdx.x; i < end; i += UNIT) {
+    Eight<F32> l;
+    l.load(a.logits, base, i, end - i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = l.get(e, end - i);
+      const int b = bins.of(v);
+      if (b == BINS - 1) continue;
+      if (b < stay) {
+        sum += left_of(a, r, v);
+      } else if (b <= hi || b == kbin) {
+        const uint32_t at = atomicAdd(&w.listed[row], 1u);
+        if (at < CANDIDATES) w.list[(int64_t)row * CANDIDATES + at] = entry_of(v, i + e);
+      }
+    }
+  }
+  uint64_t total;
+  scan_of<BIN_THREADS>(sum, part, total);
+  if (threadIdx.x == 0) w.sums[blockIdx.x] = total;
+}
+
+// Descending, in LDS; n a power of two.
+__device__ __forceinline__ void sort_entries(uint64_t* v, int n) {
+  for (int k = 2; k <= n; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      __syncthreads();
+      for (int t = threadIdx.x; t < n / 2; t += THREADS) {
+        const int i = 2 * t - (t & (j - 1)), o = i + j;  // the pair's lower place
+        const uint64_t x = v[i], y = v[o];
+        if ((x < y) == ((i & k) == 0)) v[i] = y, v[o] = x;
+      }
+    }
+  __syncthreads();
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
+  constexpr int EACH = CANDIDATES / THREADS;
+  __shared__ Shared s;
+  __shared__ uint64_t entry[CANDIDATES];
+  __shared__ int kept_entries;
+  const int row = blockIdx.x;
+  const void* p = (const uint8_t*)a.logits + (int64_t)row * a.vocab * (F32 ? 4 : 2);
+  float top;
+  if (!row_top<THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, s.top, top)) {
+    if (threadIdx.x == 0) a.tokens[row] = -1, a.logp[row] = NAN;
+    return;
+  }
+  const Rules r(a, row, top);
+  const int n = (int)w.listed[row];
+  if (n > CANDIDATES) {  // the same for all threads
+    draw_cut<F32>(a, p, row, r, s, w.chunks, w.size);
+    return;
+  }
+  const Bins bins(r);
+  const RowInfo info = w.info[row];
+  if ((int)threadIdx.x < w.chunks) s.chunk[threadIdx.x] = w.sums[(int64_t)row * w.chunks + threadIdx.x];
+  if (threadIdx.x == 0) kept_entries = 0;
+  uint64_t last = ~0ull;  // the last entry that stays; none
+  if (n > 0) {
+    int places = 2;
+    while (places < n) places *= 2;
+    for (int i = threadIdx.x; i < places; i += THREADS) entry[i] = i < n ? w.list[(int64_t)row * CANDIDATES + i] : 0;
+    sort_entries(entry, places);
+    // in order: the bins from lo to hi, then kbin's, if that is behind them
+    float l[EACH];
+    int b[EACH], in_k[EACH];
+    uint64_t weight[EACH], sum = 0, ahead = 0, total;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = threadIdx.x * EACH + j;
+      l[j] = i < n ? value_of((uint32_t)(entry[i] >> 32)) : -INFINITY;
+      b[j] = i < n ? bins.of(l[j]) : BINS;
+      weight[j] = i < n ? fixed_of(weight_of(l[j], r), a.shift) : 0;
+      ahead += b[j] < info.kbin;
+    }
+    uint64_t before_k;
+    block_scan(ahead, s.part, before_k);  // entries ahead of kbin's
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = threadIdx.x * EACH + j;
+      in_k[j] = i < n && (b[j] < info.kbin || (b[j] == info.kbin && i < (int)before_k + info.kleft));
+      if (!in_k[j]) weight[j] = 0;
+      sum += weight[j];
+    }
+    uint64_t before = block_scan(sum, s.part, total);
+    const uint64_t want = r.p < 1.0f ? part_of(r.p, info.below_lo + info.between + total) : 0;
+    int kept = 0;
+    before += info.below_lo;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      if (in_k[j] && (!(r.p < 1.0f) || (b[j] <= info.hi && before < want))) {
+        ++kept;
+        const int id = (int)~(uint32_t)entry[threadIdx.x * EACH + j];
+        const uint64_t v = left_of(a, r, l[j]);
+        if (v) atomicAdd((unsigned long long*)&s.chunk[id / w.size], (unsigned long long)v);
+      }
+      before += weight[j];
+    }
+    if (kept) atomicAdd(&kept_entries, kept);
+    __syncthreads();
+    if (kept_entries > 0) last = entry[kept_entries - 1];
+  }
+  draw<F32>(a, p, row, r, s, w.chunks, w.size, [&](float l, int i) -> uint64_t {
+    const int b = bins.of(l);
+    return b < BINS - 1 && (b < info.lo || entry_of(l, i) >= last) ? left_of(a, r, l) : 0;
+  });
+}
+
+// Tokens of a chunk: whole units, so many that the launches have about three workgroups a CU.
+static int chunk_size(int64_t rows, int vocab) {
+  const int64_t units = (vocab + UNIT - 1) / UNIT, each = rows * units / 768;
+  return (int)(each < 1 ? 1 : each > 8 ? 8 : each) * UNIT;
+}
+struct Layout {
+  int chunks, size;
+  size_t tops, sums, info, weights, counts, list, listed, bytes;
+  Layout(int64_t rows, int vocab) {
+    size = chunk_size(rows, vocab);
+    chunks = (vocab + size - 1) / size;
+    bytes = 0;
+    auto part = [&](size_t n) {
+      const size_t at = bytes;
+      bytes += (n + 15) / 16 * 16;
+      return at;
+    };
+    sums = part(rows * chunks * sizeof(uint64_t));
+    info = part(rows * sizeof(RowInfo));
+    weights = part(rows * BINS * sizeof(uint64_t));
+    list = part(rows * CANDIDATES * sizeof(uint64_t));
+    counts = part(rows * BINS * sizeof(uint32_t));
+    tops = part(rows * chunks * sizeof(float));
+    listed = part(rows * sizeof(uint32_t));
+  }
+};
+
+// Rows that one set of launches takes, which bounds the workspace: 41 KB a row.
+constexpr int BATCH = 1024;
+
+template <bool F32>
+static void launch(Args a, void* workspace, hipStream_t st) {
+  if (a.vocab <= SMALL) {
+    hipLaunchKernelGGL((sample_row_kernel<F32>), dim3(a.rows), dim3(THREADS), 0, st, a);
+    check_launch("sample_row");
+    return;
+  }
+  const Layout at(a.rows < BATCH ? a.rows : BATCH, a.vocab);
+  uint8_t* base = (uint8_t*)workspace;
+  const Work w = {(float*)(base + at.tops),       (uint64_t*)(base + at.sums),   (RowInfo*)(base + at.info),
+                  (uint64_t*)(base + at.weights), (uint32_t*)(base + at.counts), (uint64_t*)(base + at.list),
+                  (uint32_t*)(base + at.listed),  at.chunks,                     at.size};
+  for (int left = a.rows; left > 0; left -= BATCH) {
+    a.rows = left < BATCH ? left : BATCH;
+    const dim3 grid((unsigned)(a.rows * at.chunks));
+    hipLaunchKernelGGL((sample_tops_kernel<F32>), grid, dim3(BIN_THREADS), 0, st, a, w);
+    check_launch("sample_tops");
+    if (a.top_k || a.top_p || a.temperature) {  // else no row has a cut
+      hipLaunchKernelGGL((sample_bins_kernel<F32>), grid, dim3(BIN_THREADS), 0, st, a, w);
+      check_launch("sample_bins");
+    }
+    hipLaunchKernelGGL((sample_gather_kernel<F32>), grid, dim3(BIN_THREADS), 0, st, a, w);
+    check_launch("sample_gather");
+    hipLaunchKernelGGL((sample_draw_kernel<F32>), dim3(a.rows), dim3(THREADS), 0, st, a, w);
+    check_launch("sample_draw");
+    a.logits = (const uint8_t*)a.logits + (int64_t)BATCH * a.vocab * (F32 ? 4 : 2);
+    a.uniforms += BATCH;
+    if (a.temperature) a.temperature += BATCH;
+    if (a.top_k) a.top_k += BATCH;
+    if (a.top_p) a.top_p += BATCH;
+    if (a.min_p) a.min_p += BATCH;
+    a.tokens += BATCH;
+    a.logp += BATCH;
   }
 }
 
@@ -318,7 +732,10 @@ using namespace wm;
 
 extern "C" {
 
-WM_EXPORT size_t wm_sample_logits_workspace_size(int32_t rows, int32_t vocab) { return 0; }
+WM_EXPORT size_t wm_sample_logits_workspace_size(int32_t rows, int32_t vocab) {
+  if (rows < 0 || vocab <= smp::SMALL || vocab > smp::MAX_VOCAB) return 0;
+  return smp::Layout(rows < smp::BATCH ? rows : smp::BATCH, vocab).bytes;
+}
 
 WM_EXPORT int wm_sample_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab, const float* uniforms,
                                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
@@ -327,19 +744,21 @@ WM_EXPORT int wm_sample_logits(const void* logits, int32_t fp32, int32_t rows, i
     if (rows < 0) fail("wm_sample_logits: rows must not be negative");
     if (vocab < 1 || vocab > smp::MAX_VOCAB) fail("wm_sample_logits: vocab must be in 1..4194304");
     if (fp32 != 0 && fp32 != 1) fail("wm_sample_logits: fp32 must be 0 (bf16 logits) or 1");
-    const unsigned grid = grid_of("wm_sample_logits", rows, smp::THREADS);
+    grid_of("wm_sample_logits", rows, smp::THREADS);
     if (rows == 0) return;
     if (!logits || !uniforms || !tokens || !logp) fail("wm_sample_logits: null pointer");
     if ((uintptr_t)logits % (fp32 ? 4 : 2) ||
         ((uintptr_t)uniforms | (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)tokens |
          (uintptr_t)logp) % 4)
       fail("wm_sample_logits: tensors must be aligned to their elements");
+    const size_t need = wm_sample_logits_workspace_size(rows, vocab);
+    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+      fail("wm_sample_logits: workspace too small or misaligned");
     int bits = 0;
     while ((1 << bits) < vocab) ++bits;
     const smp::Args a = {logits, rows, vocab, 62 - bits < 51 ? 62 - bits : 51, uniforms, temperature, top_k, top_p, min_p, tokens, logp};
-    if (fp32) hipLaunchKernelGGL((smp::sample_kernel<true>), dim3(grid), dim3(smp::THREADS), 0, as_stream(stream), a);
-    else hipLaunchKernelGGL((smp::sample_kernel<false>), dim3(grid), dim3(smp::THREADS), 0, as_stream(stream), a);
-    check_launch("sample_logits");
+    if (fp32) smp::launch<true>(a, workspace, as_stream(stream));
+    else smp::launch<false>(a, workspace, as_stream(stream));
   });
 }
 
