@@ -11,6 +11,8 @@
 // output's rounding (2^-8) but not below fp32's: for fp32 outputs the bytes, which are bf16 values, are
 // converted to bf16 in registers, exactly, and multiplied by the bf16 instructions, whose sums are fp32's (2^-21 of the
 // magnitudes), at half the rate.
+#include <type_traits>
+
 #include "lds_dma.h"
 #include "row_units.h"
 
@@ -31,7 +33,6 @@ struct Args {
   const void* add;
   void* out;
   int tokens, n, k, blocks;
-  int vec;  // outputs of 4 consecutive weight rows are one aligned store
 };
 
 // A lane's 32 bytes of a row's block: the pieces g and 4 + g of 16 bytes, g = lane / 16, of row lane % 16 of a
@@ -94,28 +95,27 @@ __device__ __forceinline__ void store_one(const Args& a, int t, int n, float v) 
     ((uint16_t*)a.out)[at] = (uint16_t)pack_bf16(v, 0.0f);
   }
 }
-// Weight rows n .. n + 3.
+// Weight rows n .. n + 3 of token t, with what is to be added.
 template <bool F32>
-__device__ __forceinline__ void store_four(const Args& a, int t, int n, f32x4 v) {
-  if (!a.vec) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.n) store_one<F32>(a, t, n + i, v[i]);
-    return;
-  }
-  if (n >= a.n) return;  // a.n is a multiple of 4
+__device__ __forceinline__ f32x4 added(const Args& a, int t, int n, f32x4 v) {
+  if (!a.add || t >= a.tokens) return v;
   const int64_t at = (int64_t)t * a.n + n;
-  if (F32) {
-    if (a.add) v += *(const f32x4*)((const float*)a.add + at);
-    *(f32x4*)((float*)a.out + at) = v;
-  } else {
-    if (a.add) {
-      const wm_u32x2 d = *(const wm_u32x2*)((const uint16_t*)a.add + at);
+  if (n + 4 <= a.n) {
+    if (F32) {
+      const wm_u32x4 d = load16((const float*)a.add + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(d[i]);
+    } else {
+      const wm_u32x2 d = load8((const uint16_t*)a.add + at);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(i % 2 ? d[i / 2] & 0xffff0000u : d[i / 2] << 16);
     }
-    *(wm_u32x2*)((uint16_t*)a.out + at) = wm_u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.n) v[i] += F32 ? ((const float*)a.add)[at + i] : bf16_bits_to_f32(((const uint16_t*)a.add)[at + i]);
   }
+  return v;
 }
 
 // ---------------------------------------------------------------------------------
@@ -289,15 +289,14 @@ __global__ void __launch_bounds__(64 * T::WAVES) tiled_kernel(Args a, int n_tile
   const uint32_t sdst = T::SCALES + (tokens_scales ? 256u * wave : 4u * T::BM);
   soff = (uint32_t)(tokens_scales ? min(t0 + 64 * wave + lane, a.tokens - 1) - t0
                                   : min(lane, (a.n - 1) / BLOCK - n0 / BLOCK)) * (uint32_t)a.blocks * 4u;
-  auto issue = [&](int b) {
+  // Load i of block b's LOADS.
+  auto issue = [&](int b, int i) {
     const uint32_t slot = lds_addr(lds + b % T::STAGES * T::STAGE);
     // pieces behind the rows' end read the block's first one
     const uint32_t off = (uint32_t)BLOCK * b - (TAIL && BLOCK * b + 16 * piece >= a.k ? 16u * piece : 0u);
-#pragma unroll
-    for (int i = 0; i < T::WL; ++i) dma16(wbase, woff[i] + off, slot + 1024 * (wave + T::WAVES * i));
-#pragma unroll
-    for (int i = 0; i < T::XL; ++i) dma16(xbase, xoff[i] + off, slot + T::W + 1024 * (wave + T::WAVES * i));
-    dma4(sbase, soff + 4u * b, slot + sdst);
+    if (i < T::WL) dma16(wbase, woff[i] + off, slot + 1024 * (wave + T::WAVES * i));
+    else if (i < T::WL + T::XL) dma16(xbase, xoff[i - T::WL] + off, slot + T::W + 1024 * (wave + T::WAVES * (i - T::WL)));
+    else dma4(sbase, soff + 4u * b, slot + sdst);
   };
 
   f32x4 acc[T::TN][T::TM];
@@ -310,44 +309,110 @@ __global__ void __launch_bounds__(64 * T::WAVES) tiled_kernel(Args a, int n_tile
   const uint32_t wrow = (uint32_t)(16 * T::TN * wn + c) * BLOCK + pos, xrow = T::W + (uint32_t)(16 * T::TM * wm + c) * BLOCK + pos;
   const uint32_t xscale = T::SCALES + 4u * (16 * T::TM * wm + c), wscale = T::SCALES + 4u * (T::BM + 16 * T::TN * wn / BLOCK);
 
+  // Block b's sums. The multiply-adds of a matrix instruction's results stand beside the instruction TM later, so that
+  // none waits for them (the last ones of a block beside the next block's first). With AHEAD the loads of the block STAGES - 1
+  // behind it go out between the instructions of the block's first half.
+  f32x4 d[T::TM];
+  float f[T::TM];
 #pragma unroll
-  for (int p = 0; p < T::STAGES - 1; ++p)
-    if (p < a.blocks) issue(p);
-  for (int b = 0; b < a.blocks; ++b) {
-    // this step's loads have landed in every wave, and every wave is done with the slot that the next loads overwrite
-    wait_step<T::LOADS, T::STAGES - 2>(a.blocks - 1 - b);
-    if (b + T::STAGES - 1 < a.blocks) issue(b + T::STAGES - 1);
+  for (int m = 0; m < T::TM; ++m) d[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f[m] = 0.0f;
+  auto step = [&](int b, auto ahead, auto last) {
+    constexpr bool AHEAD = decltype(ahead)::value, LAST = decltype(last)::value;
     const uint8_t* s = lds + b % T::STAGES * T::STAGE;
-    const int pieces = TAIL && b == a.blocks - 1 ? (a.k - b * BLOCK) / 16 : 8;
+    const int pieces = (a.k - b * BLOCK) / 16;
     auto frag = [&](uint32_t at) {
       Frag f = {*reinterpret_cast<const uint4*>(s + at), *reinterpret_cast<const uint4*>(s + (at ^ 64u))};
-      if (TAIL) zero_behind(f, g, pieces);
+      if (TAIL && LAST) zero_behind(f, g, pieces);
       return Operand<F32>(f);
     };
-    const float ws = *reinterpret_cast<const float*>(s + wscale);
-    Operand<F32> x[T::TM];
+    Operand<F32> x[T::TM], w[2];
+    w[0] = frag(wrow);
 #pragma unroll
     for (int m = 0; m < T::TM; ++m) x[m] = frag(xrow + 16 * BLOCK * m);
-    float f[T::TM];
+    const float ws = *reinterpret_cast<const float*>(s + wscale);
+    float xs[T::TM];
 #pragma unroll
-    for (int m = 0; m < T::TM; ++m) f[m] = ws * *reinterpret_cast<const float*>(s + xscale + 64 * m);
+    for (int m = 0; m < T::TM; ++m) xs[m] = *reinterpret_cast<const float*>(s + xscale + 64 * m);
 #pragma unroll
     for (int i = 0; i < T::TN; ++i) {
-      const Operand<F32> w = frag(wrow + 16 * BLOCK * i);
+      if (i + 1 < T::TN) w[(i + 1) % 2] = frag(wrow + 16 * BLOCK * (i + 1));
+      if (AHEAD) {
+        constexpr int PER = (2 * T::LOADS + T::TN - 1) / T::TN;  // in the first half
+#pragma unroll
+        for (int q = i * PER; q < (i + 1) * PER && q < T::LOADS; ++q) issue(b + T::STAGES - 1, q);
+      }
 #pragma unroll
       for (int m = 0; m < T::TM; ++m) {
-        const f32x4 d = Operand<F32>::product(w, x[m]);
+        const f32x4 p = Operand<F32>::product(w[i % 2], x[m]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][m][e] = fmaf(d[e], f[m], acc[i][m][e]);
+        for (int e = 0; e < 4; ++e) acc[(i + T::TN - 1) % T::TN][m][e] = fmaf(d[m][e], f[m], acc[(i + T::TN - 1) % T::TN][m][e]);
+        if (i == 0) f[m] = ws * xs[m];
+        d[m] = p;
+        __builtin_amdgcn_sched_barrier(0);  // the order as it is written
       }
     }
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  int b = 0;
+  for (; b < T::STAGES - 1 && b < a.blocks; ++b)
+#pragma unroll
+    for (int i = 0; i < T::LOADS; ++i) issue(b, i);
+  // at the top of a block its loads have landed in every wave, and every wave is done with the slot that the next
+  // loads overwrite
+  for (b = 0; b + T::STAGES - 1 < a.blocks; ++b) {
+    wait_loads<T::LOADS * (T::STAGES - 2)>();
+    step(b, yes, no);
   }
+  for (; b + 1 < a.blocks; ++b) {
+    wait_step<T::LOADS, T::STAGES - 2>(a.blocks - 1 - b);
+    step(b, no, no);
+  }
+  wait_loads<0>();
+  step(b, no, yes);
+#pragma unroll
+  for (int m = 0; m < T::TM; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[T::TN - 1][m][e] = fmaf(d[m][e], f[m], acc[T::TN - 1][m][e]);
+  // Results by way of LDS, so that stores are whole runs of a row: a wave has ROWS tokens at a time there, its 16 TN weight rows
+  // each as pieces of 16 bytes, the piece's place XOR the token's.
+  wait_loads<0>();
+  constexpr int WIDE = 16 * T::TN, SIZE = F32 ? 4 : 2, EACH = 16 / SIZE, PIECES = WIDE / EACH, BYTES = 16 * WIDE * SIZE;
+  constexpr int MASK = PIECES < 16 ? PIECES - 1 : 15;
+  uint8_t* mine = lds + wave * BYTES;
+  static_assert(T::WAVES * BYTES <= T::STAGES * T::STAGE);
 #pragma unroll
   for (int m = 0; m < T::TM; ++m) {
-    const int t = t0 + 16 * (T::TM * wm + m) + c;
-    if (t >= a.tokens) continue;
+    if (m > 0) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its own reads
 #pragma unroll
-    for (int i = 0; i < T::TN; ++i) store_four<F32>(a, t, n0 + 16 * (T::TN * wn + i) + 4 * g, acc[i][m]);
+    for (int i = 0; i < T::TN; ++i) {
+      const f32x4 v = added<F32>(a, t0 + 16 * (T::TM * wm + m) + c, n0 + WIDE * wn + 16 * i + 4 * g, acc[i][m]);
+      if constexpr (F32) {
+        *reinterpret_cast<f32x4*>(mine + c * WIDE * 4 + 16 * ((4 * i + g) ^ (c & MASK))) = v;
+      } else {
+        *reinterpret_cast<wm_u32x2*>(mine + c * WIDE * 2 + 16 * ((2 * i + g / 2) ^ (c & MASK)) + 8 * (g % 2)) =
+            wm_u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < PIECES / 4; ++j) {
+      const int at = 64 * j + lane, row = at / PIECES, q = at % PIECES;
+      const int t = t0 + 16 * (T::TM * wm + m) + row, n = n0 + WIDE * wn + EACH * q;
+      const wm_u32x4 v = *reinterpret_cast<const wm_u32x4*>(mine + row * WIDE * SIZE + 16 * (q ^ (row & MASK)));
+      if (t >= a.tokens || n >= a.n) continue;
+      uint8_t* to = (uint8_t*)a.out + ((int64_t)t * a.n + n) * SIZE;
+      if (n + EACH <= a.n) {
+        store16(to, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          if (n + e >= a.n) continue;
+          if (F32) ((uint32_t*)to)[e] = v[e % 4];
+          else ((uint16_t*)to)[e] = (uint16_t)(v[e / 2 % 4] >> (16 * (e % 2)));
+        }
+      }
+    }
   }
 }
 
@@ -371,6 +436,7 @@ static void launch_tiled(const Args& a, hipStream_t s) {
 }
 
 using Large = Tile<8, 4, 2, 4, 2>;   // 256 x 256
+using Wide = Tile<4, 4, 2, 4, 3>;    // 128 x 256, for bf16 operands, which are twice the registers
 using Middle = Tile<4, 4, 2, 2, 2>;  // 128 x 128
 using Small = Tile<2, 2, 2, 2, 4>;   // 64 x 64
 
@@ -383,7 +449,11 @@ static void launch(const Args& a, hipStream_t s) {
   if (a.tokens <= 32) return launch_stream<1, 2, 3, F32>(a, s);
   if (a.tokens <= 64) return launch_stream<1, 4, 2, F32>(a, s);
   auto blocks = [&](int64_t n, int64_t t) { return ((a.n + n - 1) / n) * ((a.tokens + t - 1) / t); };
-  if (blocks(256, 256) >= 256) return launch_tiled<Large, F32>(a, s);
+  if constexpr (F32) {
+    if (blocks(128, 256) >= 256) return launch_tiled<Wide, F32>(a, s);
+  } else {
+    if (blocks(256, 256) >= 256) return launch_tiled<Large, F32>(a, s);
+  }
   if (blocks(128, 128) >= 256) return launch_tiled<Middle, F32>(a, s);
   launch_tiled<Small, F32>(a, s);
 }
@@ -408,8 +478,7 @@ WM_EXPORT int wm_linear_fp8(const void* x, const float* x_scales, int32_t tokens
     if (((uintptr_t)x | (uintptr_t)weight) % 16) fail("wm_linear_fp8: x and weight must be 16-byte aligned");
     if (((uintptr_t)x_scales | (uintptr_t)weight_scales) % 4 || ((uintptr_t)add | (uintptr_t)out) % (out_fp32 ? 4 : 2))
       fail("wm_linear_fp8: tensors must be aligned to their elements");
-    g8::Args a = {(const uint8_t*)x, x_scales, (const uint8_t*)weight, weight_scales, add, out, tokens, n, k, (k + 127) / 128, 0};
-    a.vec = n % 4 == 0 && ((uintptr_t)add | (uintptr_t)out) % (out_fp32 ? 16 : 8) == 0;
+    const g8::Args a = {(const uint8_t*)x, x_scales, (const uint8_t*)weight, weight_scales, add, out, tokens, n, k, (k + 127) / 128};
     if (out_fp32) g8::launch<true>(a, as_stream(stream));
     else g8::launch<false>(a, as_stream(stream));
   });
