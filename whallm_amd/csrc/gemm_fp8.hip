@@ -119,112 +119,144 @@ __device__ __forceinline__ f32x4 added(const Args& a, int t, int n, f32x4 v) {
 }
 
 // ---------------------------------------------------------------------------------
-// stream: few tokens. A block of 8 waves owns 16 NT weight rows x 16 MT tokens; the waves take the blocks of K in turn,
-// operands straight from memory, DEPTH blocks in flight a wave, and their sums meet in LDS, added in wave order.
-constexpr int SW = 8;
+// stream: few tokens, where the weights' way from memory is what counts. A block of W waves owns 16 TN weight rows x 16 TM
+// tokens; the waves take the blocks of K in turn, each through a ring of its own of D slots in LDS, so that no wave waits
+// for another one until the sums meet at the end, added in wave order. A block of K comes as direct loads of
+// 8 rows of 128 bytes, whole lines: X rows of tokens (8 where that is all). A wave's scales come for eight of its blocks at
+// once, 8 tokens a load: a block's alone would be a line for each token.
+template <int N>
+__device__ __forceinline__ void wait_own() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+template <int PER, int MOST>
+__device__ __forceinline__ void wait_own_steps(int ahead) {
+  if (ahead >= MOST) {
+    wait_own<PER * MOST>();
+  } else if constexpr (MOST > 0) {
+    wait_own_steps<PER, MOST - 1>(ahead);
+  }
+}
 
-template <int NT, int MT>
-struct StreamSlot {
-  Frag w[NT], x[MT];
-  float xs[MT], ws[NT];
+template <int TN_, int TM_, int X_, int W_, int D_>
+struct Stream {
+  static constexpr int TN = TN_, TM = TM_, X = X_, W = W_, D = D_;
+  static constexpr int BN = 16 * TN, BM = 16 * TM;
+  static constexpr int WEIGHTS = BN * BLOCK, SLOT = WEIGHTS + X * BLOCK;
+  static constexpr int SCALES = 32 * X + 256;  // of eight blocks: [token][8], and the weights'
+  static constexpr int LOADS = 2 * TN + X / 8;
+  static constexpr int OWN = D * SLOT + 2 * SCALES, RING = W * OWN, SUMS = W * TN * TM * 1024, LDS = RING > SUMS ? RING : SUMS;
+  static_assert(BLOCK % BN == 0 && X % 8 == 0 && (X == BM || (X == 8 && TM == 1)) && D <= 8 && LDS <= 160 * 1024 &&
+                LOADS * (D - 1) <= 63);
 };
 
-template <int NT, int MT, int DEPTH, bool F32, bool TAIL>
-__global__ void __launch_bounds__(64 * SW) stream_kernel(Args a) {
-  __shared__ float red[SW][NT * MT][4][64];
+template <typename T, bool F32, bool TAIL>
+__global__ void __launch_bounds__(64 * T::W) stream_kernel(Args a, int n_tiles) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const int c = lane % 16, g = lane / 16;
-  const int n0 = blockIdx.x * (16 * NT), t0 = blockIdx.y * (16 * MT);
-  const uint8_t *wp[NT], *xp[MT];
-  const float *xsp[MT], *wsp[NT];
+  const int n0 = blockIdx.x % n_tiles * T::BN, t0 = blockIdx.x / n_tiles * T::BM;
+  // lane l fills row l / 8, position l % 8 with the piece (l % 8) ^ (row % 8); rows past the end read the last one
+  const int lrow = lane / 8, piece = (lane % 8) ^ lrow;
+  const uint8_t* wbase = a.w + (int64_t)n0 * a.k;
+  const uint8_t* xbase = a.x + (int64_t)t0 * a.k;
+  uint32_t woff[2 * T::TN], xoff[T::X / 8];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    wp[j] = a.w + (int64_t)min(n0 + 16 * j + c, a.n - 1) * a.k + 16 * g;
-    wsp[j] = a.ws + (int64_t)(min(n0 + 16 * j, a.n - 1) / BLOCK) * a.blocks;
-  }
+  for (int i = 0; i < 2 * T::TN; ++i) woff[i] = (uint32_t)(min(n0 + 8 * i + lrow, a.n - 1) - n0) * (uint32_t)a.k + 16u * piece;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int64_t t = min(t0 + 16 * m + c, a.tokens - 1);
-    xp[m] = a.x + t * a.k + 16 * g;
-    xsp[m] = a.xs + t * a.blocks;
-  }
-  f32x4 acc[NT][MT];
+  for (int i = 0; i < T::X / 8; ++i) xoff[i] = (uint32_t)(min(t0 + 8 * i + lrow, a.tokens - 1) - t0) * (uint32_t)a.k + 16u * piece;
+  const float* xsbase = a.xs + (int64_t)t0 * a.blocks;
+  const float* wsbase = a.ws + (int64_t)(n0 / BLOCK) * a.blocks;
+  uint8_t* ring = lds + wave * T::OWN;
+  uint8_t* scales = ring + T::D * T::SLOT;
+  // the scales of this wave's blocks j .. j + 7, j a multiple of 8
+  auto issue_scales = [&](int j) {
+    const uint32_t to = lds_addr(scales + j / 8 % 2 * T::SCALES);
+    const uint32_t block = (uint32_t)min(wave + T::W * (j + lane % 8), a.blocks - 1);
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[j][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  StreamSlot<NT, MT> s[DEPTH];
-  auto load = [&](StreamSlot<NT, MT>& s, int b) {
-    int64_t lo = (int64_t)b * BLOCK, hi = lo + 64;
-    if (TAIL) {  // pieces behind the row's end read its first bytes and count as zero
-      lo = lo + 16 * g < a.k ? lo : -16 * g;
-      hi = hi + 16 * g < a.k ? hi : -16 * g;
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) s.w[j] = {gload16_nt(wp[j] + lo), gload16_nt(wp[j] + hi)};
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      s.x[m] = {gload16(xp[m] + lo), gload16(xp[m] + hi)};
-      s.xs[m] = gload<float>(xsp[m] + b);
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) s.ws[j] = wsp[j][b];
+    for (int i = 0; i < T::X / 8; ++i)
+      dma4(xsbase, 4u * ((uint32_t)(min(t0 + 8 * i + lrow, a.tokens - 1) - t0) * (uint32_t)a.blocks + block), to + 256 * i);
+    dma4(wsbase, 4u * block, to + 32 * T::X);
   };
-  auto multiply = [&](StreamSlot<NT, MT>& s, int b) {
-    if (TAIL && b == a.blocks - 1) {
-      const int pieces = (a.k - b * BLOCK) / 16;
+  auto issue = [&](int b, int slot) {
+    const uint32_t to = lds_addr(ring + slot * T::SLOT);
+    // pieces behind the rows' end read the block's first one
+    const uint32_t off = (uint32_t)BLOCK * b - (TAIL && BLOCK * b + 16 * piece >= a.k ? 16u * piece : 0u);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) zero_behind(s.w[j], g, pieces);
+    for (int i = 0; i < 2 * T::TN; ++i) dma16<(T::X <= 16)>(wbase, woff[i] + off, to + 1024 * i);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) zero_behind(s.x[m], g, pieces);
-    }
+    for (int i = 0; i < T::X / 8; ++i) dma16(xbase, xoff[i] + off, to + T::WEIGHTS + 1024 * i);
+  };
+  f32x4 acc[T::TN][T::TM];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const Operand<F32> x(s.x[m]);
+  for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const f32x4 d = Operand<F32>::product(Operand<F32>(s.w[j]), x);
-        const float f = s.xs[m] * s.ws[j];
+    for (int m = 0; m < T::TM; ++m) acc[j][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int c = lane % 16, g = lane / 16, xc = c % T::X;
+  const uint32_t pos = 16u * (uint32_t)(g ^ (c % 8));
+  auto multiply = [&](int j, int slot) {
+    const int b = wave + T::W * j;
+    const uint8_t* s = ring + slot * T::SLOT;
+    const float* sc = reinterpret_cast<const float*>(scales + j / 8 % 2 * T::SCALES) + j % 8;
+    auto frag = [&](uint32_t at) {
+      Frag f = {*reinterpret_cast<const uint4*>(s + at), *reinterpret_cast<const uint4*>(s + (at ^ 64u))};
+      if (TAIL && b == a.blocks - 1) zero_behind(f, g, (a.k - b * BLOCK) / 16);
+      return Operand<F32>(f);
+    };
+    const float ws = sc[8 * T::X];
+    Operand<F32> w[T::TN];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][m][i] = fmaf(d[i], f, acc[j][m][i]);
+    for (int i = 0; i < T::TN; ++i) w[i] = frag((16 * i + c) * BLOCK + pos);
+#pragma unroll
+    for (int m = 0; m < T::TM; ++m) {
+      const Operand<F32> x = frag(T::WEIGHTS + (16 * m + xc) * BLOCK + pos);
+      const float f = ws * sc[8 * (16 * m + xc)];
+#pragma unroll
+      for (int i = 0; i < T::TN; ++i) {
+        const f32x4 d = Operand<F32>::product(w[i], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][m][e] = fmaf(d[e], f, acc[i][m][e]);
       }
     }
   };
-  int b = wave;
+  const int mine = (a.blocks - wave + T::W - 1) / T::W;  // this wave's blocks: wave, wave + W, ..
 #pragma unroll
-  for (int u = 0; u < DEPTH; ++u) load(s[u], min(b + SW * u, a.blocks - 1));
-  for (; b + SW * DEPTH < a.blocks; b += SW * DEPTH) {
-#pragma unroll
-    for (int u = 0; u < DEPTH; ++u) {
-      multiply(s[u], b + SW * u);
-      load(s[u], min(b + SW * (DEPTH + u), a.blocks - 1));
+  for (int p = 0; p < T::D; ++p)
+    if (p < mine) {
+      if (p == 0) issue_scales(0);
+      issue(wave + T::W * p, p);
     }
+  int slot = 0;
+  for (int j = 0; j < mine; ++j) {
+    wait_own_steps<T::LOADS, T::D - 1>(mine - 1 - j);  // scales among the loads ahead make it wait for more than it must
+    multiply(j, slot);
+    if (j + T::D < mine) {
+      if ((j + T::D) % 8 == 0) issue_scales(j + T::D);
+      issue(wave + T::W * (j + T::D), slot);
+    }
+    slot = slot + 1 == T::D ? 0 : slot + 1;
   }
-#pragma unroll
-  for (int u = 0; u < DEPTH; ++u)
-    if (b + SW * u < a.blocks) multiply(s[u], b + SW * u);  // wave-uniform
 
+  if (T::W > 1) __syncthreads();  // the sums lie over the rings
+  float(*red)[T::TN * T::TM][4][64] = reinterpret_cast<float(*)[T::TN * T::TM][4][64]>(lds);
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < T::TM; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[wave][j * MT + m][i][lane] = acc[j][m][i];
+      for (int i = 0; i < 4; ++i) red[wave][j * T::TM + m][i][lane] = acc[j][m][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < 256 * NT * MT; e += 64 * SW) {
-    const int o = e % (16 * NT), tc = e / (16 * NT);  // weight row and token of the tile
-    const int at = o / 16 * MT + tc / 16, i = o % 4, l = 16 * (o % 16 / 4) + tc % 16;
+  for (int e = threadIdx.x; e < 256 * T::TN * T::TM; e += 64 * T::W) {
+    const int o = e % T::BN, tc = e / T::BN;  // weight row and token of the tile
+    const int at = o / 16 * T::TM + tc / 16, i = o % 4, l = 16 * (o % 16 / 4) + tc % 16;
     float v = red[0][at][i][l];
 #pragma unroll
-    for (int q = 1; q < SW; ++q) v += red[q][at][i][l];
+    for (int q = 1; q < T::W; ++q) v += red[q][at][i][l];
     if (t0 + tc < a.tokens && n0 + o < a.n) store_one<F32>(a, t0 + tc, n0 + o, v);
   }
 }
 
 // ---------------------------------------------------------------------------------
-// tiled: WN x WM waves, each 16 TN weight rows x 16 TM tokens. A step is a block of K: its rows of 128 bytes and its scales go
-// straight to LDS, STAGES steps at once, pieces of 16 bytes XOR-swizzled by row, so that the 8 rows of a
+// tiled: WN x WM waves, each 16 TN weight rows x 16 TM tokens. A step is KB blocks of K: their rows of 128 bytes and their scales
+// go straight to LDS, STAGES steps at once, pieces of 16 bytes XOR-swizzled by row, so that the 8 rows of a
 // ds_read_b128 cycle fall on distinct banks.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -239,15 +271,16 @@ __device__ __forceinline__ void wait_step(int ahead) {
   }
 }
 
-template <int TN_, int TM_, int WN_, int WM_, int STAGES_>
+template <int TN_, int TM_, int WN_, int WM_, int KB_, int STAGES_>
 struct Tile {
-  static constexpr int TN = TN_, TM = TM_, WN = WN_, WM = WM_, STAGES = STAGES_, WAVES = WN * WM;
+  static constexpr int TN = TN_, TM = TM_, WN = WN_, WM = WM_, KB = KB_, STAGES = STAGES_, WAVES = WN * WM;
   static constexpr int BN = 16 * TN * WN, BM = 16 * TM * WM;
-  static constexpr int W = BN * BLOCK, X = BM * BLOCK, SCALES = W + X, STAGE = SCALES + 4 * BM + 256;
-  static constexpr int WL = BN / 8 / WAVES, XL = BM / 8 / WAVES;  // row loads of a wave
-  static constexpr int LOADS = WL + XL + 1;                       // and one of scales
-  static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM / 64 < WAVES && BM % 64 == 0 && BN <= 64 * BLOCK && 128 % (16 * TN) == 0);
-  static_assert(STAGES * STAGE <= 160 * 1024);
+  static constexpr int W = BN * BLOCK, X = BM * BLOCK, SCALES = KB * (W + X);  // a stage: KB blocks' rows, then their scales
+  static constexpr int XS = BM * KB / 64, STAGE = SCALES + 256 * (XS + 1);
+  static constexpr int WL = KB * BN / 8 / WAVES, XL = KB * BM / 8 / WAVES;  // row loads of a wave
+  static constexpr int LOADS = WL + XL + 1;                                 // and one of scales
+  static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM * KB % 64 == 0 && XS < WAVES && BN * KB <= 64 * BLOCK && 128 % (16 * TN) == 0);
+  static_assert(STAGES * STAGE <= 160 * 1024 && LOADS * (STAGES - 1) <= 63);
 };
 
 // Tiles of 8 token tiles at a time, these innermost: an XCD (block b runs on XCD b % 8) works on a patch of 8 token tiles and a
@@ -276,27 +309,31 @@ __global__ void __launch_bounds__(64 * T::WAVES) tiled_kernel(Args a, int n_tile
   const int lrow = lane / 8, piece = (lane % 8) ^ lrow;
   const uint8_t* wbase = a.w + (int64_t)n0 * a.k;
   const uint8_t* xbase = a.x + (int64_t)t0 * a.k;
-  uint32_t woff[T::WL], xoff[T::XL], soff;
+  constexpr int WR = T::WL / T::KB, XR = T::XL / T::KB;  // row loads of a block
+  uint32_t woff[WR], xoff[XR];
 #pragma unroll
-  for (int i = 0; i < T::WL; ++i)
+  for (int i = 0; i < WR; ++i)
     woff[i] = (uint32_t)(min(n0 + 8 * (wave + T::WAVES * i) + lrow, a.n - 1) - n0) * (uint32_t)a.k + 16u * piece;
 #pragma unroll
-  for (int i = 0; i < T::XL; ++i)
+  for (int i = 0; i < XR; ++i)
     xoff[i] = (uint32_t)(min(t0 + 8 * (wave + T::WAVES * i) + lrow, a.tokens - 1) - t0) * (uint32_t)a.k + 16u * piece;
-  // waves below BM / 64 load 64 tokens' scales each, the others those of the weights
-  const bool tokens_scales = wave < T::BM / 64;
+  // a load of scales: KB blocks side by side of 64 / KB tokens (the waves below XS) or weight rows of blocks
+  const bool tokens_scales = wave < T::XS;
   const float* sbase = tokens_scales ? a.xs + (int64_t)t0 * a.blocks : a.ws + (int64_t)(n0 / BLOCK) * a.blocks;
-  const uint32_t sdst = T::SCALES + (tokens_scales ? 256u * wave : 4u * T::BM);
-  soff = (uint32_t)(tokens_scales ? min(t0 + 64 * wave + lane, a.tokens - 1) - t0
-                                  : min(lane, (a.n - 1) / BLOCK - n0 / BLOCK)) * (uint32_t)a.blocks * 4u;
-  // Load i of block b's LOADS.
-  auto issue = [&](int b, int i) {
-    const uint32_t slot = lds_addr(lds + b % T::STAGES * T::STAGE);
+  const uint32_t sdst = T::SCALES + 256u * (tokens_scales ? wave : T::XS);
+  const uint32_t srow = (uint32_t)(tokens_scales ? min(t0 + (64 * wave + lane) / T::KB, a.tokens - 1) - t0
+                                                 : min(lane / T::KB, (a.n - 1) / BLOCK - n0 / BLOCK)) * (uint32_t)a.blocks;
+  // Load i of the LOADS of the blocks KB step .. of a step. Blocks behind the last read that one again, and are not used.
+  auto issue = [&](int step, int i) {
+    const uint32_t slot = lds_addr(lds + step % T::STAGES * T::STAGE);
+    if (i == T::WL + T::XL) return dma4(sbase, 4u * (srow + (uint32_t)min(T::KB * step + lane % T::KB, a.blocks - 1)), slot + sdst);
+    const int kb = i < T::WL ? i / WR : (i - T::WL) / XR;
+    const int b = min(T::KB * step + kb, a.blocks - 1);
     // pieces behind the rows' end read the block's first one
     const uint32_t off = (uint32_t)BLOCK * b - (TAIL && BLOCK * b + 16 * piece >= a.k ? 16u * piece : 0u);
-    if (i < T::WL) dma16(wbase, woff[i] + off, slot + 1024 * (wave + T::WAVES * i));
-    else if (i < T::WL + T::XL) dma16(xbase, xoff[i - T::WL] + off, slot + T::W + 1024 * (wave + T::WAVES * (i - T::WL)));
-    else dma4(sbase, soff + 4u * b, slot + sdst);
+    const uint32_t to = slot + kb * (T::W + T::X);
+    if (i < T::WL) dma16(wbase, woff[i % WR] + off, to + 1024 * (wave + T::WAVES * (i % WR)));
+    else dma16(xbase, xoff[(i - T::WL) % XR] + off, to + T::W + 1024 * (wave + T::WAVES * ((i - T::WL) % XR)));
   };
 
   f32x4 acc[T::TN][T::TM];
@@ -307,69 +344,77 @@ __global__ void __launch_bounds__(64 * T::WAVES) tiled_kernel(Args a, int n_tile
   const int c = lane % 16, g = lane / 16;
   const uint32_t pos = 16u * (uint32_t)(g ^ (c % 8));
   const uint32_t wrow = (uint32_t)(16 * T::TN * wn + c) * BLOCK + pos, xrow = T::W + (uint32_t)(16 * T::TM * wm + c) * BLOCK + pos;
-  const uint32_t xscale = T::SCALES + 4u * (16 * T::TM * wm + c), wscale = T::SCALES + 4u * (T::BM + 16 * T::TN * wn / BLOCK);
+  const uint32_t xscale = T::SCALES + 4u * T::KB * (16 * T::TM * wm + c);
+  const uint32_t wscale = T::SCALES + 256u * T::XS + 4u * T::KB * (16 * T::TN * wn / BLOCK);
 
-  // Block b's sums. The multiply-adds of a matrix instruction's results stand beside the instruction TM later, so that
-  // none waits for them (the last ones of a block beside the next block's first). With AHEAD the loads of the block STAGES - 1
-  // behind it go out between the instructions of the block's first half.
+  // A step's sums. The multiply-adds of a matrix instruction's results stand beside the instruction TM later, so that
+  // none waits for them (the last ones of a block beside the next block's first). With AHEAD the loads of the step STAGES - 1
+  // behind it go out between the instructions of the step's first two thirds.
   f32x4 d[T::TM];
   float f[T::TM];
 #pragma unroll
   for (int m = 0; m < T::TM; ++m) d[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f[m] = 0.0f;
-  auto step = [&](int b, auto ahead, auto last) {
+  auto step = [&](int p, auto ahead, auto last) {
     constexpr bool AHEAD = decltype(ahead)::value, LAST = decltype(last)::value;
-    const uint8_t* s = lds + b % T::STAGES * T::STAGE;
-    const int pieces = (a.k - b * BLOCK) / 16;
-    auto frag = [&](uint32_t at) {
-      Frag f = {*reinterpret_cast<const uint4*>(s + at), *reinterpret_cast<const uint4*>(s + (at ^ 64u))};
-      if (TAIL && LAST) zero_behind(f, g, pieces);
-      return Operand<F32>(f);
-    };
-    Operand<F32> x[T::TM], w[2];
-    w[0] = frag(wrow);
+    const uint8_t* s = lds + p % T::STAGES * T::STAGE;
 #pragma unroll
-    for (int m = 0; m < T::TM; ++m) x[m] = frag(xrow + 16 * BLOCK * m);
-    const float ws = *reinterpret_cast<const float*>(s + wscale);
-    float xs[T::TM];
+    for (int kb = 0; kb < T::KB; ++kb) {
+      const int b = T::KB * p + kb;
+      if (LAST && kb > 0 && b >= a.blocks) break;
+      auto frag = [&](uint32_t at) {
+        at += kb * (T::W + T::X);
+        Frag f = {*reinterpret_cast<const uint4*>(s + at), *reinterpret_cast<const uint4*>(s + (at ^ 64u))};
+        if (TAIL && LAST && b == a.blocks - 1) zero_behind(f, g, (a.k - b * BLOCK) / 16);
+        return Operand<F32>(f);
+      };
+      Operand<F32> x[T::TM], w[2];
+      w[0] = frag(wrow);
 #pragma unroll
-    for (int m = 0; m < T::TM; ++m) xs[m] = *reinterpret_cast<const float*>(s + xscale + 64 * m);
+      for (int m = 0; m < T::TM; ++m) x[m] = frag(xrow + 16 * BLOCK * m);
+      const float ws = *reinterpret_cast<const float*>(s + wscale + 4 * kb);
+      float xs[T::TM];
 #pragma unroll
-    for (int i = 0; i < T::TN; ++i) {
-      if (i + 1 < T::TN) w[(i + 1) % 2] = frag(wrow + 16 * BLOCK * (i + 1));
-      if (AHEAD) {
-        constexpr int PER = (2 * T::LOADS + T::TN - 1) / T::TN;  // in the first half
+      for (int m = 0; m < T::TM; ++m) xs[m] = *reinterpret_cast<const float*>(s + xscale + 64 * T::KB * m + 4 * kb);
 #pragma unroll
-        for (int q = i * PER; q < (i + 1) * PER && q < T::LOADS; ++q) issue(b + T::STAGES - 1, q);
-      }
+      for (int i = 0; i < T::TN; ++i) {
+        if (i + 1 < T::TN) w[(i + 1) % 2] = frag(wrow + 16 * BLOCK * (i + 1));
+        if (AHEAD) {
+          constexpr int PER = (3 * T::LOADS + 2 * T::TN * T::KB - 1) / (2 * T::TN * T::KB);
+          const int at = kb * T::TN + i;
 #pragma unroll
-      for (int m = 0; m < T::TM; ++m) {
-        const f32x4 p = Operand<F32>::product(w[i % 2], x[m]);
+          for (int q = at * PER; q < (at + 1) * PER && q < T::LOADS; ++q) issue(p + T::STAGES - 1, q);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[(i + T::TN - 1) % T::TN][m][e] = fmaf(d[m][e], f[m], acc[(i + T::TN - 1) % T::TN][m][e]);
-        if (i == 0) f[m] = ws * xs[m];
-        d[m] = p;
-        __builtin_amdgcn_sched_barrier(0);  // the order as it is written
+        for (int m = 0; m < T::TM; ++m) {
+          const f32x4 r = Operand<F32>::product(w[i % 2], x[m]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[(i + T::TN - 1) % T::TN][m][e] = fmaf(d[m][e], f[m], acc[(i + T::TN - 1) % T::TN][m][e]);
+          if (i == 0) f[m] = ws * xs[m];
+          d[m] = r;
+          __builtin_amdgcn_sched_barrier(0);  // the order as it is written
+        }
       }
     }
   };
   const std::true_type yes;
   const std::false_type no;
-  int b = 0;
-  for (; b < T::STAGES - 1 && b < a.blocks; ++b)
+  const int steps = (a.blocks + T::KB - 1) / T::KB;
+  int p = 0;
+  for (; p < T::STAGES - 1 && p < steps; ++p)
 #pragma unroll
-    for (int i = 0; i < T::LOADS; ++i) issue(b, i);
-  // at the top of a block its loads have landed in every wave, and every wave is done with the slot that the next
+    for (int i = 0; i < T::LOADS; ++i) issue(p, i);
+  // at the top of a step its loads have landed in every wave, and every wave is done with the slot that the next
   // loads overwrite
-  for (b = 0; b + T::STAGES - 1 < a.blocks; ++b) {
+  for (p = 0; p + T::STAGES - 1 < steps; ++p) {
     wait_loads<T::LOADS * (T::STAGES - 2)>();
-    step(b, yes, no);
+    step(p, yes, no);
   }
-  for (; b + 1 < a.blocks; ++b) {
-    wait_step<T::LOADS, T::STAGES - 2>(a.blocks - 1 - b);
-    step(b, no, no);
+  for (; p + 1 < steps; ++p) {
+    wait_step<T::LOADS, T::STAGES - 2>(steps - 1 - p);
+    step(p, no, no);
   }
   wait_loads<0>();
-  step(b, no, yes);
+  step(p, no, yes);
 #pragma unroll
   for (int m = 0; m < T::TM; ++m)
 #pragma unroll
@@ -418,11 +463,12 @@ __global__ void __launch_bounds__(64 * T::WAVES) tiled_kernel(Args a, int n_tile
 
 // ---------------------------------------------------------------------------------
 
-template <int NT, int MT, int DEPTH, bool F32>
+template <typename T, bool F32>
 static void launch_stream(const Args& a, hipStream_t s) {
-  const dim3 grid((a.n + 16 * NT - 1) / (16 * NT), (a.tokens + 16 * MT - 1) / (16 * MT));
-  if (a.k % BLOCK) hipLaunchKernelGGL((stream_kernel<NT, MT, DEPTH, F32, true>), grid, dim3(64 * SW), 0, s, a);
-  else hipLaunchKernelGGL((stream_kernel<NT, MT, DEPTH, F32, false>), grid, dim3(64 * SW), 0, s, a);
+  const int64_t n_tiles = (a.n + T::BN - 1) / T::BN, t_tiles = (a.tokens + T::BM - 1) / T::BM;
+  const dim3 grid(grid_of("wm_linear_fp8", n_tiles * t_tiles, 64 * T::W));
+  if (a.k % BLOCK) hipLaunchKernelGGL((stream_kernel<T, F32, true>), grid, dim3(64 * T::W), 0, s, a, (int)n_tiles);
+  else hipLaunchKernelGGL((stream_kernel<T, F32, false>), grid, dim3(64 * T::W), 0, s, a, (int)n_tiles);
   check_launch("linear_fp8 (stream)");
 }
 
@@ -435,27 +481,47 @@ static void launch_tiled(const Args& a, hipStream_t s) {
   check_launch("linear_fp8 (tiled)");
 }
 
-using Large = Tile<8, 4, 2, 4, 2>;   // 256 x 256
-using Wide = Tile<4, 4, 2, 4, 3>;    // 128 x 256, for bf16 operands, which are twice the registers
-using Middle = Tile<4, 4, 2, 2, 2>;  // 128 x 128
-using Small = Tile<2, 2, 2, 2, 4>;   // 64 x 64
-
+// The kernel of a shape. Up to 16 tokens the weights' way from memory is all: 16 weight rows a block with 8 waves while
+// that gives two blocks a CU at most, 32 with 4 waves beyond (one token of 7168 to 4096 5.8 us and 7.3, to 24576 31.7 and
+// 26.8). Their rows pass once, so their loads are non-temporal (1 token of 7168 to 24576 30.2 us without, 26.8 with, six to
+// 129,280 154 and 134; for 64 tokens, where two blocks take a row, 12.3 with and 9.7 without).
+// Otherwise the shape with the lowest cost, rounds of 256 blocks times what a block of K takes in a round. Larger tiles move fewer
+// bytes and take more matrix instructions a barrier, smaller ones fill the chip sooner; the rounds decide. Costs are
+// in units of 10 ns, measured at one round and more of K = 7168 to bf16; fp32 takes 1.6 times of each. The sizes' times in
+// us, the cheapest first and the next ones by cost:
+//   64 x 4096 x 7168   32 x 32 10.1, 64 x 32 13.4        256 x 4096 x 7168  64 x 64 19.1, 64 x 128 23, 64 x 32 27.5
+//   128 x 4096 x 7168  64 x 32 14.5, 64 x 64 16.4        512 x 4096 x 7168  64 x 128 28, 128 x 128 34, 64 x 64 35
+//   96 x 4608 x 5120   64 x 32 11.7, 64 x 64 12.8        1024 x 4096 x 7168  128 x 128 41.5, 64 x 128 53, 128 x 256 55
+//   300 x 7168 x 2048  128 x 128 12.9, 64 x 64 18.4      2048 x 4096 x 7168  128 x 256 82, 128 x 128 91, 256 x 256 92
+//   1501 x 1283 x 2560  64 x 128 12.9, 64 x 64 16        4096 x 4096 x 7168  256 x 256 112, 128 x 256 147
 template <bool F32>
 static void launch(const Args& a, hipStream_t s) {
   if (a.tokens <= 16) {
-    if (a.n >= 16384) return launch_stream<2, 1, 3, F32>(a, s);
-    return launch_stream<1, 1, 4, F32>(a, s);
+    const bool few = a.n <= 8192;
+    if (a.tokens <= 8) return few ? launch_stream<Stream<1, 1, 8, 8, 4>, F32>(a, s) : launch_stream<Stream<2, 1, 8, 4, 3>, F32>(a, s);
+    return few ? launch_stream<Stream<1, 1, 16, 8, 4>, F32>(a, s) : launch_stream<Stream<2, 1, 16, 4, 3>, F32>(a, s);
   }
-  if (a.tokens <= 32) return launch_stream<1, 2, 3, F32>(a, s);
-  if (a.tokens <= 64) return launch_stream<1, 4, 2, F32>(a, s);
-  auto blocks = [&](int64_t n, int64_t t) { return ((a.n + n - 1) / n) * ((a.tokens + t - 1) / t); };
-  if constexpr (F32) {
-    if (blocks(128, 256) >= 256) return launch_tiled<Wide, F32>(a, s);
-  } else {
-    if (blocks(256, 256) >= 256) return launch_tiled<Large, F32>(a, s);
+  constexpr int SHAPES = F32 ? 7 : 8;  // bf16 operands are twice the registers: no 256 x 256
+  constexpr struct { int n, t, cost; } shape[8] = {{16, 32, 8}, {32, 32, 13}, {64, 32, 21}, {64, 64, 28},
+                                                   {64, 128, 45}, {128, 128, 70}, {128, 256, 135}, {256, 256, 175}};
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < SHAPES; ++i) {
+    const int64_t blocks = ((int64_t)(a.n + shape[i].n - 1) / shape[i].n) * ((a.tokens + shape[i].t - 1) / shape[i].t);
+    const int64_t cost = (blocks + 255) / 256 * shape[i].cost;
+    if (cost < least) least = cost, best = i;
   }
-  if (blocks(128, 128) >= 256) return launch_tiled<Middle, F32>(a, s);
-  launch_tiled<Small, F32>(a, s);
+  switch (best) {
+    case 0: return launch_stream<Stream<1, 2, 32, 4, 3>, F32>(a, s);
+    case 1: return launch_stream<Stream<2, 2, 32, 4, 2>, F32>(a, s);
+    case 2: return launch_stream<Stream<4, 2, 32, 4, 2>, F32>(a, s);
+    case 3: return launch_tiled<Tile<2, 1, 2, 4, 2, 4>, F32>(a, s);
+    case 4: return launch_tiled<Tile<2, 2, 2, 4, 2, 3>, F32>(a, s);
+    case 5: return launch_tiled<Tile<4, 2, 2, 4, 1, 4>, F32>(a, s);
+    case 6: return launch_tiled<Tile<4, 4, 2, 4, 1, 3>, F32>(a, s);
+    default:
+      if constexpr (!F32) launch_tiled<Tile<8, 4, 2, 4, 1, 2>, F32>(a, s);
+  }
 }
 
 }  // namespace g8
