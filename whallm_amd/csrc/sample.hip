@@ -117,18 +117,20 @@ struct Shared {
   uint64_t bcast[3];
 };
 
-__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int from) {
-  const uint32_t lo = __shfl((uint32_t)v, from, 64), hi = __shfl((uint32_t)(v >> 32), from, 64);
-  return (uint64_t)hi << 32 | lo;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t add_dpp(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((uint64_t)hi << 32 | lo);
 }
-// Sum of the lanes up to this one.
+// Sum of the lanes up to this one, by moves within rows of 16 lanes and from row to row.
 __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
-  const int lane = threadIdx.x % 64;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t o = shfl_u64(v, lane >= d ? lane - d : lane);
-    if (lane >= d) v += o;
-  }
+  v = add_dpp<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = add_dpp<0x112, 0xf>(v);
+  v = add_dpp<0x114, 0xf>(v);
+  v = add_dpp<0x118, 0xf>(v);
+  v = add_dpp<0x142, 0xa>(v);  // row_bcast 15 to rows 1 and 3
+  v = add_dpp<0x143, 0xc>(v);  // row_bcast 31 to rows 2 and 3
   return v;
 }
 // Sum of the threads before this one; `total` of all. Every thread calls it.
@@ -252,6 +254,13 @@ __device__ __forceinline__ uint64_t place_of(float u, uint64_t whole) {
   return __umul64hi((uint64_t)((u > 0.0f ? fminf(u, 1.0f - 0x1p-24f) : 0.0f) * 0x1p64f), whole);
 }
 
+// The row's results: token i of logit l, drawn among weights of this sum.
+__device__ __forceinline__ void write_token(const Args& a, int row, const Rules& r, int i, float l, uint64_t whole) {
+  const double t = l == r.top ? 0.0 : ((double)l - (double)r.top) * r.scale;
+  a.tokens[row] = i;
+  a.logp[row] = (float)((t - log2(ldexp((double)whole, -a.shift))) * 0.6931471805599453);
+}
+
 // Writes the token whose running sum passes `want`, given the chunks' sums in s.chunk. left(l, i): the weight of
 // logit l with id i, 0 if it goes. `size` is a chunk's tokens, a multiple of THREADS. Every thread calls it.
 template <bool F32, typename Left>
@@ -276,9 +285,7 @@ __device__ void draw(const Args& a, const void* p, int row, const Rules& r, Shar
     int i = first;
     float l = logit<F32>(p, i);
     for (uint64_t w; want >= before + (w = left(l, i)); l = logit<F32>(p, i)) before += w, ++i;
-    const double t = l == r.top ? 0.0 : ((double)l - (double)r.top) * r.scale;
-    a.tokens[row] = i;
-    a.logp[row] = (float)((t - log2(ldexp((double)whole, -a.shift))) * 0.6931471805599453);
+    write_token(a, row, r, i, l, whole);
   }
 }
 
@@ -330,12 +337,23 @@ __global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
 
 // ---------------------------------------------------------------------------------- larger vocabularies
 //
-// Four launches over chunks of the rows: each chunk's largest logit; weights and counts by bins of the distance from the
-// row's largest; the tokens in the bins that a cut may fall into (candidates), and the chunks' sums of those above;
-// the cut among the candidates and the draw, a workgroup a row. A bin is 1/32 of a factor of 2, so that a cut has some
-// hundreds of candidates where it falls among the bulk of the tokens and a few where it does not. Rows of more
-// candidates than there is room for (a cut among thousands of nearly equal logits) are cut by radix selection as above.
-constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048;
+// Chunks of the rows, and then a workgroup a row. A first launch finds each chunk's largest logit, and each group's of 64
+// tokens.
+//
+// With a small k (LIST_K) a row needs no other pass: of the groups' largest logits the k largest are k tokens, so
+// the tokens that top-k may keep are no smaller than the k-th of these, and lie in the few groups that reach it.
+//
+// Otherwise two more launches go over the chunks: weights and counts by bins of the distance from the row's largest logit; and
+// the tokens in the bins that a cut may fall into (candidates), with the chunks' sums of those above. A bin is
+// 1/32 of a factor of 2, so that a cut has some hundreds of candidates where it falls among the bulk of the tokens and a few
+// where it does not.
+//
+// Either way the last launch sorts the candidates, cuts and draws. Rows of more candidates than there is room for (a cut
+// among thousands of nearly equal logits) are cut by radix selection as above.
+constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048, LIST_K = 512;
+constexpr int GROUP = 64;
+
+__device__ __forceinline__ bool listed(const Rules& r) { return r.k > 0 && r.k <= LIST_K; }
 
 struct RowInfo {
   uint64_t below_lo, between;  // weights of the bins below lo, and of those between hi and kbin
@@ -351,6 +369,7 @@ struct Work {
   uint32_t* counts;     // [rows][BINS]
   uint64_t* list;       // [rows][CANDIDATES]: key and the complement of the id
   uint32_t* listed;     // [rows]
+  float* groups;        // [rows][chunks * size / GROUP]: each group's largest logit
   int chunks, size;
 };
 
@@ -406,15 +425,21 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_tops_kernel(Args a, Work w
   if (c == 0 && threadIdx.x == 0) w.listed[row] = 0;
   float t = -INFINITY;
   bool nan = false;
-  for (int i = lo + 8 * threadIdx.x; i < end; i += UNIT) {
+  for (int i = lo + 8 * threadIdx.x; i < lo + w.size; i += UNIT) {  // whole waves, also behind the vocabulary's end
     Eight<F32> l;
     l.load(a.logits, base, i, end - i);
+    float mine = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float v = l.get(e, end - i);
       nan |= v != v;
-      t = fmaxf(t, v);
+      mine = fmaxf(mine, v);
     }
+    t = fmaxf(t, mine);
+    mine = fmaxf(mine, dpp_f<0xB1>(mine));   // over 8 lanes, a group's
+    mine = fmaxf(mine, dpp_f<0x4E>(mine));
+    mine = fmaxf(mine, dpp_f<0x141>(mine));
+    if (threadIdx.x % 8 == 0) w.groups[((int64_t)row * w.chunks * w.size + i) / GROUP] = mine;
   }
   t = segment_max<64>(t);
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = t;
@@ -436,9 +461,12 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_bins_kernel(Args a, Work w
   if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, part, top)) return;
   const Rules r(a, row, top);
   const bool by_weight = r.p < 1.0f, by_count = r.k > 0;
-  if (!by_weight && !by_count) return;
+  if (listed(r) || (!by_weight && !by_count)) return;
   const Bins bins(r);
-  for (int i = threadIdx.x; i < BINS; i += BIN_THREADS) weights[i] = 0, counts[i] = 0;
+  for (int i = threadIdx.x; i < BINS; i += BIN_THREADS) {
+    if (by_weight) weights[i] = 0;
+    if (by_count) counts[i] = 0;
+  }
   __syncthreads();
   const int64_t base = (int64_t)row * a.vocab;
   const int lo = c * w.size, end = min(lo + w.size, a.vocab);
@@ -456,8 +484,9 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_bins_kernel(Args a, Work w
   }
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += BIN_THREADS) {
-    if (weights[i]) atomicAdd((unsigned long long*)&w.weights[(int64_t)row * BINS + i], (unsigned long long)weights[i]);
-    if (counts[i]) atomicAdd(&w.counts[(int64_t)row * BINS + i], counts[i]);
+    if (by_weight && weights[i])
+      atomicAdd((unsigned long long*)&w.weights[(int64_t)row * BINS + i], (unsigned long long)weights[i]);
+    if (by_count && counts[i]) atomicAdd(&w.counts[(int64_t)row * BINS + i], counts[i]);
   }
 }
 
@@ -485,12 +514,15 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
   __shared__ float top_part[BIN_THREADS / 64];
   __shared__ RowInfo info;
   __shared__ uint64_t k_below, k_in;  // weights below kbin, and in it
+  __shared__ uint64_t list[CANDIDATES];
+  __shared__ uint32_t found, first;
   const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
   float top;
   if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, top_part, top)) return;
   const Rules r(a, row, top);
+  if (listed(r)) return;
   const Bins bins(r);
-  if (threadIdx.x == 0) info = {0, 0, BINS, BINS, BINS, 0};
+  if (threadIdx.x == 0) info = {0, 0, BINS, BINS, BINS, 0}, found = 0;
   if (r.k > 0 || r.p < 1.0f) {
     uint64_t weight[EACH], sum = 0, total, before;
     uint32_t count[EACH], n = 0;
@@ -561,14 +593,20 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
       if (b < stay) {
         sum += left_of(a, r, v);
       } else if (b <= hi || b == kbin) {
-        const uint32_t at = atomicAdd(&w.listed[row], 1u);
-        if (at < CANDIDATES) w.list[(int64_t)row * CANDIDATES + at] = entry_of(v, i + e);
+        const uint32_t at = atomicAdd(&found, 1u);
+        if (at < CANDIDATES) list[at] = entry_of(v, i + e);
       }
     }
   }
   uint64_t total;
-  scan_of<BIN_THREADS>(sum, part, total);
-  if (threadIdx.x == 0) w.sums[blockIdx.x] = total;
+  scan_of<BIN_THREADS>(sum, part, total);  // and a barrier
+  if (threadIdx.x == 0) {
+    w.sums[blockIdx.x] = total;
+    first = found ? atomicAdd(&w.listed[row], found) : 0;
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < found && first + i < CANDIDATES; i += BIN_THREADS)
+    w.list[(int64_t)row * CANDIDATES + first + i] = list[i];
 }
 
 // Descending, in LDS; n a power of two.
@@ -585,12 +623,86 @@ __device__ __forceinline__ void sort_entries(uint64_t* v, int n) {
   __syncthreads();
 }
 
+// The same for up to THREADS / 2 entries, each put in its place by how many are above it. Ends with a barrier.
+__device__ __forceinline__ void rank_entries(uint64_t* v, uint64_t* other, int n) {
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t < n) {
+    const uint64_t mine = v[t];
+    int above = 0;
+    for (int i = 0; i < n; ++i) above += v[i] > mine;
+    other[above] = mine;
+  }
+  __syncthreads();
+  if (t < n) v[t] = other[t];
+  __syncthreads();
+}
+
+// The entries of a row that a small k may keep, into `entry`, and how many there are: more than CANDIDATES where they do not
+// fit. A bin that k groups' largest logits reach bounds the tokens; `counts` is BINS + CANDIDATES words.
+template <bool F32>
+__device__ int list_row(const Args& a, const Work& w, const void* p, int row, const Rules& r, const Bins& bins, Shared& s,
+                        uint64_t* entry, uint32_t* counts, uint32_t* found) {
+  constexpr int EACH = BINS / THREADS, AHEAD = 4;
+  const int groups = (a.vocab + GROUP - 1) / GROUP;
+  const float* tops = w.groups + (int64_t)row * w.chunks * w.size / GROUP;
+  uint32_t* which = counts + BINS;
+  for (int i = threadIdx.x; i < BINS; i += THREADS) counts[i] = 0;
+  if (threadIdx.x < 2) found[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s.bcast[0] = BINS - 2;
+  __syncthreads();
+  for (int g = threadIdx.x; g < groups; g += THREADS) {
+    const int b = bins.of(tops[g]);
+    if (b < BINS - 1) atomicAdd(&counts[b], 1u);
+  }
+  __syncthreads();
+  uint64_t n = 0, total;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) n += counts[threadIdx.x * EACH + j];
+  uint64_t at = block_scan(n, s.part, total);
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const uint64_t next = at + counts[threadIdx.x * EACH + j];
+    if (at < (uint64_t)r.k && next >= (uint64_t)r.k) s.bcast[0] = threadIdx.x * EACH + j;
+    at = next;
+  }
+  __syncthreads();
+  const int bound = (int)s.bcast[0];
+  for (int g = threadIdx.x; g < groups; g += THREADS) {
+    if (bins.of(tops[g]) > bound) continue;
+    const uint32_t i = atomicAdd(&found[0], 1u);
+    if (i < CANDIDATES) which[i] = g;
+  }
+  __syncthreads();
+  const uint32_t hits = found[0];
+  if (hits > CANDIDATES) return CANDIDATES + 1;
+  for (uint32_t e0 = threadIdx.x; e0 < hits * GROUP; e0 += THREADS * AHEAD) {
+    float l[AHEAD];
+    int id[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const uint32_t e = e0 + THREADS * j;
+      id[j] = e < hits * GROUP ? (int)(which[e / GROUP] * GROUP + e % GROUP) : a.vocab;
+      l[j] = id[j] < a.vocab ? logit<F32>(p, id[j]) : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (id[j] >= a.vocab || bins.of(l[j]) > bound) continue;
+      const uint32_t i = atomicAdd(&found[1], 1u);
+      if (i < CANDIDATES) entry[i] = entry_of(l[j], id[j]);
+    }
+  }
+  __syncthreads();
+  return (int)found[1];
+}
+
 template <bool F32>
 __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
   constexpr int EACH = CANDIDATES / THREADS;
   __shared__ Shared s;
-  __shared__ uint64_t entry[CANDIDATES];
+  __shared__ uint64_t entry[CANDIDATES], other[CANDIDATES];
   __shared__ int kept_entries;
+  __shared__ uint32_t found[2];
   const int row = blockIdx.x;
   const void* p = (const uint8_t*)a.logits + (int64_t)row * a.vocab * (F32 ? 4 : 2);
   float top;
@@ -599,23 +711,41 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
     return;
   }
   const Rules r(a, row, top);
-  const int n = (int)w.listed[row];
+  const Bins bins(r);
+  const bool list = listed(r);
+  RowInfo info = {0, 0, 0, BINS, BINS, 0};
+  int n;
+  if (list) {
+    n = list_row<F32>(a, w, p, row, r, bins, s, entry, (uint32_t*)other, found);
+  } else {
+    n = (int)w.listed[row];
+    info = w.info[row];
+  }
   if (n > CANDIDATES) {  // the same for all threads
     draw_cut<F32>(a, p, row, r, s, w.chunks, w.size);
     return;
   }
-  const Bins bins(r);
-  const RowInfo info = w.info[row];
-  if ((int)threadIdx.x < w.chunks) s.chunk[threadIdx.x] = w.sums[(int64_t)row * w.chunks + threadIdx.x];
+  // the weights by id: in parts of the chunks' size, or, where the list is all there is, as fine as there are threads
+  int part = w.size;
+  if (list) part = (a.vocab + THREADS - 1) / THREADS;
+  if (!list && (int)threadIdx.x < w.chunks) s.chunk[threadIdx.x] = w.sums[(int64_t)row * w.chunks + threadIdx.x];
+  if (list) s.chunk[threadIdx.x] = 0;
   if (threadIdx.x == 0) kept_entries = 0;
   uint64_t last = ~0ull;  // the last entry that stays; none
+  float l[EACH];
+  uint64_t left[EACH];
   if (n > 0) {
-    int places = 2;
-    while (places < n) places *= 2;
-    for (int i = threadIdx.x; i < places; i += THREADS) entry[i] = i < n ? w.list[(int64_t)row * CANDIDATES + i] : 0;
-    sort_entries(entry, places);
+    if (!list)
+      for (int i = threadIdx.x; i < n; i += THREADS) entry[i] = w.list[(int64_t)row * CANDIDATES + i];
+    if (n <= 512) {
+      rank_entries(entry, other, n);
+    } else {
+      int places = 1024;
+      while (places < n) places *= 2;
+      for (int i = n + threadIdx.x; i < places; i += THREADS) entry[i] = 0;
+      sort_entries(entry, places);
+    }
     // in order: the bins from lo to hi, then kbin's, if that is behind them
-    float l[EACH];
     int b[EACH], in_k[EACH];
     uint64_t weight[EACH], sum = 0, ahead = 0, total;
 #pragma unroll
@@ -631,7 +761,7 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
       const int i = threadIdx.x * EACH + j;
-      in_k[j] = i < n && (b[j] < info.kbin || (b[j] == info.kbin && i < (int)before_k + info.kleft));
+      in_k[j] = i < n && (list ? i < r.k : b[j] < info.kbin || (b[j] == info.kbin && i < (int)before_k + info.kleft));
       if (!in_k[j]) weight[j] = 0;
       sum += weight[j];
     }
@@ -641,11 +771,12 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
     before += info.below_lo;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
+      left[j] = 0;
       if (in_k[j] && (!(r.p < 1.0f) || (b[j] <= info.hi && before < want))) {
         ++kept;
+        left[j] = left_of(a, r, l[j]);
         const int id = (int)~(uint32_t)entry[threadIdx.x * EACH + j];
-        const uint64_t v = left_of(a, r, l[j]);
-        if (v) atomicAdd((unsigned long long*)&s.chunk[id / w.size], (unsigned long long)v);
+        if (left[j]) atomicAdd((unsigned long long*)&s.chunk[id / part], (unsigned long long)left[j]);
       }
       before += weight[j];
     }
@@ -653,10 +784,46 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
     __syncthreads();
     if (kept_entries > 0) last = entry[kept_entries - 1];
   }
-  draw<F32>(a, p, row, r, s, w.chunks, w.size, [&](float l, int i) -> uint64_t {
-    const int b = bins.of(l);
-    return b < BINS - 1 && (b < info.lo || entry_of(l, i) >= last) ? left_of(a, r, l) : 0;
-  });
+  if (!list) {
+    draw<F32>(a, p, row, r, s, w.chunks, w.size, [&](float l, int i) -> uint64_t {
+      const int b = bins.of(l);
+      return b < BINS - 1 && (b < info.lo || entry_of(l, i) >= last) ? left_of(a, r, l) : 0;
+    });
+    return;
+  }
+  // the part of the ids that holds the draw's place, its entries, and of these the one
+  uint64_t whole;
+  const uint64_t of_part = s.chunk[threadIdx.x];
+  const uint64_t first_of = block_scan(of_part, s.part, whole);
+  const uint64_t place = place_of(a.uniforms[row], whole);
+  if (place >= first_of && place < first_of + of_part) {
+    s.bcast[0] = threadIdx.x;
+    s.bcast[1] = first_of;
+  }
+  if (threadIdx.x == 0) kept_entries = 0;
+  __syncthreads();
+  const int at = (int)s.bcast[0];
+  const uint64_t first = s.bcast[1];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const int i = threadIdx.x * EACH + j;
+    if (i >= n || left[j] == 0) continue;
+    const int id = (int)~(uint32_t)entry[i];
+    if (id / part == at) other[atomicAdd(&kept_entries, 1)] = (uint64_t)id << 32 | (uint32_t)i;
+  }
+  __syncthreads();
+  const int few = kept_entries;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const int i = threadIdx.x * EACH + j;
+    if (i >= n || left[j] == 0) continue;
+    const int id = (int)~(uint32_t)entry[i];
+    if (id / part != at) continue;
+    uint64_t before = first;
+    for (int q = 0; q < few; ++q)
+      if ((int)(other[q] >> 32) < id) before += left_of(a, r, value_of((uint32_t)(entry[(uint32_t)other[q]] >> 32)));
+    if (place >= before && place < before + left[j]) write_token(a, row, r, id, l[j], whole);
+  }
 }
 
 // Tokens of a chunk: whole units, so many that the launches have about three workgroups a CU.
@@ -666,7 +833,7 @@ static int chunk_size(int64_t rows, int vocab) {
 }
 struct Layout {
   int chunks, size;
-  size_t tops, sums, info, weights, counts, list, listed, bytes;
+  size_t tops, sums, info, weights, counts, list, listed, groups, bytes;
   Layout(int64_t rows, int vocab) {
     size = chunk_size(rows, vocab);
     chunks = (vocab + size - 1) / size;
@@ -682,6 +849,7 @@ struct Layout {
     list = part(rows * CANDIDATES * sizeof(uint64_t));
     counts = part(rows * BINS * sizeof(uint32_t));
     tops = part(rows * chunks * sizeof(float));
+    groups = part(rows * chunks * (size / GROUP) * sizeof(float));
     listed = part(rows * sizeof(uint32_t));
   }
 };
@@ -700,7 +868,8 @@ static void launch(Args a, void* workspace, hipStream_t st) {
   uint8_t* base = (uint8_t*)workspace;
   const Work w = {(float*)(base + at.tops),       (uint64_t*)(base + at.sums),   (RowInfo*)(base + at.info),
                   (uint64_t*)(base + at.weights), (uint32_t*)(base + at.counts), (uint64_t*)(base + at.list),
-                  (uint32_t*)(base + at.listed),  at.chunks,                     at.size};
+                  (uint32_t*)(base + at.listed),  (float*)(base + at.groups),    at.chunks,
+                  at.size};
   for (int left = a.rows; left > 0; left -= BATCH) {
     a.rows = left < BATCH ? left : BATCH;
     const dim3 grid((unsigned)(a.rows * at.chunks));
