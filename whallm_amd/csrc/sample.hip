@@ -17,7 +17,8 @@ namespace wm {
 namespace smp {
 
 constexpr int MAX_VOCAB = 1 << 22;
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr int THREADS = 512, WAVES = THREADS / 64;
+constexpr int PARTS = 1024;  // a row's chunks at most
 constexpr int SMALL = 8192;  // tokens of a vocabulary that one workgroup takes
 
 struct Args {
@@ -51,7 +52,8 @@ struct Rules {
   double scale;   // log2(e) / T
   int k;
   float p, m;
-  __device__ __forceinline__ Rules(const Args& a, int row, float top_) : top(top_) {
+  // Loaded before the row's largest logit is known, which `top` is set to.
+  __device__ __forceinline__ Rules(const Args& a, int row) : top(0.0f) {
     float t = a.temperature ? a.temperature[row] : 1.0f;
     k = a.top_k ? a.top_k[row] : 0;
     p = a.top_p ? a.top_p[row] : 1.0f;
@@ -113,7 +115,7 @@ struct Shared {
   uint32_t counts[256];
   uint64_t part[WAVES];
   float top[WAVES];
-  uint64_t chunk[THREADS];  // the chunks' sums
+  uint64_t chunk[PARTS];  // the chunks' sums
   uint64_t bcast[3];
 };
 
@@ -132,6 +134,26 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
   v = add_dpp<0x142, 0xa>(v);  // row_bcast 15 to rows 1 and 3
   v = add_dpp<0x143, 0xc>(v);  // row_bcast 31 to rows 2 and 3
   return v;
+}
+// Room for `n` of this lane in a list: the first place, after the wave's lanes before. One addition a wave, whose lanes all
+// call it.
+__device__ __forceinline__ uint32_t reserve(uint32_t* counter, uint32_t n) {
+  uint32_t s = n;
+#define WM_SCAN_STEP(CTRL, ROWS) s += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)s, CTRL, ROWS, 0xf, false)
+  WM_SCAN_STEP(0x111, 0xf);
+  WM_SCAN_STEP(0x112, 0xf);
+  WM_SCAN_STEP(0x114, 0xf);
+  WM_SCAN_STEP(0x118, 0xf);
+  WM_SCAN_STEP(0x142, 0xa);
+  WM_SCAN_STEP(0x143, 0xc);
+#undef WM_SCAN_STEP
+  const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+  uint32_t first = 0;
+  if (all > 0) {
+    if (threadIdx.x % 64 == 0) first = atomicAdd(counter, all);
+    first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
+  }
+  return first + s - n;
 }
 // Sum of the threads before this one; `total` of all. Every thread calls it.
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint64_t& total) {
@@ -254,6 +276,31 @@ __device__ __forceinline__ uint64_t place_of(float u, uint64_t whole) {
   return __umul64hi((uint64_t)((u > 0.0f ? fminf(u, 1.0f - 0x1p-24f) : 0.0f) * 0x1p64f), whole);
 }
 
+// The part of `parts` that holds the draw's place, into s.bcast[0]; returns the place, the sum of all and of the parts before.
+// Every thread calls it, behind a barrier; ends with one.
+__device__ __forceinline__ uint64_t find_part(const Args& a, int row, Shared& s, int parts, uint64_t& whole, uint64_t& before) {
+  constexpr int EACH = PARTS / THREADS;
+  uint64_t v[EACH], sum = 0;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const int c = threadIdx.x * EACH + j;
+    sum += v[j] = c < parts ? s.chunk[c] : 0;
+  }
+  uint64_t at = block_scan(sum, s.part, whole);
+  const uint64_t place = place_of(a.uniforms[row], whole);
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    if (place >= at && place < at + v[j]) {
+      s.bcast[0] = threadIdx.x * EACH + j;
+      s.bcast[1] = at;
+    }
+    at += v[j];
+  }
+  __syncthreads();
+  before = s.bcast[1];
+  return place;
+}
+
 // The row's results: token i of logit l, drawn among weights of this sum.
 __device__ __forceinline__ void write_token(const Args& a, int row, const Rules& r, int i, float l, uint64_t whole) {
   const double t = l == r.top ? 0.0 : ((double)l - (double)r.top) * r.scale;
@@ -265,18 +312,11 @@ __device__ __forceinline__ void write_token(const Args& a, int row, const Rules&
 // logit l with id i, 0 if it goes. `size` is a chunk's tokens, a multiple of THREADS. Every thread calls it.
 template <bool F32, typename Left>
 __device__ void draw(const Args& a, const void* p, int row, const Rules& r, Shared& s, int chunks, int size, Left left) {
-  uint64_t whole;
+  uint64_t whole, first_of;
   __syncthreads();
-  const uint64_t of_chunk = (int)threadIdx.x < chunks ? s.chunk[threadIdx.x] : 0;
-  const uint64_t first_of = block_scan(of_chunk, s.part, whole);
-  uint64_t want = place_of(a.uniforms[row], whole);
-  if (want >= first_of && want < first_of + of_chunk) {
-    s.bcast[0] = threadIdx.x;
-    s.bcast[1] = want - first_of;
-  }
-  __syncthreads();
+  uint64_t want = find_part(a, row, s, chunks, whole, first_of);
+  want -= first_of;
   const int c = (int)s.bcast[0], each = size / THREADS;
-  want = s.bcast[1];
   const int first = c * size + (int)threadIdx.x * each, end = min(first + each, a.vocab);
   uint64_t mine = 0, total;
   for (int i = first; i < end; ++i) mine += left(logit<F32>(p, i), i);
@@ -315,6 +355,7 @@ __global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
   __shared__ Shared s;
   const int row = blockIdx.x;
   const void* p = (const uint8_t*)a.logits + (int64_t)row * a.vocab * (F32 ? 4 : 2);
+  Rules r(a, row);
   // the largest logit; a NaN's key is the largest or the smallest
   uint32_t high = 0;
   bool nan = false;
@@ -332,7 +373,8 @@ __global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
     if (threadIdx.x == 0) a.tokens[row] = -1, a.logp[row] = NAN;
     return;
   }
-  draw_cut<F32>(a, p, row, Rules(a, row, top), s, 1, SMALL);
+  r.top = top;
+  draw_cut<F32>(a, p, row, r, s, 1, SMALL);
 }
 
 // ---------------------------------------------------------------------------------- larger vocabularies
@@ -457,11 +499,10 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_bins_kernel(Args a, Work w
   __shared__ uint32_t counts[BINS];
   __shared__ float part[BIN_THREADS / 64];
   const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
-  float top;
-  if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, part, top)) return;
-  const Rules r(a, row, top);
+  Rules r(a, row);
   const bool by_weight = r.p < 1.0f, by_count = r.k > 0;
   if (listed(r) || (!by_weight && !by_count)) return;
+  if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, part, r.top)) return;
   const Bins bins(r);
   for (int i = threadIdx.x; i < BINS; i += BIN_THREADS) {
     if (by_weight) weights[i] = 0;
@@ -517,10 +558,8 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
   __shared__ uint64_t list[CANDIDATES];
   __shared__ uint32_t found, first;
   const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
-  float top;
-  if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, top_part, top)) return;
-  const Rules r(a, row, top);
-  if (listed(r)) return;
+  Rules r(a, row);
+  if (listed(r) || !row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, top_part, r.top)) return;
   const Bins bins(r);
   if (threadIdx.x == 0) info = {0, 0, BINS, BINS, BINS, 0}, found = 0;
   if (r.k > 0 || r.p < 1.0f) {
@@ -582,21 +621,25 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
   uint64_t sum = 0;
   const int64_t base = (int64_t)row * a.vocab;
   const int lo = c * w.size, end = min(lo + w.size, a.vocab);
-  for (int i = lo + 8 * threadIdx.x; i < end; i += UNIT) {
+  for (int i = lo + 8 * threadIdx.x; i < lo + w.size; i += UNIT) {  // whole waves
     Eight<F32> l;
     l.load(a.logits, base, i, end - i);
+    uint32_t hits = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float v = l.get(e, end - i);
       const int b = bins.of(v);
       if (b == BINS - 1) continue;
-      if (b < stay) {
-        sum += left_of(a, r, v);
-      } else if (b <= hi || b == kbin) {
-        const uint32_t at = atomicAdd(&found, 1u);
-        if (at < CANDIDATES) list[at] = entry_of(v, i + e);
-      }
+      if (b < stay) sum += left_of(a, r, v);
+      else if (b <= hi || b == kbin) hits |= 1u << e;
     }
+    uint32_t at = reserve(&found, __popc(hits));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (hits >> e & 1) {
+        if (at < CANDIDATES) list[at] = entry_of(l.get(e, end - i), i + e);
+        ++at;
+      }
   }
   uint64_t total;
   scan_of<BIN_THREADS>(sum, part, total);  // and a barrier
@@ -623,14 +666,21 @@ __device__ __forceinline__ void sort_entries(uint64_t* v, int n) {
   __syncthreads();
 }
 
-// The same for up to THREADS / 2 entries, each put in its place by how many are above it. Ends with a barrier.
+// The same for up to THREADS entries, each put in its place by how many are above it. Ends with a barrier.
 __device__ __forceinline__ void rank_entries(uint64_t* v, uint64_t* other, int n) {
-  __syncthreads();
   const int t = threadIdx.x;
+  if (t < 8) v[n + t] = 0;  // below every entry
+  __syncthreads();
   if (t < n) {
     const uint64_t mine = v[t];
     int above = 0;
-    for (int i = 0; i < n; ++i) above += v[i] > mine;
+    for (int i = 0; i < n; i += 8) {
+      uint64_t o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = v[i + j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) above += o[j] > mine;
+    }
     other[above] = mine;
   }
   __syncthreads();
@@ -651,6 +701,7 @@ __device__ int list_row(const Args& a, const Work& w, const void* p, int row, co
   if (threadIdx.x < 2) found[threadIdx.x] = 0;
   if (threadIdx.x == 0) s.bcast[0] = BINS - 2;
   __syncthreads();
+#pragma unroll 4
   for (int g = threadIdx.x; g < groups; g += THREADS) {
     const int b = bins.of(tops[g]);
     if (b < BINS - 1) atomicAdd(&counts[b], 1u);
@@ -668,29 +719,35 @@ __device__ int list_row(const Args& a, const Work& w, const void* p, int row, co
   }
   __syncthreads();
   const int bound = (int)s.bcast[0];
-  for (int g = threadIdx.x; g < groups; g += THREADS) {
-    if (bins.of(tops[g]) > bound) continue;
-    const uint32_t i = atomicAdd(&found[0], 1u);
-    if (i < CANDIDATES) which[i] = g;
+#pragma unroll 1
+  for (int g0 = 0; g0 < groups; g0 += THREADS) {
+    const int g = g0 + (int)threadIdx.x;
+    const bool is = g < groups && bins.of(tops[g]) <= bound;
+    const uint32_t i = reserve(&found[0], is);
+    if (is && i < CANDIDATES) which[i] = g;
   }
   __syncthreads();
   const uint32_t hits = found[0];
   if (hits > CANDIDATES) return CANDIDATES + 1;
-  for (uint32_t e0 = threadIdx.x; e0 < hits * GROUP; e0 += THREADS * AHEAD) {
+  for (uint32_t e0 = 0; e0 < hits * GROUP; e0 += THREADS * AHEAD) {
     float l[AHEAD];
     int id[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const uint32_t e = e0 + THREADS * j;
+      const uint32_t e = e0 + THREADS * j + threadIdx.x;
       id[j] = e < hits * GROUP ? (int)(which[e / GROUP] * GROUP + e % GROUP) : a.vocab;
       l[j] = id[j] < a.vocab ? logit<F32>(p, id[j]) : -INFINITY;
     }
+    uint32_t in = 0;
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (id[j] >= a.vocab || bins.of(l[j]) > bound) continue;
-      const uint32_t i = atomicAdd(&found[1], 1u);
-      if (i < CANDIDATES) entry[i] = entry_of(l[j], id[j]);
-    }
+    for (int j = 0; j < AHEAD; ++j) in |= (uint32_t)(bins.of(l[j]) <= bound) << j;
+    uint32_t i = reserve(&found[1], __popc(in));
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (in >> j & 1) {
+        if (i < CANDIDATES) entry[i] = entry_of(l[j], id[j]);
+        ++i;
+      }
   }
   __syncthreads();
   return (int)found[1];
@@ -698,25 +755,24 @@ __device__ int list_row(const Args& a, const Work& w, const void* p, int row, co
 
 template <bool F32>
 __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
-  constexpr int EACH = CANDIDATES / THREADS;
   __shared__ Shared s;
-  __shared__ uint64_t entry[CANDIDATES], other[CANDIDATES];
-  __shared__ int kept_entries;
+  // the candidates, their weights, and what lies ahead of each
+  __shared__ uint64_t entry[CANDIDATES], weight[CANDIDATES], ahead[CANDIDATES];
+  __shared__ int in_part;
   __shared__ uint32_t found[2];
   const int row = blockIdx.x;
   const void* p = (const uint8_t*)a.logits + (int64_t)row * a.vocab * (F32 ? 4 : 2);
-  float top;
-  if (!row_top<THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, s.top, top)) {
+  Rules r(a, row);
+  if (!row_top<THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, s.top, r.top)) {
     if (threadIdx.x == 0) a.tokens[row] = -1, a.logp[row] = NAN;
     return;
   }
-  const Rules r(a, row, top);
   const Bins bins(r);
   const bool list = listed(r);
   RowInfo info = {0, 0, 0, BINS, BINS, 0};
   int n;
   if (list) {
-    n = list_row<F32>(a, w, p, row, r, bins, s, entry, (uint32_t*)other, found);
+    n = list_row<F32>(a, w, p, row, r, bins, s, entry, (uint32_t*)weight, found);
   } else {
     n = (int)w.listed[row];
     info = w.info[row];
@@ -725,66 +781,65 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
     draw_cut<F32>(a, p, row, r, s, w.chunks, w.size);
     return;
   }
-  // the weights by id: in parts of the chunks' size, or, where the list is all there is, as fine as there are threads
+  // the weights by id: in parts of the chunks' size, or, where the list is all there is, a thousand
   int part = w.size;
-  if (list) part = (a.vocab + THREADS - 1) / THREADS;
-  if (!list && (int)threadIdx.x < w.chunks) s.chunk[threadIdx.x] = w.sums[(int64_t)row * w.chunks + threadIdx.x];
-  if (list) s.chunk[threadIdx.x] = 0;
-  if (threadIdx.x == 0) kept_entries = 0;
-  uint64_t last = ~0ull;  // the last entry that stays; none
-  float l[EACH];
-  uint64_t left[EACH];
-  if (n > 0) {
-    if (!list)
-      for (int i = threadIdx.x; i < n; i += THREADS) entry[i] = w.list[(int64_t)row * CANDIDATES + i];
-    if (n <= 512) {
-      rank_entries(entry, other, n);
-    } else {
-      int places = 1024;
-      while (places < n) places *= 2;
-      for (int i = n + threadIdx.x; i < places; i += THREADS) entry[i] = 0;
-      sort_entries(entry, places);
-    }
-    // in order: the bins from lo to hi, then kbin's, if that is behind them
-    int b[EACH], in_k[EACH];
-    uint64_t weight[EACH], sum = 0, ahead = 0, total;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int i = threadIdx.x * EACH + j;
-      l[j] = i < n ? value_of((uint32_t)(entry[i] >> 32)) : -INFINITY;
-      b[j] = i < n ? bins.of(l[j]) : BINS;
-      weight[j] = i < n ? fixed_of(weight_of(l[j], r), a.shift) : 0;
-      ahead += b[j] < info.kbin;
-    }
-    uint64_t before_k;
-    block_scan(ahead, s.part, before_k);  // entries ahead of kbin's
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int i = threadIdx.x * EACH + j;
-      in_k[j] = i < n && (list ? i < r.k : b[j] < info.kbin || (b[j] == info.kbin && i < (int)before_k + info.kleft));
-      if (!in_k[j]) weight[j] = 0;
-      sum += weight[j];
-    }
-    uint64_t before = block_scan(sum, s.part, total);
-    const uint64_t want = r.p < 1.0f ? part_of(r.p, info.below_lo + info.between + total) : 0;
-    int kept = 0;
-    before += info.below_lo;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      left[j] = 0;
-      if (in_k[j] && (!(r.p < 1.0f) || (b[j] <= info.hi && before < want))) {
-        ++kept;
-        left[j] = left_of(a, r, l[j]);
-        const int id = (int)~(uint32_t)entry[threadIdx.x * EACH + j];
-        if (left[j]) atomicAdd((unsigned long long*)&s.chunk[id / part], (unsigned long long)left[j]);
-      }
-      before += weight[j];
-    }
-    if (kept) atomicAdd(&kept_entries, kept);
-    __syncthreads();
-    if (kept_entries > 0) last = entry[kept_entries - 1];
+  if (list) part = (a.vocab + PARTS - 1) / PARTS;
+  if (threadIdx.x == 0) in_part = 0;
+  for (int c = threadIdx.x; c < PARTS; c += THREADS) s.chunk[c] = !list && c < w.chunks ? w.sums[(int64_t)row * w.chunks + c] : 0;
+  if (!list)
+    for (int i = threadIdx.x; i < n; i += THREADS) entry[i] = w.list[(int64_t)row * CANDIDATES + i];
+  if (n <= THREADS) {
+    rank_entries(entry, weight, n);
+  } else {
+    int places = 2 * THREADS;
+    while (places < n) places *= 2;
+    for (int i = n + threadIdx.x; i < places; i += THREADS) entry[i] = 0;
+    sort_entries(entry, places);
   }
+  // In order: the bins from lo to hi, then kbin's, if that is behind them. Entries ahead of kbin's:
+  int before_k = 0;
   if (!list) {
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += THREADS) {
+      const int i = i0 + (int)threadIdx.x;
+      before_k += __syncthreads_count(i < n && bins.of(value_of((uint32_t)(entry[i] >> 32))) < info.kbin);
+    }
+  }
+  uint64_t sum = info.below_lo;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    const int i = i0 + (int)threadIdx.x;
+    uint64_t v = 0, total;
+    bool stays = false;
+    if (i < n) {
+      const float l = value_of((uint32_t)(entry[i] >> 32));
+      const int b = bins.of(l);
+      const double e = weight_of(l, r);
+      stays = e >= (double)r.m;
+      if (list ? i < r.k : b < info.kbin || (b == info.kbin && i < before_k + info.kleft)) v = fixed_of(e, a.shift);
+    }
+    const uint64_t before = sum + block_scan(v, s.part, total);
+    if (i < n) {
+      weight[i] = v | (uint64_t)stays << 63;
+      ahead[i] = before;
+    }
+    sum += total;
+  }
+  const uint64_t want = r.p < 1.0f ? part_of(r.p, sum + info.between) : ~0ull;
+  int kept = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    const int i = i0 + (int)threadIdx.x;
+    const uint64_t v = i < n ? weight[i] : 0;
+    // a token of top-k whose weight is 0 does not matter, nor does one between hi and kbin: it has more than `want` ahead
+    const bool keep = (v << 1) != 0 && ahead[i] < want;
+    kept += __syncthreads_count(keep);
+    if (i < n) weight[i] = keep && v >> 63 ? v << 1 >> 1 : 0;
+    if (keep && v >> 63) atomicAdd((unsigned long long*)&s.chunk[(int)~(uint32_t)entry[i] / part], (unsigned long long)(v << 1 >> 1));
+  }
+  __syncthreads();
+  if (!list) {
+    const uint64_t last = kept > 0 ? entry[kept - 1] : ~0ull;  // the last entry that stays
     draw<F32>(a, p, row, r, s, w.chunks, w.size, [&](float l, int i) -> uint64_t {
       const int b = bins.of(l);
       return b < BINS - 1 && (b < info.lo || entry_of(l, i) >= last) ? left_of(a, r, l) : 0;
@@ -792,44 +847,32 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
     return;
   }
   // the part of the ids that holds the draw's place, its entries, and of these the one
-  uint64_t whole;
-  const uint64_t of_part = s.chunk[threadIdx.x];
-  const uint64_t first_of = block_scan(of_part, s.part, whole);
-  const uint64_t place = place_of(a.uniforms[row], whole);
-  if (place >= first_of && place < first_of + of_part) {
-    s.bcast[0] = threadIdx.x;
-    s.bcast[1] = first_of;
-  }
-  if (threadIdx.x == 0) kept_entries = 0;
-  __syncthreads();
+  uint64_t whole, first;
+  const uint64_t place = find_part(a, row, s, PARTS, whole, first);
   const int at = (int)s.bcast[0];
-  const uint64_t first = s.bcast[1];
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const int i = threadIdx.x * EACH + j;
-    if (i >= n || left[j] == 0) continue;
-    const int id = (int)~(uint32_t)entry[i];
-    if (id / part == at) other[atomicAdd(&kept_entries, 1)] = (uint64_t)id << 32 | (uint32_t)i;
-  }
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += THREADS)
+    if (weight[i] && (int)~(uint32_t)entry[i] / part == at) ahead[atomicAdd(&in_part, 1)] = i;
   __syncthreads();
-  const int few = kept_entries;
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const int i = threadIdx.x * EACH + j;
-    if (i >= n || left[j] == 0) continue;
-    const int id = (int)~(uint32_t)entry[i];
-    if (id / part != at) continue;
+  const int few = in_part;
+#pragma unroll 1
+  for (int j = threadIdx.x; j < few; j += THREADS) {
+    const int i = (int)ahead[j], id = (int)~(uint32_t)entry[i];
     uint64_t before = first;
-    for (int q = 0; q < few; ++q)
-      if ((int)(other[q] >> 32) < id) before += left_of(a, r, value_of((uint32_t)(entry[(uint32_t)other[q]] >> 32)));
-    if (place >= before && place < before + left[j]) write_token(a, row, r, id, l[j], whole);
+#pragma unroll 1
+    for (int q = 0; q < few; ++q) {
+      const int o = (int)ahead[q];
+      if ((int)~(uint32_t)entry[o] < id) before += weight[o];
+    }
+    if (place >= before && place < before + weight[i]) write_token(a, row, r, id, value_of((uint32_t)(entry[i] >> 32)), whole);
   }
 }
 
 // Tokens of a chunk: whole units, so many that the launches have about three workgroups a CU.
 static int chunk_size(int64_t rows, int vocab) {
+  constexpr int MOST = 2;
   const int64_t units = (vocab + UNIT - 1) / UNIT, each = rows * units / 768;
-  return (int)(each < 1 ? 1 : each > 8 ? 8 : each) * UNIT;
+  return (int)(each < 1 ? 1 : each > MOST ? MOST : each) * UNIT;
 }
 struct Layout {
   int chunks, size;
