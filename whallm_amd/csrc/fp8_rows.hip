@@ -80,53 +80,44 @@ struct RowArgs {
   int64_t units;    // rows * blocks
 };
 
-// 16 lanes a block, UNITS blocks a lane group with their loads in flight together.
-template <bool F32, bool SWIGLU, bool WHOLE, int UNITS>
+// 16 lanes a block. (Four blocks a group of lanes, their loads in flight together, took 4.0 us for 256 rows of 7168 and 65.2 for
+// 16,384; one 3.3 and 64.5.)
+template <bool F32, bool SWIGLU, bool WHOLE>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(RowArgs a, Fp8Out o) {
   const int lane = threadIdx.x % 16;
-  const int64_t first = (int64_t)blockIdx.x * (16 * UNITS) + threadIdx.x / 16;
-  Row8<F32> x[UNITS], up[UNITS];
-  int64_t row[UNITS];
-  int col[UNITS];
-#pragma unroll
-  for (int k = 0; k < UNITS; ++k) {
-    const int64_t unit = first + 16 * k;
-    x[k].clear();
-    if (SWIGLU) up[k].clear();
-    row[k] = unit / a.blocks;
-    col[k] = (int)(unit - row[k] * a.blocks) * FP8_BLOCK + 8 * lane;
-    if (unit < a.units && col[k] < a.width) {
-      const int n = a.width - col[k];
-      if (SWIGLU) {
-        const int64_t at = row[k] * 2 * a.width + col[k];
-        x[k].template load<WHOLE>(a.x, at + a.gate_at, n);
-        up[k].template load<WHOLE>(a.x, at + (a.width - a.gate_at), n);
-      } else {
-        x[k].template load<WHOLE>(a.x, row[k] * a.width + col[k], n);
-      }
+  const int64_t unit = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const int64_t row = unit / a.blocks;
+  const int col = (int)(unit - row * a.blocks) * FP8_BLOCK + 8 * lane, n = a.width - col;
+  const bool in = unit < a.units && n > 0;
+  Row8<F32> x, up;
+  x.clear();
+  if (SWIGLU) up.clear();
+  if (in) {
+    if (SWIGLU) {
+      const int64_t at = row * 2 * a.width + col;
+      x.template load<WHOLE>(a.x, at + a.gate_at, n);
+      up.template load<WHOLE>(a.x, at + (a.width - a.gate_at), n);
+    } else {
+      x.template load<WHOLE>(a.x, row * a.width + col, n);
     }
   }
+  float v[8];
 #pragma unroll
-  for (int k = 0; k < UNITS; ++k) {
-    const int64_t unit = first + 16 * k;
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = x[k].get(i);
-      if (SWIGLU) {
-        float u = up[k].get(i);
-        if (a.limit > 0.0f) {  // NaN passes
-          v[i] = __builtin_elementwise_minimum(v[i], a.limit);
-          u = __builtin_elementwise_maximum(__builtin_elementwise_minimum(u, a.limit), -a.limit);
-        }
-        v[i] = v[i] * sigmoid_f32(v[i]) * u;
+  for (int i = 0; i < 8; ++i) {
+    v[i] = x.get(i);
+    if (SWIGLU) {
+      float u = up.get(i);
+      if (a.limit > 0.0f) {  // NaN passes
+        v[i] = __builtin_elementwise_minimum(v[i], a.limit);
+        u = __builtin_elementwise_maximum(__builtin_elementwise_minimum(u, a.limit), -a.limit);
       }
+      v[i] = v[i] * sigmoid_f32(v[i]) * u;
     }
-    const float s = block_scale(v, o.pow2);
-    if (unit < a.units && col[k] < a.width) {
-      store_e4m3<WHOLE>(o.q + row[k] * a.width + col[k], a.width - col[k], to_e4m3(v, 1.0f / s));
-      if (lane == 0) o.scales[unit] = s;
-    }
+  }
+  const float s = block_scale(v, o.pow2);
+  if (in) {
+    store_e4m3<WHOLE>(o.q + row * a.width + col, n, to_e4m3(v, 1.0f / s));
+    if (lane == 0) o.scales[unit] = s;
   }
 }
 
@@ -221,15 +212,10 @@ static void norm_fp8(const Fp8NormArgs& a, const Fp8Out& o, hipStream_t s) {
   check_launch("norm_fp8");
 }
 
-// Blocks of 128 a group of lanes takes, by how many there are.
-constexpr int64_t FP8_MANY = 1 << 16;
-
 template <bool F32, bool SWIGLU, bool WHOLE>
 static void fp8_rows(const RowArgs& a, const Fp8Out& o, hipStream_t s) {
-  const int each = a.units >= FP8_MANY ? 4 : 1;
-  const dim3 grid(grid_of("wm_fp8_rows", (a.units + 16 * each - 1) / (16 * each), 256));
-  if (each == 4) hipLaunchKernelGGL((fp8_rows_kernel<F32, SWIGLU, WHOLE, 4>), grid, dim3(256), 0, s, a, o);
-  else hipLaunchKernelGGL((fp8_rows_kernel<F32, SWIGLU, WHOLE, 1>), grid, dim3(256), 0, s, a, o);
+  const dim3 grid(grid_of("wm_fp8_rows", (a.units + 15) / 16, 256));
+  hipLaunchKernelGGL((fp8_rows_kernel<F32, SWIGLU, WHOLE>), grid, dim3(256), 0, s, a, o);
   check_launch("fp8_rows");
 }
 
@@ -272,7 +258,7 @@ WM_EXPORT int wm_fp8_rows(const void* x, int32_t fp32, int32_t rows, int32_t wid
     if (pow2 != 0 && pow2 != 1) fail("wm_fp8_rows: pow2 must be 0 or 1");
     if (!(limit >= 0.0f)) fail("wm_fp8_rows: limit must not be negative");
     const int64_t blocks = (width + FP8_BLOCK - 1) / FP8_BLOCK, units = rows * blocks;
-    grid_of("wm_fp8_rows", (units + 63) / 64, 256);
+    grid_of("wm_fp8_rows", (units + 15) / 16, 256);
     if (rows == 0) return;
     if (!x || !q || !scales) fail("wm_fp8_rows: null pointer");
     if ((uintptr_t)x % (fp32 ? 4 : 2) || (uintptr_t)scales % 4) fail("wm_fp8_rows: tensors must be aligned to their elements");

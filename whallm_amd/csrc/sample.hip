@@ -19,7 +19,10 @@ namespace smp {
 constexpr int MAX_VOCAB = 1 << 22;
 constexpr int THREADS = 512, WAVES = THREADS / 64;
 constexpr int PARTS = 1024;  // a row's chunks at most
-constexpr int SMALL = 8192;  // tokens of a vocabulary that one workgroup takes
+// Tokens of a vocabulary that one workgroup takes in one launch, passing them several times from its L2. With top-k 50 and top-p 0.9,
+// top-p alone and neither, one row: 24, 21 and 12 us of 2048 tokens (in chunks 39, 23 and 15), 31, 25 and 13 of 4096 (16, 25
+// and 16), 51, 45 and 18 of 8192 (16, 26 and 17); 512 rows likewise.
+constexpr int SMALL = 2048;
 
 struct Args {
   const void* logits;
@@ -67,37 +70,33 @@ struct Rules {
   }
 };
 
-// 2^x for x <= 0, to 2^-51 of it: x split into a whole number and a rest of at most 1/2, whose power is its
-// series in the rest times ln 2. 0 from 2^-64 on, which no fixed-point weight holds.
-__device__ __forceinline__ double exp2_f64(double x) {
-  if (!(x > -64.0)) return 0.0;
-  constexpr double LN2 = 0.6931471805599453;
-  const double n = rint(x), f = (x - n) * LN2;
-  double s = 1.0 / 479001600.0;
-  s = fma(s, f, 1.0 / 39916800.0);
-  s = fma(s, f, 1.0 / 3628800.0);
-  s = fma(s, f, 1.0 / 362880.0);
-  s = fma(s, f, 1.0 / 40320.0);
-  s = fma(s, f, 1.0 / 5040.0);
-  s = fma(s, f, 1.0 / 720.0);
-  s = fma(s, f, 1.0 / 120.0);
-  s = fma(s, f, 1.0 / 24.0);
-  s = fma(s, f, 1.0 / 6.0);
-  s = fma(s, f, 0.5);
-  s = fma(s, f, 1.0);
-  s = fma(s, f, 1.0);
-  return ldexp(s, (int)n);
-}
-
-// e of a logit.
+// e of a logit, to 2^-51 of it, without a branch. With x = (l - L) log2(e) / T, n the whole number next to it and f = x - n
+//   e = 2^n sum_j (f ln 2)^j / j!     |f| <= 1/2, so that what lies behind j = 12 is below 2^-52
+// x ends at -100, far below what a weight's integer holds; a masked logit is there too, where T is infinite (NaN) as well.
 __device__ __forceinline__ double weight_of(float l, const Rules& r) {
-  if (l == r.top) return 1.0;
-  if (l == -INFINITY || r.top == INFINITY) return 0.0;
-  return exp2_f64(((double)l - (double)r.top) * r.scale);
+  constexpr double L1 = 0.6931471805599453, L2 = L1 * L1, L3 = L2 * L1, L4 = L2 * L2, L6 = L4 * L2, L8 = L4 * L4;
+  constexpr double WHOLE = 0x1.8p52;  // added to x it leaves n in the sum's low bits
+  const double x = fmax(((double)l - (double)r.top) * r.scale, -100.0);
+  const double t = x + WHOLE, f = x - (t - WHOLE);
+  double s = L8 * L4 / 479001600.0;
+  s = fma(s, f, L8 * L3 / 39916800.0);
+  s = fma(s, f, L8 * L2 / 3628800.0);
+  s = fma(s, f, L8 * L1 / 362880.0);
+  s = fma(s, f, L8 / 40320.0);
+  s = fma(s, f, L6 * L1 / 5040.0);
+  s = fma(s, f, L6 / 720.0);
+  s = fma(s, f, L4 * L1 / 120.0);
+  s = fma(s, f, L4 / 24.0);
+  s = fma(s, f, L3 / 6.0);
+  s = fma(s, f, L2 / 2.0);
+  s = fma(s, f, L1);
+  s = fma(s, f, 1.0);
+  const double e = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, s) + (__builtin_bit_cast(uint64_t, t) << 52));
+  return l == r.top ? 1.0 : e;  // also where both are infinite
 }
 // e to a multiple of 2^-shift, as an integer: adding 2^52 leaves it in the sum's low bits (shift is at most 51).
 __device__ __forceinline__ uint64_t fixed_of(double e, int shift) {
-  const double v = ldexp(e, shift) + 0x1p52;
+  const double v = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, e) + ((uint64_t)shift << 52)) + 0x1p52;
   return __builtin_bit_cast(uint64_t, v) & ((1ull << 52) - 1);
 }
 
@@ -392,10 +391,14 @@ __global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
 //
 // Either way the last launch sorts the candidates, cuts and draws. Rows of more candidates than there is room for (a cut
 // among thousands of nearly equal logits) are cut by radix selection as above.
-constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048, LIST_K = 512;
-constexpr int GROUP = 64;
+constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048;
+constexpr int MOST = 2;  // units of a chunk at most
 
-__device__ __forceinline__ bool listed(const Rules& r) { return r.k > 0 && r.k <= LIST_K; }
+// A row's candidates come from its groups while k is small and at most 3/4 of the groups: beyond, the groups' bound sinks fast.
+// By the groups and by the bins, one row of 129,280 tokens: k 48 18 and 22 us, 128 22 both, 256 28 and 22; 256 rows 52 and 109,
+// 56 and 110, 64 and 112. One row of 8192 (128 groups): k 96 18.5 and 22, 128 28 and 23.
+constexpr int GROUP = 64, LIST_K = 256;
+__device__ __forceinline__ bool listed(const Args& a, const Rules& r) { return r.k > 0 && r.k <= min(LIST_K, a.vocab / GROUP * 3 / 4); }
 
 struct RowInfo {
   uint64_t below_lo, between;  // weights of the bins below lo, and of those between hi and kbin
@@ -454,6 +457,20 @@ struct Eight {
   __device__ __forceinline__ float get(int e, int n) const { return e < n ? raw.get(e) + 0.0f : -INFINITY; }
 };
 
+// A thread's logits of a chunk, all on their way at once: before what the launch has to know of the row.
+template <bool F32>
+struct ChunkLogits {
+  Eight<F32> l[MOST];
+  __device__ __forceinline__ void load(const void* logits, int64_t base, int lo, int end, int size) {
+#pragma unroll
+    for (int u = 0; u < MOST; ++u)
+      if (u * UNIT < size) {
+        const int i = lo + u * UNIT + 8 * (int)threadIdx.x;
+        l[u].load(logits, base, i, end - i);
+      }
+  }
+};
+
 template <bool F32>
 __global__ void __launch_bounds__(BIN_THREADS) sample_tops_kernel(Args a, Work w) {
   __shared__ float part[BIN_THREADS / 64];
@@ -501,7 +518,11 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_bins_kernel(Args a, Work w
   const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
   Rules r(a, row);
   const bool by_weight = r.p < 1.0f, by_count = r.k > 0;
-  if (listed(r) || (!by_weight && !by_count)) return;
+  if (listed(a, r) || (!by_weight && !by_count)) return;
+  const int64_t base = (int64_t)row * a.vocab;
+  const int lo = c * w.size, end = min(lo + w.size, a.vocab);
+  ChunkLogits<F32> here;
+  here.load(a.logits, base, lo, end, w.size);
   if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, part, r.top)) return;
   const Bins bins(r);
   for (int i = threadIdx.x; i < BINS; i += BIN_THREADS) {
@@ -509,14 +530,13 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_bins_kernel(Args a, Work w
     if (by_count) counts[i] = 0;
   }
   __syncthreads();
-  const int64_t base = (int64_t)row * a.vocab;
-  const int lo = c * w.size, end = min(lo + w.size, a.vocab);
-  for (int i = lo + 8 * threadIdx.x; i < end; i += UNIT) {
-    Eight<F32> l;
-    l.load(a.logits, base, i, end - i);
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    const int i = lo + u * UNIT + 8 * (int)threadIdx.x;
+    if (u * UNIT >= w.size || i >= end) break;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = l.get(e, end - i);
+      const float v = here.l[u].get(e, end - i);
       const int b = bins.of(v);
       if (b == BINS - 1) continue;
       if (by_count) atomicAdd(&counts[b], 1u);
@@ -559,7 +579,12 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
   __shared__ uint32_t found, first;
   const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
   Rules r(a, row);
-  if (listed(r) || !row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, top_part, r.top)) return;
+  if (listed(a, r)) return;
+  const int64_t base = (int64_t)row * a.vocab;
+  const int lo = c * w.size, end = min(lo + w.size, a.vocab);
+  ChunkLogits<F32> here;
+  here.load(a.logits, base, lo, end, w.size);
+  if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, top_part, r.top)) return;
   const Bins bins(r);
   if (threadIdx.x == 0) info = {0, 0, BINS, BINS, BINS, 0}, found = 0;
   if (r.k > 0 || r.p < 1.0f) {
@@ -619,15 +644,14 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
   if (c == 0 && threadIdx.x == 0) w.info[row] = info;
   const int stay = info.lo, hi = info.hi, kbin = info.kbin;
   uint64_t sum = 0;
-  const int64_t base = (int64_t)row * a.vocab;
-  const int lo = c * w.size, end = min(lo + w.size, a.vocab);
-  for (int i = lo + 8 * threadIdx.x; i < lo + w.size; i += UNIT) {  // whole waves
-    Eight<F32> l;
-    l.load(a.logits, base, i, end - i);
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    if (u * UNIT >= w.size) break;
+    const int i = lo + u * UNIT + 8 * (int)threadIdx.x;  // whole waves, also behind the vocabulary's end
     uint32_t hits = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = l.get(e, end - i);
+      const float v = here.l[u].get(e, end - i);
       const int b = bins.of(v);
       if (b == BINS - 1) continue;
       if (b < stay) sum += left_of(a, r, v);
@@ -637,7 +661,7 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (hits >> e & 1) {
-        if (at < CANDIDATES) list[at] = entry_of(l.get(e, end - i), i + e);
+        if (at < CANDIDATES) list[at] = entry_of(here.l[u].get(e, end - i), i + e);
         ++at;
       }
   }
@@ -768,7 +792,7 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
     return;
   }
   const Bins bins(r);
-  const bool list = listed(r);
+  const bool list = listed(a, r);
   RowInfo info = {0, 0, 0, BINS, BINS, 0};
   int n;
   if (list) {
@@ -788,7 +812,7 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
   for (int c = threadIdx.x; c < PARTS; c += THREADS) s.chunk[c] = !list && c < w.chunks ? w.sums[(int64_t)row * w.chunks + c] : 0;
   if (!list)
     for (int i = threadIdx.x; i < n; i += THREADS) entry[i] = w.list[(int64_t)row * CANDIDATES + i];
-  if (n <= THREADS) {
+  if (n <= THREADS) {  // (50 of 129,280 tokens 18 us so and 29 by the sort; 512 46 both)
     rank_entries(entry, weight, n);
   } else {
     int places = 2 * THREADS;
@@ -868,9 +892,10 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
   }
 }
 
-// Tokens of a chunk: whole units, so many that the launches have about three workgroups a CU.
+// Tokens of a chunk: whole units, so many that the launches have about three workgroups a CU, two at most: more of them make the
+// draw's walk through one chunk longer, fewer add work a chunk. At most 1, 2 and 4 take, with top-p alone, 422, 348
+// and 365 us for 512 rows of 129,280 tokens and 120, 109 and 141 for 512 of 32,768; with no rule 203, 201, 237 and 64, 68, 108.
 static int chunk_size(int64_t rows, int vocab) {
-  constexpr int MOST = 2;
   const int64_t units = (vocab + UNIT - 1) / UNIT, each = rows * units / 768;
   return (int)(each < 1 ? 1 : each > MOST ? MOST : each) * UNIT;
 }
