@@ -272,3 +272,48 @@ def test_past_32_bits(device):
     assert torch.equal(tokens[-3:], t) and torch.equal(logp[-3:], lp)
     same = (u[:-3].double() * V).floor().int()
     assert (tokens[:-3] - same).abs().max() <= 1
+
+
+@pytest.mark.parametrize("R,V", [(3, 2048), (3, 2049), (1023, 2050), (1024, 2049), (1025, 2051), (2050, 2060)])
+def test_sets_of_rows(device, R, V):
+    """Around the vocabularies of one launch a row, and the rows of one set of launches."""
+    rng = np.random.default_rng([R, V])
+    temp = rng.uniform(0.3, 1.6, R)
+    temp[R // 2] = 0.0
+    v = values(rng, R, V, RULES["kpm"])
+    v["k"][-1], v["p"][0] = 20, 1.0
+    check(device, head(rng, R, V), rng.random(R).astype(np.float32), temp, **v)
+
+
+@pytest.mark.parametrize("V", [2049, 4096, 8200, 70000])
+def test_k_around_the_groups(device, V):
+    """Cuts at and next to every k at which the way to the candidates changes; all of the largest logits in one group, or one in
+    each; more equal logits in the groups than there is room for."""
+    rng = np.random.default_rng(V)
+    groups = V // 64
+    ks = sorted({1, 2, 63, 64, 65, 255, 256, 257, groups * 3 // 4, groups * 3 // 4 + 1, groups, groups + 1, 511, 512, 513, V - 1, V})
+    n = len(ks)
+    rows = [head(rng, 1, V)[0] for _ in range(4)]
+    rows[1][:64] += 40.0
+    rows[2][::64] += 40.0
+    rows[3] = torch.round(rows[3] * 0.2)                   # few values
+    for l in rows:
+        u = rng.random(n).astype(np.float32)
+        check(device, l.repeat(n, 1), u, k=ks, least_clear=0.8)
+        check(device, l.repeat(n, 1), u, k=ks, p=np.full(n, 0.83), m=np.full(n, 0.001), least_clear=0.8)
+
+
+def test_rows_do_not_depend_on_their_batch(device):
+    rng = np.random.default_rng(21)
+    R, V = 40, 9000
+    logits = head(rng, R, V).to(device)
+    u, t = torch.rand(R, device=device), torch.rand(R, device=device) + 0.2
+    k = torch.randint(0, 400, (R,), device=device, dtype=torch.int32)
+    p = torch.rand(R, device=device)
+    tokens, logp = wa.sample_logits(logits, u, t, k, p)
+    for r in (0, 7, 39):
+        a, b = wa.sample_logits(logits[r:r + 1], u[r:r + 1], t[r:r + 1], k[r:r + 1], p[r:r + 1])
+        assert int(a) == int(tokens[r]) and float(b) == float(logp[r])
+    many = 300
+    a, b = wa.sample_logits(logits[3:4].repeat(many, 1), u[3:4].repeat(many), t[3:4].repeat(many), k[3:4].repeat(many), p[3:4].repeat(many))
+    assert bool((a == tokens[3]).all()) and bool((b == logp[3]).all())
