@@ -229,13 +229,14 @@ __global__ void __launch_bounds__(64 * T::W) stream_kernel(Args a, int n_tiles) 
     wait_own_steps<T::LOADS, T::D - 1>(mine - 1 - j);  // scales among the loads ahead make it wait for more than it must
     multiply(j, slot);
     if (j + T::D < mine) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's reads have come back
       if ((j + T::D) % 8 == 0) issue_scales(j + T::D);
       issue(wave + T::W * (j + T::D), slot);
     }
     slot = slot + 1 == T::D ? 0 : slot + 1;
   }
 
-  if (T::W > 1) __syncthreads();  // the sums lie over the rings
+  __syncthreads();  // the sums lie over the rings
   float(*red)[T::TN * T::TM][4][64] = reinterpret_cast<float(*)[T::TN * T::TM][4][64]>(lds);
 #pragma unroll
   for (int j = 0; j < T::TN; ++j)
