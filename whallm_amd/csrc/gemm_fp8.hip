@@ -11,6 +11,10 @@
 // output's rounding (2^-8) but not below fp32's: for fp32 outputs the bytes, which are bf16 values, are
 // converted to bf16 in registers, exactly, and multiplied by the bf16 instructions, whose sums are fp32's (2^-21 of the
 // magnitudes), at half the rate.
+//
+// Few tokens are bound by the weights' bytes (1 token of 7168 to 4096 5.3 us, 5.5 TB/s; 6 tokens to 129,280 in fp32 132 us,
+// 7.0 TB/s), many by the matrix units and what a tile does before and behind its loop (16,384 tokens of 7168 to 4096 453 us,
+// 2.12 PFLOP/s; 8192^3 524 us, 2.10).
 #include <type_traits>
 
 #include "lds_dma.h"

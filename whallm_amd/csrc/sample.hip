@@ -9,6 +9,11 @@
 // another order would move. So weights are fixed point: e in fp64, rounded to a multiple of 2^-s, s from
 // the vocabulary's size so that no sum passes 2^62. Sums of integers do not depend on their order; every token
 // is off by at most 2^-(s + 1) of the largest one's weight (2^-46 for 129,280 tokens).
+//
+// A few rows are bound by dependent launches and, in the last one, by a workgroup's chain of barriers (1 row of 129,280 fp32
+// logits, top-k and top-p: 19 us, of it 11 to 15 the last launch; 5 rows with top-p alone 27); many rows by the instructions a token
+// takes where there is no small top-k (512 rows 316 us with top-p alone), and by HBM where there is (256 rows with top-k 50 51 us,
+// 2.6 TB/s).
 #include <cmath>
 
 #include "norm_rows.h"
