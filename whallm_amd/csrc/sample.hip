@@ -717,24 +717,49 @@ __device__ __forceinline__ void rank_entries(uint64_t* v, uint64_t* other, int n
   __syncthreads();
 }
 
+// The first groups' largest logits, a thread's own in registers: requested before anything else is known of the row.
+struct Groups {
+  static constexpr int KEPT = 4;
+  float kept[KEPT];
+  const float* tops;
+  int groups;
+  __device__ __forceinline__ Groups(const Args& a, const Work& w, int row)
+      : tops(w.groups + (int64_t)row * w.chunks * w.size / GROUP), groups((a.vocab + GROUP - 1) / GROUP) {
+#pragma unroll
+    for (int j = 0; j < KEPT; ++j) {
+      const int g = THREADS * j + (int)threadIdx.x;
+      kept[j] = g < groups ? tops[g] : -INFINITY;
+    }
+  }
+  // f(group, its largest logit) for whole waves; groups behind the last are -inf.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int j = 0; j < KEPT; ++j)
+      if (THREADS * j < groups) f(THREADS * j + (int)threadIdx.x, kept[j]);
+#pragma unroll 1
+    for (int g0 = THREADS * KEPT; g0 < groups; g0 += THREADS) {
+      const int g = g0 + (int)threadIdx.x;
+      f(g, g < groups ? tops[g] : -INFINITY);
+    }
+  }
+};
+
 // The entries of a row that a small k may keep, into `entry`, and how many there are: more than CANDIDATES where they do not
 // fit. A bin that k groups' largest logits reach bounds the tokens; `counts` is BINS + CANDIDATES words.
 template <bool F32>
-__device__ int list_row(const Args& a, const Work& w, const void* p, int row, const Rules& r, const Bins& bins, Shared& s,
+__device__ int list_row(const Args& a, const Groups& groups, const void* p, const Rules& r, const Bins& bins, Shared& s,
                         uint64_t* entry, uint32_t* counts, uint32_t* found) {
-  constexpr int EACH = BINS / THREADS, AHEAD = 4;
-  const int groups = (a.vocab + GROUP - 1) / GROUP;
-  const float* tops = w.groups + (int64_t)row * w.chunks * w.size / GROUP;
+  constexpr int EACH = BINS / THREADS, AHEAD = 8;
   uint32_t* which = counts + BINS;
   for (int i = threadIdx.x; i < BINS; i += THREADS) counts[i] = 0;
   if (threadIdx.x < 2) found[threadIdx.x] = 0;
   if (threadIdx.x == 0) s.bcast[0] = BINS - 2;
   __syncthreads();
-#pragma unroll 4
-  for (int g = threadIdx.x; g < groups; g += THREADS) {
-    const int b = bins.of(tops[g]);
+  groups.each([&](int, float top) {
+    const int b = bins.of(top);
     if (b < BINS - 1) atomicAdd(&counts[b], 1u);
-  }
+  });
   __syncthreads();
   uint64_t n = 0, total;
 #pragma unroll
@@ -748,13 +773,11 @@ __device__ int list_row(const Args& a, const Work& w, const void* p, int row, co
   }
   __syncthreads();
   const int bound = (int)s.bcast[0];
-#pragma unroll 1
-  for (int g0 = 0; g0 < groups; g0 += THREADS) {
-    const int g = g0 + (int)threadIdx.x;
-    const bool is = g < groups && bins.of(tops[g]) <= bound;
+  groups.each([&](int g, float top) {
+    const bool is = bins.of(top) <= bound;
     const uint32_t i = reserve(&found[0], is);
     if (is && i < CANDIDATES) which[i] = g;
-  }
+  });
   __syncthreads();
   const uint32_t hits = found[0];
   if (hits > CANDIDATES) return CANDIDATES + 1;
@@ -792,6 +815,7 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
   const int row = blockIdx.x;
   const void* p = (const uint8_t*)a.logits + (int64_t)row * a.vocab * (F32 ? 4 : 2);
   Rules r(a, row);
+  const Groups groups(a, w, row);
   if (!row_top<THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, s.top, r.top)) {
     if (threadIdx.x == 0) a.tokens[row] = -1, a.logp[row] = NAN;
     return;
@@ -801,7 +825,7 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
   RowInfo info = {0, 0, 0, BINS, BINS, 0};
   int n;
   if (list) {
-    n = list_row<F32>(a, w, p, row, r, bins, s, entry, (uint32_t*)weight, found);
+    n = list_row<F32>(a, groups, p, r, bins, s, entry, (uint32_t*)weight, found);
   } else {
     n = (int)w.listed[row];
     info = w.info[row];
