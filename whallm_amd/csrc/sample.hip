@@ -405,6 +405,9 @@ constexpr int MOST = 2;  // units of a chunk at most
 constexpr int GROUP = 64, LIST_K = 256;
 __device__ __forceinline__ bool listed(const Args& a, const Rules& r) { return r.k > 0 && r.k <= min(LIST_K, a.vocab / GROUP * 3 / 4); }
 
+// Rows whose cut takes bins.
+__device__ __forceinline__ bool binned(const Args& a, const Rules& r) { return !listed(a, r) && (r.k > 0 || r.p < 1.0f); }
+
 struct RowInfo {
   uint64_t below_lo, between;  // weights of the bins below lo, and of those between hi and kbin
   int32_t lo, hi;              // bins below lo stay, bins above hi go by top-p
@@ -482,20 +485,25 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_tops_kernel(Args a, Work w
   const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
   const int64_t base = (int64_t)row * a.vocab;
   const int lo = c * w.size, end = min(lo + w.size, a.vocab);
-  for (int i = c * BIN_THREADS + threadIdx.x; i < BINS; i += w.chunks * BIN_THREADS) {
-    w.weights[(int64_t)row * BINS + i] = 0;
-    w.counts[(int64_t)row * BINS + i] = 0;
+  ChunkLogits<F32> here;
+  here.load(a.logits, base, lo, end, w.size);
+  if (binned(a, Rules(a, row))) {
+    for (int i = c * BIN_THREADS + threadIdx.x; i < BINS; i += w.chunks * BIN_THREADS) {
+      w.weights[(int64_t)row * BINS + i] = 0;
+      w.counts[(int64_t)row * BINS + i] = 0;
+    }
   }
   if (c == 0 && threadIdx.x == 0) w.listed[row] = 0;
   float t = -INFINITY;
   bool nan = false;
-  for (int i = lo + 8 * threadIdx.x; i < lo + w.size; i += UNIT) {  // whole waves, also behind the vocabulary's end
-    Eight<F32> l;
-    l.load(a.logits, base, i, end - i);
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    if (u * UNIT >= w.size) break;
+    const int i = lo + u * UNIT + 8 * (int)threadIdx.x;  // whole waves, also behind the vocabulary's end
     float mine = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = l.get(e, end - i);
+      const float v = here.l[u].get(e, end - i);
       nan |= v != v;
       mine = fmaxf(mine, v);
     }
@@ -523,7 +531,7 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_bins_kernel(Args a, Work w
   const int row = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
   Rules r(a, row);
   const bool by_weight = r.p < 1.0f, by_count = r.k > 0;
-  if (listed(a, r) || (!by_weight && !by_count)) return;
+  if (!binned(a, r)) return;
   const int64_t base = (int64_t)row * a.vocab;
   const int lo = c * w.size, end = min(lo + w.size, a.vocab);
   ChunkLogits<F32> here;
@@ -592,7 +600,7 @@ __global__ void __launch_bounds__(BIN_THREADS) sample_gather_kernel(Args a, Work
   if (!row_top<BIN_THREADS>(w.tops + (int64_t)row * w.chunks, w.chunks, top_part, r.top)) return;
   const Bins bins(r);
   if (threadIdx.x == 0) info = {0, 0, BINS, BINS, BINS, 0}, found = 0;
-  if (r.k > 0 || r.p < 1.0f) {
+  if (binned(a, r)) {
     uint64_t weight[EACH], sum = 0, total, before;
     uint32_t count[EACH], n = 0;
 #pragma unroll
