@@ -87,6 +87,14 @@ def test_many_tokens(device, M, N, K, out):
     run(device, M, N, K, out, with_add=N % 2 == 0, whole=True)
 
 
+@pytest.mark.parametrize("out", ["bf16", "fp32"])
+@pytest.mark.parametrize("M,N,K", [(40, 25003, 4112), (64, 24576, 4096), (100, 25001, 4112), (128, 24640, 4224)])
+def test_weights_past_the_caches(device, M, N, K, out):
+    """One token tile and 100 MB of weights or more: odd and whole numbers of blocks and rows."""
+    run(device, M, N, K, out, with_add=N % 2 == 1, whole=True)
+    run(device, M, N, K, out, with_add=N % 2 == 0, whole=False)
+
+
 @pytest.mark.parametrize("M", [1, 20, 50, 100, 700])
 def test_forms_of_the_inputs(device, M):
     """uint8, batch dims, strides, views off 16 bytes, no tokens: the same bits."""

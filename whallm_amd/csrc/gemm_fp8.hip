@@ -276,8 +276,9 @@ __device__ __forceinline__ void wait_step(int ahead) {
   }
 }
 
-template <int TN_, int TM_, int WN_, int WM_, int KB_, int STAGES_>
+template <int TN_, int TM_, int WN_, int WM_, int KB_, int STAGES_, bool ONCE_ = false>
 struct Tile {
+  static constexpr bool ONCE = ONCE_;  // the weights pass once: loads with the non-temporal hint
   static constexpr int TN = TN_, TM = TM_, WN = WN_, WM = WM_, KB = KB_, STAGES = STAGES_, WAVES = WN * WM;
   static constexpr int BN = 16 * TN * WN, BM = 16 * TM * WM;
   static constexpr int W = BN * BLOCK, X = BM * BLOCK, SCALES = KB * (W + X);  // a stage: KB blocks' rows, then their scales
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(64 * T::WAVES) tiled_kernel(Args a, int n_tile
     // pieces behind the rows' end read the block's first one
     const uint32_t off = (uint32_t)BLOCK * b - (TAIL && BLOCK * b + 16 * piece >= a.k ? 16u * piece : 0u);
     const uint32_t to = slot + kb * (T::W + T::X);
-    if (i < T::WL) dma16(wbase, woff[i % WR] + off, to + 1024 * (wave + T::WAVES * (i % WR)));
+    if (i < T::WL) dma16<T::ONCE>(wbase, woff[i % WR] + off, to + 1024 * (wave + T::WAVES * (i % WR)));
     else dma16(xbase, xoff[(i - T::WL) % XR] + off, to + T::W + 1024 * (wave + T::WAVES * ((i - T::WL) % XR)));
   };
 
@@ -499,6 +500,12 @@ static void launch_tiled(const Args& a, hipStream_t s) {
 //   96 x 4608 x 5120   64 x 32 11.7, 64 x 64 12.8        1024 x 4096 x 7168  128 x 128 41.5, 64 x 128 53, 128 x 256 55
 //   300 x 7168 x 2048  128 x 128 12.9, 64 x 64 18.4      2048 x 4096 x 7168  128 x 256 82, 128 x 128 91, 256 x 256 92
 //   1501 x 1283 x 2560  64 x 128 12.9, 64 x 64 16        4096 x 4096 x 7168  256 x 256 112, 128 x 256 147
+//
+// One token tile of 64 x 64 or 128 x 128 and weights that no cache holds from call to call: they pass once, with twice the blocks of K
+// a step, so longer runs of a row, two steps deep, and non-temporal loads (in turn without and with; 64 x 24576 x 7168
+// 58.4 and 49.4, 128 x 129280 x 7168 287 and 254, to fp32 313 and 292, 64 x 20480 x 5120 (105 MB) 43.4 and 36.1; 64 x 16384 x 5120
+// (84 MB, held by the 256 MB cache) 17.1 and 22.9, 128 x 32768 x 2048 (67 MB) 22.4 and 22.6).
+constexpr int64_t ONCE_BYTES = 100000000;
 template <bool F32>
 static void launch(const Args& a, hipStream_t s) {
   if (a.tokens <= 16) {
@@ -516,13 +523,18 @@ static void launch(const Args& a, hipStream_t s) {
     const int64_t cost = (blocks + 255) / 256 * shape[i].cost;
     if (cost < least) least = cost, best = i;
   }
+  const bool once = a.tokens <= shape[best].t && (int64_t)a.n * a.k >= ONCE_BYTES;
   switch (best) {
     case 0: return launch_stream<Stream<1, 2, 32, 4, 3>, F32>(a, s);
     case 1: return launch_stream<Stream<2, 2, 32, 4, 2>, F32>(a, s);
     case 2: return launch_stream<Stream<4, 2, 32, 4, 2>, F32>(a, s);
-    case 3: return launch_tiled<Tile<2, 1, 2, 4, 2, 4>, F32>(a, s);
+    case 3:
+      if (once) return launch_tiled<Tile<2, 1, 2, 4, 4, 2, true>, F32>(a, s);
+      return launch_tiled<Tile<2, 1, 2, 4, 2, 4>, F32>(a, s);
     case 4: return launch_tiled<Tile<2, 2, 2, 4, 2, 3>, F32>(a, s);
-    case 5: return launch_tiled<Tile<4, 2, 2, 4, 1, 4>, F32>(a, s);
+    case 5:
+      if (once) return launch_tiled<Tile<4, 2, 2, 4, 2, 2, true>, F32>(a, s);
+      return launch_tiled<Tile<4, 2, 2, 4, 1, 4>, F32>(a, s);
     case 6: return launch_tiled<Tile<4, 4, 2, 4, 1, 3>, F32>(a, s);
     default:
       if constexpr (!F32) launch_tiled<Tile<8, 4, 2, 4, 1, 2>, F32>(a, s);
