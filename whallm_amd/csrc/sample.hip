@@ -24,6 +24,7 @@ namespace smp {
 constexpr int MAX_VOCAB = 1 << 22;
 constexpr int THREADS = 512, WAVES = THREADS / 64;
 constexpr int PARTS = 1024;  // a row's chunks at most
+constexpr int MOST = 2;      // units of a chunk at most
 // Tokens of a vocabulary that one workgroup takes in one launch, passing them several times from its L2. With top-k 50 and top-p 0.9,
 // top-p alone and neither, one row: 24, 21 and 12 us of 2048 tokens (in chunks 39, 23 and 15), 31, 25 and 13 of 4096 (16, 25
 // and 16), 51, 45 and 18 of 8192 (16, 26 and 17); 512 rows likewise.
@@ -312,24 +313,44 @@ __device__ __forceinline__ void write_token(const Args& a, int row, const Rules&
   a.logp[row] = (float)((t - log2(ldexp((double)whole, -a.shift))) * 0.6931471805599453);
 }
 
-// Writes the token whose running sum passes `want`, given the chunks' sums in s.chunk. left(l, i): the weight of
-// logit l with id i, 0 if it goes. `size` is a chunk's tokens, a multiple of THREADS. Every thread calls it.
+// Eight logits of a chunk from token i on, `n` of them there; the others are -inf.
+template <bool F32>
+struct Eight {
+  Row8<F32> raw;
+  __device__ __forceinline__ void load(const void* logits, int64_t base, int i, int n) {
+    raw.clear();
+    if (n > 0) raw.template load<false>(logits, base + i, n);
+  }
+  __device__ __forceinline__ float get(int e, int n) const { return e < n ? raw.get(e) + 0.0f : -INFINITY; }
+};
+
+// Writes the token whose running sum passes the draw's place, given the chunks' sums in s.chunk. left(l, i): the weight of
+// logit l with id i, 0 if it goes. `size` is a chunk's tokens, MOST * 8 * THREADS at most and a multiple of 4 * THREADS. Every
+// thread calls it.
 template <bool F32, typename Left>
-__device__ void draw(const Args& a, const void* p, int row, const Rules& r, Shared& s, int chunks, int size, Left left) {
+__device__ void draw(const Args& a, int row, const Rules& r, Shared& s, int chunks, int size, Left left) {
   uint64_t whole, first_of;
   __syncthreads();
-  uint64_t want = find_part(a, row, s, chunks, whole, first_of);
-  want -= first_of;
+  const uint64_t want = find_part(a, row, s, chunks, whole, first_of) - first_of;
   const int c = (int)s.bcast[0], each = size / THREADS;
   const int first = c * size + (int)threadIdx.x * each, end = min(first + each, a.vocab);
-  uint64_t mine = 0, total;
-  for (int i = first; i < end; ++i) mine += left(logit<F32>(p, i), i);
+  float l[8 * MOST];
+  uint64_t w[8 * MOST], mine = 0, total;
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    Eight<F32> raw;
+    const int i = first + 8 * u;
+    raw.load(a.logits, (int64_t)row * a.vocab, i, end - i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l[8 * u + e] = raw.get(e, end - i);
+  }
+#pragma unroll
+  for (int j = 0; j < 8 * MOST; ++j) mine += w[j] = l[j] == -INFINITY ? 0 : left(l[j], first + j);
   uint64_t before = block_scan(mine, s.part, total);
-  if (want >= before && want < before + mine) {
-    int i = first;
-    float l = logit<F32>(p, i);
-    for (uint64_t w; want >= before + (w = left(l, i)); l = logit<F32>(p, i)) before += w, ++i;
-    write_token(a, row, r, i, l, whole);
+#pragma unroll
+  for (int j = 0; j < 8 * MOST; ++j) {
+    if (want >= before && want < before + w[j]) write_token(a, row, r, first + j, l[j], whole);
+    before += w[j];
   }
 }
 
@@ -350,7 +371,7 @@ __device__ void draw_cut(const Args& a, const void* p, int row, const Rules& r, 
     block_scan(v, s.part, total);
     if (threadIdx.x == 0) s.chunk[c] = total;
   }
-  draw<F32>(a, p, row, r, s, chunks, size, left);
+  draw<F32>(a, row, r, s, chunks, size, left);
 }
 
 // Vocabularies of one chunk: a workgroup a row does all of it.
@@ -397,7 +418,6 @@ __global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
 // Either way the last launch sorts the candidates, cuts and draws. Rows of more candidates than there is room for (a cut
 // among thousands of nearly equal logits) are cut by radix selection as above.
 constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048;
-constexpr int MOST = 2;  // units of a chunk at most
 
 // A row's candidates come from its groups while k is small and at most 3/4 of the groups: beyond, the groups' bound sinks fast.
 // By the groups and by the bins, one row of 129,280 tokens: k 48 18 and 22 us, 128 22 both, 256 28 and 22; 256 rows 52 and 109,
@@ -453,17 +473,6 @@ __device__ __forceinline__ bool row_top(const float* tops, int chunks, float* pa
   top = t;
   return !nan && t != -INFINITY;
 }
-
-// Eight logits of a chunk from token i on, `n` of them there; the others are -inf.
-template <bool F32>
-struct Eight {
-  Row8<F32> raw;
-  __device__ __forceinline__ void load(const void* logits, int64_t base, int i, int n) {
-    raw.clear();
-    if (n > 0) raw.template load<false>(logits, base + i, n);
-  }
-  __device__ __forceinline__ float get(int e, int n) const { return e < n ? raw.get(e) + 0.0f : -INFINITY; }
-};
 
 // A thread's logits of a chunk, all on their way at once: before what the launch has to know of the row.
 template <bool F32>
@@ -901,7 +910,7 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
   __syncthreads();
   if (!list) {
     const uint64_t last = kept > 0 ? entry[kept - 1] : ~0ull;  // the last entry that stays
-    draw<F32>(a, p, row, r, s, w.chunks, w.size, [&](float l, int i) -> uint64_t {
+    draw<F32>(a, row, r, s, w.chunks, w.size, [&](float l, int i) -> uint64_t {
       const int b = bins.of(l);
       return b < BINS - 1 && (b < info.lo || entry_of(l, i) >= last) ? left_of(a, r, l) : 0;
     });
