@@ -659,7 +659,8 @@ WM_EXPORT int wm_fp8_rows(const void* x, int32_t fp32, int32_t rows, int32_t wid
  * x [tokens, k] and weight [n, k] bytes, 16-byte aligned, k a multiple of 16 up to 1048576; x_scales
  * [tokens, ceil(k / 128)], weight_scales [ceil(n / 128), ceil(k / 128)]; add (nullable) and out
  * [tokens, n] bf16, or fp32 where out_fp32 is 1, aligned to their elements. out may be add; it
- * overlaps no other input. Blocks are added up in fp32. Within a block the FP8 matrix
+ * overlaps no other input. Blocks are added up in fp32, each times the product of its two scales, rounded
+ * to fp32 (which loses bits below 2^-126 and is infinite from 2^128 on). Within a block the FP8 matrix
  * instructions drop what is below about 2^-13 of the sum's largest products; with fp32 outputs the
  * bytes are multiplied as bf16, whose sums are fp32's. */
 WM_EXPORT int wm_linear_fp8(const void* x, const float* x_scales, int32_t tokens, int32_t k, const void* weight,

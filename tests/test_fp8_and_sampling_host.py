@@ -146,7 +146,7 @@ def test_residual_out_over_an_input():
     (ops.quantize_fp8, torch.empty(2 ** 31, 1, device="meta"), {}, "below 2"),
     (ops.swiglu_fp8, torch.zeros(2, 7), {}, "2 I"), (ops.swiglu_fp8, torch.zeros(2, 8, dtype=torch.int32), {}, "bfloat16 or float32"),
     (ops.swiglu_fp8, torch.empty(1, (1 << 21) + 2, device="meta"), {}, "at most"),
-    (ops.swiglu_fp8, torch.zeros(2, 8), {"limit": -1.0}, "limit"), (ops.swiglu_fp8, torch.zeros(2, 8), {"limit": float("nan")}, "limit")])
+    (ops.swiglu_fp8, torch.zeros(2, 8), {"limit": 1e-60}, "limit"), (ops.swiglu_fp8, torch.zeros(2, 8), {"limit": -1.0}, "limit"), (ops.swiglu_fp8, torch.zeros(2, 8), {"limit": float("nan")}, "limit")])
 def test_rows_refusals(call, x, kw, msg):
     with pytest.raises(ValueError, match=msg):
         call(x, **kw)

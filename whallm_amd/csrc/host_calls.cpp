@@ -426,6 +426,7 @@ std::tuple<Tensor, Tensor> fp8_rows(const char* name, const Tensor& x_, bool swi
   if (W > 1 << 20) refuse("rows must have at most 1048576 values");
   if (T > INT32_MAX) refuse("rows must be below 2^31");
   if (!(limit >= 0)) refuse("limit must not be negative");
+  if (limit > 0 && (float)limit == 0.0f) refuse("limit must be 0 or a number that fp32 holds");
   const c10::Device device = device_of({&x});
   const On on(device);
   const Fp8Rows o(x.sizes(), W, device);
