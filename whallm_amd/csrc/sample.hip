@@ -11,9 +11,9 @@
 // is off by at most 2^-(s + 1) of the largest one's weight (2^-46 for 129,280 tokens).
 //
 // A few rows are bound by dependent launches and, in the last one, by a workgroup's chain of barriers (1 row of 129,280 fp32
-// logits, top-k and top-p: 19 us, of it 11 to 15 the last launch; 5 rows with top-p alone 27); many rows by the instructions a token
-// takes where there is no small top-k (512 rows 316 us with top-p alone), and by HBM where there is (256 rows with top-k 50 51 us,
-// 2.6 TB/s).
+// logits, top-k and top-p: 17 to 20 us, of it 9 to 13 the last launch; 5 rows with top-p alone 27); many rows by the instructions a token
+// takes where there is no small top-k (512 rows 313 us with top-p alone), and by HBM where there is (256 rows with top-k 50 47 us,
+// 2.8 TB/s).
 #include <cmath>
 
 #include "norm_rows.h"
@@ -25,9 +25,9 @@ constexpr int MAX_VOCAB = 1 << 22;
 constexpr int THREADS = 512, WAVES = THREADS / 64;
 constexpr int PARTS = 1024;  // a row's chunks at most
 constexpr int MOST = 2;      // units of a chunk at most
-// Tokens of a vocabulary that one workgroup takes in one launch, passing them several times from its L2. With top-k 50 and top-p 0.9,
-// top-p alone and neither, one row: 24, 21 and 12 us of 2048 tokens (in chunks 39, 23 and 15), 31, 25 and 13 of 4096 (16, 25
-// and 16), 51, 45 and 18 of 8192 (16, 26 and 17); 512 rows likewise.
+// Tokens of a vocabulary that one workgroup takes in one launch, passing them several times from its L2. With top-k 48 and top-p 0.9,
+// top-p alone and neither, one row: 22, 18 and 9 us of 2048 tokens (in chunks 22, 22 and 14), 24, 21 and 10 of 3000 (23, 23
+// and 15), 28, 24 and 10 of 4096 (16, 24 and 15), 48, 39 and 15 of 8192 (15, 25 and 15); 512 rows likewise.
 constexpr int SMALL = 2048;
 
 struct Args {
@@ -420,8 +420,8 @@ __global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
 constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048;
 
 // A row's candidates come from its groups while k is small and at most 3/4 of the groups: beyond, the groups' bound sinks fast.
-// By the groups and by the bins, one row of 129,280 tokens: k 48 18 and 22 us, 128 22 both, 256 28 and 22; 256 rows 52 and 109,
-// 56 and 110, 64 and 112. One row of 8192 (128 groups): k 96 18.5 and 22, 128 28 and 23.
+// By the groups and by the bins, one row of 129,280 tokens: k 48 16.4 and 21 us, 128 20.5 and 21.6, 256 26 and 22; 256 rows 47
+// and 108, 51 and 106, 60 and 109. One row of 8192 (128 groups): k 96 18.6 and 21.8, 128 28 and 23.
 constexpr int GROUP = 64, LIST_K = 256;
 __device__ __forceinline__ bool listed(const Args& a, const Rules& r) { return r.k > 0 && r.k <= min(LIST_K, a.vocab / GROUP * 3 / 4); }
 
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
   for (int c = threadIdx.x; c < PARTS; c += THREADS) s.chunk[c] = !list && c < w.chunks ? w.sums[(int64_t)row * w.chunks + c] : 0;
   if (!list)
     for (int i = threadIdx.x; i < n; i += THREADS) entry[i] = w.list[(int64_t)row * CANDIDATES + i];
-  if (n <= THREADS) {  // (50 of 129,280 tokens 18 us so and 29 by the sort; 512 46 both)
+  if (n <= THREADS) {  // (a row of 129,280 tokens with top-k 48 16 us so and 28 by the sort, 256 26 and 35)
     rank_entries(entry, weight, n);
   } else {
     int places = 2 * THREADS;
@@ -939,8 +939,8 @@ __global__ void __launch_bounds__(THREADS) sample_draw_kernel(Args a, Work w) {
 }
 
 // Tokens of a chunk: whole units, so many that the launches have about three workgroups a CU, two at most: more of them make the
-// draw's walk through one chunk longer, fewer add work a chunk. At most 1, 2 and 4 take, with top-p alone, 422, 348
-// and 365 us for 512 rows of 129,280 tokens and 120, 109 and 141 for 512 of 32,768; with no rule 203, 201, 237 and 64, 68, 108.
+// draw's part of one chunk longer, fewer add work a chunk. At most 1, 2 and 4 take, with top-p alone, 390, 313
+// and 328 us for 512 rows of 129,280 tokens and 118, 109 and 132 for 512 of 32,768; with no rule 180, 177, 200 and 57, 62, 87.
 static int chunk_size(int64_t rows, int vocab) {
   const int64_t units = (vocab + UNIT - 1) / UNIT, each = rows * units / 768;
   return (int)(each < 1 ? 1 : each > MOST ? MOST : each) * UNIT;
