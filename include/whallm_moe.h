@@ -729,8 +729,8 @@ WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, 
  * top_p 1 and more; min_p 0 and below (above 1 counts as 1); NaN. Logits of -inf (masked) are never
  * drawn; the largest may be +inf, which then shares with its equals alone. A row with a NaN or with nothing
  * but -inf gives token -1 and logp NaN. Weights are fixed point (2^-46 of the largest for vocabularies
- * around 131072), so that no result depends on an order of sums. tokens int32 [rows], logp fp32 [rows].
- * vocab up to 4194304. workspace: wm_sample_logits_workspace_size bytes, 16-byte aligned. */
+ * around 2^17), so that no result depends on an order of sums. tokens int32 [rows], logp fp32 [rows].
+ * vocab up to 4194304, rows up to 8388607. workspace: wm_sample_logits_workspace_size bytes, 16-byte aligned. */
 WM_EXPORT size_t wm_sample_logits_workspace_size(int32_t rows, int32_t vocab);
 WM_EXPORT int wm_sample_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab, const float* uniforms,
                                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,

@@ -22,6 +22,7 @@ namespace wm {
 namespace smp {
 
 constexpr int MAX_VOCAB = 1 << 22;
+// One row of 129,280 tokens with top-k 48: 16.2 us, with 256 threads 19.7, with 1024 18.2 (k 256: 26.7, 41.5, 24.8).
 constexpr int THREADS = 512, WAVES = THREADS / 64;
 constexpr int PARTS = 1024;  // a row's chunks at most
 constexpr int MOST = 2;      // units of a chunk at most
