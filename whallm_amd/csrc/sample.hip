@@ -449,11 +449,20 @@ struct Work {
 
 __device__ __forceinline__ uint64_t entry_of(float l, int i) { return (uint64_t)key_of(l) << 32 | (uint32_t)~i; }
 
-// A row's bins: monotone in the logit, BINS - 1 where the weight is 0 (from 2^-63.9 on).
+// A row's bins: monotone in the logit, BINS - 1 where the weight is 0 (from 2^-63.9 on). Distances are taken h times, h a power
+// of two, so that neither they nor the scale leave fp32 where the weight is not 0: a quarter for temperatures of 0.7 and more
+// (the types' largest values are 2^129 apart), 2^60 for ones below 2^-60 (differences of 2^-149 count there) among logits below 2^60;
+// larger logits are 2^36 apart or equal. Between, h is 1, and a distance past fp32 has weight 0.
 struct Bins {
-  float top, scale;
-  __device__ __forceinline__ explicit Bins(const Rules& r) : top(r.top), scale((float)(32.0 * r.scale)) {}
-  __device__ __forceinline__ int of(float l) const { return l == top ? 0 : (int)fminf((top - l) * scale, (float)(BINS - 1)); }
+  float top, h, top_h, scale;
+  __device__ __forceinline__ explicit Bins(const Rules& r) : top(r.top) {
+    const double s = 32.0 * r.scale;
+    const bool large = s <= 64.0, small = s >= 0x1p66 && fabsf(top) < 0x1p60f;
+    h = large ? 0.25f : small ? 0x1p60f : 1.0f;
+    top_h = top * h;
+    scale = (float)(large ? 4.0 * s : small ? 0x1p-60 * s : s);
+  }
+  __device__ __forceinline__ int of(float l) const { return l == top ? 0 : (int)fminf(fmaf(-l, h, top_h) * scale, (float)(BINS - 1)); }
 };
 
 // The row's largest logit from its chunks'; false for a row that has nothing to draw. Every thread calls it.
