@@ -999,7 +999,7 @@ static void launch(Args a, void* workspace, hipStream_t st) {
     const dim3 grid((unsigned)(a.rows * at.chunks));
     hipLaunchKernelGGL((sample_tops_kernel<F32>), grid, dim3(BIN_THREADS), 0, st, a, w);
     check_launch("sample_tops");
-    if (a.top_k || a.top_p || a.temperature) {  // else no row has a cut
+    if (a.top_k || a.top_p) {  // else no row takes bins: a greedy row's k of 1 is listed
       hipLaunchKernelGGL((sample_bins_kernel<F32>), grid, dim3(BIN_THREADS), 0, st, a, w);
       check_launch("sample_bins");
     }
