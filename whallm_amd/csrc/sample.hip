@@ -118,7 +118,6 @@ struct Cut {
 
 struct Shared {
   uint64_t sums[256];
-  uint32_t counts[256];
   uint64_t part[WAVES];
   float top[WAVES];
   uint64_t chunk[PARTS];  // the chunks' sums
