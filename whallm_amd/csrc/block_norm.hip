@@ -375,9 +375,6 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(const float* __restr
   }
 }
 
-// How a row is held: by `group` threads (0: a workgroup of `threads`), 8 v columns each. Short rows have 16 threads
-// or a wave, four waves a workgroup (16000 tokens of 100, captured, 5.5 us and the gradients 12.6, with a workgroup a
-// row 12.0 and 42); rows of more than 8192 columns 16 columns a thread, since a workgroup has 1024.
 // The gradient pass has what a CU holds at once, one workgroup of long rows (4001 tokens of 5120: 69.7 us, two in turn
 // 74.8), and adds a row a workgroup to the second launch's work: 8 tokens a group or more, 4 where rows are
 // short and no eights (their loads take longer), unless that leaves CUs without one: 18775 tokens of 479 with a

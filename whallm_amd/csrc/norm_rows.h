@@ -132,6 +132,9 @@ struct Weight8 {
   __device__ __forceinline__ float get(float offset, int i) const { return w.get(i) + offset; }
 };
 
+// How a row is held: by `group` threads (0: a workgroup of `threads`), 8 v columns each. Short rows have 16 threads
+// or a wave, four waves a workgroup (16000 tokens of 100, captured, 5.5 us and the gradients 12.6, with a workgroup a
+// row 12.0 and 42); rows of more than 8192 columns 16 columns a thread, since a workgroup has 1024.
 struct NormShape {
   int group, v, threads;
 };
