@@ -7,6 +7,7 @@
 // wm_last_error() where the C call does.
 #include <torch/extension.h>
 
+#include <cmath>
 #include <initializer_list>
 #include <optional>
 #include <string>
@@ -394,6 +395,8 @@ py::tuple norm_fp8(const Tensor& residual_, const Maybe& y_, const Maybe& weight
   const int64_t H = residual_.size(-1), T = residual_.numel() / H;
   if (T > INT32_MAX) refuse("tokens must be below 2^31");
   if (!(eps >= 0)) refuse("eps must not be negative");
+  if (((float)eps == 0.0f) != (eps == 0) || std::isinf((float)eps) != std::isinf(eps)) refuse("eps must be 0 or a number that fp32 holds");
+  if (std::isinf((float)weight_offset) != std::isinf(weight_offset)) refuse("weight_offset must be a number that fp32 holds");
   const Maybe y = of_type(y_, at::kBFloat16, "y"), weight = of_type(weight_, at::kBFloat16, "weight");
   if (y && y->sizes() != residual_.sizes()) refuse("y must match residual");
   if (weight && (weight->dim() != 1 || weight->size(0) != H)) refuse("weight must be [H]");
