@@ -646,7 +646,8 @@ WM_EXPORT int wm_slot_cache_route_state(wm_slot_cache* cache, double* scores, in
  *
  * wm_fp8_rows: v = the rows of x, bf16 or fp32 [rows, width]; with swiglu x is [rows, 2 width] and
  * v = silu(gate) * up, the gate's half first (the other one with up_first), clamped as the experts'
- * are where limit is above 0: gate to at most limit, up to -limit..limit. width 1..1048576. */
+ * are where limit is above 0: gate to at most limit, up to -limit..limit; silu counts as 0 for gates
+ * below -87.3, where it is less than 1.2e-36. width 1..1048576. */
 WM_EXPORT int wm_norm_fp8(const void* residual, int32_t fp32, const void* y, const void* weight, float weight_offset,
                           float eps, int32_t tokens, int32_t hidden, int32_t pow2, void* residual_out, void* q,
                           float* scales, void* x, void* stream);
@@ -729,7 +730,9 @@ WM_EXPORT int wm_process_logits(const void* logits, int32_t fp32, int32_t rows, 
  * top_p 1 and more; min_p 0 and below (above 1 counts as 1); NaN. Logits of -inf (masked) are never
  * drawn; the largest may be +inf, which then shares with its equals alone. A row with a NaN or with nothing
  * but -inf gives token -1 and logp NaN. Weights are fixed point (2^-46 of the largest for vocabularies
- * around 2^17), so that no result depends on an order of sums. tokens int32 [rows], logp fp32 [rows].
+ * around 2^17), so that no result depends on an order of sums. Time depends on the values: a row whose cut
+ * falls among more than 2048 tokens of nearly equal logits is cut by one workgroup, up to 35 times as
+ * long as others (0.4 to 0.8 ms of 129,280 tokens). tokens int32 [rows], logp fp32 [rows].
  * vocab up to 4194304, rows up to 8388607. workspace: wm_sample_logits_workspace_size bytes, 16-byte aligned. */
 WM_EXPORT size_t wm_sample_logits_workspace_size(int32_t rows, int32_t vocab);
 WM_EXPORT int wm_sample_logits(const void* logits, int32_t fp32, int32_t rows, int32_t vocab, const float* uniforms,

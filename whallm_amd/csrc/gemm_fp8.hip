@@ -12,9 +12,9 @@
 // converted to bf16 in registers, exactly, and multiplied by the bf16 instructions, whose sums are fp32's (2^-21 of the
 // magnitudes), at half the rate.
 //
-// Few tokens are bound by the weights' bytes (1 token of 7168 to 4096 5.3 us, 5.5 TB/s; 6 tokens to 129,280 in fp32 132 us,
-// 7.0 TB/s), many by the matrix units and what a tile does before and behind its loop (16,384 tokens of 7168 to 4096 453 us,
-// 2.12 PFLOP/s; 8192^3 524 us, 2.10).
+// Few tokens are bound by the weights' bytes (captured calls, 1 token of 7168 to 4096: 4.7 us with the weights in the caches,
+// 6.8 from memory, 4.3 TB/s; 6 tokens to 129,280 in fp32 141 us, 6.6 TB/s), many by the matrix units and what a tile does
+// before and behind its loop (16,384 tokens of 7168 to 4096 452 us, 2.13 PFLOP/s; 8192^3 524 us, 2.10).
 #include <type_traits>
 
 #include "lds_dma.h"
@@ -487,7 +487,9 @@ static void launch_tiled(const Args& a, hipStream_t s) {
   check_launch("linear_fp8 (tiled)");
 }
 
-// The kernel of a shape. Up to 16 tokens the weights' way from memory is all: 16 weight rows a block with 8 waves while
+// The kernel of a shape. All times here but those of the last paragraph are of calls in a row on one to three matrices, which
+// the 256 MB cache holds where they are small; from memory the shapes of 1 to 256 tokens take 1.2 to 1.5 times as
+// long (captured, 32, 96 and 256 tokens of 5120 to 4608: 7.6, 11.7 and 18.6 us warm, 11.1, 14.8 and 25.1 cold). Up to 16 tokens the weights' way from memory is all: 16 weight rows a block with 8 waves while
 // that gives two blocks a CU at most, 32 with 4 waves beyond (one token of 7168 to 4096 5.8 us and 7.3, to 24576 31.7 and
 // 26.8). Their rows pass once, so their loads are non-temporal (1 token of 7168 to 24576 30.2 us without, 26.8 with, six to
 // 129,280 154 and 134; for 64 tokens, where two blocks take a row, 12.3 with and 9.7 without).
@@ -501,10 +503,13 @@ static void launch_tiled(const Args& a, hipStream_t s) {
 //   300 x 7168 x 2048  128 x 128 12.9, 64 x 64 18.4      2048 x 4096 x 7168  128 x 256 82, 128 x 128 91, 256 x 256 92
 //   1501 x 1283 x 2560  64 x 128 12.9, 64 x 64 16        4096 x 4096 x 7168  256 x 256 112, 128 x 256 147
 //
-// One token tile of 64 x 64 or 128 x 128 and weights that no cache holds from call to call: they pass once, with twice the blocks of K
-// a step, so longer runs of a row, two steps deep, and non-temporal loads (in turn without and with; 64 x 24576 x 7168
-// 58.4 and 49.4, 128 x 129280 x 7168 287 and 254, to fp32 313 and 292, 64 x 20480 x 5120 (105 MB) 43.4 and 36.1; 64 x 16384 x 5120
-// (84 MB, held by the 256 MB cache) 17.1 and 22.9, 128 x 32768 x 2048 (67 MB) 22.4 and 22.6).
+// Where the choice falls on the 64 x 64 or the 128 x 128 tile, one token tile and weights that no cache holds from call to
+// call pass once, with twice the blocks of K a step, so longer runs of a row, two steps deep, and non-temporal loads (in turn
+// without and with; 64 x 24576 x 7168 58.4 and 49.4, 128 x 129280 x 7168 287 and 254, to fp32 313 and 292, 64 x 20480 x 5120 (105 MB)
+// 43.4 and 36.1; 64 x 16384 x 5120 (84 MB, held by the 256 MB cache) 17.1 and 22.9, 128 x 32768 x 2048 (67 MB) 22.4 and 22.6).
+// The other shapes have no such form. The streams of 32 tokens read large weights at 5.1 to 5.4 TB/s as they are (17, 24 and 32 x
+// 129280 x 7168 172, 177 and 183 us, to fp32 179, 182 and 191; 32 x 24576 x 7168 39); 64 x 128 tiles, which 65 to 128 tokens
+// of 16384 x 7168 (117 MB) take, at 3.1 to 3.3 (37 to 40 us cold).
 constexpr int64_t ONCE_BYTES = 100000000;
 template <bool F32>
 static void launch(const Args& a, hipStream_t s) {

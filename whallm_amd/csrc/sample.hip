@@ -11,9 +11,10 @@
 // is off by at most 2^-(s + 1) of the largest one's weight (2^-46 for 129,280 tokens).
 //
 // A few rows are bound by dependent launches and, in the last one, by a workgroup's chain of barriers (1 row of 129,280 fp32
-// logits, top-k and top-p: 17 to 20 us, of it 9 to 13 the last launch; 5 rows with top-p alone 27); many rows by the instructions a token
-// takes where there is no small top-k (512 rows 313 us with top-p alone), and by HBM where there is (256 rows with top-k 50 47 us,
-// 2.8 TB/s).
+// logits, top-k and top-p: 17 to 20 us, of it 9 to 13 the last launch; 5 rows with top-p alone 28); many rows by the instructions a token
+// takes where there is no small top-k (512 rows of fp32 314 us with top-p alone), and by HBM where there is (256 rows of fp32 with
+// top-k 50 47 us, 2.8 TB/s). Rows whose cut falls among more than CANDIDATES tokens of one bin take up to 35 times a row's
+// usual time (below).
 #include <cmath>
 
 #include "norm_rows.h"
@@ -415,8 +416,13 @@ __global__ void __launch_bounds__(THREADS) sample_row_kernel(Args a) {
 // 1/32 of a factor of 2, so that a cut has some hundreds of candidates where it falls among the bulk of the tokens and a few
 // where it does not.
 //
-// Either way the last launch sorts the candidates, cuts and draws. Rows of more candidates than there is room for (a cut
-// among thousands of nearly equal logits) are cut by radix selection as above.
+// Either way the last launch sorts the candidates, cuts and draws. Rows of more candidates than there is room for are
+// cut by radix selection as above: their one workgroup passes the row seven times for top-p and twelve with top-k too. That
+// is not rare for bf16: values of magnitude 8 to 16 are 1/16 apart, so that one value alone can be thousands of tokens of the tail.
+// Normal logits of mean -10 and deviation 1.5 have 2100 candidates of 129,280 at top-p 0.9 and T 1, fp32 ones of
+// deviation 1 at T 2 and top-p 0.8 as many; equal logits have all of them, for a greedy row as well. One row of 129,280 in
+// bf16 with top-p 0.9: 25 us a head's logits, 56 the normal ones below the limit, 400 to 540 above it, 716 equal ones (greedy
+// 565); 192 rows 104, 159, 876 and 952 (657).
 constexpr int BINS = 2048, BIN_THREADS = 512, UNIT = 8 * BIN_THREADS, CANDIDATES = 2048;
 
 // A row's candidates come from its groups while k is small and at most 3/4 of the groups: beyond, the groups' bound sinks fast.
@@ -977,7 +983,8 @@ struct Layout {
   }
 };
 
-// Rows that one set of launches takes, which bounds the workspace: 41 KB a row.
+// Rows that one set of launches takes, which bounds the workspace: a row has 41 KB, vocab / 16 bytes of groups and 12 bytes a
+// chunk (49 KB of 129,280 tokens, 309 KB of 4,194,304, and so 316 MB at most).
 constexpr int BATCH = 1024;
 
 template <bool F32>

@@ -956,8 +956,9 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, we
     [ceil(N / 128), ceil(K / 128)] (dequant_fp8_blocks' form), both float8_e4m3fn or uint8, K a multiple of 16
     -> [.., N] in ``out_dtype`` (bf16 or fp32), plus ``add`` of that shape and type.
 
-    fp32 results are exact to fp32's rounding (a head's logits); bf16 ones take the FP8 matrix instructions at twice
-    the rate. The gradient of x before its rounding is linear_fp8 of dy and the transposed weights and scales."""
+    fp32 results (a head's logits) have fp32 sums throughout, off by at most (140 + K / 128) 2^-24 of the sum of
+    magnitudes; bf16 ones take the FP8 matrix instructions at twice the rate, whose sums of 128 products drop what
+    is below about 2^-13 of the largest. The gradient of x before its rounding is linear_fp8 of dy and the transposed weights and scales."""
     return _lib.host_calls().linear_fp8(x, x_scales, weight, weight_scales, out_dtype, add)
 
 
@@ -989,7 +990,8 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
     say), one number of [0, 1) a row in ``uniforms``, and per row temperature, top_k (int32), top_p and min_p, fp32
     [rows], applied in this order. Returns (tokens int32 [rows], log-probabilities fp32 [rows] of the drawn tokens among
     those left). A temperature of 0 takes the largest logit, top_k 0, top_p 1 and min_p 0 are off; a row with a NaN
-    or nothing to draw gives token -1. Everything is on the device, so a captured call follows its values."""
+    or nothing to draw gives token -1. Everything is on the device, so a captured call follows its values. Rows whose cut
+    falls among thousands of equal or nearly equal logits take up to 35 times as long as others."""
     return _lib.host_calls().sample_logits(logits, uniforms, temperature, top_k, top_p, min_p)
 
 
